@@ -14,7 +14,8 @@ CSRC = os.path.join(HERE, "csrc")
 OUTDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(OUTDIR, "libmechta_kv.so")
 SOURCES = ["kv_store.cpp", "kv_root.cpp", "kv_append.hip", "kv_produce.hip", "kv_decode.hip", "kv_prefill.hip",
-           "kv_attn32.hip", "flint_store.cpp", "flint_kv.hip"]
+           "kv_attn32.hip", "flint_store.cpp", "flint_kv.hip", "paged_book.cpp", "paged_store.cpp", "paged_rows.hip",
+           "paged_attn.hip"]
 # prefill: MFMA accumulators in VGPRs, so the rare lazy rescale of O is plain VALU work instead of AGPR round trips;
 # flint_kv: the same for the decodes' score accumulators, which the softmax reads every subtile (no accumulator-register
 # reads: f16 full-layer decode 20.4-20.5 against 20.8-20.9 us, sliding layer 10.3-10.4 against 10.6-10.7 us)

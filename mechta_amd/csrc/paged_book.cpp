@@ -1,0 +1,237 @@
+// paged_book.cpp -- which pages belong to whom, and how a batch's attention is cut into work (paged_book.h).
+#include "paged_book.h"
+
+#include <algorithm>
+#include <climits>
+
+#include "../../include/mechta_kv.h"
+
+namespace mkv {
+namespace paged {
+
+void Book::init(int pages_, int page_, int seqs_, int ctx_) {
+    pages = free = pages_;
+    page = page_;
+    seqs = seqs_;
+    ctx = ctx_;
+    owners.assign(pages, 0);
+    open.assign(((size_t)pages + 63) / 64, ~0ull);
+    if (pages % 64) open.back() = (1ull << (pages % 64)) - 1;
+    low = 0;
+    table.assign(seqs, {});
+    len.assign(seqs, 0);
+    fresh.assign(seqs, 0);
+}
+
+int Book::take() {  // the free page of the lowest number; one is free
+    while (!open[low]) low++;
+    const int p = (int)(low * 64 + __builtin_ctzll(open[low]));
+    open[low] &= open[low] - 1;
+    free--;
+    owners[p] = 1;
+    return p;
+}
+
+void Book::drop(int p) {
+    if (--owners[p]) return;
+    open[p / 64] |= 1ull << (p % 64);
+    low = std::min(low, (size_t)p / 64);
+    free++;
+}
+
+int Book::distinct(const char* who, int n, const int* seq) const {
+    if (n < 0) return fail(MKV_E_ARG, "%s: %d sequences", who, n);
+    if (n && !seq) return fail(MKV_E_ARG, "%s: NULL argument", who);
+    std::vector<bool> seen(seqs, false);
+    for (int i = 0; i < n; i++) {
+        if (seq[i] < 0 || seq[i] >= seqs) return fail(MKV_E_ARG, "%s: sequence %d outside [0, %d)", who, seq[i], seqs);
+        if (seen[seq[i]]) return fail(MKV_E_ARG, "%s: sequence %d twice", who, seq[i]);
+        seen[seq[i]] = true;
+    }
+    return MKV_OK;
+}
+
+int Book::reserve(const char* who, int n, const int* seq, const int* count) {
+    if (int rc = distinct(who, n, seq)) return rc;
+    if (n && !count) return fail(MKV_E_ARG, "%s: NULL argument", who);
+    long long want = 0;
+    for (int i = 0; i < n; i++) {
+        if (count[i] < 0) return fail(MKV_E_ARG, "%s: %d positions for sequence %d", who, count[i], seq[i]);
+        if (count[i] > ctx - len[seq[i]])
+            return fail(MKV_E_POS, "%s: sequence %d of %d positions plus %d: more than the context %d", who, seq[i],
+                        len[seq[i]], count[i], ctx);
+        want += need(len[seq[i]] + count[i]) - (int)table[seq[i]].size();
+    }
+    if (want > free) return fail(MKV_E_NOMEM, "%s: %lld pages needed, %d free", who, want, free);
+    for (int i = 0; i < n; i++) table[seq[i]].reserve(need(len[seq[i]] + count[i]));  // nothing throws behind this
+    for (int i = 0; i < n; i++) {
+        std::vector<int>& t = table[seq[i]];
+        len[seq[i]] += count[i];
+        stale(seq[i], (int)t.size());
+        while ((int)t.size() < need(len[seq[i]])) t.push_back(take());
+    }
+    return MKV_OK;
+}
+
+int Book::fork(const char* who, int n, const int* src, const int* dst, const int* upto, bool own,
+               std::vector<Pair>& copies) {
+    if (int rc = distinct(who, n, dst)) return rc;
+    if (n && !src) return fail(MKV_E_ARG, "%s: NULL argument", who);
+    std::vector<bool> is_dst(seqs, false);
+    for (int i = 0; i < n; i++) is_dst[dst[i]] = true;
+    long long want = 0;
+    for (int i = 0; i < n; i++) {
+        if (src[i] < 0 || src[i] >= seqs) return fail(MKV_E_ARG, "%s: sequence %d outside [0, %d)", who, src[i], seqs);
+        if (is_dst[src[i]]) return fail(MKV_E_ARG, "%s: sequence %d is both source and destination", who, src[i]);
+        if (!table[dst[i]].empty()) return fail(MKV_E_ARG, "%s: destination %d is not empty", who, dst[i]);
+        const int m = upto ? upto[i] : len[src[i]];
+        if (m < 0 || m > len[src[i]])
+            return fail(MKV_E_POS, "%s: %d positions of sequence %d, which has %d", who, m, src[i], len[src[i]]);
+        want += own ? need(m) : m % page ? 1 : 0;
+    }
+    if (want > free) return fail(MKV_E_NOMEM, "%s: %lld pages needed, %d free", who, want, free);
+    copies.reserve(want);  // nothing throws behind these
+    for (int i = 0; i < n; i++) table[dst[i]].reserve(need(upto ? upto[i] : len[src[i]]));
+    for (int i = 0; i < n; i++) {
+        const int m = upto ? upto[i] : len[src[i]], full = own ? 0 : m / page;
+        const std::vector<int>& from = table[src[i]];
+        std::vector<int>& t = table[dst[i]];
+        t.assign(from.begin(), from.begin() + full);
+        for (int p : t) owners[p]++;
+        for (int k = full; k < need(m); k++) {
+            t.push_back(take());
+            copies.push_back({from[k], t[k]});
+        }
+        len[dst[i]] = m;
+        stale(dst[i], 0);
+    }
+    return MKV_OK;
+}
+
+int Book::release(const char* who, int n, const int* seq) {
+    if (int rc = distinct(who, n, seq)) return rc;
+    for (int i = 0; i < n; i++) {
+        for (int p : table[seq[i]]) drop(p);
+        table[seq[i]].clear();
+        len[seq[i]] = 0;
+        fresh[seq[i]] = 0;
+    }
+    return MKV_OK;
+}
+
+int Book::set_len(const char* who, int seq, int n, std::vector<Pair>& copies) {
+    if (int rc = distinct(who, 1, &seq)) return rc;
+    if (n < 0 || n > len[seq])
+        return fail(MKV_E_POS, "%s: length %d of sequence %d, which has %d", who, n, seq, len[seq]);
+    std::vector<int>& t = table[seq];
+    const int keep = need(n);
+    const bool shared = n % page && owners[t[keep - 1]] > 1;
+    if (shared) {
+        bool given = false;  // the pages given back may serve as the copy
+        for (int k = keep; k < (int)t.size(); k++) given |= owners[t[k]] == 1;
+        if (!free && !given) return fail(MKV_E_NOMEM, "%s: no free page for a copy of a shared one", who);
+    }
+    if (shared) copies.reserve(1);  // nothing throws behind this
+    while ((int)t.size() > keep) {
+        drop(t.back());
+        t.pop_back();
+    }
+    if (shared) {
+        const int was = t.back();
+        t.back() = take();
+        copies.push_back({was, t.back()});
+        owners[was]--;
+        stale(seq, keep - 1);
+    }
+    stale(seq, keep);
+    len[seq] = n;
+    return MKV_OK;
+}
+
+int Book::compact(std::vector<Pair>& copies) {
+    const int used = pages - free;
+    std::vector<int> to(pages);
+    copies.reserve(std::min(used, free));  // nothing throws behind these
+    int hole = 0;
+    for (int p = 0; p < pages; p++) to[p] = p;
+    for (int p = used; p < pages; p++) {
+        if (!owners[p]) continue;
+        while (owners[hole]) hole++;  // there are as many holes below `used` as pages in use behind it
+        to[p] = hole;
+        owners[hole] = owners[p];
+        owners[p] = 0;
+        copies.push_back({p, hole});
+    }
+    for (int s = 0; s < seqs; s++)
+        for (int k = 0; k < (int)table[s].size(); k++)
+            if (to[table[s][k]] != table[s][k]) {
+                stale(s, k);
+                table[s][k] = to[table[s][k]];
+            }
+    for (size_t w = 0; w < open.size(); w++) open[w] = 0;
+    for (int p = used; p < pages; p++) open[p / 64] |= 1ull << (p % 64);
+    low = (size_t)used / 64;
+    if (low >= open.size()) low = open.size() - 1;
+    return (int)copies.size();
+}
+
+// ---- plans ----
+
+constexpr int ROWS[KINDS] = {16, 32, 32};  // query rows of a tile
+constexpr int SPLITS = 1024;               // work-groups that splits may add to a plan
+
+size_t most_items(const Shape& g, int tokens, int seqs) {
+    const size_t rows = (size_t)tokens * (g.q_heads / g.kv_heads);
+    return (rows / ROWS[FEW] + seqs) * g.kv_heads + SPLITS;
+}
+size_t most_joins(const Shape& g, int tokens, int seqs) { return most_items(g, tokens, seqs) - SPLITS; }
+
+void plan_window(const Shape& g, const std::vector<Member>& batch, int window, Plan& out) {
+    for (auto& v : out.items) v.clear();
+    out.joins.clear();
+    struct Tile {
+        int member, tok0, row0, k0, k1, kind;
+    };
+    std::vector<Tile> tiles;
+    const int group = g.q_heads / g.kv_heads;
+    long long keys = 0;
+    int tok0 = 0;
+    for (int i = 0; i < (int)batch.size(); i++) {
+        const Member& m = batch[i];
+        const int rows = m.count * group, pos0 = m.len - m.count;
+        const int kind = rows <= ROWS[FEW] ? FEW : SOME;
+        for (int r = 0; r < rows; r += ROWS[kind]) {
+            const int last = (std::min(r + ROWS[kind], rows) - 1) / group;
+            const int lo = window ? std::max(0, pos0 + r / group - window + 1) : 0;
+            tiles.push_back({i, tok0, r, lo / KEYS * KEYS, pos0 + last + 1, kind});
+            keys += (long long)(tiles.back().k1 - tiles.back().k0) * g.kv_heads;
+        }
+        tok0 += m.count;
+    }
+    // Splits: about two work-groups per CU, of 256 positions at least (two tiles for each of a work-group's waves).
+    const long long chunk = std::max(256ll, (keys + 511) / 512);
+    int part = 0;
+    for (const Tile& t : tiles) {
+        const Member& m = batch[t.member];
+        const int rows = m.count * group, count = std::min(ROWS[t.kind], rows - t.row0);
+        const int units = (t.k1 - t.k0 + KEYS - 1) / KEYS;
+        int splits = (int)std::min((long long)units, (t.k1 - t.k0 + chunk - 1) / chunk);
+        splits = std::min(splits, (PART_ROWS - part) / (count * g.kv_heads));
+        if (splits < 2) splits = 1;
+        for (int head = 0; head < g.kv_heads; head++) {
+            for (int s = 0; s < splits; s++) {
+                const int a = t.k0 + (int)((long long)units * s / splits) * KEYS;
+                const int b = s + 1 < splits ? t.k0 + (int)((long long)units * (s + 1) / splits) * KEYS : t.k1;
+                out.items[t.kind].push_back({m.seq, head, t.tok0, t.row0, rows, m.len - m.count, a, b,
+                                             splits > 1 ? part + s * count : -1, {0, 0, 0}});
+            }
+            if (splits > 1) {
+                out.joins.push_back({head, t.tok0, t.row0, count, part, splits, {0, 0}});
+                part += splits * count;
+            }
+        }
+    }
+}
+
+}  // namespace paged
+}  // namespace mkv

@@ -1,0 +1,286 @@
+// paged_rows.hip -- what moves rows of the paged cache: uploads of its tables, page copies, the append with rotary
+// positions, rotary positions alone, rows out of the pages. All bound by memory or, small, by their launch.
+#include <algorithm>
+
+#include "paged_device.h"
+
+namespace mkv {
+namespace paged {
+namespace {
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// ---- uploads: segments of words out of pinned host memory into place, a work-group each ----
+__global__ void __launch_bounds__(256) apply_kernel(int* __restrict__ dev, const unsigned* __restrict__ stage) {
+    const Segment s = ((const Segment*)stage)[blockIdx.x];
+    for (unsigned i = threadIdx.x; i < s.words; i += 256) dev[s.dst + i] = (int)stage[s.src + i];
+}
+
+// ---- page copies: every plane (layer, K|V) of a list of pages. Sources and destinations of a launch are different
+// pages. A unit is 4 KB of one plane's page (the least page of the least shape): 16 bytes a thread, four units in flight.
+constexpr int PAIRS = 256;  // of a launch, in its arguments
+struct PairList {
+    Pair p[PAIRS];
+};
+constexpr int UNITS = 4;
+__global__ void __launch_bounds__(256) copy_kernel(char* __restrict__ pool, PairList list, unsigned units, unsigned per_page,
+                                                   unsigned planes, size_t page_bytes, size_t plane_bytes) {
+    const unsigned u0 = blockIdx.x * UNITS;
+    u32x4 x[UNITS];
+    size_t to[UNITS];
+#pragma unroll
+    for (int i = 0; i < UNITS; i++) {
+        const unsigned u = min(u0 + i, units - 1);
+        const unsigned at = u % per_page, rest = u / per_page, plane = rest % planes, pair = rest / planes;
+        const size_t off = plane * plane_bytes + (size_t)at * 4096 + threadIdx.x * 16;
+        to[i] = off + list.p[pair].dst * page_bytes;
+        x[i] = __builtin_nontemporal_load((const u32x4*)(pool + off + list.p[pair].src * page_bytes));
+    }
+#pragma unroll
+    for (int i = 0; i < UNITS; i++)
+        if (u0 + i < units) __builtin_nontemporal_store(x[i], (u32x4*)(pool + to[i]));
+}
+
+// ---- rotary positions ----
+// cos and sin of a position's pairs: the angle in whole turns in 64 bits, its fraction alone goes on in 32.
+__device__ inline float2 turn(const RopeArgs& r, int pos, int pair) {
+    const double t = (double)pos * r.turns[pair];
+    const float f = 2.f * (float)(t - rint(t));
+    float s, c;
+    sincospif(f, &s, &c);
+    return make_float2(c * r.amplitude, s * r.amplitude);
+}
+__device__ inline void rotate_pair(float& a, float& b, float2 cs) {
+    const float x = a * cs.x - b * cs.y;
+    b = b * cs.x + a * cs.y;
+    a = x;
+}
+
+// One unit of a row's rotation: 8 elements of either side of their pairs (half layout), 8 elements (interleaved), 8
+// elements that are copied; without 8-element alignment a pair or an element. Whoever reads an element writes it, so a
+// row may be rotated in place. cs: the row's pairs. to(d): where element d (and, for units of 8, those behind it) goes.
+template <typename T, bool WIDE>
+__device__ inline int row_units(int dim, int rot, int layout) {
+    if (!WIDE) return rot / 2 + dim - rot;
+    return layout == MPG_HALF ? rot / 16 + (dim - rot) / 8 : dim / 8;
+}
+template <typename T, bool WIDE, typename To>
+__device__ inline void rotate_unit(const T* __restrict__ x, int u, int rot, int layout, const float2* cs, To to) {
+    if constexpr (!WIDE) {
+        if (u >= rot / 2) {
+            *to(rot / 2 + u) = x[rot / 2 + u];
+            return;
+        }
+        const int i = layout == MPG_HALF ? u : 2 * u, j = layout == MPG_HALF ? u + rot / 2 : 2 * u + 1;
+        float a = (float)x[i], b = (float)x[j];
+        rotate_pair(a, b, cs[u]);
+        *to(i) = (T)a;
+        *to(j) = (T)b;
+    } else if (layout == MPG_HALF && u < rot / 16) {
+        Vec8<T> a = load8(x + 8 * u), b = load8(x + rot / 2 + 8 * u);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            float p = (float)a[e], q = (float)b[e];
+            rotate_pair(p, q, cs[8 * u + e]);
+            a[e] = (T)p;
+            b[e] = (T)q;
+        }
+        store8(to(8 * u), a);
+        store8(to(rot / 2 + 8 * u), b);
+    } else {
+        const int d = layout == MPG_HALF ? rot / 2 + 8 * u : 8 * u;
+        Vec8<T> a = load8(x + d);
+        if (d < rot) {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                float p = (float)a[e], q = (float)a[e + 1];
+                rotate_pair(p, q, cs[(d + e) / 2]);
+                a[e] = (T)p;
+                a[e + 1] = (T)q;
+            }
+        }
+        store8(to(d), a);
+    }
+}
+
+constexpr int ROT_ROWS = 8;  // rows of a work-group: their angles are shared by the heads
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(256) rotate_kernel(RopeArgs r, int rows, int heads, int dim, const T* x, int64_t x_row,
+                                                     int64_t x_head, const int* __restrict__ pos, T* out, int64_t o_row,
+                                                     int64_t o_head) {
+    extern __shared__ float2 cs[];  // [ROT_ROWS][r.dim / 2]
+    const int row0 = blockIdx.x * ROT_ROWS, n = min(ROT_ROWS, rows - row0), half = r.dim / 2;
+    for (int i = threadIdx.x; i < n * half; i += 256) cs[i] = turn(r, pos[row0 + i / half], i % half);
+    __syncthreads();
+    const int units = row_units<T, WIDE>(dim, r.dim, r.layout), all = n * heads * units;
+    for (int i = threadIdx.x + 256 * blockIdx.y; i < all; i += 256 * gridDim.y) {
+        const int u = i % units, head = i / units % heads, row = i / units / heads;
+        T* const o = out + (row0 + row) * o_row + head * o_head;
+        rotate_unit<T, WIDE>(x + (row0 + row) * x_row + head * x_head, u, r.dim, r.layout, cs + row * half,
+                             [&](int d) { return o + d; });
+    }
+}
+
+// ---- append ----
+// Work-group = (run of new tokens inside one 32-position block of a page, kv head): the head's K rows, rotated, its V
+// rows, and the query heads that read it, rotated. A V block that is all new is turned in registers (8 positions of 8
+// dims a thread) and written in 16-byte pieces, others element by element.
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(256) append_kernel(const Run* __restrict__ runs, const int* __restrict__ nruns,
+                                                     const int* __restrict__ table, int most_pages, int page, int dim,
+                                                     int group, T* __restrict__ kpool, T* __restrict__ vpool, int rows,
+                                                     const T* __restrict__ k, int64_t k_tok, int64_t k_head,
+                                                     const T* __restrict__ v, int64_t v_tok, int64_t v_head, const T* q,
+                                                     int64_t q_tok, int64_t q_head, T* q_out, RopeArgs r) {
+    extern __shared__ float2 cs[];  // [KEYS][r.dim / 2]
+    const int head = blockIdx.y, kv_heads = gridDim.y, half = r.dim / 2;
+    const int units = row_units<T, WIDE>(dim, r.dim, r.layout), count = *nruns;
+    for (int i = blockIdx.x; i < count; i += gridDim.x) {
+        Run run = runs[i];
+        run.count = min(run.count, rows - run.tok);
+        if (run.count <= 0) continue;
+        const size_t p = table[(size_t)run.seq * most_pages + run.pos / page];
+        const size_t base = (p * kv_heads + head) * page * dim;  // the head's part of the page
+        const int in = run.pos % page;
+        __syncthreads();  // the table of the run before has been read
+        for (int j = threadIdx.x; j < run.count * half; j += 256) cs[j] = turn(r, run.pos + j / half, j % half);
+        __syncthreads();
+        const int per = q ? group + 1 : 1;  // rows a token: its K row, then query heads
+        for (int j = threadIdx.x; j < run.count * per * units; j += 256) {
+            const int u = j % units, row = j / units, t = row / per, which = row % per;
+            const int64_t tok = run.tok + t;
+            if (which == 0) {
+                const int pos = in + t;
+                T* const o = kpool + base + (size_t)(pos / 16) * 16 * dim + pos % 16 * 8;
+                rotate_unit<T, WIDE>(k + tok * k_tok + head * k_head, u, r.dim, r.layout, cs + t * half,
+                                     [&](int d) { return o + d / 8 * 128 + d % 8; });
+            } else {
+                const int h = head * group + which - 1;
+                T* const o = q_out + (tok * kv_heads * group + h) * dim;
+                rotate_unit<T, WIDE>(q + tok * q_tok + h * q_head, u, r.dim, r.layout, cs + t * half,
+                                     [&](int d) { return o + d; });
+            }
+        }
+        const T* const vs = v + run.tok * v_tok + head * v_head;
+        T* const vb = vpool + base + (size_t)(in / KEYS) * KEYS * dim;
+        if (run.count == KEYS) {
+            for (int j = threadIdx.x; j < dim / 2; j += 256) {  // (group of 8 positions, 8 dims)
+                const int g = j / (dim / 8), d = j % (dim / 8) * 8;
+                Vec8<T> x[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = load8(vs + (16 * (e / 4) + 4 * g + e % 4) * v_tok + d);
+#pragma unroll
+                for (int c = 0; c < 8; c++)
+                    store8(vb + (g * dim + d + c) * 8,
+                           Vec8<T>{x[0][c], x[1][c], x[2][c], x[3][c], x[4][c], x[5][c], x[6][c], x[7][c]});
+            }
+        } else {
+            for (int j = threadIdx.x; j < run.count * dim / 8; j += 256) {
+                const int t = j / (dim / 8), d = j % (dim / 8) * 8, at = in % KEYS + t;
+                const Vec8<T> x = load8(vs + t * v_tok + d);
+                T* const o = vb + (at % 16 / 4 * dim + d) * 8 + at / 16 * 4 + at % 4;
+#pragma unroll
+                for (int c = 0; c < 8; c++) o[c * 8] = x[c];
+            }
+        }
+    }
+}
+
+// ---- rows out of the pages: 8 elements a thread ----
+template <typename T>
+__global__ void __launch_bounds__(256) read_kernel(const T* __restrict__ pool, const int* __restrict__ table, int page,
+                                                   int kv_heads, int dim, int is_v, int p0, int p1, T* __restrict__ dst) {
+    const size_t per = (size_t)kv_heads * dim / 8, i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= per * (p1 - p0)) return;
+    const int pos = p0 + (int)(i / per), head = (int)(i % per) / (dim / 8), d = (int)(i % (dim / 8)) * 8, in = pos % page;
+    const T* const b = pool + ((size_t)table[pos / page] * kv_heads + head) * page * dim;
+    Vec8<T> x;
+    if (!is_v) {
+        x = load8(b + (size_t)(in / 16) * 16 * dim + d * 16 + in % 16 * 8);
+    } else {
+        const T* const s = b + (size_t)(in / KEYS) * KEYS * dim + (in % 16 / 4 * dim + d) * 8 + in % KEYS / 16 * 4 + in % 4;
+#pragma unroll
+        for (int c = 0; c < 8; c++) x[c] = s[c * 8];
+    }
+    store8(dst + i * 8, x);
+}
+
+template <typename T>
+hipError_t append_as(const Geometry& g, char* pool, int layer, const int* table, const Run* runs, const int* nruns, int grid,
+                     int rows, const Rows& k, const Rows& v, const Rows& q, void* q_out, const RopeArgs* rope, hipStream_t s) {
+    RopeArgs none{};
+    none.layout = MPG_HALF;
+    const RopeArgs& r = rope ? *rope : none;
+    T* const kp = (T*)pool + (size_t)layer * 2 * g.plane_elems();
+    const size_t lds = (size_t)KEYS * (r.dim / 2) * sizeof(float2);
+    const auto kernel = r.dim % 16 ? append_kernel<T, false> : append_kernel<T, true>;
+    kernel<<<dim3(grid, g.kv_heads), dim3(256), lds, s>>>(runs, nruns, table, g.most_pages, g.page, g.head_dim,
+                                                          g.q_heads / g.kv_heads, kp, kp + g.plane_elems(), rows,
+                                                          (const T*)k.p, k.tok, k.head, (const T*)v.p, v.tok, v.head,
+                                                          (const T*)q.p, q.tok, q.head, (T*)q_out, r);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t rotate_as(const RopeArgs& r, int rows, int heads, int dim, const Rows& x, const int* pos, const Rows& out,
+                     hipStream_t s) {
+    const bool wide = r.dim % 16 == 0 && dim % 8 == 0 && x.tok % 8 == 0 && x.head % 8 == 0 && out.tok % 8 == 0 &&
+                      out.head % 8 == 0 && (uintptr_t)x.p % 16 == 0 && (uintptr_t)out.p % 16 == 0;
+    const size_t lds = (size_t)ROT_ROWS * (r.dim / 2) * sizeof(float2);
+    const auto kernel = wide ? rotate_kernel<T, true> : rotate_kernel<T, false>;
+    kernel<<<dim3((rows + ROT_ROWS - 1) / ROT_ROWS), dim3(256), lds, s>>>(r, rows, heads, dim, (const T*)x.p, x.tok, x.head,
+                                                                         pos, (T*)out.p, out.tok, out.head);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_apply(int* dev, const unsigned* stage, int segments, hipStream_t s) {
+    apply_kernel<<<dim3(segments), dim3(256), 0, s>>>(dev, stage);
+    return hipGetLastError();
+}
+
+hipError_t launch_copies(const Geometry& g, char* pool, const Pair* pairs, int n, hipStream_t s) {
+    const size_t page = g.page_elems() * 2;
+    const unsigned planes = 2 * g.layers, per_page = (unsigned)(page / 4096);
+    // pairs of a launch: in its arguments, its units counted in 31 bits
+    const int most = (int)std::max<size_t>(1, std::min<size_t>(PAIRS, (1ull << 31) / ((size_t)planes * per_page)));
+    for (int i = 0; i < n; i += most) {
+        PairList list;
+        const int m = std::min(most, n - i);
+        std::copy(pairs + i, pairs + i + m, list.p);
+        std::fill(list.p + m, list.p + PAIRS, Pair{0, 0});
+        const unsigned units = (unsigned)m * planes * per_page;
+        copy_kernel<<<dim3((units + UNITS - 1) / UNITS), dim3(256), 0, s>>>(pool, list, units, per_page, planes, page,
+                                                                           g.plane_elems() * 2);
+        if (const hipError_t e = hipGetLastError()) return e;
+    }
+    return hipSuccess;
+}
+
+hipError_t launch_append(const Geometry& g, char* pool, int layer, const int* table, const Run* runs, const int* nruns,
+                         int grid, int rows, const Rows& k, const Rows& v, const Rows& q, void* q_out, const RopeArgs* rope,
+                         hipStream_t s) {
+    return g.fmt == MKV_F16 ? append_as<_Float16>(g, pool, layer, table, runs, nruns, grid, rows, k, v, q, q_out, rope, s)
+                            : append_as<__bf16>(g, pool, layer, table, runs, nruns, grid, rows, k, v, q, q_out, rope, s);
+}
+
+hipError_t launch_read(const Geometry& g, const char* pool, int layer, int which, const int* table, int p0, int p1, void* dst,
+                       hipStream_t s) {
+    const size_t threads = (size_t)(p1 - p0) * g.kv_heads * g.head_dim / 8;
+    const char* const base = pool + ((size_t)layer * 2 + which) * g.plane_elems() * 2;
+    // both types are 16 bits that are only moved
+    read_kernel<_Float16><<<dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s>>>(
+        (const _Float16*)base, table, g.page, g.kv_heads, g.head_dim, which == MKV_V, p0, p1, (_Float16*)dst);
+    return hipGetLastError();
+}
+
+hipError_t launch_rotate(const RopeArgs& r, int fmt, int rows, int heads, int dim, const Rows& x, const int* pos,
+                         const Rows& out, hipStream_t s) {
+    return fmt == MKV_F16   ? rotate_as<_Float16>(r, rows, heads, dim, x, pos, out, s)
+           : fmt == MKV_F32 ? rotate_as<float>(r, rows, heads, dim, x, pos, out, s)
+                            : rotate_as<__bf16>(r, rows, heads, dim, x, pos, out, s);
+}
+
+}  // namespace paged
+}  // namespace mkv

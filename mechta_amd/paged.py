@@ -1,0 +1,341 @@
+"""Python mirror of the paged cache's C ABI (include/mechta_paged.h), over the same libmechta_kv.so.
+
+Many sequences share one pool of pages: PagedKv keeps the pages, forks, copies, frees and compacts them, appends the new
+tokens of a batch (rotating K and q) and attends over the pages; rotate() applies rotary positions alone. Every compute
+call goes through the HIP library.
+"""
+import ctypes
+
+from mechta_amd import F16, F32, K, V, MkvError, lib as _mkv_lib  # noqa: F401
+
+BF16 = 2
+
+# every symbol include/mechta_paged.h declares
+SYMBOLS = ["mpg_rope_freqs", "mpg_rotate", "mpg_bytes", "mpg_create", "mpg_destroy", "mpg_set_stream", "mpg_sync",
+           "mpg_len", "mpg_table", "mpg_free_pages", "mpg_pages", "mpg_reserve", "mpg_begin", "mpg_set_len", "mpg_fork",
+           "mpg_copy", "mpg_free", "mpg_compact", "mpg_append", "mpg_attend", "mpg_read_rows"]
+
+LAYOUTS = {"half": 0, "interleaved": 1}
+SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
+
+_done = False
+
+
+class _Rope(ctypes.Structure):
+    _fields_ = [("dim", ctypes.c_int), ("layout", ctypes.c_int), ("scaling", ctypes.c_int), ("original", ctypes.c_int),
+                ("base", ctypes.c_double), ("factor", ctypes.c_double), ("beta_fast", ctypes.c_double),
+                ("beta_slow", ctypes.c_double), ("low", ctypes.c_double), ("high", ctypes.c_double),
+                ("amplitude", ctypes.c_double)]
+
+
+class _Config(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("layers", "q_heads", "kv_heads", "head_dim", "fmt", "pages", "page", "seqs",
+                                            "ctx", "tokens")]
+
+
+def lib():
+    global _done
+    L = _mkv_lib()
+    if not _done:
+        P, I, F, S, L64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_int64
+        R, C, IP, DP = ctypes.POINTER(_Rope), ctypes.POINTER(_Config), ctypes.POINTER(I), ctypes.POINTER(ctypes.c_double)
+        sig = {
+            "mpg_rope_freqs": ([R, DP, DP], I),
+            "mpg_rotate": ([R, I, I, I, I, P, L64, L64, P, P, L64, L64, P], I),
+            "mpg_bytes": ([C], S),
+            "mpg_create": ([ctypes.POINTER(P), C, IP, R, P], I),
+            "mpg_destroy": ([P], I),
+            "mpg_set_stream": ([P, P], I),
+            "mpg_sync": ([P], I),
+            "mpg_len": ([P, I, IP], I),
+            "mpg_table": ([P, I, IP, I], I),
+            "mpg_free_pages": ([P, IP], I),
+            "mpg_pages": ([P, I, I, ctypes.POINTER(P)], I),
+            "mpg_reserve": ([P, I, IP, IP], I),
+            "mpg_begin": ([P, I, IP, IP, IP], I),
+            "mpg_set_len": ([P, I, I], I),
+            "mpg_fork": ([P, I, IP, IP, IP], I),
+            "mpg_copy": ([P, I, IP, IP], I),
+            "mpg_free": ([P, I, IP], I),
+            "mpg_compact": ([P, IP], I),
+            "mpg_append": ([P, I, I, P, L64, L64, P, L64, L64, P, L64, L64, P, I], I),
+            "mpg_attend": ([P, I, I, P, L64, L64, F, P, P, L64, L64, P], I),
+            "mpg_read_rows": ([P, I, I, I, I, I, P], I),
+        }
+        for name, (args, res) in sig.items():
+            f = getattr(L, name)
+            f.argtypes = args
+            f.restype = res
+        _done = True
+    return L
+
+
+def _check(rc):
+    if rc < 0:
+        raise MkvError(rc, lib().mkv_last_error().decode())
+    return rc
+
+
+def _ints(xs, n=None, what="list"):
+    xs = [int(x) for x in xs]
+    if n is not None and len(xs) != n:
+        raise ValueError(f"{what} has {len(xs)} entries, {n} needed")
+    return (ctypes.c_int * max(len(xs), 1))(*xs)
+
+
+def _dtype(fmt):
+    import torch
+    return {F16: torch.float16, F32: torch.float32, BF16: torch.bfloat16}[fmt]
+
+
+class Rope:
+    """Rotary positions: the first `dim` elements of a head turn, in pairs (i, i + dim/2) ("half") or (2i, 2i + 1)
+    ("interleaved"). scaling: "none", "linear", "ntk", "yarn" or "bands", by `factor`, with the context `original` that
+    the model was trained on for the last two (include/mechta_paged.h has the formulas)."""
+
+    def __init__(self, dim, layout="half", base=10000.0, scaling="none", factor=1.0, original=0, beta_fast=32.0,
+                 beta_slow=1.0, low=1.0, high=4.0, amplitude=0.0):
+        if layout not in LAYOUTS:
+            raise ValueError(f"layout {layout!r}: one of {', '.join(LAYOUTS)}")
+        if scaling not in SCALINGS:
+            raise ValueError(f"scaling {scaling!r}: one of {', '.join(SCALINGS)}")
+        self.c = _Rope(dim, LAYOUTS[layout], SCALINGS[scaling], int(original), base, factor, beta_fast, beta_slow, low,
+                       high, amplitude)
+        self.dim = dim
+        self.freqs()  # refuses what the library does
+
+    def freqs(self):
+        """(turning speed of each pair in radians per position, amplitude)."""
+        th, amp = (ctypes.c_double * max(self.dim // 2, 1))(), ctypes.c_double()
+        _check(lib().mpg_rope_freqs(ctypes.byref(self.c), th, ctypes.byref(amp)))
+        return list(th), amp.value
+
+
+def _rows(t, heads, dim, dtype, device, what):
+    """Checks a [rows, heads, dim] tensor whose last dimension is contiguous; returns its pointer and strides."""
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, {device} needed")
+    if t.dtype != dtype:
+        raise ValueError(f"{what} is {t.dtype}, {dtype} needed")
+    if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or (dim is not None and t.shape[2] != dim):
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, (rows, {heads or 'heads'}, {dim or 'dim'}) needed")
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError(f"the last dimension of {what} must be contiguous")
+    return ctypes.c_void_p(t.data_ptr()), t.stride(0), t.stride(1)
+
+
+def rotate(x, pos, rope, out=None):
+    """x [rows, heads, dim] (f16, bf16 or f32) rotated at the positions pos [rows] (int32), into `out` (may be x), on
+    torch's current stream of x's device."""
+    import torch
+    fmts = {torch.float16: F16, torch.float32: F32, torch.bfloat16: BF16}
+    if x.device.type != "cuda":
+        raise ValueError("x must be a device tensor")
+    if x.dtype not in fmts:
+        raise ValueError(f"x is {x.dtype}: float16, bfloat16 or float32 needed")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    a = _rows(x, None, None, x.dtype, x.device, "x")
+    b = _rows(out, x.shape[1], x.shape[2], x.dtype, x.device, "out")
+    if out.shape[0] != x.shape[0]:
+        raise ValueError(f"out has {out.shape[0]} rows, x {x.shape[0]}")
+    if pos.device != x.device or pos.dtype != torch.int32 or pos.shape != x.shape[:1] or not pos.is_contiguous():
+        raise ValueError(f"pos must be {x.shape[0]} contiguous int32 on {x.device}")
+    with torch.cuda.device(x.device):
+        _check(lib().mpg_rotate(ctypes.byref(rope.c), fmts[x.dtype], x.shape[0], x.shape[1], x.shape[2], *a,
+                                ctypes.c_void_p(pos.data_ptr()), *b,
+                                ctypes.c_void_p(torch.cuda.current_stream(x.device).cuda_stream)))
+    return out
+
+
+class PagedKv:
+    """The paged cache of `layers` layers: `pages` pages of `page` positions for up to `seqs` sequences of up to `ctx`
+    positions; batches of up to `tokens` new tokens. fmt: F16 or BF16 (pages, q, k, v, gate, out). windows: per layer the
+    positions a token sees, itself included (0 or None: all). rope: what append() rotates by. Calls are ordered on
+    `stream` (default: torch's current stream).
+
+        kv.begin([0, 3], [1, 512])            # one new token for sequence 0, 512 for sequence 3
+        for layer in range(layers):
+            q = kv.append(layer, k, v, q)     # [513, heads, dim] each; q comes back rotated
+            out = kv.attend(layer, q)
+    """
+
+    def __init__(self, layers, q_heads, kv_heads, head_dim, pages, page=64, seqs=64, ctx=262144, fmt=F16, tokens=8192,
+                 windows=None, rope=None, stream=None):
+        import torch
+        self._h = ctypes.c_void_p()
+        s = stream if stream is not None else torch.cuda.current_stream()
+        self._stream, self.device = s, s.device
+        self.layers, self.q_heads, self.kv_heads, self.head_dim = layers, q_heads, kv_heads, head_dim
+        self.num_pages, self.page, self.seqs, self.ctx, self.fmt, self.rope = pages, page, seqs, ctx, fmt, rope
+        self._config = _Config(layers, q_heads, kv_heads, head_dim, fmt, pages, page, seqs, ctx, tokens)
+        w = None if windows is None else _ints([x or 0 for x in windows], layers, "windows")
+        with torch.cuda.device(self.device):
+            _check(lib().mpg_create(ctypes.byref(self._h), ctypes.byref(self._config), w,
+                                    None if rope is None else ctypes.byref(rope.c), ctypes.c_void_p(s.cuda_stream)))
+        self.dtype = _dtype(fmt)
+
+    def close(self):
+        if getattr(self, "_h", None):
+            lib().mpg_destroy(self._h)
+            self._h = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *a):
+        self.close()
+
+    @property
+    def handle(self):
+        """The handle's mpg_t* (ctypes.c_void_p), for a caller that calls the C ABI through lib() directly."""
+        return self._h
+
+    def set_stream(self, stream):
+        if stream.device != self.device:
+            raise ValueError(f"the stream is on {stream.device}, the cache on {self.device}")
+        self._stream = stream
+        _check(lib().mpg_set_stream(self._h, ctypes.c_void_p(stream.cuda_stream)))
+
+    def sync(self):
+        _check(lib().mpg_sync(self._h))
+
+    # ---- sequences and pages ----
+
+    def length(self, seq):
+        n = ctypes.c_int()
+        _check(lib().mpg_len(self._h, seq, ctypes.byref(n)))
+        return n.value
+
+    def table(self, seq):
+        """The sequence's pages, in order."""
+        n = _check(lib().mpg_table(self._h, seq, None, 0))
+        t = (ctypes.c_int * max(n, 1))()
+        _check(lib().mpg_table(self._h, seq, t, n))
+        return list(t)[:n]
+
+    def free_pages(self):
+        n = ctypes.c_int()
+        _check(lib().mpg_free_pages(self._h, ctypes.byref(n)))
+        return n.value
+
+    def reserve(self, seqs, counts):
+        """Lengthens the sequences by `counts` positions that the caller fills in itself (pages())."""
+        _check(lib().mpg_reserve(self._h, len(seqs), _ints(seqs), _ints(counts, len(seqs), "counts")))
+
+    def begin(self, seqs, counts):
+        """Lengthens the sequences by `counts` new tokens and makes them the batch of the appends and attention that
+        follow; returns the number of tokens."""
+        n = ctypes.c_int()
+        _check(lib().mpg_begin(self._h, len(seqs), _ints(seqs), _ints(counts, len(seqs), "counts"), ctypes.byref(n)))
+        return n.value
+
+    def set_len(self, seq, n):
+        """Shortens a sequence (rollback)."""
+        _check(lib().mpg_set_len(self._h, seq, n))
+
+    def fork(self, src, dst, lens=None):
+        """Each empty dst[i] becomes the first lens[i] positions of src[i] (all by default); full pages are shared."""
+        n = len(dst)
+        _check(lib().mpg_fork(self._h, n, _ints(src, n, "src"), _ints(dst),
+                              None if lens is None else _ints(lens, n, "lens")))
+
+    def copy(self, src, dst):
+        """Each empty dst[i] becomes src[i] on pages of its own."""
+        n = len(dst)
+        _check(lib().mpg_copy(self._h, n, _ints(src, n, "src"), _ints(dst)))
+
+    def free(self, seqs):
+        _check(lib().mpg_free(self._h, len(seqs), _ints(seqs)))
+
+    def compact(self):
+        """Moves pages so that those in use are the lowest; returns how many moved."""
+        n = ctypes.c_int()
+        _check(lib().mpg_compact(self._h, ctypes.byref(n)))
+        return n.value
+
+    def pages(self, layer, which):
+        """A layer's K or V pages as a tensor over the pool: K [page][kv head][pos/16][d/8][16][8], V [page][kv head]
+        [pos/32][4][d][8] (element e of group g of V: position 16 (e/4) + 4 g + e%4 of its 32)."""
+        import torch
+        base = ctypes.c_void_p()
+        _check(lib().mpg_pages(self._h, layer, which, ctypes.byref(base)))
+        h, p, d = self.kv_heads, self.page, self.head_dim
+        shape = (self.num_pages, h, p // 16, d // 8, 16, 8) if which == K else (self.num_pages, h, p // 32, 4, d, 8)
+
+        class _Mem:  # the tensor keeps the cache alive
+            owner = self
+            __cuda_array_interface__ = {"shape": shape, "typestr": "<i2", "data": (base.value, False), "version": 2}
+
+        return torch.as_tensor(_Mem(), device=self.device).view(self.dtype)
+
+    def read_rows(self, layer, which, seq, p0=0, p1=None, out=None):
+        """Positions [p0, p1) of a sequence's K or V, [p1 - p0, kv_heads, head_dim]."""
+        import torch
+        if p1 is None:
+            p1 = self.length(seq)
+        n = max(0, p1 - p0)
+        if out is None:
+            out = torch.empty((n, self.kv_heads, self.head_dim), dtype=self.dtype, device=self.device)
+        _rows(out, self.kv_heads, self.head_dim, self.dtype, self.device, "out")
+        if out.shape[0] != n or not out.is_contiguous():
+            raise ValueError(f"out must be {n} contiguous rows")
+        _check(lib().mpg_read_rows(self._h, layer, which, seq, p0, p1, ctypes.c_void_p(out.data_ptr())))
+        return out
+
+    # ---- the layers' calls ----
+
+    def append(self, layer, k, v, q=None, q_out=None, rotate=None):
+        """Writes the batch's k and v [tokens, kv_heads, head_dim] into the pages, k rotated (rotate=False: it is already;
+        default: if the cache has a rope). With q [tokens, q_heads, head_dim]: returns it rotated, in q_out (may be q)."""
+        import torch
+        rows = k.shape[0]
+        ka = _rows(k, self.kv_heads, self.head_dim, self.dtype, self.device, "k")
+        va = _rows(v, self.kv_heads, self.head_dim, self.dtype, self.device, "v")
+        if v.shape[0] != rows or (q is not None and q.shape[0] != rows):
+            raise ValueError("k, v and q differ in rows")
+        qa, qo = (None, 0, 0), None
+        if q is not None:
+            qa = _rows(q, self.q_heads, self.head_dim, self.dtype, self.device, "q")
+            if q_out is None:
+                q_out = torch.empty((rows, self.q_heads, self.head_dim), dtype=self.dtype, device=self.device)
+            _rows(q_out, self.q_heads, self.head_dim, self.dtype, self.device, "q_out")
+            if q_out.shape[0] != rows or not q_out.is_contiguous():
+                raise ValueError(f"q_out must be {rows} contiguous rows")
+            qo = ctypes.c_void_p(q_out.data_ptr())
+        if rotate is None:
+            rotate = self.rope is not None
+        _check(lib().mpg_append(self._h, layer, rows, *ka, *va, *qa, qo, 1 if rotate else 0))
+        return q_out
+
+    def attend(self, layer, q, scale=None, sinks=None, gate=None, out=None):
+        """Attention of the batch's tokens: q [tokens, q_heads, head_dim] -> out of the same shape. scale: 1/sqrt(head_dim)
+        by default; sinks [q_heads] f32; gate as q: out = attention * sigmoid(gate)."""
+        import torch
+        qa = _rows(q, self.q_heads, self.head_dim, self.dtype, self.device, "q")
+        rows = q.shape[0]
+        if out is None:
+            out = torch.empty((rows, self.q_heads, self.head_dim), dtype=self.dtype, device=self.device)
+        _rows(out, self.q_heads, self.head_dim, self.dtype, self.device, "out")
+        if out.shape[0] != rows or not out.is_contiguous():
+            raise ValueError(f"out must be {rows} contiguous rows")
+        ga, sp = (None, 0, 0), None
+        if gate is not None:
+            ga = _rows(gate, self.q_heads, self.head_dim, self.dtype, self.device, "gate")
+            if gate.shape[0] != rows:
+                raise ValueError("q and gate differ in rows")
+        if sinks is not None:
+            if sinks.device != self.device or sinks.dtype != torch.float32 or sinks.shape != (self.q_heads,) \
+                    or not sinks.is_contiguous():
+                raise ValueError(f"sinks must be {self.q_heads} contiguous float32 on {self.device}")
+            sp = ctypes.c_void_p(sinks.data_ptr())
+        if scale is None:
+            scale = self.head_dim ** -0.5
+        _check(lib().mpg_attend(self._h, layer, rows, *qa, scale, sp, *ga, ctypes.c_void_p(out.data_ptr())))
+        return out
