@@ -260,10 +260,10 @@ def _prepare_own(case, s):
             for which in (0, 1):
                 kv.pages(layer, which).copy_(s["pool"][layer, which].view(kv.pages(layer, which).shape))
         if case["op"] == "fork":
-            kv.begin([0], [case["length"]])
+            kv.reserve([0], [case["length"]])
         else:  # slot 1 holds the pages below the conversation in slot 0
-            kv.begin([1], [s["n"] * case["page"]])
-            kv.begin([0], [s["n"] * case["page"]])
+            kv.reserve([1], [s["n"] * case["page"]])
+            kv.reserve([0], [s["n"] * case["page"]])
         del s["pool"]
         return dict(s, kv=kv)
     n = len(s["counts"])
