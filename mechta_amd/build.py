@@ -26,7 +26,9 @@ SOURCES = ["kv_store.cpp", "kv_root.cpp", "kv_append.hip", "kv_produce.hip", "kv
 EXTRA = {"kv_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-fno-honor-nans", "-mllvm",
                             "-amdgpu-sched-strategy=max-ilp"], "kv_decode.hip": ["-fno-honor-nans", "-mllvm", "-amdgpu-sched-strategy=max-ilp"],
          "kv_attn32.hip": ["-fno-honor-nans"], "flint_kv.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-fno-honor-nans"],
-         "kv_produce.hip": ["-ffp-contract=off"]}
+         "kv_produce.hip": ["-ffp-contract=off"],
+         # accumulators in VGPRs: few_rows of heads of 256 and 32 rows fits its registers (with AGPRs it spilled 35)
+         "paged_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 # measurement aid of bench.py (a plain HBM read of a given size), its own library: not part of the KV-cache ABI
 PROBE_SRC, PROBE_LIB = "hbm_probe.hip", os.path.join(OUTDIR, "libmkv_probe.so")
 ARCH = os.environ.get("MKV_OFFLOAD_ARCH", "gfx950")

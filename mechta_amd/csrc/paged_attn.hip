@@ -3,23 +3,27 @@
 // Row r of a sequence's query rows is (token r / group, query head head * group + r % group): the query heads of a kv head
 // and the tokens of a chunk share the keys they read. A work-group takes a tile of rows and a range of keys (Item); where
 // a tile's keys are split, join_kernel puts the splits together.
+#include "mkv_device.h"
 #include "paged_device.h"
 
 namespace mkv {
 namespace paged {
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float NEG_INF = -__builtin_huge_valf();
 
 __device__ inline f32x4 mfma16(Vec8<_Float16> a, Vec8<_Float16> b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 __device__ inline f32x4 mfma16(Vec8<__bf16> a, Vec8<__bf16> b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+__device__ inline f32x16 mfma32(Vec8<_Float16> a, Vec8<_Float16> b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ inline f32x16 mfma32(Vec8<__bf16> a, Vec8<__bf16> b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
 // The weights 2^(s - ref) of a row are rounded to the cache's type for the matrix units (half a step: 2^-11 of a weight
@@ -32,15 +36,13 @@ struct Weights;
 template <>
 struct Weights<_Float16> {
     static constexpr float LIFT = 10.f, LAZY = 5.f;
-    static constexpr unsigned INF2 = 0x7C007C00u;
+    static constexpr unsigned short INF = 0x7C00;
 };
 template <>
 struct Weights<__bf16> {
     static constexpr float LIFT = 0.f, LAZY = 8.f;
-    static constexpr unsigned INF2 = 0x7F807F80u;
+    static constexpr unsigned short INF = 0x7F80;
 };
-
-__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 struct Args {
     const int* table;
@@ -62,15 +64,15 @@ template <typename T, int D>
 __device__ inline void finish(const Args& a, int tok, int head, int d, f32x4 acc, float m, float l) {
     if (a.sinks) {  // m is the reference of acc and l, in log2 units
         const float s = a.sinks[head] * LOG2E, top = fmaxf(m, s);
-        const float f = m == NEG_INF ? 0.f : exp2_fast(m - top);
+        const float f = m == NEG_INF ? 0.f : fast_exp2(m - top);
         acc *= f;
-        l = l * f + exp2_fast(s - top);
+        l = l * f + fast_exp2(s - top);
     }
     acc *= 1.f / l;
     if (a.gate) {
         const Vec4<T> g = *(const Vec4<T>*)((const T*)a.gate + tok * a.g_tok + head * a.g_head + d);
 #pragma unroll
-        for (int i = 0; i < 4; i++) acc[i] *= 1.f / (1.f + exp2_fast(-LOG2E * (float)g[i]));
+        for (int i = 0; i < 4; i++) acc[i] *= 1.f / (1.f + fast_exp2(-LOG2E * (float)g[i]));
     }
     Vec4<T> o;
 #pragma unroll
@@ -78,7 +80,10 @@ __device__ inline void finish(const Args& a, int tok, int head, int d, f32x4 acc
     *(Vec4<T>*)((T*)a.out + ((size_t)tok * a.q_heads + head) * D + d) = o;
 }
 
-// Whether any of a wave's V operands holds an infinity or NaN.
+// Infinities and NaN of V in positions that some of a wave's rows do not see: 0 x NaN would reach those rows through the
+// products. Only tiles that cross a row's bounds can hold such (edge tiles); there the operands are looked through, and
+// what is not finite is taken as zero. The rows that see it get it after the loop, by plain additions, value by value
+// (add_odd): slow, and rare.
 template <typename T, int N>
 __device__ inline bool odd_values(const Vec8<T> (&v)[N]) {
     typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
@@ -89,36 +94,25 @@ __device__ inline bool odd_values(const Vec8<T> (&v)[N]) {
 #pragma unroll
         for (int j = 0; j < 4; j++) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, x[j] & 0x7FFF7FFFu));
     }
-    constexpr unsigned short inf = Weights<T>::INF2 & 0xFFFF;
-    return __any(top.x >= inf || top.y >= inf);
+    return __any(top.x >= Weights<T>::INF || top.y >= Weights<T>::INF);
 }
-
-// P.V where a tile's V holds infinities or NaN that some row does not see (0 x NaN would reach it): the finite part as
-// ever, and per row how many +inf, -inf and NaN of each dim it sees, counted by the matrix units (a tile has 32
-// positions: at most 32 of each), which then decide the sum.
-template <typename T, int NRT>
-__device__ inline void odd_product(Vec8<T> v, const Vec8<T> (&p)[NRT], const Vec8<T> (&seen)[NRT],
-                                                     f32x4 (&o)[NRT]) {
-    Vec8<T> fine, odd;
+template <typename T>
+__device__ inline Vec8<T> finite(Vec8<T> v) {
+    typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+    u16x8 x = __builtin_bit_cast(u16x8, v);
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const float x = (float)v[e];
-        const bool nan = x != x, inf = __builtin_isinf(x);
-        fine[e] = nan || inf ? (T)0.f : v[e];
-        odd[e] = (T)(nan ? 16384.f : inf ? (x > 0 ? 1.f : 128.f) : 0.f);
-    }
+    for (int e = 0; e < 8; e++) x[e] = (x[e] & 0x7FFF) >= Weights<T>::INF ? 0 : x[e];
+    return __builtin_bit_cast(Vec8<T>, x);
+}
+// v: element 0 of dim 0 of a 32-position block of V; position x of it, dims d .. d + 3, added to o where not finite
+template <typename T, int D>
+__device__ inline f32x4 add_odd(const T* v, int x, int d, bool seen, f32x4 o) {
+    const unsigned short* const p = (const unsigned short*)v + (size_t)((x % 16 / 4) * D + d) * 8 + x / 16 * 4 + x % 4;
 #pragma unroll
-    for (int t = 0; t < NRT; t++) {
-        o[t] = mfma16(fine, p[t], o[t]);
-        const f32x4 c = mfma16(odd, seen[t], f32x4{});
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int n = (int)c[i];
-            if (n & 127) o[t][i] += -NEG_INF;
-            if (n >> 7 & 127) o[t][i] += NEG_INF;
-            if (n >> 14) o[t][i] = __builtin_nanf("");
-        }
-    }
+    for (int i = 0; i < 4; i++)
+        if (seen && (p[8 * i] & 0x7FFF) >= Weights<T>::INF) o[i] += (float)__builtin_bit_cast(T, p[8 * i]);
+    __builtin_amdgcn_sched_barrier(0);  // a few registers at a time
+    return o;
 }
 
 // ---- few rows: NRT x 16 query rows against keys streamed once ----
@@ -133,6 +127,9 @@ template <typename T, int D, int NRT>
 __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, const Item* __restrict__ items,
                                                                        const int* __restrict__ nitems) {
     constexpr int NS = D / 32, NV = D / 16;
+    // Q in registers, or where they are scarce (two waves a SIMD, heads of 256) in LDS, rows 16 bytes apart in the banks
+    constexpr bool QLDS = D == 256 && NRT == 1;
+    __shared__ __attribute__((aligned(16))) T sq[QLDS ? 16 : 1][D + 8];
     __shared__ __attribute__((aligned(16))) float so[4][16][D + 4];
     __shared__ float sm[4][16], sl[4][16];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
@@ -148,7 +145,7 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
         const int all_hi = it.pos0 + it.row0 / a.group;
         const int all_lo = a.window ? it.pos0 + last_row / a.group - a.window + 1 : 0;
 
-        Vec8<T> q[NRT][NS];
+        Vec8<T> q[NRT][QLDS ? 1 : NS];
         int lo[NRT], hi[NRT];  // keys the lane's row sees
 #pragma unroll
         for (int t = 0; t < NRT; t++) {
@@ -157,9 +154,19 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
             hi[t] = is ? it.pos0 + tok : -1;
             lo[t] = a.window ? it.pos0 + tok - a.window + 1 : 0;
             const T* const src = (const T*)a.q + (int64_t)(it.tok0 + tok) * a.q_tok + head * a.q_head + 8 * g;
+            if constexpr (QLDS) {
+                // each wave brings a quarter of the rows' dims
 #pragma unroll
-            for (int s = 0; s < NS; s++) q[t][s] = is ? load8(src + 32 * s) : Vec8<T>{};
+                for (int s = 0; s < NS / 4; s++) {
+                    const int d = 32 * (w * (NS / 4) + s);
+                    *(Vec8<T>*)&sq[r][d + 8 * g] = is ? load8(src + d) : Vec8<T>{};
+                }
+            } else {
+#pragma unroll
+                for (int s = 0; s < NS; s++) q[t][s] = is ? load8(src + 32 * s) : Vec8<T>{};
+            }
         }
+        if constexpr (QLDS) __syncthreads();
         f32x4 o[NRT][NV];
         float m[NRT], l[NRT];  // the reference of the row's weights (log2 units), the lane's share of their sum
 #pragma unroll
@@ -186,6 +193,7 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
 #pragma unroll
             for (int i = 0; i < NV; i++) vf[i] = load8(vp + off + (g * D + 16 * i + r) * 8);
         };
+        bool odd = false;
         if (w < blocks) {
             size_t off = offset(w, page_of(w));
             load_k(off);
@@ -201,9 +209,11 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
 #pragma unroll
                 for (int i = 0; i < NS; i++)
 #pragma unroll
-                    for (int t = 0; t < NRT; t++)
+                    for (int t = 0; t < NRT; t++) {
+                        const Vec8<T> x = QLDS ? *(const Vec8<T>*)&sq[r][32 * i + 8 * g] : q[t][QLDS ? 0 : i];
 #pragma unroll
-                        for (int b = 0; b < 2; b++) s[t][b] = mfma16(kf[b][i], q[t][i], s[t][b]);
+                        for (int b = 0; b < 2; b++) s[t][b] = mfma16(kf[b][i], x, s[t][b]);
+                    }
                 load_k(next);
                 const int k0 = key_of(j);
                 const bool edge = k0 + KEYS - 1 > all_hi || k0 < all_lo;
@@ -223,7 +233,7 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
                     top = fmaxf(top, __shfl_xor(top, 32)) * a.scale2 - Weights<T>::LIFT;
                     const bool move = m[t] != NEG_INF && top > m[t] + Weights<T>::LAZY;
                     if (__any(move)) {
-                        const float f = move ? exp2_fast(m[t] - top) : 1.f;
+                        const float f = move ? fast_exp2(m[t] - top) : 1.f;
                         l[t] *= f;
 #pragma unroll
                         for (int i = 0; i < NV; i++) o[t][i] *= f;
@@ -232,37 +242,39 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
                     const float ref = m[t] == NEG_INF ? 0.f : m[t];
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        const float x = exp2_fast(__builtin_fmaf(s[t][e / 4][e % 4], a.scale2, -ref));
+                        const float x = fast_exp2(__builtin_fmaf(s[t][e / 4][e % 4], a.scale2, -ref));
                         l[t] += x;
                         p[t][e] = (T)x;
                     }
                 }
                 if (edge && odd_values(vf)) {
-                    Vec8<T> seen[NRT];
+                    odd = true;
 #pragma unroll
-                    for (int t = 0; t < NRT; t++)
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const int key = k0 + e / 4 * 16 + 4 * g + e % 4;
-                            seen[t][e] = (T)(key > hi[t] || key < lo[t] ? 0.f : 1.f);
-                        }
-#pragma unroll
-                    for (int i = 0; i < NV; i++) {
-                        f32x4 x[NRT];
-#pragma unroll
-                        for (int t = 0; t < NRT; t++) x[t] = o[t][i];
-                        odd_product<T, NRT>(vf[i], p, seen, x);
-#pragma unroll
-                        for (int t = 0; t < NRT; t++) o[t][i] = x[t];
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < NV; i++)
-#pragma unroll
-                        for (int t = 0; t < NRT; t++) o[t][i] = mfma16(vf[i], p[t], o[t][i]);
+                    for (int i = 0; i < NV; i++) vf[i] = finite(vf[i]);
                 }
+#pragma unroll
+                for (int i = 0; i < NV; i++)
+#pragma unroll
+                    for (int t = 0; t < NRT; t++) o[t][i] = mfma16(vf[i], p[t], o[t][i]);
                 load_v(next);
                 off = next;
+            }
+        }
+        if (odd) {
+            for (int j = w; j < blocks; j += 4) {
+                const int k0 = key_of(j);
+                if (k0 + KEYS - 1 <= all_hi && k0 >= all_lo) continue;
+                const T* const v = vp + offset(j, page_of(j));
+                for (int x = 0; x < KEYS; x++) {
+#pragma unroll
+                    for (int t = 0; t < NRT; t++) {
+                        const bool seen = k0 + x <= hi[t] && k0 + x >= lo[t];
+                        if (!__any(seen)) continue;
+#pragma unroll
+                        for (int i = 0; i < NV; i++)
+                            o[t][i] = add_odd<T, D>(v, x, 16 * i + 4 * g, seen, o[t][i]);
+                    }
+                }
             }
         }
         // the four waves' states of 16 rows at a time
@@ -284,7 +296,7 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
             float f[4], total = 0.f;
 #pragma unroll
             for (int x = 0; x < 4; x++) {
-                f[x] = sm[x][rr] == NEG_INF ? 0.f : exp2_fast(sm[x][rr] - top);
+                f[x] = sm[x][rr] == NEG_INF ? 0.f : fast_exp2(sm[x][rr] - top);
                 total += f[x] * sl[x][rr];
             }
 #pragma unroll
@@ -312,29 +324,356 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
     }
 }
 
-// ---- splits of a tile's rows put together: D / 4 lanes a row, four dims each ----
+// ---- chunks: tiles of 256 or 128 query rows against 32-position tiles of keys shared in LDS ----
+// 8 waves. KS = 1: each has 32 rows of the work-group's 256 and takes every key tile. KS = 2: waves 0-3 have the 32-row
+// parts of 128 rows and take the even tiles, waves 4-7 the same rows and the odd tiles; their states meet in LDS at the end.
+// A key tile (32 x D of K and of V, contiguous in a page) comes into a ring in LDS by direct loads. Per tile and wave:
+//   S^T[32 keys][32 rows] = K . Q^T    D / 16 of 32x32x16, K rows read in the order `key` below: register i = 8 s + e of lane
+//                                      half h holds key 16 (e / 4) + 4 (2 s + h) + e % 4, which is element e of V's group
+//                                      2 s + h: the scores become the B operand of the next product where they are
+//   softmax of the lane's row in registers (two lanes a row)
+//   O^T[D][32 rows] += V^T . P^T       D / 16 of 32x32x16; a lane's values all belong to its row, so a moved reference is a
+//                                      factor per lane
+template <int D, int KS>
+struct Chunk {
+    static constexpr int NW = 8, RW = NW / KS;        // waves, waves over the rows
+    static constexpr int TILE = KEYS * D * 2;         // bytes of a tile's K, or V
+    static constexpr int STEP = 2 * KS * TILE;        // the tiles that are computed at once
+    static constexpr int RING = D == 64 ? 65536 : 131072;
+    static constexpr int SLOTS = RING / STEP;
+    static constexpr int LOADS = 2 * TILE / 1024 / RW;  // 1 KB pieces of its tile (K, then V) that a wave copies
+    static_assert(LOADS >= 1 && SLOTS >= 2, "ring");
+};
+
+template <int LOADS, int MOST>
+__device__ inline void wait_loads(int later) {  // until at most `later` <= MOST steps of LOADS loads are on their way
+    if constexpr (MOST == 0) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    } else {
+        if (later >= MOST) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS * MOST) : "memory");
+        else wait_loads<LOADS, MOST - 1>(later);
+    }
+}
+
+template <typename T, int D, int KS>
+__global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict__ items, const int* __restrict__ nitems) {
+    using C = Chunk<D, KS>;
+    constexpr int NS = D / 16, NB = D / 32;
+    __shared__ __attribute__((aligned(16))) unsigned char ring[C::RING];
+    __shared__ float sm[C::NW][32], sl[C::NW][32];
+    __shared__ int odd;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h = lane >> 5;
+    const int wr = w % C::RW, kg = w / C::RW;
+    const int count = *nitems;
+    const unsigned lds0 = (unsigned)(uintptr_t)(lds_void*)ring + kg * 2 * C::TILE + wr * C::LOADS * 1024;
+    const unsigned voff = lane * 16;
+    // the K row a lane feeds: m = r goes to key 16 (m / 8 % 2) + 8 (m / 16) + m % 8
+    const int kaddr = (r >> 3 & 1) * 16 * D * 2 + ((r >> 4) * 8 + (r & 7)) * 16 + h * 256;
+    const int vaddr = h * D * 16 + r * 16;
+    for (int n = blockIdx.x; n < count; n += gridDim.x) {
+        const Item it = items[n];
+        const size_t page_bytes = (size_t)a.kv_heads * a.page * D * 2;
+        const char* const kp = (const char*)a.kpool + (size_t)it.head * a.page * D * 2;
+        const char* const vp = (const char*)a.vpool + (size_t)it.head * a.page * D * 2;
+        const int* const table = a.table + (size_t)it.seq * a.most_pages;
+        const int tiles = (it.k1 - it.k0 + KEYS - 1) / KEYS, steps = (tiles + KS - 1) / KS;
+        const int mine = (tiles - kg + KS - 1) / KS;  // tiles of this key group
+        auto page_of = [&](int j) {  // of this group's tile of step j
+            return table[(it.k0 + KEYS * min(KS * j + kg, tiles - 1)) >> a.page_shift];
+        };
+        auto issue = [&](int j, int page) {
+            if (j >= mine) return;
+            const int in = (it.k0 + KEYS * (KS * j + kg)) & (a.page - 1);
+            const size_t off = page * page_bytes + (size_t)in * D * 2;
+            const unsigned dst = lds0 + (j % C::SLOTS) * C::STEP;
+#pragma unroll
+            for (int i = 0; i < C::LOADS; i++) {
+                const int piece = wr * C::LOADS + i, per = C::TILE / 1024;
+                dma16s((piece < per ? kp : vp - C::TILE) + off + piece * 1024, voff, dst + i * 1024);
+            }
+        };
+        // infinities and NaN of V in a tile that crosses some row's bounds: each wave looks through the pieces it has copied
+        // and puts zeros there before the others read them (add_odd brings them in after the loop)
+        auto mend = [&](int j) {
+#pragma unroll
+            for (int i = 0; i < C::LOADS; i++) {
+                if (wr * C::LOADS + i < C::TILE / 1024) continue;  // K
+                Vec8<T>* const x = (Vec8<T>*)(ring + (j % C::SLOTS) * C::STEP + kg * 2 * C::TILE + (wr * C::LOADS + i) * 1024 + lane * 16);
+                const Vec8<T> v[1] = {*x};
+                if (odd_values(v)) {
+                    *x = finite(v[0]);
+                    odd = 1;
+                }
+            }
+        };
+        __syncthreads();  // the ring and the flag of the item before have been read
+        if (threadIdx.x == 0) odd = 0;
+        __syncthreads();
+        for (int j = 0; j < C::SLOTS - 1; j++) issue(j, page_of(j));
+        int page = page_of(C::SLOTS - 1);
+
+        const int row = it.row0 + 32 * wr + r, last_row = min(it.row0 + 32 * C::RW, it.rows) - 1;
+        const int tok = row / a.group, head = it.head * a.group + row % a.group;
+        const bool is = row <= last_row && it.tok0 + tok < a.rows;
+        const int hi = is ? it.pos0 + tok : -1, lo = a.window ? it.pos0 + tok - a.window + 1 : 0;
+        // keys in [tile_lo, tile_hi] are seen by all rows of the work-group
+        const int tile_hi = it.pos0 + it.row0 / a.group, tile_lo = a.window ? it.pos0 + last_row / a.group - a.window + 1 : 0;
+        // bounds of the wave's rows: keys all of them see are in [all_lo, all_hi], keys any sees in [any_lo, any_hi]
+        const int row_a = it.row0 + 32 * wr, row_b = min(row_a + 31, last_row);
+        const int all_hi = it.pos0 + row_a / a.group, any_lo = a.window ? all_hi - a.window + 1 : 0;
+        const int any_hi = row_b < row_a ? -1 : it.pos0 + row_b / a.group;
+        const int all_lo = a.window ? any_hi - a.window + 1 : 0;
+        Vec8<T> q[NS];
+        const T* const src = (const T*)a.q + (int64_t)(it.tok0 + tok) * a.q_tok + head * a.q_head + 8 * h;
+#pragma unroll
+        for (int s = 0; s < NS; s++) q[s] = is ? load8(src + 16 * s) : Vec8<T>{};
+        f32x16 o[NB];
+#pragma unroll
+        for (int i = 0; i < NB; i++) o[i] = f32x16{};
+        float m = NEG_INF, l = 0.f;
+
+        for (int j = 0; j < steps; j++) {
+            const int k0 = it.k0 + KEYS * (KS * j + kg);
+            wait_loads<C::LOADS, C::SLOTS - 2>(min(mine - 1 - j, C::SLOTS - 2));
+            if (j < mine && (k0 + KEYS - 1 > tile_hi || k0 < tile_lo)) mend(j);
+            lds_barrier();  // step j is in LDS for every wave, and every wave is done with step j - 1
+            issue(j + C::SLOTS - 1, page);
+            page = page_of(j + C::SLOTS);
+            if (j >= mine) break;
+            if (k0 > any_hi || k0 + KEYS <= any_lo) continue;
+            const unsigned char* const ks = ring + (j % C::SLOTS) * C::STEP + kg * 2 * C::TILE + kaddr;
+            const unsigned char* const vs = ring + (j % C::SLOTS) * C::STEP + kg * 2 * C::TILE + C::TILE + vaddr;
+            f32x16 s = f32x16{};
+            {
+                constexpr int AHEAD = 3;  // K operands on their way ahead of the products
+                Vec8<T> k[AHEAD];
+#pragma unroll
+                for (int i = 0; i < AHEAD; i++) k[i] = *(const Vec8<T>*)(ks + i * 512);
+#pragma unroll
+                for (int i = 0; i < NS; i++) {
+                    const Vec8<T> x = k[i % AHEAD];
+                    if (i + AHEAD < NS) k[i % AHEAD] = *(const Vec8<T>*)(ks + (i + AHEAD) * 512);
+                    s = mfma32(x, q[i], s);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+                for (int i = 0; i < NS - AHEAD; i++) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+            }
+            const bool edge = k0 + KEYS - 1 > all_hi || k0 < all_lo;
+            auto key = [&](int i) { return k0 + i % 8 / 4 * 16 + 4 * (i / 8 * 2 + h) + i % 4; };
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (key(i) > hi || key(i) < lo) s[i] = NEG_INF;
+            }
+            float top = fmaxf(s[0], s[1]);  // the compiler's: it waits for the products
+#pragma unroll
+            for (int i = 2; i < 16; i += 2) top = vmax3(top, s[i], s[i + 1]);
+            top = max_xor32(top) * a.scale2 - Weights<T>::LIFT;
+            const bool move = m != NEG_INF && top > m + Weights<T>::LAZY;
+            if (__any(move)) {
+                const float f = move ? fast_exp2(m - top) : 1.f;
+                l *= f;
+#pragma unroll
+                for (int i = 0; i < NB; i++) o[i] *= f;
+            }
+            if (move || m == NEG_INF) m = top;
+            const float ref = m == NEG_INF ? 0.f : m;
+            Vec8<T> p[2];
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float x = fast_exp2(__builtin_fmaf(s[i], a.scale2, -ref));
+                sum += x;
+                p[i / 8][i % 8] = (T)x;
+            }
+            l += sum;
+            auto v_of = [&](int i) {  // operand i: dim block i % NB, groups 2 (i / NB) + h
+                return *(const Vec8<T>*)(vs + (i / NB) * 2 * D * 16 + (i % NB) * 512);
+            };
+            {
+                constexpr int AHEAD = 3;
+                Vec8<T> v[AHEAD];
+#pragma unroll
+                for (int i = 0; i < AHEAD; i++) v[i] = v_of(i);
+#pragma unroll
+                for (int i = 0; i < 2 * NB; i++) {
+                    const Vec8<T> x = v[i % AHEAD];
+                    if (i + AHEAD < 2 * NB) v[i % AHEAD] = v_of(i + AHEAD);
+                    o[i % NB] = mfma32(x, p[i / NB], o[i % NB]);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+                for (int i = 0; i < 2 * NB - AHEAD; i++) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+            }
+        }
+        __syncthreads();
+        if (odd) {
+            for (int j = 0; j < mine; j++) {
+                const int k0 = it.k0 + KEYS * (KS * j + kg);
+                if (k0 + KEYS - 1 <= tile_hi && k0 >= tile_lo) continue;
+                const T* const v = (const T*)vp + page_of(j) * (page_bytes / 2) + (size_t)(k0 & (a.page - 1)) * D;
+                for (int x = 0; x < KEYS; x++) {
+                    const bool seen = k0 + x <= hi && k0 + x >= lo;
+                    if (!__any(seen)) continue;
+#pragma unroll
+                    for (int i = 0; i < 4 * NB; i++) {
+                        f32x4 y = {o[i / 4][i % 4 * 4], o[i / 4][i % 4 * 4 + 1], o[i / 4][i % 4 * 4 + 2], o[i / 4][i % 4 * 4 + 3]};
+                        y = add_odd<T, D>(v, x, 32 * (i / 4) + 8 * (i % 4) + 4 * h, seen, y);
+#pragma unroll
+                        for (int c = 0; c < 4; c++) o[i / 4][i % 4 * 4 + c] = y[c];
+                    }
+                }
+            }
+        }
+        l += __shfl_xor(l, 32);
+        // o[b][4 c + i]: dim 32 b + 8 c + 4 h + i of row r
+        auto put = [&](int b0, int b1) {
+            if (!is) return;
+            const size_t at = it.part + 32 * wr + r;
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+                if (b >= b0 && b < b1) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const f32x4 x = {o[b][4 * c], o[b][4 * c + 1], o[b][4 * c + 2], o[b][4 * c + 3]};
+                        const int d = 32 * b + 8 * c + 4 * h;
+                        if (it.part < 0) finish<T, D>(a, it.tok0 + tok, head, d, x, m, l);
+                        else *(f32x4*)(a.pacc + at * D + d) = x;
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        };
+        if constexpr (KS == 1) {
+            put(0, NB);
+        } else {
+            // two states of each row, in waves w and w ^ RW: both taken to the larger reference, each wave finishes half of
+            // the dims with its partner's half of them, which goes through the ring
+            if (h == 0) {
+                sm[w][r] = m;
+                sl[w][r] = l;
+            }
+            __syncthreads();
+            const float mo = sm[w ^ C::RW][r], lo2 = sl[w ^ C::RW][r], top = fmaxf(m, mo);
+            const float f = m == NEG_INF ? 0.f : fast_exp2(m - top), fo = mo == NEG_INF ? 0.f : fast_exp2(mo - top);
+            f32x4* const give = (f32x4*)ring + w * (NB / 2 * 256) + lane;
+            const f32x4* const take = (const f32x4*)ring + (w ^ C::RW) * (NB / 2 * 256) + lane;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                if (m == NEG_INF) o[b] = f32x16{};
+                else o[b] *= f;
+                if (b / (NB / 2) != kg) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        give[(b % (NB / 2) * 4 + c) * 64] = f32x4{o[b][4 * c], o[b][4 * c + 1], o[b][4 * c + 2], o[b][4 * c + 3]};
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+                if (b / (NB / 2) == kg) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const f32x4 x = take[(b % (NB / 2) * 4 + c) * 64];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) o[b][4 * c + i] += x[i];
+                    }
+                }
+            m = top;
+            l = l * f + lo2 * fo;
+            if (kg == 0) put(0, NB / 2);
+            else put(NB / 2, NB);
+        }
+        if (it.part >= 0 && kg == 0 && h == 0 && is) {
+            a.pm[it.part + 32 * wr + r] = m;
+            a.pl[it.part + 32 * wr + r] = l;
+        }
+    }
+}
+
+// ---- splits of a tile's rows put together ----
+// D / 4 lanes hold a row's dims, four each. Of few splits the 1024 / D such groups of a work-group take a row each; of
+// JOIN_WIDE and more they share a row: each adds up every so many of its splits, with the splits' factors in LDS.
+constexpr int JOIN_WIDE = 8;
 template <typename T, int D>
 __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restrict__ joins, const int* __restrict__ njoins) {
-    constexpr int LANES = D / 4, ROWS = 256 / LANES;
-    const int count = *njoins;
+    constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+    __shared__ float factor[SPLITS_MOST];
+    __shared__ __attribute__((aligned(16))) f32x4 sa[GROUPS][LANES];
+    __shared__ float red[2][4];
+    const int count = *njoins, tid = threadIdx.x, part = tid / LANES, lane = tid % LANES, d = lane * 4;
     for (int n = blockIdx.x; n < count; n += gridDim.x) {
         const Join j = joins[n];
-        for (int r = blockIdx.y * ROWS + threadIdx.x / LANES; r < j.count; r += gridDim.y * ROWS) {
-            const int row = j.row0 + r, tok = j.tok0 + row / a.group, d = threadIdx.x % LANES * 4;
+        if (j.splits < JOIN_WIDE) {
+            for (int r = blockIdx.y * GROUPS + part; r < j.count; r += gridDim.y * GROUPS) {
+                const int row = j.row0 + r, tok = j.tok0 + row / a.group;
+                if (tok >= a.rows) continue;
+                float m[JOIN_WIDE], top = NEG_INF, total = 0.f;
+                f32x4 x[JOIN_WIDE], acc = f32x4{};
+#pragma unroll
+                for (int s = 0; s < JOIN_WIDE; s++) {  // splits behind the last: the last again, not counted
+                    const size_t at = j.part + r + (size_t)min(s, j.splits - 1) * j.count;
+                    m[s] = s < j.splits ? a.pm[at] : NEG_INF;
+                    x[s] = *(const f32x4*)(a.pacc + at * D + d);
+                    top = fmaxf(top, m[s]);
+                }
+#pragma unroll
+                for (int s = 0; s < JOIN_WIDE; s++) {
+                    const float f = m[s] == NEG_INF ? 0.f : fast_exp2(m[s] - top);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[i] += f == 0.f ? 0.f : f * x[s][i];
+                    total += f * a.pl[j.part + r + (size_t)min(s, j.splits - 1) * j.count];
+                }
+                finish<T, D>(a, tok, j.head * a.group + row % a.group, d, acc, top, total);
+            }
+            continue;
+        }
+        for (int r = blockIdx.y; r < j.count; r += gridDim.y) {
+            const int row = j.row0 + r, tok = j.tok0 + row / a.group;
             if (tok >= a.rows) continue;
             const size_t first = j.part + r;
             float top = NEG_INF;
-            for (int s = 0; s < j.splits; s++) top = fmaxf(top, a.pm[first + (size_t)s * j.count]);
-            f32x4 acc = f32x4{};
+            for (int s = tid; s < j.splits; s += 256) top = fmaxf(top, a.pm[first + (size_t)s * j.count]);
+#pragma unroll
+            for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+            __syncthreads();  // the row before has been read
+            if (tid % 64 == 0) red[0][tid / 64] = top;
+            __syncthreads();
+            top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
             float total = 0.f;
-            for (int s = 0; s < j.splits; s++) {
-                const size_t at = first + (size_t)s * j.count;
-                const float m = a.pm[at], f = m == NEG_INF ? 0.f : exp2_fast(m - top);
-                const f32x4 x = *(const f32x4*)(a.pacc + at * D + d);
+            for (int s = tid; s < j.splits; s += 256) {
+                const float m = a.pm[first + (size_t)s * j.count], f = m == NEG_INF ? 0.f : fast_exp2(m - top);
+                factor[s] = f;
+                total += f == 0.f ? 0.f : f * a.pl[first + (size_t)s * j.count];
+            }
+#pragma unroll
+            for (int x = 1; x < 64; x *= 2) total += __shfl_xor(total, x);
+            if (tid % 64 == 0) red[1][tid / 64] = total;
+            __syncthreads();
+            total = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+            f32x4 acc = f32x4{};
+            const float* const src = a.pacc + first * D + d;
+            const size_t step = (size_t)j.count * D;
+#pragma unroll 8
+            for (int s = part; s < j.splits; s += GROUPS) {
+                const float f = factor[s];
+                const f32x4 x = *(const f32x4*)(src + s * step);
 #pragma unroll
                 for (int i = 0; i < 4; i++) acc[i] += f == 0.f ? 0.f : f * x[i];
-                total += f * a.pl[at];
             }
+            sa[part][lane] = acc;
+            __syncthreads();
+            if (part) continue;
+#pragma unroll
+            for (int x = 1; x < GROUPS; x++) acc += sa[x][lane];
             finish<T, D>(a, tok, j.head * a.group + row % a.group, d, acc, top, total);
         }
     }
@@ -376,9 +715,16 @@ hipError_t attend_as(const Geometry& g, const AttendArgs& x, const int* batch, c
         few_rows<T, D, 2><<<dim3(grid[SOME]), dim3(256), 0, s>>>(a, (const Item*)(batch + l.items[SOME]), batch + SOME);
         e = hipGetLastError();
     }
+    if (grid[HALF] && e == hipSuccess) {
+        chunk_rows<T, D, 2><<<dim3(grid[HALF]), dim3(512), 0, s>>>(a, (const Item*)(batch + l.items[HALF]), batch + HALF);
+        e = hipGetLastError();
+    }
+    if (grid[MANY] && e == hipSuccess) {
+        chunk_rows<T, D, 1><<<dim3(grid[MANY]), dim3(512), 0, s>>>(a, (const Item*)(batch + l.items[MANY]), batch + MANY);
+        e = hipGetLastError();
+    }
     if (join_grid && e == hipSuccess) {
-        constexpr int rows = 256 / (D / 4);
-        join_kernel<T, D><<<dim3(join_grid, 32 / rows), dim3(256), 0, s>>>(a, (const Join*)(batch + l.joins), batch + KINDS);
+        join_kernel<T, D><<<dim3(join_grid, 32), dim3(256), 0, s>>>(a, (const Join*)(batch + l.joins), batch + KINDS);
         e = hipGetLastError();
     }
     return e;

@@ -177,44 +177,106 @@ int Book::compact(std::vector<Pair>& copies) {
 
 // ---- plans ----
 
-constexpr int ROWS[KINDS] = {16, 32, 32};  // query rows of a tile
-constexpr int SPLITS = 1024;               // work-groups that splits may add to a plan
+constexpr int XCDS = 8;  // the dispatcher deals consecutive work-groups round robin to the dies, each with its own L2
 
 size_t most_items(const Shape& g, int tokens, int seqs) {
     const size_t rows = (size_t)tokens * (g.q_heads / g.kv_heads);
-    return (rows / ROWS[FEW] + seqs) * g.kv_heads + SPLITS;
+    return (rows / TILE_ROWS[FEW] + seqs) * g.kv_heads + SPLITS_MOST;
 }
-size_t most_joins(const Shape& g, int tokens, int seqs) { return most_items(g, tokens, seqs) - SPLITS; }
+size_t most_joins(const Shape& g, int tokens, int seqs) { return most_items(g, tokens, seqs) - SPLITS_MOST; }
+
+namespace {
+struct Tile {
+    int member, tok0, row0, k0, k1, kind;
+};
+// Work-groups that run at once: 256 CUs, two to a CU except for the widest accumulators and for chunks.
+int resident(int kind, int head_dim) { return kind == FEW || (kind == SOME && head_dim <= 128) ? 512 : 256; }
+}  // namespace
+
+// Dies take the items of a list in turn (position i: die i % 8). The tiles of one (sequence, head, split) stream the same
+// keys, so they go to one die, dealt over several where they are more than a die's share of the work; on a die the longest
+// comes first.
+static void deal(std::vector<Item>& items) {
+    struct Bunch {
+        long long work;
+        std::vector<int> at;
+    };
+    std::vector<Bunch> bunches;
+    long long all = 0;
+    auto work = [&](const Item& i) { return (long long)(i.k1 - i.k0) + 2 * KEYS; };
+    for (const Item& i : items) all += work(i);
+    for (size_t i = 0; i < items.size();) {  // items of a bunch lie together
+        size_t e = i;
+        long long w = 0;
+        while (e < items.size() && items[e].seq == items[i].seq && items[e].head == items[i].head && items[e].split == items[i].split)
+            w += work(items[e++]);
+        const int ways = (int)std::min<long long>(e - i, std::max<long long>(1, (w * XCDS + all - 1) / std::max(1ll, all)));
+        for (int k = 0; k < ways; k++) {
+            Bunch b{0, {}};
+            for (size_t x = i + k; x < e; x += ways) {
+                b.work += work(items[x]);
+                b.at.push_back((int)x);
+            }
+            bunches.push_back(std::move(b));
+        }
+        i = e;
+    }
+    std::stable_sort(bunches.begin(), bunches.end(), [](const Bunch& a, const Bunch& b) { return a.work > b.work; });
+    long long load[XCDS] = {};
+    std::vector<int> mine[XCDS];
+    for (const Bunch& b : bunches) {
+        const int x = (int)(std::min_element(load, load + XCDS) - load);
+        load[x] += b.work;
+        mine[x].insert(mine[x].end(), b.at.begin(), b.at.end());
+    }
+    std::vector<Item> out;
+    out.reserve(items.size());
+    size_t next[XCDS] = {};
+    for (auto& m : mine)
+        std::stable_sort(m.begin(), m.end(), [&](int a, int b) { return work(items[a]) > work(items[b]); });
+    for (size_t i = 0; i < items.size(); i++) {
+        int x = i % XCDS;
+        if (next[x] == mine[x].size())  // that die has all of its own: the one with the most left gives
+            for (int y = 0; y < XCDS; y++)
+                if (mine[y].size() - next[y] > mine[x].size() - next[x]) x = y;
+        out.push_back(items[mine[x][next[x]++]]);
+    }
+    items.swap(out);
+}
 
 void plan_window(const Shape& g, const std::vector<Member>& batch, int window, Plan& out) {
     for (auto& v : out.items) v.clear();
     out.joins.clear();
-    struct Tile {
-        int member, tok0, row0, k0, k1, kind;
-    };
-    std::vector<Tile> tiles;
     const int group = g.q_heads / g.kv_heads;
-    long long keys = 0;
+    // Tiles of 256 rows where they fill the card, of 128 (and two key groups) where they do not.
+    long long wide = 0;
+    for (const Member& m : batch) {
+        const long long rows = (long long)m.count * group;
+        if (rows > TILE_ROWS[SOME]) wide += (rows + TILE_ROWS[MANY] - 1) / TILE_ROWS[MANY] * g.kv_heads;
+    }
+    const int chunk_kind = wide >= 256 ? MANY : HALF;
+    std::vector<Tile> tiles;
+    long long keys[KINDS] = {};
     int tok0 = 0;
     for (int i = 0; i < (int)batch.size(); i++) {
         const Member& m = batch[i];
         const int rows = m.count * group, pos0 = m.len - m.count;
-        const int kind = rows <= ROWS[FEW] ? FEW : SOME;
-        for (int r = 0; r < rows; r += ROWS[kind]) {
-            const int last = (std::min(r + ROWS[kind], rows) - 1) / group;
+        const int kind = rows <= TILE_ROWS[FEW] ? FEW : rows <= TILE_ROWS[SOME] ? SOME : chunk_kind;
+        for (int r = 0; r < rows; r += TILE_ROWS[kind]) {
+            const int last = (std::min(r + TILE_ROWS[kind], rows) - 1) / group;
             const int lo = window ? std::max(0, pos0 + r / group - window + 1) : 0;
             tiles.push_back({i, tok0, r, lo / KEYS * KEYS, pos0 + last + 1, kind});
-            keys += (long long)(tiles.back().k1 - tiles.back().k0) * g.kv_heads;
+            keys[kind] += (long long)(tiles.back().k1 - tiles.back().k0) * g.kv_heads;
         }
         tok0 += m.count;
     }
-    // Splits: about two work-groups per CU, of 256 positions at least (two tiles for each of a work-group's waves).
-    const long long chunk = std::max(256ll, (keys + 511) / 512);
+    // Splits: as many work-groups as run at once, of 256 positions at least (two tiles for each wave of few rows).
     int part = 0;
     for (const Tile& t : tiles) {
         const Member& m = batch[t.member];
-        const int rows = m.count * group, count = std::min(ROWS[t.kind], rows - t.row0);
-        const int units = (t.k1 - t.k0 + KEYS - 1) / KEYS;
+        const int rows = m.count * group, count = std::min(TILE_ROWS[t.kind], rows - t.row0);
+        const int units = (t.k1 - t.k0 + KEYS - 1) / KEYS, run = resident(t.kind, g.head_dim);
+        const long long chunk = std::max(256ll, (keys[t.kind] + run - 1) / run);
         int splits = (int)std::min((long long)units, (t.k1 - t.k0 + chunk - 1) / chunk);
         splits = std::min(splits, (PART_ROWS - part) / (count * g.kv_heads));
         if (splits < 2) splits = 1;
@@ -223,13 +285,19 @@ void plan_window(const Shape& g, const std::vector<Member>& batch, int window, P
                 const int a = t.k0 + (int)((long long)units * s / splits) * KEYS;
                 const int b = s + 1 < splits ? t.k0 + (int)((long long)units * (s + 1) / splits) * KEYS : t.k1;
                 out.items[t.kind].push_back({m.seq, head, t.tok0, t.row0, rows, m.len - m.count, a, b,
-                                             splits > 1 ? part + s * count : -1, {0, 0, 0}});
+                                             splits > 1 ? part + s * count : -1, s, {0, 0}});
             }
             if (splits > 1) {
                 out.joins.push_back({head, t.tok0, t.row0, count, part, splits, {0, 0}});
                 part += splits * count;
             }
         }
+    }
+    for (auto& list : out.items) {
+        std::stable_sort(list.begin(), list.end(), [](const Item& a, const Item& b) {
+            return a.seq != b.seq ? a.seq < b.seq : a.head != b.head ? a.head < b.head : a.split < b.split;
+        });
+        deal(list);
     }
 }
 

@@ -52,7 +52,7 @@ struct Item {
     int pos0;        // position of the sequence's first new token
     int k0, k1;      // k0 a multiple of KEYS
     int part;        // first row of the split partials it writes, -1: it writes the output
-    int pad[3];
+    int split, pad[2];
 };
 // Join of a tile's splits: split s of row r at part + s * count + r.
 struct Join {
@@ -62,7 +62,9 @@ struct Join {
 struct Run {
     int seq, tok, pos, count;
 };
-enum { FEW = 0, SOME = 1, MANY = 2, KINDS = 3 };  // Item lists by rows of a tile: <= 16, <= 32, chunks
+enum { FEW, SOME, HALF, MANY, KINDS };  // Item lists by the rows of a tile: 16, 32, 128, 256
+constexpr int TILE_ROWS[KINDS] = {16, 32, 128, 256};
+constexpr int SPLITS_MOST = 1024;  // splits of a tile at most; work-groups that splits add to a plan at most
 struct Plan {
     std::vector<Item> items[KINDS];
     std::vector<Join> joins;

@@ -12,6 +12,7 @@ struct Lists {
     size_t items[KINDS], joins, words;  // word offsets of the lists; words of the whole
 };
 constexpr size_t COUNTS = 8;  // words: items of each kind, joins
+static_assert(KINDS < COUNTS, "counts");
 
 struct Geometry {
     int layers, q_heads, kv_heads, head_dim, fmt, pages, page, most_pages;  // most_pages: of a sequence

@@ -148,6 +148,24 @@ def rotate(x, pos, rope, out=None):
     return out
 
 
+class _Handle:
+    """Owns an mpg_t*: the cache and every tensor over its pages hold it."""
+
+    def __init__(self):
+        self.ptr = ctypes.c_void_p()
+
+    def close(self):
+        if self.ptr:
+            lib().mpg_destroy(self.ptr)
+            self.ptr = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 class PagedKv:
     """The paged cache of `layers` layers: `pages` pages of `page` positions for up to `seqs` sequences of up to `ctx`
     positions; batches of up to `tokens` new tokens. fmt: F16 or BF16 (pages, q, k, v, gate, out). windows: per layer the
@@ -163,7 +181,7 @@ class PagedKv:
     def __init__(self, layers, q_heads, kv_heads, head_dim, pages, page=64, seqs=64, ctx=262144, fmt=F16, tokens=8192,
                  windows=None, rope=None, stream=None):
         import torch
-        self._h = ctypes.c_void_p()
+        self._owner = _Handle()
         s = stream if stream is not None else torch.cuda.current_stream()
         self._stream, self.device = s, s.device
         self.layers, self.q_heads, self.kv_heads, self.head_dim = layers, q_heads, kv_heads, head_dim
@@ -171,20 +189,17 @@ class PagedKv:
         self._config = _Config(layers, q_heads, kv_heads, head_dim, fmt, pages, page, seqs, ctx, tokens)
         w = None if windows is None else _ints([x or 0 for x in windows], layers, "windows")
         with torch.cuda.device(self.device):
-            _check(lib().mpg_create(ctypes.byref(self._h), ctypes.byref(self._config), w,
+            _check(lib().mpg_create(ctypes.byref(self._owner.ptr), ctypes.byref(self._config), w,
                                     None if rope is None else ctypes.byref(rope.c), ctypes.c_void_p(s.cuda_stream)))
+        self._h = self._owner.ptr
         self.dtype = _dtype(fmt)
+        self._views = {}
 
     def close(self):
-        if getattr(self, "_h", None):
-            lib().mpg_destroy(self._h)
-            self._h = ctypes.c_void_p()
-
-    def __del__(self):
-        try:
-            self.close()
-        except Exception:
-            pass
+        """Frees the cache's memory now (tensors that pages() gave must not be used any more); without it, it is freed with
+        the last of the cache and those tensors."""
+        self._owner.close()
+        self._h = self._owner.ptr
 
     def __enter__(self):
         return self
@@ -264,16 +279,18 @@ class PagedKv:
         """A layer's K or V pages as a tensor over the pool: K [page][kv head][pos/16][d/8][16][8], V [page][kv head]
         [pos/32][4][d][8] (element e of group g of V: position 16 (e/4) + 4 g + e%4 of its 32)."""
         import torch
-        base = ctypes.c_void_p()
-        _check(lib().mpg_pages(self._h, layer, which, ctypes.byref(base)))
-        h, p, d = self.kv_heads, self.page, self.head_dim
-        shape = (self.num_pages, h, p // 16, d // 8, 16, 8) if which == K else (self.num_pages, h, p // 32, 4, d, 8)
+        if (layer, which) not in self._views:
+            base = ctypes.c_void_p()
+            _check(lib().mpg_pages(self._h, layer, which, ctypes.byref(base)))
+            h, p, d = self.kv_heads, self.page, self.head_dim
+            shape = (self.num_pages, h, p // 16, d // 8, 16, 8) if which == K else (self.num_pages, h, p // 32, 4, d, 8)
 
-        class _Mem:  # the tensor keeps the cache alive
-            owner = self
-            __cuda_array_interface__ = {"shape": shape, "typestr": "<i2", "data": (base.value, False), "version": 2}
+            class _Mem:  # the tensor keeps the memory
+                owner = self._owner
+                __cuda_array_interface__ = {"shape": shape, "typestr": "<i2", "data": (base.value, False), "version": 2}
 
-        return torch.as_tensor(_Mem(), device=self.device).view(self.dtype)
+            self._views[layer, which] = torch.as_tensor(_Mem(), device=self.device).view(self.dtype)
+        return self._views[layer, which]
 
     def read_rows(self, layer, which, seq, p0=0, p1=None, out=None):
         """Positions [p0, p1) of a sequence's K or V, [p1 - p0, kv_heads, head_dim]."""

@@ -205,19 +205,19 @@ def test_refusals_change_nothing(shim):
 # ---- plans ----
 
 def make_plan(L, q_heads, kv_heads, dim, batch, window):
-    sizes = ints([0] * 4)
+    sizes = ints([0] * 5)
     L.shim_plan(q_heads, kv_heads, dim, len(batch), ints([x for m in batch for x in m]), window, sizes)
     items = []
-    for kind in range(3):
+    for kind in range(4):
         buf = ints([0] * (12 * sizes[kind] + 1))
         L.shim_items(kind, buf)
         items.append([list(buf[12 * i:12 * i + 9]) for i in range(sizes[kind])])
-    buf = ints([0] * (8 * sizes[3] + 1))
+    buf = ints([0] * (8 * sizes[4] + 1))
     L.shim_joins(buf)
-    return items, [list(buf[8 * i:8 * i + 6]) for i in range(sizes[3])]
+    return items, [list(buf[8 * i:8 * i + 6]) for i in range(sizes[4])]
 
 
-TILE = {0: 16, 1: 32, 2: 256}
+TILE = {0: 16, 1: 32, 2: 128, 3: 256}
 
 
 @pytest.mark.parametrize("seed", range(40))
@@ -239,7 +239,7 @@ def test_a_plan_covers_every_score_once(shim, seed):
         first[s] = at
         at += c
     tiles = {}
-    for kind in range(3):
+    for kind in range(4):
         for seq, head, tok0, row0, rows, pos0, k0, k1, part in items[kind]:
             _, c, n = batch[seq]
             assert tok0 == first[seq] and rows == c * group and pos0 == n - c and 0 <= head < kv
