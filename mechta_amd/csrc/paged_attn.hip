@@ -3,6 +3,8 @@
 // Row r of a sequence's query rows is (token r / group, query head head * group + r % group): the query heads of a kv head
 // and the tokens of a chunk share the keys they read. A work-group takes a tile of rows and a range of keys (Item); where
 // a tile's keys are split, join_kernel puts the splits together.
+#include <type_traits>
+
 #include "mkv_device.h"
 #include "paged_device.h"
 
@@ -11,6 +13,8 @@ namespace paged {
 namespace {
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+// lambdas that hold a kernel's registers by reference: one that is not inlined puts them into memory
+#define INLINE __attribute__((always_inline))
 
 __device__ inline f32x4 mfma16(Vec8<_Float16> a, Vec8<_Float16> b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -58,6 +62,11 @@ struct Args {
     float scale2;  // scale * log2 e
     float *pm, *pl, *pacc;
 };
+
+__device__ inline Item load_item(const Item* p) {
+    const Uniform<int> x = uniform((const int*)p);
+    return Item{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], x[8], 0, {0, 0}};
+}
 
 // Four dims of a finished row: acc / l with the sink in the sum, gated, rounded once.
 template <typename T, int D>
@@ -133,13 +142,13 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
     __shared__ __attribute__((aligned(16))) float so[4][16][D + 4];
     __shared__ float sm[4][16], sl[4][16];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-    const int count = *nitems;
+    const int count = *uniform(nitems);
     for (int n = blockIdx.x; n < count; n += gridDim.x) {
-        const Item it = items[n];
+        const Item it = load_item(items + n);
         const T* const kp = (const T*)a.kpool + (size_t)it.head * a.page * D;
         const T* const vp = (const T*)a.vpool + (size_t)it.head * a.page * D;
         const size_t page_elems = (size_t)a.kv_heads * a.page * D;
-        const int* const table = a.table + (size_t)it.seq * a.most_pages;
+        const Uniform<int> table = uniform(a.table) + (size_t)it.seq * a.most_pages;
         const int last_row = min(it.row0 + 16 * NRT, it.rows) - 1;
         // blocks with every key in [all_lo, all_hi] are seen by all rows whole
         const int all_hi = it.pos0 + it.row0 / a.group;
@@ -324,81 +333,102 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
     }
 }
 
-// ---- chunks: tiles of 256 or 128 query rows against 32-position tiles of keys shared in LDS ----
-// 8 waves. KS = 1: each has 32 rows of the work-group's 256 and takes every key tile. KS = 2: waves 0-3 have the 32-row
-// parts of 128 rows and take the even tiles, waves 4-7 the same rows and the odd tiles; their states meet in LDS at the end.
-// A key tile (32 x D of K and of V, contiguous in a page) comes into a ring in LDS by direct loads. Per tile and wave:
-//   S^T[32 keys][32 rows] = K . Q^T    D / 16 of 32x32x16, K rows read in the order `key` below: register i = 8 s + e of lane
-//                                      half h holds key 16 (e / 4) + 4 (2 s + h) + e % 4, which is element e of V's group
-//                                      2 s + h: the scores become the B operand of the next product where they are
-//   softmax of the lane's row in registers (two lanes a row)
-//   O^T[D][32 rows] += V^T . P^T       D / 16 of 32x32x16; a lane's values all belong to its row, so a moved reference is a
-//                                      factor per lane
+// ---- chunks: tiles of 256 or 128 query rows against keys shared in LDS ----
+// 8 waves, two to a SIMD (w and w + 4). KS = 1: each has 32 rows of the work-group's 256 and takes every key. KS = 2: waves
+// 0-3 have the 32-row parts of 128 rows and waves 4-7 the same rows; a step has keys for either, and the states meet in LDS
+// at the end. Per step of KT keys a wave does
+//   matrix phase   O^T[D][32 rows] += V^T . P^T of the step before, S^T[KT keys][32 rows] = K . Q^T of this one
+//                  (32x32x16; K rows are read in such an order that register i = 8 s + e of lane half h holds key
+//                  16 (e / 4) + 4 (2 s + h) + e % 4 of its 32, element e of V's group 2 s + h: the scores become the B
+//                  operand of the next product where they are, and a lane's values of O all belong to its row)
+//   softmax phase  of its row (two lanes a row), in registers
+// with a barrier behind each. Waves 4-7 run one phase behind waves 0-3, so of a SIMD's two waves one feeds the matrix unit
+// while the other computes weights. K and V come by direct loads into rings of SL steps each; a phase's barrier hands over
+// what has landed and frees what has been read.
 template <int D, int KS>
 struct Chunk {
-    static constexpr int NW = 8, RW = NW / KS;        // waves, waves over the rows
-    static constexpr int TILE = KEYS * D * 2;         // bytes of a tile's K, or V
-    static constexpr int STEP = 2 * KS * TILE;        // the tiles that are computed at once
-    static constexpr int RING = D == 64 ? 65536 : 131072;
-    static constexpr int SLOTS = RING / STEP;
-    static constexpr int LOADS = 2 * TILE / 1024 / RW;  // 1 KB pieces of its tile (K, then V) that a wave copies
-    static_assert(LOADS >= 1 && SLOTS >= 2, "ring");
+    static constexpr int NW = 8, RW = NW / KS;                   // waves, waves over the rows
+    static constexpr int KT = D <= 128 && KS == 1 ? 64 : KEYS;   // keys of a step for a wave
+    static constexpr int SUB = KT / KEYS;                        // 32-key tiles of it
+    static constexpr int TILE = KEYS * D * 2;                    // bytes of a tile's K, or V
+    static constexpr int KTILE = TILE + 256;                     // in LDS: K's second 16 keys 128 bytes on (banks)
+    static constexpr int KSTEP = KS * SUB * KTILE, VSTEP = KS * SUB * TILE;
+    static constexpr int SL = D == 256 && KS == 2 ? 2 : 4;
+    static constexpr int PIECES = SUB * TILE / 1024 / RW;        // 1 KB pieces of K, and of V, a wave copies a step
+    static constexpr int LDS = SL * (KSTEP + VSTEP);
+    static_assert(PIECES >= 1 && TILE / 1024 % PIECES == 0 && LDS <= 150 * 1024, "rings");
 };
-
-template <int LOADS, int MOST>
-__device__ inline void wait_loads(int later) {  // until at most `later` <= MOST steps of LOADS loads are on their way
-    if constexpr (MOST == 0) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    } else {
-        if (later >= MOST) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS * MOST) : "memory");
-        else wait_loads<LOADS, MOST - 1>(later);
-    }
-}
 
 template <typename T, int D, int KS>
 __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict__ items, const int* __restrict__ nitems) {
     using C = Chunk<D, KS>;
-    constexpr int NS = D / 16, NB = D / 32;
-    __shared__ __attribute__((aligned(16))) unsigned char ring[C::RING];
+    constexpr int NS = D / 16, NB = D / 32, SUB = C::SUB, SL = C::SL;
+    __shared__ __attribute__((aligned(1024))) unsigned char ring[C::LDS];
     __shared__ float sm[C::NW][32], sl[C::NW][32];
     __shared__ int odd;
+    unsigned char* const kring = ring;
+    unsigned char* const vring = ring + SL * C::KSTEP;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h = lane >> 5;
     const int wr = w % C::RW, kg = w / C::RW;
-    const int count = *nitems;
-    const unsigned lds0 = (unsigned)(uintptr_t)(lds_void*)ring + kg * 2 * C::TILE + wr * C::LOADS * 1024;
-    const unsigned voff = lane * 16;
+    const bool late = w >= 4;  // the SIMD's second wave
+    const int count = *uniform(nitems);
+    const unsigned lds_k = (unsigned)(uintptr_t)(lds_void*)ring, lds_v = lds_k + SL * C::KSTEP, voff = lane * 16;
     // the K row a lane feeds: m = r goes to key 16 (m / 8 % 2) + 8 (m / 16) + m % 8
-    const int kaddr = (r >> 3 & 1) * 16 * D * 2 + ((r >> 4) * 8 + (r & 7)) * 16 + h * 256;
-    const int vaddr = h * D * 16 + r * 16;
+    const int kaddr = kg * SUB * C::KTILE + (r >> 3 & 1) * (16 * D * 2 + 128) + ((r >> 4) * 8 + (r & 7)) * 16 + h * 256;
+    const int vaddr = kg * SUB * C::TILE + h * D * 16 + r * 16;
     for (int n = blockIdx.x; n < count; n += gridDim.x) {
-        const Item it = items[n];
+        const Item it = load_item(items + n);
         const size_t page_bytes = (size_t)a.kv_heads * a.page * D * 2;
         const char* const kp = (const char*)a.kpool + (size_t)it.head * a.page * D * 2;
         const char* const vp = (const char*)a.vpool + (size_t)it.head * a.page * D * 2;
-        const int* const table = a.table + (size_t)it.seq * a.most_pages;
-        const int tiles = (it.k1 - it.k0 + KEYS - 1) / KEYS, steps = (tiles + KS - 1) / KS;
-        const int mine = (tiles - kg + KS - 1) / KS;  // tiles of this key group
-        auto page_of = [&](int j) {  // of this group's tile of step j
-            return table[(it.k0 + KEYS * min(KS * j + kg, tiles - 1)) >> a.page_shift];
-        };
-        auto issue = [&](int j, int page) {
-            if (j >= mine) return;
-            const int in = (it.k0 + KEYS * (KS * j + kg)) & (a.page - 1);
-            const size_t off = page * page_bytes + (size_t)in * D * 2;
-            const unsigned dst = lds0 + (j % C::SLOTS) * C::STEP;
+        const Uniform<int> table = uniform(a.table) + (size_t)it.seq * a.most_pages;
+        const int tiles = (it.k1 - it.k0 + KEYS - 1) / KEYS, steps = (tiles + KS * SUB - 1) / (KS * SUB);
+        // step j of key group x: tiles (j * KS + x) * SUB .. + SUB - 1; behind the last tile the last again, whose keys then
+        // lie behind every row's bound (k1 at most)
+        auto tile_of = [&](int j, int t) { return (j * KS + kg) * SUB + t; };
+        // A wave's pieces of a step lie in one tile. Where that is in the pages is looked up a step ahead: the look-up's
+        // latency stood in front of every copy otherwise.
+        constexpr int PER = C::TILE / 1024;
+        const int own = wr * C::PIECES / PER, at0 = wr * C::PIECES % PER;
+        auto key_of = [&](int j) { return it.k0 + KEYS * min(tile_of(min(j, steps - 1), own), tiles - 1); };
+        auto page_of = [&](int j) { return table[key_of(j) >> a.page_shift]; };
+        auto offset = [&](int j, int page) { return page * page_bytes + (size_t)(key_of(j) & (a.page - 1)) * D * 2 + at0 * 1024; };
+        auto issue_k = [&](int j, size_t off) {
+            const unsigned to = lds_k + j % SL * C::KSTEP + (kg * SUB + own) * C::KTILE + at0 * 1024;
 #pragma unroll
-            for (int i = 0; i < C::LOADS; i++) {
-                const int piece = wr * C::LOADS + i, per = C::TILE / 1024;
-                dma16s((piece < per ? kp : vp - C::TILE) + off + piece * 1024, voff, dst + i * 1024);
-            }
+            for (int p = 0; p < C::PIECES; p++) dma16s(kp + off + p * 1024, voff, to + p * 1024 + (at0 + p >= PER / 2 ? 128 : 0));
         };
+        auto issue_v = [&](int j, size_t off) {
+            const unsigned to = lds_v + j % SL * C::VSTEP + (kg * SUB + own) * C::TILE + at0 * 1024;
+#pragma unroll
+            for (int p = 0; p < C::PIECES; p++) dma16s(vp + off + p * 1024, voff, to + p * 1024);
+        };
+        __syncthreads();  // the rings and the flag of the item before have been read
+        if (threadIdx.x == 0) odd = 0;
+#pragma unroll
+        for (int j = 0; j < SL - 1; j++) {
+            const size_t off = offset(j, page_of(j));
+            issue_k(j, off);
+            if (j < SL - 2) issue_v(j, off);
+        }
+        size_t v_next = offset(SL - 2, page_of(SL - 2)), k_next = offset(SL - 1, page_of(SL - 1));  // of the next copies
+
+        const int row = it.row0 + 32 * wr + r, last_row = min(it.row0 + 32 * C::RW, it.rows) - 1;
+        const int tok = row / a.group, head = it.head * a.group + row % a.group;
+        const bool is = row <= last_row && it.tok0 + tok < a.rows;
+        const int hi = is ? min(it.pos0 + tok, it.k1 - 1) : -1, lo = a.window ? it.pos0 + tok - a.window + 1 : 0;
+        // keys in [tile_lo, tile_hi] are seen by all rows of the work-group, in [all_lo, all_hi] by all of the wave's
+        const int tile_hi = min(it.pos0 + it.row0 / a.group, it.k1 - 1), tile_lo = a.window ? it.pos0 + last_row / a.group - a.window + 1 : 0;
+        const int all_hi = min(it.pos0 + (it.row0 + 32 * wr) / a.group, it.k1 - 1);
+        const int all_lo = a.window ? it.pos0 + min(it.row0 + 32 * wr + 31, last_row) / a.group - a.window + 1 : 0;
         // infinities and NaN of V in a tile that crosses some row's bounds: each wave looks through the pieces it has copied
         // and puts zeros there before the others read them (add_odd brings them in after the loop)
-        auto mend = [&](int j) {
+        auto mend = [&](int j) INLINE {
 #pragma unroll
-            for (int i = 0; i < C::LOADS; i++) {
-                if (wr * C::LOADS + i < C::TILE / 1024) continue;  // K
-                Vec8<T>* const x = (Vec8<T>*)(ring + (j % C::SLOTS) * C::STEP + kg * 2 * C::TILE + (wr * C::LOADS + i) * 1024 + lane * 16);
+            for (int p = 0; p < C::PIECES; p++) {
+                const int at = wr * C::PIECES + p, k0 = it.k0 + KEYS * tile_of(j, own);
+                if (k0 + KEYS - 1 <= tile_hi && k0 >= tile_lo) break;
+                Vec8<T>* const x = (Vec8<T>*)(vring + j % SL * C::VSTEP + kg * SUB * C::TILE + at * 1024 + lane * 16);
                 const Vec8<T> v[1] = {*x};
                 if (odd_values(v)) {
                     *x = finite(v[0]);
@@ -406,73 +436,71 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
                 }
             }
         };
-        __syncthreads();  // the ring and the flag of the item before have been read
-        if (threadIdx.x == 0) odd = 0;
-        __syncthreads();
-        for (int j = 0; j < C::SLOTS - 1; j++) issue(j, page_of(j));
-        int page = page_of(C::SLOTS - 1);
-
-        const int row = it.row0 + 32 * wr + r, last_row = min(it.row0 + 32 * C::RW, it.rows) - 1;
-        const int tok = row / a.group, head = it.head * a.group + row % a.group;
-        const bool is = row <= last_row && it.tok0 + tok < a.rows;
-        const int hi = is ? it.pos0 + tok : -1, lo = a.window ? it.pos0 + tok - a.window + 1 : 0;
-        // keys in [tile_lo, tile_hi] are seen by all rows of the work-group
-        const int tile_hi = it.pos0 + it.row0 / a.group, tile_lo = a.window ? it.pos0 + last_row / a.group - a.window + 1 : 0;
-        // bounds of the wave's rows: keys all of them see are in [all_lo, all_hi], keys any sees in [any_lo, any_hi]
-        const int row_a = it.row0 + 32 * wr, row_b = min(row_a + 31, last_row);
-        const int all_hi = it.pos0 + row_a / a.group, any_lo = a.window ? all_hi - a.window + 1 : 0;
-        const int any_hi = row_b < row_a ? -1 : it.pos0 + row_b / a.group;
-        const int all_lo = a.window ? any_hi - a.window + 1 : 0;
         Vec8<T> q[NS];
         const T* const src = (const T*)a.q + (int64_t)(it.tok0 + tok) * a.q_tok + head * a.q_head + 8 * h;
 #pragma unroll
         for (int s = 0; s < NS; s++) q[s] = is ? load8(src + 16 * s) : Vec8<T>{};
-        f32x16 o[NB];
+        f32x16 o[NB], s[SUB];
+        Vec8<T> p[2 * SUB];
 #pragma unroll
         for (int i = 0; i < NB; i++) o[i] = f32x16{};
         float m = NEG_INF, l = 0.f;
 
-        for (int j = 0; j < steps; j++) {
-            const int k0 = it.k0 + KEYS * (KS * j + kg);
-            wait_loads<C::LOADS, C::SLOTS - 2>(min(mine - 1 - j, C::SLOTS - 2));
-            if (j < mine && (k0 + KEYS - 1 > tile_hi || k0 < tile_lo)) mend(j);
-            lds_barrier();  // step j is in LDS for every wave, and every wave is done with step j - 1
-            issue(j + C::SLOTS - 1, page);
-            page = page_of(j + C::SLOTS);
-            if (j >= mine) break;
-            if (k0 > any_hi || k0 + KEYS <= any_lo) continue;
-            const unsigned char* const ks = ring + (j % C::SLOTS) * C::STEP + kg * 2 * C::TILE + kaddr;
-            const unsigned char* const vs = ring + (j % C::SLOTS) * C::STEP + kg * 2 * C::TILE + C::TILE + vaddr;
-            f32x16 s = f32x16{};
-            {
-                constexpr int AHEAD = 3;  // K operands on their way ahead of the products
-                Vec8<T> k[AHEAD];
+        // What a wave has copied of step i's K and of the V of the step before has landed, mended. Behind it may be on their
+        // way: what it issued after those.
+        auto landed = [&](int i) INLINE {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * C::PIECES * (SL - 2)) : "memory");
+            if (i > 0) mend(i - 1);
+        };
+        auto k_of = [&](int i, int x) {  // operand x of step i: tile x / NS, dims 16 (x % NS) ..
+            return *(const Vec8<T>*)(kring + i % SL * C::KSTEP + kaddr + x / NS * C::KTILE + x % NS * 512);
+        };
+        auto v_of = [&](int i, int x) {  // dim block x % NB, tile x / NB / 2, groups 2 (x / NB % 2) + h
+            return *(const Vec8<T>*)(vring + i % SL * C::VSTEP + vaddr + x / NB / 2 * C::TILE + x / NB % 2 * 2 * D * 16 + x % NB * 512);
+        };
+        constexpr int AHEAD = D == 256 ? 3 : 4, NK = NS * SUB, NVO = 2 * NB * SUB;  // operands on their way ahead; of a step
+        auto products = [&](int i, auto with_v, auto with_k) INLINE {  // P.V of step i - 1, scores of step i
+            constexpr bool PV = decltype(with_v)::value, QK = decltype(with_k)::value;
+            constexpr int ALL = (PV ? NVO : 0) + (QK ? NK : 0), V0 = PV ? NVO : 0;
+            Vec8<T> x[AHEAD];
+            auto get = [&](int y) { return y < V0 ? v_of(i - 1, y) : k_of(i, y - V0); };
 #pragma unroll
-                for (int i = 0; i < AHEAD; i++) k[i] = *(const Vec8<T>*)(ks + i * 512);
+            for (int y = 0; y < AHEAD; y++) x[y] = get(y);
+            if constexpr (QK) {
 #pragma unroll
-                for (int i = 0; i < NS; i++) {
-                    const Vec8<T> x = k[i % AHEAD];
-                    if (i + AHEAD < NS) k[i % AHEAD] = *(const Vec8<T>*)(ks + (i + AHEAD) * 512);
-                    s = mfma32(x, q[i], s);
-                }
-                __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
-#pragma unroll
-                for (int i = 0; i < NS - AHEAD; i++) {
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                }
-                __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+                for (int t = 0; t < SUB; t++) s[t] = f32x16{};
             }
-            const bool edge = k0 + KEYS - 1 > all_hi || k0 < all_lo;
-            auto key = [&](int i) { return k0 + i % 8 / 4 * 16 + 4 * (i / 8 * 2 + h) + i % 4; };
-            if (edge) {
 #pragma unroll
-                for (int i = 0; i < 16; i++)
-                    if (key(i) > hi || key(i) < lo) s[i] = NEG_INF;
+            for (int y = 0; y < ALL; y++) {
+                const Vec8<T> z = x[y % AHEAD];
+                if (y + AHEAD < ALL) x[y % AHEAD] = get(y + AHEAD);
+                if (y < V0) o[y % NB] = mfma32(z, p[y / NB], o[y % NB]);
+                else s[(y - V0) / NS] = mfma32(z, q[(y - V0) % NS], s[(y - V0) / NS]);
             }
-            float top = fmaxf(s[0], s[1]);  // the compiler's: it waits for the products
+            __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
 #pragma unroll
-            for (int i = 2; i < 16; i += 2) top = vmax3(top, s[i], s[i + 1]);
+            for (int y = 0; y < ALL - AHEAD; y++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+        };
+        auto softmax = [&](int j) INLINE {
+            float top = NEG_INF;
+#pragma unroll
+            for (int t = 0; t < SUB; t++) {
+                const int k0 = it.k0 + KEYS * tile_of(j, t);
+                if (k0 + KEYS - 1 > all_hi || k0 < all_lo) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int key = k0 + i % 8 / 4 * 16 + 4 * (i / 8 * 2 + h) + i % 4;
+                        if (key > hi || key < lo) s[t][i] = NEG_INF;
+                    }
+                }
+                top = fmaxf(top, fmaxf(s[t][0], s[t][1]));  // the compiler's: it waits for the products
+#pragma unroll
+                for (int i = 2; i < 16; i += 2) top = vmax3(top, s[t][i], s[t][i + 1]);
+            }
             top = max_xor32(top) * a.scale2 - Weights<T>::LIFT;
             const bool move = m != NEG_INF && top > m + Weights<T>::LAZY;
             if (__any(move)) {
@@ -483,44 +511,53 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
             }
             if (move || m == NEG_INF) m = top;
             const float ref = m == NEG_INF ? 0.f : m;
-            Vec8<T> p[2];
             float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float x = fast_exp2(__builtin_fmaf(s[i], a.scale2, -ref));
-                sum += x;
-                p[i / 8][i % 8] = (T)x;
-            }
+            for (int t = 0; t < SUB; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float x = fast_exp2(__builtin_fmaf(s[t][i], a.scale2, -ref));
+                    sum += x;
+                    p[2 * t + i / 8][i % 8] = (T)x;
+                }
             l += sum;
-            auto v_of = [&](int i) {  // operand i: dim block i % NB, groups 2 (i / NB) + h
-                return *(const Vec8<T>*)(vs + (i / NB) * 2 * D * 16 + (i % NB) * 512);
-            };
-            {
-                constexpr int AHEAD = 3;
-                Vec8<T> v[AHEAD];
-#pragma unroll
-                for (int i = 0; i < AHEAD; i++) v[i] = v_of(i);
-#pragma unroll
-                for (int i = 0; i < 2 * NB; i++) {
-                    const Vec8<T> x = v[i % AHEAD];
-                    if (i + AHEAD < 2 * NB) v[i % AHEAD] = v_of(i + AHEAD);
-                    o[i % NB] = mfma32(x, p[i / NB], o[i % NB]);
-                }
-                __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
-#pragma unroll
-                for (int i = 0; i < 2 * NB - AHEAD; i++) {
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                }
-                __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
-            }
-        }
+        };
+        auto phase_end = [&](bool wait, int i) INLINE {  // wait: this wave's copies for step i are due
+            __builtin_amdgcn_sched_barrier(0);
+            if (wait) landed(i);
+            lds_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        using std::false_type;
+        using std::true_type;
+        phase_end(true, 0);
+        if (late) phase_end(false, 0);
+        // Copies for a step are due before waves 0-3 begin its matrix phase: at the end of their softmax phase, of the others'
+        // matrix phase; with two key groups each copies for itself and has its softmax phase too.
+        auto step = [&](int i, auto with_v) INLINE {
+            issue_v(i + SL - 2, v_next);
+            issue_k(i + SL - 1, k_next);
+            __builtin_amdgcn_s_setprio(1);
+            products(i, with_v, true_type{});
+            __builtin_amdgcn_s_setprio(0);
+            phase_end(KS == 1 && late, i + 1);
+            const int page = page_of(i + SL);
+            softmax(i);
+            v_next = k_next;
+            k_next = offset(i + SL, page);
+            phase_end(KS == 2 || !late, i + 1);
+        };
+        step(0, false_type{});
+        for (int i = 1; i < steps; i++) step(i, true_type{});
+        products(steps, true_type{}, false_type{});
+        if (!late) phase_end(false, 0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // copies that no step needs write the rings no more behind this
         __syncthreads();
         if (odd) {
-            for (int j = 0; j < mine; j++) {
-                const int k0 = it.k0 + KEYS * (KS * j + kg);
-                if (k0 + KEYS - 1 <= tile_hi && k0 >= tile_lo) continue;
-                const T* const v = (const T*)vp + page_of(j) * (page_bytes / 2) + (size_t)(k0 & (a.page - 1)) * D;
+            for (int j = 0; j < tiles; j++) {
+                const int k0 = it.k0 + KEYS * j;
+                if (j / SUB % KS != kg || (k0 + KEYS - 1 <= tile_hi && k0 >= tile_lo)) continue;
+                const T* const v = (const T*)vp + table[k0 >> a.page_shift] * (page_bytes / 2) + (size_t)(k0 & (a.page - 1)) * D;
                 for (int x = 0; x < KEYS; x++) {
                     const bool seen = k0 + x <= hi && k0 + x >= lo;
                     if (!__any(seen)) continue;
