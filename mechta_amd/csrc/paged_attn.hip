@@ -89,6 +89,36 @@ __device__ inline void finish(const Args& a, int tok, int head, int d, f32x4 acc
     *(Vec4<T>*)((T*)a.out + ((size_t)tok * a.q_heads + head) * D + d) = o;
 }
 
+// The factor of a finished row's sums: 1 / l, with the sink (m: the reference of acc and l, in log2 units).
+__device__ inline float row_factor(const Args& a, int head, float m, float l) {
+    if (!a.sinks) return 1.f / l;
+    const float s = a.sinks[head] * LOG2E, top = fmaxf(m, s), f = m == NEG_INF ? 0.f : fast_exp2(m - top);
+    return f / (l * f + fast_exp2(s - top));
+}
+// Eight dims of a finished row: gated, rounded once.
+template <typename T, int D>
+__device__ inline void store_out(const Args& a, int tok, int head, int d, f32x4 lo, f32x4 hi) {
+    float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    if (a.gate) {
+        const Vec8<T> g = load8((const T*)a.gate + tok * a.g_tok + head * a.g_head + d);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] *= 1.f / (1.f + fast_exp2(-LOG2E * (float)g[i]));
+    }
+    Vec8<T> o;
+#pragma unroll
+    for (int i = 0; i < 8; i++) o[i] = (T)x[i];
+    store8((T*)a.out + ((size_t)tok * a.q_heads + head) * D + d, o);
+}
+
+__device__ inline float add_pair(_Float16 a, _Float16 b, float c) {
+    typedef _Float16 pair __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(pair{a, b}, pair{(_Float16)1.f, (_Float16)1.f}, c, false);
+}
+__device__ inline float add_pair(__bf16 a, __bf16 b, float c) {
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(pair{a, b}, pair{(__bf16)1.f, (__bf16)1.f}, c, false);
+}
+
 // Infinities and NaN of V in positions that some of a wave's rows do not see: 0 x NaN would reach those rows through the
 // products. Only tiles that cross a row's bounds can hold such (edge tiles); there the operands are looked through, and
 // what is not finite is taken as zero. The rows that see it get it after the loop, by plain additions, value by value
@@ -403,15 +433,22 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
 #pragma unroll
             for (int p = 0; p < C::PIECES; p++) dma16s(vp + off + p * 1024, voff, to + p * 1024);
         };
+        // Copies go out in the softmax phase, which is the shorter one (in the matrix phase they took 430 of its 1,700
+        // cycles): K of step i + SL - 1 + LEAD and V of the step before it in that of step i, into the places of K of step i - 1
+        // + LEAD and of the V before it. With two key groups those have been read by then; with one, waves 4-7 are still at
+        // K of step i.
+        constexpr int LEAD = KS == 2 ? 1 : 0;
+        static_assert(LEAD || SL >= 3, "waves 4-7 wait in front of their copies of a step");
         __syncthreads();  // the rings and the flag of the item before have been read
         if (threadIdx.x == 0) odd = 0;
 #pragma unroll
-        for (int j = 0; j < SL - 1; j++) {
+        for (int j = 0; j < SL - 1 + LEAD; j++) {
             const size_t off = offset(j, page_of(j));
             issue_k(j, off);
-            if (j < SL - 2) issue_v(j, off);
+            if (j < SL - 2 + LEAD) issue_v(j, off);
         }
-        size_t v_next = offset(SL - 2, page_of(SL - 2)), k_next = offset(SL - 1, page_of(SL - 1));  // of the next copies
+        // of the next copies: V of the one, K of the other
+        size_t v_next = offset(SL - 2 + LEAD, page_of(SL - 2 + LEAD)), k_next = offset(SL - 1 + LEAD, page_of(SL - 1 + LEAD));
 
         const int row = it.row0 + 32 * wr + r, last_row = min(it.row0 + 32 * C::RW, it.rows) - 1;
         const int tok = row / a.group, head = it.head * a.group + row % a.group;
@@ -447,9 +484,9 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
         float m = NEG_INF, l = 0.f;
 
         // What a wave has copied of step i's K and of the V of the step before has landed, mended. Behind it may be on their
-        // way: what it issued after those.
-        auto landed = [&](int i) INLINE {
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * C::PIECES * (SL - 2)) : "memory");
+        // way: what it issued after those, `behind` steps' K and V.
+        auto landed = [&](int i, auto behind) INLINE {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * C::PIECES * decltype(behind)::value) : "memory");
             if (i > 0) mend(i - 1);
         };
         auto k_of = [&](int i, int x) {  // operand x of step i: tile x / NS, dims 16 (x % NS) ..
@@ -516,41 +553,50 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
             for (int t = 0; t < SUB; t++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const float x = fast_exp2(__builtin_fmaf(s[t][i], a.scale2, -ref));
-                    sum += x;
-                    p[2 * t + i / 8][i % 8] = (T)x;
+                    p[2 * t + i / 8][i % 8] = (T)fast_exp2(__builtin_fmaf(s[t][i], a.scale2, -ref));
+                    if (i % 2) sum = add_pair(p[2 * t + i / 8][i % 8 - 1], p[2 * t + i / 8][i % 8], sum);
                 }
             l += sum;
+            // the weights are done here, not where they are used: the compiler moved the exponentials behind the phase's
+            // barrier, into the matrix phase
+#pragma unroll
+            for (int t = 0; t < 2 * SUB; t++) {
+                u32x4 x = __builtin_bit_cast(u32x4, p[t]);
+                asm volatile("" : "+v"(x));
+                p[t] = __builtin_bit_cast(Vec8<T>, x);
+            }
         };
-        auto phase_end = [&](bool wait, int i) INLINE {  // wait: this wave's copies for step i are due
+        auto phase_end = [&](bool wait, int i, auto behind) INLINE {  // wait: this wave's copies for step i are due
             __builtin_amdgcn_sched_barrier(0);
-            if (wait) landed(i);
+            if (wait) landed(i, behind);
             lds_barrier();
             __builtin_amdgcn_sched_barrier(0);
         };
         using std::false_type;
         using std::true_type;
-        phase_end(true, 0);
-        if (late) phase_end(false, 0);
+        const std::integral_constant<int, SL - 2 + LEAD> behind{};
+        phase_end(true, 0, behind);
+        if (late) phase_end(false, 0, behind);
         // Copies for a step are due before waves 0-3 begin its matrix phase: at the end of their softmax phase, of the others'
         // matrix phase; with two key groups each copies for itself and has its softmax phase too.
         auto step = [&](int i, auto with_v) INLINE {
-            issue_v(i + SL - 2, v_next);
-            issue_k(i + SL - 1, k_next);
             __builtin_amdgcn_s_setprio(1);
             products(i, with_v, true_type{});
             __builtin_amdgcn_s_setprio(0);
-            phase_end(KS == 1 && late, i + 1);
-            const int page = page_of(i + SL);
+            phase_end(KS == 1 && late, i + 1, std::integral_constant<int, KS == 1 ? SL - 3 : 0>{});
+            issue_v(i + SL - 2 + LEAD, v_next);
+            issue_k(i + SL - 1 + LEAD, k_next);
+            __builtin_amdgcn_sched_barrier(0);
+            const int page = page_of(i + SL + LEAD);
             softmax(i);
             v_next = k_next;
-            k_next = offset(i + SL, page);
-            phase_end(KS == 2 || !late, i + 1);
+            k_next = offset(i + SL + LEAD, page);
+            phase_end(KS == 2 || !late, i + 1, behind);
         };
         step(0, false_type{});
         for (int i = 1; i < steps; i++) step(i, true_type{});
         products(steps, true_type{}, false_type{});
-        if (!late) phase_end(false, 0);
+        if (!late) phase_end(false, 0, behind);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // copies that no step needs write the rings no more behind this
         __syncthreads();
         if (odd) {
@@ -572,25 +618,53 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
             }
         }
         l += __shfl_xor(l, 32);
-        // o[b][4 c + i]: dim 32 b + 8 c + 4 h + i of row r
-        auto put = [&](int b0, int b1) {
-            if (!is) return;
-            const size_t at = it.part + 32 * wr + r;
+        // o[b][4 c + i]: dim 32 b + 8 c + 4 h + i of row r. The rows go out through the wave's part of the rings, which nobody
+        // reads any more, BLOCKS x 32 dims at a time: whole runs of a row, with the gate read in such runs too.
+        constexpr int OB = NB / KS, BLOCKS = D == 64 ? 1 : 2, DW = 32 * BLOCKS, ROW = DW + 4, PER_ROW = DW / 8;
+        static_assert(C::NW * 32 * ROW * 4 <= C::LDS, "output rows");
+        float* const rows_lds = (float*)ring + w * 32 * ROW;
+        auto put = [&](auto first, float factor) INLINE {  // blocks first .. first + BLOCKS - 1, times the factor of the lane's row
 #pragma unroll
-            for (int b = 0; b < NB; b++)
-                if (b >= b0 && b < b1) {
+            for (int b = 0; b < BLOCKS; b++)
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const f32x4 x = {o[b][4 * c], o[b][4 * c + 1], o[b][4 * c + 2], o[b][4 * c + 3]};
-                        const int d = 32 * b + 8 * c + 4 * h;
-                        if (it.part < 0) finish<T, D>(a, it.tok0 + tok, head, d, x, m, l);
-                        else *(f32x4*)(a.pacc + at * D + d) = x;
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
+                for (int c = 0; c < 4; c++) {
+                    f32x4 x;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[i] = o[first + b][4 * c + i] * factor;
+                    *(f32x4*)(rows_lds + r * ROW + 32 * b + 8 * c + 4 * h) = x;
                 }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+            for (int i = lane; i < 32 * PER_ROW; i += 64) {
+                const int x = i / PER_ROW, d = i % PER_ROW * 8, row = it.row0 + 32 * wr + x;
+                const int tok = it.tok0 + row / a.group, head = it.head * a.group + row % a.group;
+                if (row > last_row || tok >= a.rows) continue;
+                const f32x4 lo = *(const f32x4*)(rows_lds + x * ROW + d), hi = *(const f32x4*)(rows_lds + x * ROW + d + 4);
+                const int dim = 32 * first + d;
+                if (it.part >= 0) {
+                    float* const to = a.pacc + (size_t)(it.part + 32 * wr + x) * D + dim;
+                    *(f32x4*)to = lo;
+                    *(f32x4*)(to + 4) = hi;
+                } else {
+                    store_out<T, D>(a, tok, head, dim, lo, hi);
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
         };
+        auto finish_rows = [&](auto first) INLINE {
+            const float factor = it.part >= 0 ? 1.f : row_factor(a, min(head, a.q_heads - 1), m, l);
+            constexpr int B = decltype(first)::value;
+            put(first, factor);
+            if constexpr (OB > BLOCKS) put(std::integral_constant<int, B + BLOCKS>{}, factor);
+            if constexpr (OB > 2 * BLOCKS) {
+                put(std::integral_constant<int, B + 2 * BLOCKS>{}, factor);
+                put(std::integral_constant<int, B + 3 * BLOCKS>{}, factor);
+            }
+        };
+        const std::integral_constant<int, 0> low{};
+        const std::integral_constant<int, NB / 2> high{};
         if constexpr (KS == 1) {
-            put(0, NB);
+            finish_rows(low);
         } else {
             // two states of each row, in waves w and w ^ RW: both taken to the larger reference, each wave finishes half of
             // the dims with its partner's half of them, which goes through the ring
@@ -626,8 +700,9 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
                 }
             m = top;
             l = l * f + lo2 * fo;
-            if (kg == 0) put(0, NB / 2);
-            else put(NB / 2, NB);
+            __syncthreads();  // what was given has been taken
+            if (kg == 0) finish_rows(low);
+            else finish_rows(high);
         }
         if (it.part >= 0 && kg == 0 && h == 0 && is) {
             a.pm[it.part + 32 * wr + r] = m;
