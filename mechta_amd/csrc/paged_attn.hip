@@ -372,9 +372,9 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
 //                  16 (e / 4) + 4 (2 s + h) + e % 4 of its 32, element e of V's group 2 s + h: the scores become the B
 //                  operand of the next product where they are, and a lane's values of O all belong to its row)
 //   softmax phase  of its row (two lanes a row), in registers
-// with a barrier behind each. Waves 4-7 run one phase behind waves 0-3, so of a SIMD's two waves one feeds the matrix unit
-// while the other computes weights. K and V come by direct loads into rings of SL steps each; a phase's barrier hands over
-// what has landed and frees what has been read.
+// Waves 4-7 run one phase behind waves 0-3, so of a SIMD's two waves one feeds the matrix unit while the other computes
+// weights. K and V come by direct loads into rings of SL steps each; barriers hand over what has landed and free what has
+// been read.
 template <int D, int KS>
 struct Chunk {
     static constexpr int NW = 8, RW = NW / KS;                   // waves, waves over the rows
@@ -433,12 +433,13 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
 #pragma unroll
             for (int p = 0; p < C::PIECES; p++) dma16s(vp + off + p * 1024, voff, to + p * 1024);
         };
-        // Copies go out in the softmax phase, which is the shorter one (in the matrix phase they took 430 of its 1,700
-        // cycles): K of step i + SL - 1 + LEAD and V of the step before it in that of step i, into the places of K of step i - 1
-        // + LEAD and of the V before it. With two key groups those have been read by then; with one, waves 4-7 are still at
-        // K of step i.
-        constexpr int LEAD = KS == 2 ? 1 : 0;
-        static_assert(LEAD || SL >= 3, "waves 4-7 wait in front of their copies of a step");
+        // ONE: a barrier a step; with rings of two steps two, and copies a step further ahead. Copies go out in the softmax
+        // phase, which is the shorter one (in the matrix phase they took 430 of its 1,700 cycles): K of step i + SL - 1 + LEAD
+        // and V of the step before it in that of step i, into the places of K of step i - 1 + LEAD and of the V before it.
+        // Those have been read by then: ONE, before the barrier in front of waves 0-3's step i, behind waves 4-7's matrix phase
+        // i - 1; else by the wave's own key group, before the barrier in front.
+        constexpr bool ONE = SL >= 3;
+        constexpr int LEAD = ONE ? 0 : 1;
         __syncthreads();  // the rings and the flag of the item before have been read
         if (threadIdx.x == 0) odd = 0;
 #pragma unroll
@@ -576,14 +577,15 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
         using std::true_type;
         const std::integral_constant<int, SL - 2 + LEAD> behind{};
         phase_end(true, 0, behind);
-        if (late) phase_end(false, 0, behind);
-        // Copies for a step are due before waves 0-3 begin its matrix phase: at the end of their softmax phase, of the others'
-        // matrix phase; with two key groups each copies for itself and has its softmax phase too.
+        if (!ONE && late) phase_end(false, 0, behind);
+        // ONE: barrier i + 1 stands behind waves 0-3's softmax phase i and waves 4-7's matrix phase i; copies for step i + 1 are
+        // due in front of it. Else barriers stand behind every phase; copies are due at the end of the softmax phase.
         auto step = [&](int i, auto with_v) INLINE {
             __builtin_amdgcn_s_setprio(1);
             products(i, with_v, true_type{});
             __builtin_amdgcn_s_setprio(0);
-            phase_end(KS == 1 && late, i + 1, std::integral_constant<int, KS == 1 ? SL - 3 : 0>{});
+            if (!ONE || late) phase_end(ONE, i + 1, std::integral_constant<int, ONE ? SL - 3 : 0>{});
+            __builtin_amdgcn_sched_barrier(0);
             issue_v(i + SL - 2 + LEAD, v_next);
             issue_k(i + SL - 1 + LEAD, k_next);
             __builtin_amdgcn_sched_barrier(0);
@@ -591,12 +593,12 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
             softmax(i);
             v_next = k_next;
             k_next = offset(i + SL + LEAD, page);
-            phase_end(KS == 2 || !late, i + 1, behind);
+            if (!ONE || !late) phase_end(true, i + 1, behind);
         };
         step(0, false_type{});
         for (int i = 1; i < steps; i++) step(i, true_type{});
         products(steps, true_type{}, false_type{});
-        if (!late) phase_end(false, 0, behind);
+        if (!ONE && !late) phase_end(false, 0, behind);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // copies that no step needs write the rings no more behind this
         __syncthreads();
         if (odd) {
