@@ -68,46 +68,41 @@ __device__ inline Item load_item(const Item* p) {
     return Item{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], x[8], 0, {0, 0}};
 }
 
-// Four dims of a finished row: acc / l with the sink in the sum, gated, rounded once.
-template <typename T, int D>
-__device__ inline void finish(const Args& a, int tok, int head, int d, f32x4 acc, float m, float l) {
-    if (a.sinks) {  // m is the reference of acc and l, in log2 units
-        const float s = a.sinks[head] * LOG2E, top = fmaxf(m, s);
-        const float f = m == NEG_INF ? 0.f : fast_exp2(m - top);
-        acc *= f;
-        l = l * f + fast_exp2(s - top);
-    }
-    acc *= 1.f / l;
-    if (a.gate) {
-        const Vec4<T> g = *(const Vec4<T>*)((const T*)a.gate + tok * a.g_tok + head * a.g_head + d);
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc[i] *= 1.f / (1.f + fast_exp2(-LOG2E * (float)g[i]));
-    }
-    Vec4<T> o;
-#pragma unroll
-    for (int i = 0; i < 4; i++) o[i] = (T)acc[i];
-    *(Vec4<T>*)((T*)a.out + ((size_t)tok * a.q_heads + head) * D + d) = o;
-}
-
 // The factor of a finished row's sums: 1 / l, with the sink (m: the reference of acc and l, in log2 units).
 __device__ inline float row_factor(const Args& a, int head, float m, float l) {
-    if (!a.sinks) return 1.f / l;
+    if (!a.sinks) return __builtin_amdgcn_rcpf(l);  // 2^-23: far below the output's rounding
     const float s = a.sinks[head] * LOG2E, top = fmaxf(m, s), f = m == NEG_INF ? 0.f : fast_exp2(m - top);
-    return f / (l * f + fast_exp2(s - top));
+    return f * __builtin_amdgcn_rcpf(l * f + fast_exp2(s - top));
 }
-// Eight dims of a finished row: gated, rounded once.
-template <typename T, int D>
-__device__ inline void store_out(const Args& a, int tok, int head, int d, f32x4 lo, f32x4 hi) {
-    float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+// N dims of a finished row: gated, rounded once.
+template <typename T, int D, int N>
+__device__ inline void store_out(const Args& a, int tok, int head, int d, const float (&x)[N]) {
+    typedef T vec __attribute__((ext_vector_type(N)));
+    vec o;
     if (a.gate) {
-        const Vec8<T> g = load8((const T*)a.gate + tok * a.g_tok + head * a.g_head + d);
+        const vec g = *(const vec*)((const T*)a.gate + tok * a.g_tok + head * a.g_head + d);
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] *= 1.f / (1.f + fast_exp2(-LOG2E * (float)g[i]));
+        for (int i = 0; i < N; i++) o[i] = (T)(x[i] * __builtin_amdgcn_rcpf(1.f + fast_exp2(-LOG2E * (float)g[i])));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) o[i] = (T)x[i];
     }
-    Vec8<T> o;
-#pragma unroll
-    for (int i = 0; i < 8; i++) o[i] = (T)x[i];
-    store8((T*)a.out + ((size_t)tok * a.q_heads + head) * D + d, o);
+    *(vec*)((T*)a.out + ((size_t)tok * a.q_heads + head) * D + d) = o;
+}
+
+// The maximum, or sum, over lanes l and l ^ 16, in every lane: two registers that both hold x exchange their odd and even
+// rows of 16 lanes.
+__device__ inline float max_xor16(float x) {
+    float y;
+    asm volatile("v_mov_b32 %0, %1" : "=v"(y) : "v"(x));
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    return vmax(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float add_xor16(float x) {
+    float y;
+    asm volatile("v_mov_b32 %0, %1" : "=v"(y) : "v"(x));
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 __device__ inline float add_pair(_Float16 a, _Float16 b, float c) {
@@ -172,18 +167,45 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
     __shared__ __attribute__((aligned(16))) float so[4][16][D + 4];
     __shared__ float sm[4][16], sl[4][16];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const unsigned klane = lane * 16, vlane = g * D * 16 + r * 16;  // a lane's bytes of a K operand's KB, of a V group
     const int count = *uniform(nitems);
     for (int n = blockIdx.x; n < count; n += gridDim.x) {
         const Item it = load_item(items + n);
-        const T* const kp = (const T*)a.kpool + (size_t)it.head * a.page * D;
-        const T* const vp = (const T*)a.vpool + (size_t)it.head * a.page * D;
-        const size_t page_elems = (size_t)a.kv_heads * a.page * D;
+        const size_t page_bytes = (size_t)a.kv_heads * a.page * D * 2;
+        const char* const kp = (const char*)a.kpool + (size_t)it.head * a.page * D * 2;
+        const char* const vp = (const char*)a.vpool + (size_t)it.head * a.page * D * 2;
         const Uniform<int> table = uniform(a.table) + (size_t)it.seq * a.most_pages;
         const int last_row = min(it.row0 + 16 * NRT, it.rows) - 1;
         // blocks with every key in [all_lo, all_hi] are seen by all rows whole
         const int all_hi = it.pos0 + it.row0 / a.group;
         const int all_lo = a.window ? it.pos0 + last_row / a.group - a.window + 1 : 0;
-
+        const int blocks = (it.k1 - it.k0 + KEYS - 1) / KEYS;
+        auto key_of = [&](int j) { return it.k0 + KEYS * j; };
+        auto page_of = [&](int j) { return table[key_of(min(j, blocks - 1)) >> a.page_shift]; };
+        auto offset = [&](int j, int page) {  // of block j in K and V, its page known
+            return page * page_bytes + (size_t)(key_of(j) & (a.page - 1)) * D * 2;
+        };
+        Vec8<T> kf[2][NS], vf[NV];
+        // read once: non-temporal. A uniform base and a lane's 32-bit offset: no 64-bit address per lane and load.
+        auto load_k = [&](size_t off) INLINE {
+#pragma unroll
+            for (int s = 0; s < NS; s++)
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+                    kf[b][s] = __builtin_nontemporal_load((const Vec8<T>*)(kp + off + b * 16 * D * 2 + s * 1024 + klane));
+        };
+        auto load_v = [&](size_t off) INLINE {
+#pragma unroll
+            for (int i = 0; i < NV; i++) vf[i] = __builtin_nontemporal_load((const Vec8<T>*)(vp + off + i * 256 + vlane));
+        };
+        size_t off = 0;
+        int page = 0;
+        if (w < blocks) {  // the first block is on its way while Q is prepared
+            off = offset(w, page_of(w));
+            load_k(off);
+            load_v(off);
+            page = page_of(w + 4);
+        }
         Vec8<T> q[NRT][QLDS ? 1 : NS];
         int lo[NRT], hi[NRT];  // keys the lane's row sees
 #pragma unroll
@@ -205,7 +227,7 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
                 for (int s = 0; s < NS; s++) q[t][s] = is ? load8(src + 32 * s) : Vec8<T>{};
             }
         }
-        if constexpr (QLDS) __syncthreads();
+        if constexpr (QLDS) lds_barrier();
         f32x4 o[NRT][NV];
         float m[NRT], l[NRT];  // the reference of the row's weights (log2 units), the lane's share of their sum
 #pragma unroll
@@ -215,122 +237,95 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
 #pragma unroll
             for (int i = 0; i < NV; i++) o[t][i] = f32x4{};
         }
-        const int blocks = (it.k1 - it.k0 + KEYS - 1) / KEYS;
-        auto key_of = [&](int j) { return it.k0 + KEYS * j; };
-        auto page_of = [&](int j) { return table[key_of(min(j, blocks - 1)) >> a.page_shift]; };
-        auto offset = [&](int j, int page) {  // of block j, its page known
-            return page * page_elems + (size_t)(key_of(j) & (a.page - 1)) * D;
-        };
-        Vec8<T> kf[2][NS], vf[NV];
-        auto load_k = [&](size_t off) {
-#pragma unroll
-            for (int s = 0; s < NS; s++)
-#pragma unroll
-                for (int b = 0; b < 2; b++) kf[b][s] = load8(kp + off + b * 16 * D + (4 * s + g) * 128 + r * 8);
-        };
-        auto load_v = [&](size_t off) {
-#pragma unroll
-            for (int i = 0; i < NV; i++) vf[i] = load8(vp + off + (g * D + 16 * i + r) * 8);
-        };
         bool odd = false;
-        if (w < blocks) {
-            size_t off = offset(w, page_of(w));
-            load_k(off);
-            load_v(off);
-            int page = page_of(w + 4);
-            for (int j = w; j < blocks; j += 4) {
-                const int jn = j + 4 < blocks ? j + 4 : j;
-                const size_t next = j + 4 < blocks ? offset(jn, page) : off;
-                page = page_of(j + 8);
-                f32x4 s[NRT][2];
+        for (int j = w; j < blocks; j += 4) {
+            const size_t next = j + 4 < blocks ? offset(j + 4, page) : off;
+            page = page_of(j + 8);
+            f32x4 s[NRT][2];
 #pragma unroll
-                for (int t = 0; t < NRT; t++) s[t][0] = s[t][1] = f32x4{};
+            for (int t = 0; t < NRT; t++) s[t][0] = s[t][1] = f32x4{};
 #pragma unroll
-                for (int i = 0; i < NS; i++)
-#pragma unroll
-                    for (int t = 0; t < NRT; t++) {
-                        const Vec8<T> x = QLDS ? *(const Vec8<T>*)&sq[r][32 * i + 8 * g] : q[t][QLDS ? 0 : i];
-#pragma unroll
-                        for (int b = 0; b < 2; b++) s[t][b] = mfma16(kf[b][i], x, s[t][b]);
-                    }
-                load_k(next);
-                const int k0 = key_of(j);
-                const bool edge = k0 + KEYS - 1 > all_hi || k0 < all_lo;
-                Vec8<T> p[NRT];
+            for (int i = 0; i < NS; i++)
 #pragma unroll
                 for (int t = 0; t < NRT; t++) {
-                    if (edge) {
+                    const Vec8<T> x = QLDS ? *(const Vec8<T>*)&sq[r][32 * i + 8 * g] : q[t][QLDS ? 0 : i];
 #pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const int key = k0 + e / 4 * 16 + 4 * g + e % 4;
-                            if (key > hi[t] || key < lo[t]) s[t][e / 4][e % 4] = NEG_INF;
-                        }
-                    }
-                    float top = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
-                                      fmaxf(fmaxf(s[t][1][0], s[t][1][1]), fmaxf(s[t][1][2], s[t][1][3])));
-                    top = fmaxf(top, __shfl_xor(top, 16));
-                    top = fmaxf(top, __shfl_xor(top, 32)) * a.scale2 - Weights<T>::LIFT;
-                    const bool move = m[t] != NEG_INF && top > m[t] + Weights<T>::LAZY;
-                    if (__any(move)) {
-                        const float f = move ? fast_exp2(m[t] - top) : 1.f;
-                        l[t] *= f;
+                    for (int b = 0; b < 2; b++) s[t][b] = mfma16(kf[b][i], x, s[t][b]);
+                }
+            load_k(next);
+            const int k0 = key_of(j);
+            const bool edge = k0 + KEYS - 1 > all_hi || k0 < all_lo;
+            Vec8<T> p[NRT];
 #pragma unroll
-                        for (int i = 0; i < NV; i++) o[t][i] *= f;
-                    }
-                    if (move || m[t] == NEG_INF) m[t] = top;
-                    const float ref = m[t] == NEG_INF ? 0.f : m[t];
+            for (int t = 0; t < NRT; t++) {
+                if (edge) {
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        const float x = fast_exp2(__builtin_fmaf(s[t][e / 4][e % 4], a.scale2, -ref));
-                        l[t] += x;
-                        p[t][e] = (T)x;
+                        const int key = k0 + e / 4 * 16 + 4 * g + e % 4;
+                        if (key > hi[t] || key < lo[t]) s[t][e / 4][e % 4] = NEG_INF;
                     }
                 }
-                if (edge && odd_values(vf)) {
-                    odd = true;
+                float top = fmaxf(s[t][0][0], s[t][1][0]);  // the compiler's: it waits for both products
+                top = vmax3(vmax3(vmax3(top, s[t][0][1], s[t][0][2]), s[t][0][3], s[t][1][1]), s[t][1][2], s[t][1][3]);
+                top = max_xor32(max_xor16(top)) * a.scale2 - Weights<T>::LIFT;
+                const bool move = m[t] != NEG_INF && top > m[t] + Weights<T>::LAZY;
+                if (__any(move)) {
+                    const float f = move ? fast_exp2(m[t] - top) : 1.f;
+                    l[t] *= f;
 #pragma unroll
-                    for (int i = 0; i < NV; i++) vf[i] = finite(vf[i]);
+                    for (int i = 0; i < NV; i++) o[t][i] *= f;
                 }
+                if (move || m[t] == NEG_INF) m[t] = top;
+                const float ref = m[t] == NEG_INF ? 0.f : m[t];
 #pragma unroll
-                for (int i = 0; i < NV; i++)
-#pragma unroll
-                    for (int t = 0; t < NRT; t++) o[t][i] = mfma16(vf[i], p[t], o[t][i]);
-                load_v(next);
-                off = next;
+                for (int e = 0; e < 8; e++) {
+                    p[t][e] = (T)fast_exp2(__builtin_fmaf(s[t][e / 4][e % 4], a.scale2, -ref));
+                    if (e % 2) l[t] = add_pair(p[t][e - 1], p[t][e], l[t]);
+                }
             }
+            if (edge && odd_values(vf)) {
+                odd = true;
+#pragma unroll
+                for (int i = 0; i < NV; i++) vf[i] = finite(vf[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < NV; i++)
+#pragma unroll
+                for (int t = 0; t < NRT; t++) o[t][i] = mfma16(vf[i], p[t], o[t][i]);
+            load_v(next);
+            off = next;
         }
         if (odd) {
             for (int j = w; j < blocks; j += 4) {
                 const int k0 = key_of(j);
                 if (k0 + KEYS - 1 <= all_hi && k0 >= all_lo) continue;
-                const T* const v = vp + offset(j, page_of(j));
+                const T* const v = (const T*)(vp + offset(j, page_of(j)));
                 for (int x = 0; x < KEYS; x++) {
 #pragma unroll
                     for (int t = 0; t < NRT; t++) {
                         const bool seen = k0 + x <= hi[t] && k0 + x >= lo[t];
                         if (!__any(seen)) continue;
 #pragma unroll
-                        for (int i = 0; i < NV; i++)
-                            o[t][i] = add_odd<T, D>(v, x, 16 * i + 4 * g, seen, o[t][i]);
+                        for (int i = 0; i < NV; i++) o[t][i] = add_odd<T, D>(v, x, 16 * i + 4 * g, seen, o[t][i]);
                     }
                 }
             }
         }
-        // the four waves' states of 16 rows at a time
+        // the four waves' states of 16 rows at a time: 16 threads a row, 8 dims each and again
 #pragma unroll
         for (int t = 0; t < NRT; t++) {
-            float sum = l[t] + __shfl_xor(l[t], 16);
-            sum += __shfl_xor(sum, 32);
-            __syncthreads();  // the states before have been read
+            const float sum = add_xor32(add_xor16(l[t]));
+            lds_barrier();  // the states before have been read
             if (g == 0) {
                 sm[w][r] = m[t];
                 sl[w][r] = sum;
             }
 #pragma unroll
             for (int i = 0; i < NV; i++) *(f32x4*)&so[w][r][16 * i + 4 * g] = o[t][i];
-            __syncthreads();
+            lds_barrier();
             const int rr = threadIdx.x >> 4, row = it.row0 + 16 * t + rr, tok = it.tok0 + row / a.group;
             if (row > last_row || tok >= a.rows) continue;
+            const int head = it.head * a.group + row % a.group;
             const float top = fmaxf(fmaxf(sm[0][rr], sm[1][rr]), fmaxf(sm[2][rr], sm[3][rr]));
             float f[4], total = 0.f;
 #pragma unroll
@@ -338,26 +333,34 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
                 f[x] = sm[x][rr] == NEG_INF ? 0.f : fast_exp2(sm[x][rr] - top);
                 total += f[x] * sl[x][rr];
             }
+            const float factor = it.part < 0 ? row_factor(a, head, top, total) : 1.f;
 #pragma unroll
-            for (int c = 0; c < D / 64; c++) {
-                const int d = ((int)(threadIdx.x & 15) + 16 * c) * 4;
-                f32x4 acc = f32x4{};
+            for (int c = 0; c < (D + 127) / 128; c++) {
+                const int d = ((int)(threadIdx.x & 15) + 16 * c) * 8;
+                if (d >= D) continue;
+                f32x4 acc[2] = {f32x4{}, f32x4{}};
 #pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    const f32x4 y = *(const f32x4*)&so[x][rr][d];
+                for (int x = 0; x < 4; x++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) acc[i] += f[x] == 0.f ? 0.f : f[x] * y[i];
-                }
-                if (it.part < 0) {
-                    finish<T, D>(a, tok, it.head * a.group + row % a.group, d, acc, top, total);
-                } else {
-                    const size_t at = it.part + 16 * t + rr;
-                    *(f32x4*)(a.pacc + at * D + d) = acc;
-                    if (d == 0) {
-                        a.pm[at] = top;
-                        a.pl[at] = total;
+                    for (int y = 0; y < 2; y++) {
+                        const f32x4 z = *(const f32x4*)&so[x][rr][d + 4 * y];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[y][i] += f[x] == 0.f ? 0.f : f[x] * z[i];
                     }
+                acc[0] *= factor;
+                acc[1] *= factor;
+                if (it.part < 0) {
+                    const float x[8] = {acc[0][0], acc[0][1], acc[0][2], acc[0][3], acc[1][0], acc[1][1], acc[1][2], acc[1][3]};
+                    store_out<T, D, 8>(a, tok, head, d, x);
+                } else {
+                    float* const to = a.pacc + (size_t)(it.part + 16 * t + rr) * D + d;
+                    *(f32x4*)to = acc[0];
+                    *(f32x4*)(to + 4) = acc[1];
                 }
+            }
+            if (it.part >= 0 && (threadIdx.x & 15) == 0) {
+                a.pm[it.part + 16 * t + rr] = top;
+                a.pl[it.part + 16 * t + rr] = total;
             }
         }
     }
@@ -648,7 +651,8 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
                     *(f32x4*)to = lo;
                     *(f32x4*)(to + 4) = hi;
                 } else {
-                    store_out<T, D>(a, tok, head, dim, lo, hi);
+                    const float y[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                    store_out<T, D, 8>(a, tok, head, dim, y);
                 }
             }
             __builtin_amdgcn_wave_barrier();
@@ -723,7 +727,12 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
     __shared__ float factor[SPLITS_MOST];
     __shared__ __attribute__((aligned(16))) f32x4 sa[GROUPS][LANES];
     __shared__ float red[2][4];
-    const int count = *njoins, tid = threadIdx.x, part = tid / LANES, lane = tid % LANES, d = lane * 4;
+    const int count = *uniform(njoins), tid = threadIdx.x, part = tid / LANES, lane = tid % LANES, d = lane * 4;
+    auto finish = [&](int tok, int head, f32x4 acc, float m, float l) INLINE {
+        acc *= row_factor(a, head, m, l);
+        const float x[4] = {acc[0], acc[1], acc[2], acc[3]};
+        store_out<T, D, 4>(a, tok, head, d, x);
+    };
     for (int n = blockIdx.x; n < count; n += gridDim.x) {
         const Join j = joins[n];
         if (j.splits < JOIN_WIDE) {
@@ -746,7 +755,7 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
                     for (int i = 0; i < 4; i++) acc[i] += f == 0.f ? 0.f : f * x[s][i];
                     total += f * a.pl[j.part + r + (size_t)min(s, j.splits - 1) * j.count];
                 }
-                finish<T, D>(a, tok, j.head * a.group + row % a.group, d, acc, top, total);
+                finish(tok, j.head * a.group + row % a.group, acc, top, total);
             }
             continue;
         }
@@ -788,7 +797,7 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
             if (part) continue;
 #pragma unroll
             for (int x = 1; x < GROUPS; x++) acc += sa[x][lane];
-            finish<T, D>(a, tok, j.head * a.group + row % a.group, d, acc, top, total);
+            finish(tok, j.head * a.group + row % a.group, acc, top, total);
         }
     }
 }
