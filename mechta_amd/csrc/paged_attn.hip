@@ -3,6 +3,7 @@
 // Row r of a sequence's query rows is (token r / group, query head head * group + r % group): the query heads of a kv head
 // and the tokens of a chunk share the keys they read. A work-group takes a tile of rows and a range of keys (Item); where
 // a tile's keys are split, join_kernel puts the splits together.
+#include <algorithm>
 #include <type_traits>
 
 #include "mkv_device.h"
@@ -718,58 +719,88 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
 }
 
 // ---- splits of a tile's rows put together ----
-// D / 4 lanes hold a row's dims, four each. Of few splits the 1024 / D such groups of a work-group take a row each; of
-// JOIN_WIDE and more they share a row: each adds up every so many of its splits, with the splits' factors in LDS.
-constexpr int JOIN_WIDE = 8;
+// Up to JOIN_FEW splits: D / 4 lanes hold a row, four dims each, and read its splits all at once; a work-group takes 1024 / D
+// rows. More: a work-group takes 64 dims of a row; 16 lanes hold them, and each 16 lanes add up every 16th split, with the
+// splits' factors in LDS. (A row whole in a work-group, 32 rows of 121 splits: 7.9 us; by 64 dims 5.2.)
+constexpr int JOIN_FEW = 8, JOIN_DIMS = 64;
 template <typename T, int D>
 __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restrict__ joins, const int* __restrict__ njoins) {
-    constexpr int LANES = D / 4, GROUPS = 256 / LANES;
     __shared__ float factor[SPLITS_MOST];
-    __shared__ __attribute__((aligned(16))) f32x4 sa[GROUPS][LANES];
+    __shared__ __attribute__((aligned(16))) f32x4 sa[16][16];
     __shared__ float red[2][4];
-    const int count = *uniform(njoins), tid = threadIdx.x, part = tid / LANES, lane = tid % LANES, d = lane * 4;
-    auto finish = [&](int tok, int head, f32x4 acc, float m, float l) INLINE {
+    const int count = *uniform(njoins), tid = threadIdx.x;
+    auto finish = [&](int tok, int head, int d, f32x4 acc, float m, float l) INLINE {
         acc *= row_factor(a, head, m, l);
         const float x[4] = {acc[0], acc[1], acc[2], acc[3]};
         store_out<T, D, 4>(a, tok, head, d, x);
     };
     for (int n = blockIdx.x; n < count; n += gridDim.x) {
-        const Join j = joins[n];
-        if (j.splits < JOIN_WIDE) {
-            for (int r = blockIdx.y * GROUPS + part; r < j.count; r += gridDim.y * GROUPS) {
+        const Uniform<int> ji = uniform((const int*)(joins + n));
+        const Join j{ji[0], ji[1], ji[2], ji[3], ji[4], ji[5], {0, 0}};
+        if (j.splits <= JOIN_FEW) {
+            constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+            const int d = tid % LANES * 4;
+            for (int r = blockIdx.y * GROUPS + tid / LANES; r < j.count; r += gridDim.y * GROUPS) {
                 const int row = j.row0 + r, tok = j.tok0 + row / a.group;
                 if (tok >= a.rows) continue;
-                float m[JOIN_WIDE], top = NEG_INF, total = 0.f;
-                f32x4 x[JOIN_WIDE], acc = f32x4{};
+                f32x4 acc = f32x4{};
+                float top = NEG_INF, total = 0.f;
+                auto four = [&](int s0) INLINE {  // splits s0 .. s0 + 3; those behind the last: the last again, not counted
+                    float m[4], l[4];
+                    f32x4 x[4];
 #pragma unroll
-                for (int s = 0; s < JOIN_WIDE; s++) {  // splits behind the last: the last again, not counted
-                    const size_t at = j.part + r + (size_t)min(s, j.splits - 1) * j.count;
-                    m[s] = s < j.splits ? a.pm[at] : NEG_INF;
-                    x[s] = *(const f32x4*)(a.pacc + at * D + d);
-                    top = fmaxf(top, m[s]);
-                }
+                    for (int s = 0; s < 4; s++) {
+                        const size_t at = j.part + r + (size_t)min(s0 + s, j.splits - 1) * j.count;
+                        m[s] = a.pm[at];
+                        l[s] = a.pl[at];
+                        x[s] = *(const f32x4*)(a.pacc + at * D + d);
+                    }
+                    const float was = top;
 #pragma unroll
-                for (int s = 0; s < JOIN_WIDE; s++) {
-                    const float f = m[s] == NEG_INF ? 0.f : fast_exp2(m[s] - top);
+                    for (int s = 0; s < 4; s++) {
+                        if (s0 + s >= j.splits) m[s] = NEG_INF;
+                        top = fmaxf(top, m[s]);
+                    }
+                    if (s0) {
+                        const float f = was == NEG_INF ? 0.f : fast_exp2(was - top);
+                        acc *= f;
+                        total *= f;
+                    }
 #pragma unroll
-                    for (int i = 0; i < 4; i++) acc[i] += f == 0.f ? 0.f : f * x[s][i];
-                    total += f * a.pl[j.part + r + (size_t)min(s, j.splits - 1) * j.count];
-                }
-                finish(tok, j.head * a.group + row % a.group, acc, top, total);
+                    for (int s = 0; s < 4; s++) {
+                        const float f = m[s] == NEG_INF ? 0.f : fast_exp2(m[s] - top);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[i] += f == 0.f ? 0.f : f * x[s][i];
+                        total += f == 0.f ? 0.f : f * l[s];
+                    }
+                };
+                four(0);
+                if (j.splits > 4) four(4);
+                finish(tok, j.head * a.group + row % a.group, d, acc, top, total);
             }
             continue;
         }
-        for (int r = blockIdx.y; r < j.count; r += gridDim.y) {
+        constexpr int PER_ROW = D / JOIN_DIMS;
+        const int part = tid / 16, lane = tid % 16;
+        for (int u = blockIdx.y; u < j.count * PER_ROW; u += gridDim.y) {
+            const int r = u / PER_ROW, d = u % PER_ROW * JOIN_DIMS + lane * 4;
             const int row = j.row0 + r, tok = j.tok0 + row / a.group;
             if (tok >= a.rows) continue;
             const size_t first = j.part + r;
             float top = NEG_INF;
             for (int s = tid; s < j.splits; s += 256) top = fmaxf(top, a.pm[first + (size_t)s * j.count]);
+            // the first splits' values are on their way meanwhile
+            constexpr int EARLY = 8;
+            const float* const src = a.pacc + first * D + d;
+            const size_t step = (size_t)j.count * D;
+            f32x4 x[EARLY];
 #pragma unroll
-            for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+            for (int i = 0; i < EARLY; i++) x[i] = *(const f32x4*)(src + min(part + 16 * i, j.splits - 1) * step);
+#pragma unroll
+            for (int i = 1; i < 64; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
             __syncthreads();  // the row before has been read
             if (tid % 64 == 0) red[0][tid / 64] = top;
-            __syncthreads();
+            lds_barrier();
             top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
             float total = 0.f;
             for (int s = tid; s < j.splits; s += 256) {
@@ -778,26 +809,28 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
                 total += f == 0.f ? 0.f : f * a.pl[first + (size_t)s * j.count];
             }
 #pragma unroll
-            for (int x = 1; x < 64; x *= 2) total += __shfl_xor(total, x);
+            for (int i = 1; i < 64; i *= 2) total += __shfl_xor(total, i);
             if (tid % 64 == 0) red[1][tid / 64] = total;
-            __syncthreads();
+            lds_barrier();
             total = red[1][0] + red[1][1] + red[1][2] + red[1][3];
             f32x4 acc = f32x4{};
-            const float* const src = a.pacc + first * D + d;
-            const size_t step = (size_t)j.count * D;
-#pragma unroll 8
-            for (int s = part; s < j.splits; s += GROUPS) {
+            auto add = [&](int s, f32x4 y) INLINE {
                 const float f = factor[s];
-                const f32x4 x = *(const f32x4*)(src + s * step);
 #pragma unroll
-                for (int i = 0; i < 4; i++) acc[i] += f == 0.f ? 0.f : f * x[i];
-            }
+                for (int c = 0; c < 4; c++) acc[c] += f == 0.f ? 0.f : f * y[c];
+            };
+#pragma unroll
+            for (int i = 0; i < EARLY; i++)
+                if (part + 16 * i < j.splits) add(part + 16 * i, x[i]);
+#pragma unroll 4
+            for (int s = part + 16 * EARLY; s < j.splits; s += 16) add(s, *(const f32x4*)(src + s * step));
             sa[part][lane] = acc;
-            __syncthreads();
+            lds_barrier();
             if (part) continue;
+            acc = sa[0][lane];
 #pragma unroll
-            for (int x = 1; x < GROUPS; x++) acc += sa[x][lane];
-            finish(tok, j.head * a.group + row % a.group, acc, top, total);
+            for (int i = 1; i < 16; i++) acc += sa[i][lane];
+            finish(tok, j.head * a.group + row % a.group, d, acc, top, total);
         }
     }
 }
@@ -847,7 +880,14 @@ hipError_t attend_as(const Geometry& g, const AttendArgs& x, const int* batch, c
         e = hipGetLastError();
     }
     if (join_grid && e == hipSuccess) {
-        join_kernel<T, D><<<dim3(join_grid, 32), dim3(256), 0, s>>>(a, (const Join*)(batch + l.joins), batch + KINDS);
+        // work-groups for a join: the most that one of them has rows for
+        int join_rows = 1;
+        for (const Join& j : *x.joins) {
+            const int groups = 1024 / D;
+            join_rows = std::max(join_rows, j.splits <= JOIN_FEW ? (j.count + groups - 1) / groups : j.count * (D / JOIN_DIMS));
+        }
+        if (x.captured) join_rows = 32;
+        join_kernel<T, D><<<dim3(join_grid, join_rows), dim3(256), 0, s>>>(a, (const Join*)(batch + l.joins), batch + KINDS);
         e = hipGetLastError();
     }
     return e;

@@ -54,6 +54,8 @@ struct AttendArgs {
     void* out;
     float scale;
     float *pm, *pl, *pacc;  // split partials: reference maximum, sum, accumulator rows
+    const std::vector<Join>* joins;  // the plan's, for the launch's shape
+    bool captured;                   // a captured launch serves any plan
 };
 // grid[kind] work-groups for each kind of item (0: not launched), joins likewise; lists and counts on the device.
 hipError_t launch_attend(const Geometry& g, const AttendArgs& a, const int* batch, const Lists& l, const int* grid,

@@ -617,6 +617,8 @@ int mpg_attend(mpg_t* h, int layer, int rows, const void* q, int64_t q_tok, int6
     a.pm = h->part;
     a.pl = h->part + PART_ROWS;
     a.pacc = h->part + 2 * (size_t)PART_ROWS;
+    a.joins = &p.joins;
+    a.captured = cap != 0;
     int grid[KINDS];
     for (int k = 0; k < KINDS; k++) grid[k] = cap ? GRAPH_GRID : (int)p.items[k].size();
     const hipError_t e = launch_attend(h->g, a, h->dev + h->batch_at + w * h->lists.words, h->lists, grid,
