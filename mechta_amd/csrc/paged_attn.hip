@@ -719,10 +719,10 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
 }
 
 // ---- splits of a tile's rows put together ----
-// Up to JOIN_FEW splits: D / 4 lanes hold a row, four dims each, and read its splits all at once; a work-group takes 1024 / D
-// rows. More: a work-group takes 64 dims of a row; 16 lanes hold them, and each 16 lanes add up every 16th split, with the
+// D / 4 lanes hold a row, four dims each, and read its splits four at a time; a work-group takes 1024 / D rows. Wide: a
+// work-group takes 64 dims of a row; 16 lanes hold them, and each 16 lanes add up every 16th split, with the
 // splits' factors in LDS. (A row whole in a work-group, 32 rows of 121 splits: 7.9 us; by 64 dims 5.2.)
-constexpr int JOIN_FEW = 8, JOIN_DIMS = 64;
+constexpr int JOIN_DIMS = 64;
 template <typename T, int D>
 __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restrict__ joins, const int* __restrict__ njoins) {
     __shared__ float factor[SPLITS_MOST];
@@ -736,8 +736,8 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
     };
     for (int n = blockIdx.x; n < count; n += gridDim.x) {
         const Uniform<int> ji = uniform((const int*)(joins + n));
-        const Join j{ji[0], ji[1], ji[2], ji[3], ji[4], ji[5], {0, 0}};
-        if (j.splits <= JOIN_FEW) {
+        const Join j{ji[0], ji[1], ji[2], ji[3], ji[4], ji[5], ji[6], 0};
+        if (!j.wide) {
             constexpr int LANES = D / 4, GROUPS = 256 / LANES;
             const int d = tid % LANES * 4;
             for (int r = blockIdx.y * GROUPS + tid / LANES; r < j.count; r += gridDim.y * GROUPS) {
@@ -775,7 +775,7 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
                     }
                 };
                 four(0);
-                if (j.splits > 4) four(4);
+                for (int s = 4; s < j.splits; s += 4) four(s);
                 finish(tok, j.head * a.group + row % a.group, d, acc, top, total);
             }
             continue;
@@ -884,7 +884,7 @@ hipError_t attend_as(const Geometry& g, const AttendArgs& x, const int* batch, c
         int join_rows = 1;
         for (const Join& j : *x.joins) {
             const int groups = 1024 / D;
-            join_rows = std::max(join_rows, j.splits <= JOIN_FEW ? (j.count + groups - 1) / groups : j.count * (D / JOIN_DIMS));
+            join_rows = std::max(join_rows, j.wide ? j.count * (D / JOIN_DIMS) : (j.count + groups - 1) / groups);
         }
         if (x.captured) join_rows = 32;
         join_kernel<T, D><<<dim3(join_grid, join_rows), dim3(256), 0, s>>>(a, (const Join*)(batch + l.joins), batch + KINDS);

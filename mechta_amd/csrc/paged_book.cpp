@@ -189,9 +189,12 @@ namespace {
 struct Tile {
     int member, tok0, row0, k0, k1, kind;
 };
-constexpr int LEAST_KEYS = 256;  // of a piece: two tiles for each wave of few rows
-// Work-groups that run at once: 256 CUs, two to a CU except for the widest accumulators and for chunks.
-int resident(int kind, int head_dim) { return kind == FEW || (kind == SOME && head_dim <= 128) ? 512 : 256; }
+constexpr int LEAST_KEYS = 128;  // of a piece: a tile for each wave of few rows
+// Pieces of a kind's tiles: about as many as CUs. Few rows stream fastest from 216 work-groups (1 token at 131,072 positions of
+// 2 x 256: 128 / 192 / 216 / 240 / 256 / 512 of them 59.1 / 51.4 / 51.3 / 52.0 / 52.6 / 59.8 us; 64 sequences of 4 x 128 at
+// 3,000: 256 / 512 / 768 64.1 / 69.5 / 71.9) -- or from 256 where 216 would leave a quarter of them without work.
+constexpr int CUS = 256, STREAMS = 216;
+constexpr int WIDE_SPLITS = 8, WIDE_ROWS = 512;
 }  // namespace
 
 // Dies take the items of a list in turn (position i: die i % 8). The tiles of one (sequence, head, split) stream the same
@@ -276,26 +279,37 @@ void plan_window(const Shape& g, const std::vector<Member>& batch, int window, P
     // two rounds: 118 us against 65.) Tiles that are more than run at once are cut where they are longer than a share.
     long long most[KINDS];
     for (int k = 0; k < KINDS; k++) {
-        const int run = resident(k, g.head_dim);
-        long long lo = LEAST_KEYS / KEYS, hi = lo, tiles_here = 0, share = (keys[k] + run - 1) / run;
+        const long long least = LEAST_KEYS / KEYS, share = (keys[k] + CUS - 1) / CUS;
+        long long longest = least, whole = 0;
         for (const Tile& t : tiles)
             if (t.kind == k) {
-                hi = std::max<long long>(hi, (t.k1 - t.k0 + KEYS - 1) / KEYS);
-                tiles_here += g.kv_heads;
+                longest = std::max<long long>(longest, (t.k1 - t.k0 + KEYS - 1) / KEYS);
+                whole += g.kv_heads;
             }
-        if (tiles_here > run) {
-            most[k] = std::max(lo, (share + KEYS - 1) / KEYS) * KEYS;
-            continue;
-        }
-        while (lo < hi) {  // the least length, in units of KEYS, that gives no more pieces than places
-            const long long mid = (lo + hi) / 2;
+        auto pieces = [&](long long length) {  // of at most so many KEYS
             long long n = 0;
             for (const Tile& t : tiles)
-                if (t.kind == k) n += ((t.k1 - t.k0 + KEYS - 1) / KEYS + mid - 1) / mid * g.kv_heads;
-            if (n <= run) hi = mid;
-            else lo = mid + 1;
+                if (t.kind == k) n += ((t.k1 - t.k0 + KEYS - 1) / KEYS + length - 1) / length * g.kv_heads;
+            return n;
+        };
+        auto shortest = [&](int places) {  // the least length that gives no more pieces than places
+            long long lo = least, hi = longest;
+            while (lo < hi) {
+                const long long mid = (lo + hi) / 2;
+                if (pieces(mid) <= places) hi = mid;
+                else lo = mid + 1;
+            }
+            return lo;
+        };
+        const bool few = k == FEW || k == SOME;
+        long long length;
+        if (whole > CUS) {
+            length = std::max(least, (share + KEYS - 1) / KEYS);
+        } else {
+            length = shortest(few && whole <= STREAMS ? STREAMS : CUS);
+            if (few && pieces(length) < STREAMS * 3 / 4) length = shortest(CUS);
         }
-        most[k] = lo * KEYS;
+        most[k] = length * KEYS;
     }
     int part = 0;
     for (const Tile& t : tiles) {
@@ -313,11 +327,16 @@ void plan_window(const Shape& g, const std::vector<Member>& batch, int window, P
                                              splits > 1 ? part + s * count : -1, s, {0, 0}});
             }
             if (splits > 1) {
-                out.joins.push_back({head, t.tok0, t.row0, count, part, splits, {0, 0}});
+                out.joins.push_back({head, t.tok0, t.row0, count, part, splits, 0, 0});
                 part += splits * count;
             }
         }
     }
+    // Many splits of few rows are read by many work-groups at once; of many rows the rows are work enough (3,200 rows of 9
+    // splits by 64 dims each: 45 us, row by row 14).
+    long long rows = 0;
+    for (const Join& j : out.joins) rows += j.count;
+    for (Join& j : out.joins) j.wide = j.splits > WIDE_SPLITS && rows <= WIDE_ROWS;
     for (auto& list : out.items) {
         std::stable_sort(list.begin(), list.end(), [](const Item& a, const Item& b) {
             return a.seq != b.seq ? a.seq < b.seq : a.head != b.head ? a.head < b.head : a.split < b.split;

@@ -54,9 +54,9 @@ struct Item {
     int part;        // first row of the split partials it writes, -1: it writes the output
     int split, pad[2];
 };
-// Join of a tile's splits: split s of row r at part + s * count + r.
+// Join of a tile's splits: split s of row r at part + s * count + r. wide: a work-group for every 64 dims of a row.
 struct Join {
-    int head, tok0, row0, count, part, splits, pad[2];
+    int head, tok0, row0, count, part, splits, wide, pad;
 };
 // A run of at most KEYS new tokens inside one KEYS-aligned run of positions.
 struct Run {
