@@ -248,69 +248,110 @@ static void deal(std::vector<Item>& items) {
     items.swap(out);
 }
 
+namespace {
+int pieces_of(const Tile& t, long long length) {  // of at most so many KEYS
+    return (int)(((t.k1 - t.k0 + KEYS - 1) / KEYS + length - 1) / length);
+}
+
+// The least length of a piece (in KEYS) that gives no more pieces than places.
+long long shortest(const std::vector<Tile>& tiles, int kv_heads, int places) {
+    long long lo = LEAST_KEYS / KEYS, hi = lo;
+    for (const Tile& t : tiles) hi = std::max(hi, (long long)(t.k1 - t.k0 + KEYS - 1) / KEYS);
+    while (lo < hi) {
+        const long long mid = (lo + hi) / 2;
+        long long n = 0;
+        for (const Tile& t : tiles) n += (long long)pieces_of(t, mid) * kv_heads;
+        if (n <= places) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+// Few rows: tiles that are more than the CUs are cut where they are longer than a CU's share, others into as many pieces as
+// stream fastest.
+long long few_length(const std::vector<Tile>& tiles, int kv_heads) {
+    const long long whole = (long long)tiles.size() * kv_heads;
+    if (whole > CUS) {
+        long long keys = 0;
+        for (const Tile& t : tiles) keys += (long long)(t.k1 - t.k0) * kv_heads;
+        return std::max<long long>(LEAST_KEYS, (keys + CUS - 1) / CUS) / KEYS;
+    }
+    const long long length = shortest(tiles, kv_heads, whole <= STREAMS ? STREAMS : CUS);
+    long long n = 0;
+    for (const Tile& t : tiles) n += (long long)pieces_of(t, length) * kv_heads;
+    return n < STREAMS * 3 / 4 ? shortest(tiles, kv_heads, CUS) : length;
+}
+
+// Chunks: the cheapest length of a piece by a model of the call in us: a piece's keys, 9 for its beginning and end, the split
+// partials written and read back at 5 TB/s and 3 for the launch that joins them. us per key of a work-group: heads of 64 /
+// 128 / 256 in tiles of 256 rows .0155 / .029 / .062, of 128 rows .0107 / .0162 / .0295. (Pieces that are more than the CUs
+// run in rounds; half a mean piece is added for the last one. Where CUs stand idle behind short pieces the card, limited by its
+// power, runs the others faster: up to .65 of the time.)
+long long chunk_length(const std::vector<Tile>& tiles, const Shape& g, int kind, double& cost) {
+    static const double us[2][3] = {{.0107, .0162, .0295}, {.0155, .029, .062}};
+    const double key = us[kind == MANY][g.head_dim / 128];
+    long long longest = LEAST_KEYS / KEYS, best = longest;
+    for (const Tile& t : tiles) longest = std::max(longest, (long long)(t.k1 - t.k0 + KEYS - 1) / KEYS);
+    cost = 1e30;
+    for (long long length = longest;; length = length * 7 / 8) {  // from whole tiles down
+        if (length < LEAST_KEYS / KEYS) break;
+        long long n = 0, sum = 0, rows = 0, most = 0;
+        for (const Tile& t : tiles) {
+            const int p = pieces_of(t, length);
+            const long long keys = t.k1 - t.k0;
+            n += (long long)p * g.kv_heads;
+            sum += keys * g.kv_heads;
+            most = std::max(most, (keys + p - 1) / p);
+            if (p > 1) rows += (long long)p * TILE_ROWS[kind] * g.kv_heads;
+        }
+        const double busy = (double)sum / ((double)CUS * most);
+        double c = n <= CUS ? most * key * (.65 + .35 * std::min(1., busy)) + 9 : (double)sum / CUS * key + 9. * n / CUS + .5 * sum / n * key;
+        if (rows) c += 3 + 8. * g.head_dim * rows / 5e6;
+        if (c < cost) {
+            cost = c;
+            best = length;
+        }
+        if (rows > PART_ROWS) break;  // no room for more
+    }
+    return best;
+}
+}  // namespace
+
 void plan_window(const Shape& g, const std::vector<Member>& batch, int window, Plan& out) {
     for (auto& v : out.items) v.clear();
     out.joins.clear();
     const int group = g.q_heads / g.kv_heads;
-    // Tiles of 256 rows where they fill the card, of 128 (and two key groups) where they do not.
-    long long wide = 0;
-    for (const Member& m : batch) {
-        const long long rows = (long long)m.count * group;
-        if (rows > TILE_ROWS[SOME]) wide += (rows + TILE_ROWS[MANY] - 1) / TILE_ROWS[MANY] * g.kv_heads;
-    }
-    const int chunk_kind = wide >= 256 ? MANY : HALF;
-    std::vector<Tile> tiles;
-    long long keys[KINDS] = {};
-    int tok0 = 0;
-    for (int i = 0; i < (int)batch.size(); i++) {
+    std::vector<Tile> by_kind[KINDS];
+    auto add = [&](int i, int tok0, int kind) {
         const Member& m = batch[i];
         const int rows = m.count * group, pos0 = m.len - m.count;
-        const int kind = rows <= TILE_ROWS[FEW] ? FEW : rows <= TILE_ROWS[SOME] ? SOME : chunk_kind;
         for (int r = 0; r < rows; r += TILE_ROWS[kind]) {
             const int last = (std::min(r + TILE_ROWS[kind], rows) - 1) / group;
             const int lo = window ? std::max(0, pos0 + r / group - window + 1) : 0;
-            tiles.push_back({i, tok0, r, lo / KEYS * KEYS, pos0 + last + 1, kind});
-            keys[kind] += (long long)(tiles.back().k1 - tiles.back().k0) * g.kv_heads;
+            by_kind[kind].push_back({i, tok0, r, lo / KEYS * KEYS, pos0 + last + 1, kind});
         }
-        tok0 += m.count;
+    };
+    int tok0 = 0;
+    for (int i = 0; i < (int)batch.size(); i++) {
+        const int rows = batch[i].count * group;
+        if (rows <= TILE_ROWS[SOME]) {
+            add(i, tok0, rows <= TILE_ROWS[FEW] ? FEW : SOME);
+        } else {  // either size of tile is a candidate
+            add(i, tok0, HALF);
+            add(i, tok0, MANY);
+        }
+        tok0 += batch[i].count;
     }
-    // Splits: every kind's tiles are cut into pieces of at most so many keys that they are as many as work-groups run at
-    // once. (By the share of a work-group instead, 64 tiles of 9,016 to 9,512 keys became 288 pieces for 256 places, and took
-    // two rounds: 118 us against 65.) Tiles that are more than run at once are cut where they are longer than a share.
+    long long length[KINDS];
+    for (int k : {FEW, SOME}) length[k] = few_length(by_kind[k], g.kv_heads);
+    double half, many;
+    length[HALF] = chunk_length(by_kind[HALF], g, HALF, half);
+    length[MANY] = chunk_length(by_kind[MANY], g, MANY, many);
+    by_kind[half <= many ? MANY : HALF].clear();
+    std::vector<Tile> tiles;
+    for (const auto& v : by_kind) tiles.insert(tiles.end(), v.begin(), v.end());
     long long most[KINDS];
-    for (int k = 0; k < KINDS; k++) {
-        const long long least = LEAST_KEYS / KEYS, share = (keys[k] + CUS - 1) / CUS;
-        long long longest = least, whole = 0;
-        for (const Tile& t : tiles)
-            if (t.kind == k) {
-                longest = std::max<long long>(longest, (t.k1 - t.k0 + KEYS - 1) / KEYS);
-                whole += g.kv_heads;
-            }
-        auto pieces = [&](long long length) {  // of at most so many KEYS
-            long long n = 0;
-            for (const Tile& t : tiles)
-                if (t.kind == k) n += ((t.k1 - t.k0 + KEYS - 1) / KEYS + length - 1) / length * g.kv_heads;
-            return n;
-        };
-        auto shortest = [&](int places) {  // the least length that gives no more pieces than places
-            long long lo = least, hi = longest;
-            while (lo < hi) {
-                const long long mid = (lo + hi) / 2;
-                if (pieces(mid) <= places) hi = mid;
-                else lo = mid + 1;
-            }
-            return lo;
-        };
-        const bool few = k == FEW || k == SOME;
-        long long length;
-        if (whole > CUS) {
-            length = std::max(least, (share + KEYS - 1) / KEYS);
-        } else {
-            length = shortest(few && whole <= STREAMS ? STREAMS : CUS);
-            if (few && pieces(length) < STREAMS * 3 / 4) length = shortest(CUS);
-        }
-        most[k] = length * KEYS;
-    }
+    for (int k = 0; k < KINDS; k++) most[k] = length[k] * KEYS;
     int part = 0;
     for (const Tile& t : tiles) {
         const Member& m = batch[t.member];
