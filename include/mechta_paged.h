@@ -85,13 +85,20 @@ typedef struct mpg_rope {
     double amplitude;                /* 0: 1, and for MPG_YARN 0.1 ln factor + 1 */
 } mpg_rope;
 
+/* What a rotation goes by, worked out once: whole turns per position of each pair, th_i / (2 pi). */
+typedef struct mpg_turns {
+    double turns[MPG_ROPE_DIM_MAX / 2];
+    float amplitude;
+    int dim, layout;
+} mpg_turns;
+int mpg_rope_turns(const mpg_rope* r, mpg_turns* turns);
 /* th_i of the dim/2 pairs, scaled, and the amplitude (host). */
 int mpg_rope_freqs(const mpg_rope* r, double* freqs, double* amplitude);
 /* Rotates rows x heads vectors of dim elements at the positions pos[row] (device, int32): out = x rotated, its elements
  * behind r->dim copied. fmt: MKV_F16, MKV_F32 or MPG_BF16. x and out (device): element (row, head, d) at
  * row x *_row + head x *_head + d; out may be x with x's strides, and overlap it in no other way. On the current device,
  * enqueued on `stream`. Products and sums in f32, rounded once. */
-int mpg_rotate(const mpg_rope* r, int fmt, int rows, int heads, int dim, const void* x, int64_t x_row, int64_t x_head,
+int mpg_rotate(const mpg_turns* r, int fmt, int rows, int heads, int dim, const void* x, int64_t x_row, int64_t x_head,
                const int* pos, void* out, int64_t o_row, int64_t o_head, void* stream);
 
 /* Device bytes mpg_create allocates for the configuration (0 if it would refuse it). */

@@ -25,11 +25,7 @@ struct Rows {  // a caller's rows: element (token, head, d) at token * tok + hea
     int64_t tok, head;
 };
 
-struct RopeArgs {
-    double turns[MPG_ROPE_DIM_MAX / 2];  // whole turns per position of each pair
-    float amplitude;
-    int dim, layout;
-};
+using RopeArgs = mpg_turns;
 
 struct Segment {
     unsigned dst, src, words, pad;

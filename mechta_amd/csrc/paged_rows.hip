@@ -103,84 +103,135 @@ __device__ inline void rotate_unit(const T* __restrict__ x, int u, int rot, int 
     }
 }
 
+// A thread's places in a grid of rows x heads x units, `by` apart, without a division each.
+struct Walk {
+    int row, head, unit, rows_by, heads_by, units_by, heads, units;
+    __device__ Walk(int at, int by, int heads_, int units_) : heads(heads_), units(units_) {
+        split(at, row, head, unit);
+        split(by, rows_by, heads_by, units_by);
+    }
+    __device__ void split(int x, int& r, int& h, int& u) const {
+        u = x % units;
+        x /= units;
+        h = x % heads;
+        r = x / heads;
+    }
+    __device__ void next() {
+        unit += units_by;
+        head += heads_by;
+        row += rows_by;
+        if (unit >= units) {
+            unit -= units;
+            head++;
+        }
+        if (head >= heads) {
+            head -= heads;
+            row++;
+        }
+    }
+};
+
 constexpr int ROT_ROWS = 8;  // rows of a work-group: their angles are shared by the heads
+// n rows of `heads` heads from x (row and head strides) to out, cs: their pairs
+template <typename T, bool WIDE>
+__device__ inline void rotate_rows(const RopeArgs& r, int n, int heads, int dim, const T* x, int64_t x_row, int64_t x_head,
+                                   T* out, int64_t o_row, int64_t o_head, const float2* cs, int at, int by) {
+    const int half = r.dim / 2;
+    for (Walk w(at, by, heads, row_units<T, WIDE>(dim, r.dim, r.layout)); w.row < n; w.next()) {
+        T* const o = out + w.row * o_row + w.head * o_head;
+        rotate_unit<T, WIDE>(x + w.row * x_row + w.head * x_head, w.unit, r.dim, r.layout, cs + w.row * half,
+                             [&](int d) { return o + d; });
+    }
+}
+
+// Work-group = ROT_ROWS rows; where those are few, blockIdx.y shares out their heads.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) rotate_kernel(RopeArgs r, int rows, int heads, int dim, const T* x, int64_t x_row,
                                                      int64_t x_head, const int* __restrict__ pos, T* out, int64_t o_row,
                                                      int64_t o_head) {
     extern __shared__ float2 cs[];  // [ROT_ROWS][r.dim / 2]
     const int row0 = blockIdx.x * ROT_ROWS, n = min(ROT_ROWS, rows - row0), half = r.dim / 2;
-    for (int i = threadIdx.x; i < n * half; i += 256) cs[i] = turn(r, pos[row0 + i / half], i % half);
+    for (Walk w(threadIdx.x, 256, 1, half); w.row < n; w.next()) cs[w.row * half + w.unit] = turn(r, pos[row0 + w.row], w.unit);
     __syncthreads();
-    const int units = row_units<T, WIDE>(dim, r.dim, r.layout), all = n * heads * units;
-    for (int i = threadIdx.x + 256 * blockIdx.y; i < all; i += 256 * gridDim.y) {
-        const int u = i % units, head = i / units % heads, row = i / units / heads;
-        T* const o = out + (row0 + row) * o_row + head * o_head;
-        rotate_unit<T, WIDE>(x + (row0 + row) * x_row + head * x_head, u, r.dim, r.layout, cs + row * half,
-                             [&](int d) { return o + d; });
-    }
+    rotate_rows<T, WIDE>(r, n, heads, dim, x + row0 * x_row, x_row, x_head, out + row0 * o_row, o_row, o_head, cs,
+                         threadIdx.x + 256 * blockIdx.y, 256 * gridDim.y);
 }
 
 // ---- append ----
-// Work-group = (run of new tokens inside one 32-position block of a page, kv head): the head's K rows, rotated, its V
-// rows, and the query heads that read it, rotated. A V block that is all new is turned in registers (8 positions of 8
-// dims a thread) and written in 16-byte pieces, others element by element.
+// For a run of new tokens inside one 32-position block of a page: work-groups y = 0 .. 3 rotate the query heads of 8 tokens
+// each; the last one takes the run's K and V. K rows are rotated into LDS and leave in the pages' order, 16 positions side
+// by side. A V block that is all new is turned in registers (8 positions of 8 dims a thread) and written in 16-byte
+// pieces, others element by element.
+constexpr int Q_PARTS = KEYS / ROT_ROWS;
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) append_kernel(const Run* __restrict__ runs, const int* __restrict__ nruns,
                                                      const int* __restrict__ table, int most_pages, int page, int dim,
-                                                     int group, T* __restrict__ kpool, T* __restrict__ vpool, int rows,
-                                                     const T* __restrict__ k, int64_t k_tok, int64_t k_head,
+                                                     int kv_heads, int q_heads, T* __restrict__ kpool, T* __restrict__ vpool,
+                                                     int rows, const T* __restrict__ k, int64_t k_tok, int64_t k_head,
                                                      const T* __restrict__ v, int64_t v_tok, int64_t v_head, const T* q,
                                                      int64_t q_tok, int64_t q_head, T* q_out, RopeArgs r) {
-    extern __shared__ float2 cs[];  // [KEYS][r.dim / 2]
-    const int head = blockIdx.y, kv_heads = gridDim.y, half = r.dim / 2;
-    const int units = row_units<T, WIDE>(dim, r.dim, r.layout), count = *nruns;
+    extern __shared__ float2 cs[];  // [tokens][r.dim / 2], behind it K rows [KEYS][dim + 8]
+    const int half = r.dim / 2, tid = threadIdx.x, count = *uniform(nruns);
     for (int i = blockIdx.x; i < count; i += gridDim.x) {
-        Run run = runs[i];
+        const Uniform<int> ri = uniform((const int*)(runs + i));
+        Run run{ri[0], ri[1], ri[2], ri[3]};
         run.count = min(run.count, rows - run.tok);
-        if (run.count <= 0) continue;
-        const size_t p = table[(size_t)run.seq * most_pages + run.pos / page];
-        const size_t base = (p * kv_heads + head) * page * dim;  // the head's part of the page
-        const int in = run.pos % page;
-        __syncthreads();  // the table of the run before has been read
-        for (int j = threadIdx.x; j < run.count * half; j += 256) cs[j] = turn(r, run.pos + j / half, j % half);
-        __syncthreads();
-        const int per = q ? group + 1 : 1;  // rows a token: its K row, then query heads
-        for (int j = threadIdx.x; j < run.count * per * units; j += 256) {
-            const int u = j % units, row = j / units, t = row / per, which = row % per;
-            const int64_t tok = run.tok + t;
-            if (which == 0) {
-                const int pos = in + t;
-                T* const o = kpool + base + (size_t)(pos / 16) * 16 * dim + pos % 16 * 8;
-                rotate_unit<T, WIDE>(k + tok * k_tok + head * k_head, u, r.dim, r.layout, cs + t * half,
-                                     [&](int d) { return o + d / 8 * 128 + d % 8; });
-            } else {
-                const int h = head * group + which - 1;
-                T* const o = q_out + (tok * kv_heads * group + h) * dim;
-                rotate_unit<T, WIDE>(q + tok * q_tok + h * q_head, u, r.dim, r.layout, cs + t * half,
-                                     [&](int d) { return o + d; });
-            }
+        if (blockIdx.y < gridDim.y - 1) {  // query heads
+            const int t0 = blockIdx.y * ROT_ROWS, n = min(ROT_ROWS, run.count - t0);
+            if (n <= 0) continue;
+            __syncthreads();  // the angles before have been read
+            for (Walk w(tid, 256, 1, half); w.row < n; w.next())
+                cs[w.row * half + w.unit] = turn(r, run.pos + t0 + w.row, w.unit);
+            __syncthreads();
+            const int64_t tok = run.tok + t0;
+            rotate_rows<T, WIDE>(r, n, q_heads, dim, q + tok * q_tok, q_tok, q_head, q_out + tok * q_heads * dim,
+                                 (int64_t)q_heads * dim, dim, cs, tid, 256);
+            continue;
         }
-        const T* const vs = v + run.tok * v_tok + head * v_head;
-        T* const vb = vpool + base + (size_t)(in / KEYS) * KEYS * dim;
-        if (run.count == KEYS) {
-            for (int j = threadIdx.x; j < dim / 2; j += 256) {  // (group of 8 positions, 8 dims)
-                const int g = j / (dim / 8), d = j % (dim / 8) * 8;
-                Vec8<T> x[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) x[e] = load8(vs + (16 * (e / 4) + 4 * g + e % 4) * v_tok + d);
-#pragma unroll
-                for (int c = 0; c < 8; c++)
-                    store8(vb + (g * dim + d + c) * 8,
-                           Vec8<T>{x[0][c], x[1][c], x[2][c], x[3][c], x[4][c], x[5][c], x[6][c], x[7][c]});
+        if (run.count <= 0) continue;
+        const size_t p = uniform(table)[(size_t)run.seq * most_pages + run.pos / page];
+        const int in = run.pos % page, at = in % KEYS, stride = dim + 8;
+        T* const kt = (T*)(cs + KEYS * half);
+        __syncthreads();  // what stood in LDS has been read
+        if (half > 0)
+            for (Walk w(tid, 256, 1, half); w.row < run.count; w.next())
+                cs[w.row * half + w.unit] = turn(r, run.pos + w.row, w.unit);
+        const int units = row_units<T, WIDE>(dim, r.dim, r.layout), chunks = dim / 8;
+        for (int head = 0; head < kv_heads; head++) {
+            __syncthreads();
+            const T* const ks = k + run.tok * k_tok + head * k_head;
+            for (Walk w(tid, 256, 1, units); w.row < run.count; w.next()) {
+                T* const o = kt + w.row * stride;
+                rotate_unit<T, WIDE>(ks + w.row * k_tok, w.unit, r.dim, r.layout, cs + w.row * half, [&](int d) { return o + d; });
             }
-        } else {
-            for (int j = threadIdx.x; j < run.count * dim / 8; j += 256) {
-                const int t = j / (dim / 8), d = j % (dim / 8) * 8, at = in % KEYS + t;
-                const Vec8<T> x = load8(vs + t * v_tok + d);
-                T* const o = vb + (at % 16 / 4 * dim + d) * 8 + at / 16 * 4 + at % 4;
+            __syncthreads();
+            const size_t base = (p * kv_heads + head) * page * dim + (size_t)(in / KEYS) * KEYS * dim;  // of the 32-position block
+            T* const kb = kpool + base;
+            for (int j = tid; j < KEYS * chunks; j += 256) {  // 16-byte pieces in the pages' order
+                const int pos = j % 16 + j / (16 * chunks) * 16, t = pos - at;
+                if (t >= 0 && t < run.count) store8(kb + j * 8, load8(kt + t * stride + j / 16 % chunks * 8));
+            }
+            const T* const vs = v + run.tok * v_tok + head * v_head;
+            T* const vb = vpool + base;
+            if (run.count == KEYS) {
+                for (int j = tid; j < dim / 2; j += 256) {  // (group of 8 positions, 8 dims)
+                    const int g = j / chunks, d = j % chunks * 8;
+                    Vec8<T> x[8];
 #pragma unroll
-                for (int c = 0; c < 8; c++) o[c * 8] = x[c];
+                    for (int e = 0; e < 8; e++) x[e] = load8(vs + (16 * (e / 4) + 4 * g + e % 4) * v_tok + d);
+#pragma unroll
+                    for (int c = 0; c < 8; c++)
+                        store8(vb + (g * dim + d + c) * 8,
+                               Vec8<T>{x[0][c], x[1][c], x[2][c], x[3][c], x[4][c], x[5][c], x[6][c], x[7][c]});
+                }
+            } else {
+                for (Walk w(tid, 256, 1, chunks); w.row < run.count; w.next()) {
+                    const int d = w.unit * 8, b = at + w.row;
+                    const Vec8<T> x = load8(vs + w.row * v_tok + d);
+                    T* const o = vb + (b % 16 / 4 * dim + d) * 8 + b / 16 * 4 + b % 4;
+#pragma unroll
+                    for (int c = 0; c < 8; c++) o[c * 8] = x[c];
+                }
             }
         }
     }
@@ -212,12 +263,11 @@ hipError_t append_as(const Geometry& g, char* pool, int layer, const int* table,
     none.layout = MPG_HALF;
     const RopeArgs& r = rope ? *rope : none;
     T* const kp = (T*)pool + (size_t)layer * 2 * g.plane_elems();
-    const size_t lds = (size_t)KEYS * (r.dim / 2) * sizeof(float2);
+    const size_t lds = (size_t)KEYS * (r.dim / 2) * sizeof(float2) + (size_t)KEYS * (g.head_dim + 8) * sizeof(T);
     const auto kernel = r.dim % 16 ? append_kernel<T, false> : append_kernel<T, true>;
-    kernel<<<dim3(grid, g.kv_heads), dim3(256), lds, s>>>(runs, nruns, table, g.most_pages, g.page, g.head_dim,
-                                                          g.q_heads / g.kv_heads, kp, kp + g.plane_elems(), rows,
-                                                          (const T*)k.p, k.tok, k.head, (const T*)v.p, v.tok, v.head,
-                                                          (const T*)q.p, q.tok, q.head, (T*)q_out, r);
+    kernel<<<dim3(grid, q.p ? Q_PARTS + 1 : 1), dim3(256), lds, s>>>(
+        runs, nruns, table, g.most_pages, g.page, g.head_dim, g.kv_heads, g.q_heads, kp, kp + g.plane_elems(), rows,
+        (const T*)k.p, k.tok, k.head, (const T*)v.p, v.tok, v.head, (const T*)q.p, q.tok, q.head, (T*)q_out, r);
     return hipGetLastError();
 }
 
@@ -228,7 +278,10 @@ hipError_t rotate_as(const RopeArgs& r, int rows, int heads, int dim, const Rows
                       out.head % 8 == 0 && (uintptr_t)x.p % 16 == 0 && (uintptr_t)out.p % 16 == 0;
     const size_t lds = (size_t)ROT_ROWS * (r.dim / 2) * sizeof(float2);
     const auto kernel = wide ? rotate_kernel<T, true> : rotate_kernel<T, false>;
-    kernel<<<dim3((rows + ROT_ROWS - 1) / ROT_ROWS), dim3(256), lds, s>>>(r, rows, heads, dim, (const T*)x.p, x.tok, x.head,
+    const int groups = (rows + ROT_ROWS - 1) / ROT_ROWS, n = rows < ROT_ROWS ? rows : ROT_ROWS;
+    // few rows of many heads: heads shared out, a unit or two a thread
+    const int y = groups >= 256 ? 1 : std::max(1, std::min(256 / groups, n * heads * (dim / 16) / 512));
+    kernel<<<dim3(groups, y), dim3(256), lds, s>>>(r, rows, heads, dim, (const T*)x.p, x.tok, x.head,
                                                                          pos, (T*)out.p, out.tok, out.head);
     return hipGetLastError();
 }

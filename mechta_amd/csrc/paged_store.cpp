@@ -311,9 +311,18 @@ int mpg_rope_freqs(const mpg_rope* r, double* th, double* amplitude) {
     return MKV_OK;
 }
 
-int mpg_rotate(const mpg_rope* r, int fmt, int rows, int heads, int dim, const void* x, int64_t x_row, int64_t x_head,
+int mpg_rope_turns(const mpg_rope* r, mpg_turns* turns) {
+    if (int rc = check_rope("mpg_rope_turns", r)) return rc;
+    if (!turns) return fail(MKV_E_ARG, "mpg_rope_turns: NULL argument");
+    *turns = rope_args(*r);
+    return MKV_OK;
+}
+
+int mpg_rotate(const mpg_turns* r, int fmt, int rows, int heads, int dim, const void* x, int64_t x_row, int64_t x_head,
                const int* pos, void* out, int64_t o_row, int64_t o_head, void* stream) {
-    if (int rc = check_rope("mpg_rotate", r)) return rc;
+    if (!r) return fail(MKV_E_ARG, "mpg_rotate: NULL argument");
+    if (r->dim < 2 || r->dim > MPG_ROPE_DIM_MAX || r->dim % 2 || (r->layout != MPG_HALF && r->layout != MPG_INTERLEAVED))
+        return fail(MKV_E_ARG, "mpg_rotate: rotated dim %d, layout %d", r->dim, r->layout);
     if (fmt != MKV_F16 && fmt != MKV_F32 && fmt != MPG_BF16) return fail(MKV_E_ARG, "mpg_rotate: format %d", fmt);
     if (rows < 0 || heads < 0 || heads > 65536) return fail(MKV_E_ARG, "mpg_rotate: %d rows x %d heads", rows, heads);
     if (dim < r->dim || dim > 4096) return fail(MKV_E_ARG, "mpg_rotate: heads of %d elements, %d of them rotated", dim, r->dim);
@@ -324,7 +333,7 @@ int mpg_rotate(const mpg_rope* r, int fmt, int rows, int heads, int dim, const v
     const size_t bytes = fmt == MKV_F32 ? 4 : 2;
     if ((uintptr_t)x % bytes || (uintptr_t)out % bytes || (uintptr_t)pos % 4)
         return fail(MKV_E_ARG, "mpg_rotate: misaligned pointer");
-    const hipError_t e = launch_rotate(rope_args(*r), fmt, rows, heads, dim, Rows{x, x_row, x_head}, pos,
+    const hipError_t e = launch_rotate(*r, fmt, rows, heads, dim, Rows{x, x_row, x_head}, pos,
                                        Rows{out, o_row, o_head}, (hipStream_t)stream);
     return e == hipSuccess ? MKV_OK : hip_fail(e, "mpg_rotate");
 }

@@ -11,13 +11,14 @@ from mechta_amd import F16, F32, K, V, MkvError, lib as _mkv_lib  # noqa: F401
 BF16 = 2
 
 # every symbol include/mechta_paged.h declares
-SYMBOLS = ["mpg_rope_freqs", "mpg_rotate", "mpg_bytes", "mpg_create", "mpg_destroy", "mpg_set_stream", "mpg_sync",
+SYMBOLS = ["mpg_rope_freqs", "mpg_rope_turns", "mpg_rotate", "mpg_bytes", "mpg_create", "mpg_destroy", "mpg_set_stream", "mpg_sync",
            "mpg_len", "mpg_table", "mpg_free_pages", "mpg_pages", "mpg_reserve", "mpg_begin", "mpg_set_len", "mpg_fork",
            "mpg_copy", "mpg_free", "mpg_compact", "mpg_append", "mpg_attend", "mpg_read_rows"]
 
 LAYOUTS = {"half": 0, "interleaved": 1}
 SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
 
+_FORMATS = {}  # torch's element types, filled in on first use
 _done = False
 
 
@@ -26,6 +27,11 @@ class _Rope(ctypes.Structure):
                 ("base", ctypes.c_double), ("factor", ctypes.c_double), ("beta_fast", ctypes.c_double),
                 ("beta_slow", ctypes.c_double), ("low", ctypes.c_double), ("high", ctypes.c_double),
                 ("amplitude", ctypes.c_double)]
+
+
+class _Turns(ctypes.Structure):
+    _fields_ = [("turns", ctypes.c_double * 256), ("amplitude", ctypes.c_float), ("dim", ctypes.c_int),
+                ("layout", ctypes.c_int)]
 
 
 class _Config(ctypes.Structure):
@@ -38,10 +44,12 @@ def lib():
     L = _mkv_lib()
     if not _done:
         P, I, F, S, L64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_int64
-        R, C, IP, DP = ctypes.POINTER(_Rope), ctypes.POINTER(_Config), ctypes.POINTER(I), ctypes.POINTER(ctypes.c_double)
+        R, T, C = ctypes.POINTER(_Rope), P, ctypes.POINTER(_Config)
+        IP, DP = ctypes.POINTER(I), ctypes.POINTER(ctypes.c_double)
         sig = {
             "mpg_rope_freqs": ([R, DP, DP], I),
-            "mpg_rotate": ([R, I, I, I, I, P, L64, L64, P, P, L64, L64, P], I),
+            "mpg_rope_turns": ([R, T], I),
+            "mpg_rotate": ([T, I, I, I, I, P, L64, L64, P, P, L64, L64, P], I),
             "mpg_bytes": ([C], S),
             "mpg_create": ([ctypes.POINTER(P), C, IP, R, P], I),
             "mpg_destroy": ([P], I),
@@ -102,7 +110,9 @@ class Rope:
         self.c = _Rope(dim, LAYOUTS[layout], SCALINGS[scaling], int(original), base, factor, beta_fast, beta_slow, low,
                        high, amplitude)
         self.dim = dim
-        self.freqs()  # refuses what the library does
+        self._turns = _Turns()
+        _check(lib().mpg_rope_turns(ctypes.byref(self.c), ctypes.byref(self._turns)))
+        self._ptr = ctypes.addressof(self._turns)
 
     def freqs(self):
         """(turning speed of each pair in radians per position, amplitude)."""
@@ -112,39 +122,53 @@ class Rope:
 
 
 def _rows(t, heads, dim, dtype, device, what):
-    """Checks a [rows, heads, dim] tensor whose last dimension is contiguous; returns its pointer and strides."""
+    """Checks a [rows, heads, dim] tensor whose last dimension is contiguous; returns its address and strides."""
+    shape, stride = t.shape, t.stride()
+    if t.dtype is dtype and t.device == device and len(shape) == 3 and shape[1] == heads and shape[2] == dim \
+            and (stride[2] == 1 or dim == 1):
+        return t.data_ptr(), stride[0], stride[1]
     if t.device != device:
         raise ValueError(f"{what} is on {t.device}, {device} needed")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise ValueError(f"{what} is {t.dtype}, {dtype} needed")
-    if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or (dim is not None and t.shape[2] != dim):
-        raise ValueError(f"{what} has shape {tuple(t.shape)}, (rows, {heads or 'heads'}, {dim or 'dim'}) needed")
-    if t.shape[2] > 1 and t.stride(2) != 1:
-        raise ValueError(f"the last dimension of {what} must be contiguous")
-    return ctypes.c_void_p(t.data_ptr()), t.stride(0), t.stride(1)
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
+        raise ValueError(f"{what} has shape {tuple(shape)}, (rows, {heads}, {dim}) needed")
+    raise ValueError(f"the last dimension of {what} must be contiguous")
 
 
 def rotate(x, pos, rope, out=None):
     """x [rows, heads, dim] (f16, bf16 or f32) rotated at the positions pos [rows] (int32), into `out` (may be x), on
     torch's current stream of x's device."""
     import torch
-    fmts = {torch.float16: F16, torch.float32: F32, torch.bfloat16: BF16}
-    if x.device.type != "cuda":
+    dtype, device, shape = x.dtype, x.device, x.shape
+    fmt = _FORMATS.get(dtype)
+    if fmt is None:
+        if x.is_floating_point() and not _FORMATS:
+            _FORMATS.update({torch.float16: F16, torch.float32: F32, torch.bfloat16: BF16})
+        fmt = _FORMATS.get(dtype)
+        if fmt is None:
+            raise ValueError(f"x is {dtype}: float16, bfloat16 or float32 needed")
+    if device.type != "cuda":
         raise ValueError("x must be a device tensor")
-    if x.dtype not in fmts:
-        raise ValueError(f"x is {x.dtype}: float16, bfloat16 or float32 needed")
+    if len(shape) != 3:
+        raise ValueError(f"x has shape {tuple(shape)}, (rows, heads, dim) needed")
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    a = _rows(x, None, None, x.dtype, x.device, "x")
-    b = _rows(out, x.shape[1], x.shape[2], x.dtype, x.device, "out")
-    if out.shape[0] != x.shape[0]:
-        raise ValueError(f"out has {out.shape[0]} rows, x {x.shape[0]}")
-    if pos.device != x.device or pos.dtype != torch.int32 or pos.shape != x.shape[:1] or not pos.is_contiguous():
-        raise ValueError(f"pos must be {x.shape[0]} contiguous int32 on {x.device}")
-    with torch.cuda.device(x.device):
-        _check(lib().mpg_rotate(ctypes.byref(rope.c), fmts[x.dtype], x.shape[0], x.shape[1], x.shape[2], *a,
-                                ctypes.c_void_p(pos.data_ptr()), *b,
-                                ctypes.c_void_p(torch.cuda.current_stream(x.device).cuda_stream)))
+        out = torch.empty(shape, dtype=dtype, device=device)
+    elif out.shape[:1] != shape[:1]:
+        raise ValueError(f"out has shape {tuple(out.shape)}, x {tuple(shape)}")
+    rows, heads, dim = shape
+    xp, xr, xh = _rows(x, heads, dim, dtype, device, "x")
+    op, orow, oh = _rows(out, heads, dim, dtype, device, "out")
+    if pos.device != device or pos.dtype is not torch.int32 or pos.shape != shape[:1] or not pos.is_contiguous():
+        raise ValueError(f"pos must be {rows} contiguous int32 on {device}")
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        rc = lib().mpg_rotate(rope._ptr, fmt, rows, heads, dim, xp, xr, xh, pos.data_ptr(), op, orow, oh, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = lib().mpg_rotate(rope._ptr, fmt, rows, heads, dim, xp, xr, xh, pos.data_ptr(), op, orow, oh, stream)
+    if rc:
+        _check(rc)
     return out
 
 
@@ -194,6 +218,7 @@ class PagedKv:
         self._h = self._owner.ptr
         self.dtype = _dtype(fmt)
         self._views = {}
+        self._lib, self._empty, self._float32, self._scale = lib(), torch.empty, torch.float32, head_dim ** -0.5
 
     def close(self):
         """Frees the cache's memory now (tensors that pages() gave must not be used any more); without it, it is freed with
@@ -308,51 +333,57 @@ class PagedKv:
 
     # ---- the layers' calls ----
 
+    def _whole(self, t, rows, what):
+        """The address of a contiguous [rows, q_heads, head_dim] tensor that takes an output."""
+        p = _rows(t, self.q_heads, self.head_dim, self.dtype, self.device, what)[0]
+        if t.shape[0] != rows or not t.is_contiguous():
+            raise ValueError(f"{what} must be {rows} contiguous rows")
+        return p
+
     def append(self, layer, k, v, q=None, q_out=None, rotate=None):
         """Writes the batch's k and v [tokens, kv_heads, head_dim] into the pages, k rotated (rotate=False: it is already;
         default: if the cache has a rope). With q [tokens, q_heads, head_dim]: returns it rotated, in q_out (may be q)."""
-        import torch
-        rows = k.shape[0]
-        ka = _rows(k, self.kv_heads, self.head_dim, self.dtype, self.device, "k")
-        va = _rows(v, self.kv_heads, self.head_dim, self.dtype, self.device, "v")
+        rows, h, d = k.shape[0], self.kv_heads, self.head_dim
+        kp, kt, kh = _rows(k, h, d, self.dtype, self.device, "k")
+        vp, vt, vh = _rows(v, h, d, self.dtype, self.device, "v")
         if v.shape[0] != rows or (q is not None and q.shape[0] != rows):
             raise ValueError("k, v and q differ in rows")
-        qa, qo = (None, 0, 0), None
+        qp, qt, qh, qo = None, 0, 0, None
         if q is not None:
-            qa = _rows(q, self.q_heads, self.head_dim, self.dtype, self.device, "q")
+            qp, qt, qh = _rows(q, self.q_heads, d, self.dtype, self.device, "q")
             if q_out is None:
-                q_out = torch.empty((rows, self.q_heads, self.head_dim), dtype=self.dtype, device=self.device)
-            _rows(q_out, self.q_heads, self.head_dim, self.dtype, self.device, "q_out")
-            if q_out.shape[0] != rows or not q_out.is_contiguous():
-                raise ValueError(f"q_out must be {rows} contiguous rows")
-            qo = ctypes.c_void_p(q_out.data_ptr())
+                q_out = self._empty((rows, self.q_heads, d), dtype=self.dtype, device=self.device)
+                qo = q_out.data_ptr()
+            else:
+                qo = self._whole(q_out, rows, "q_out")
         if rotate is None:
             rotate = self.rope is not None
-        _check(lib().mpg_append(self._h, layer, rows, *ka, *va, *qa, qo, 1 if rotate else 0))
+        rc = self._lib.mpg_append(self._h, layer, rows, kp, kt, kh, vp, vt, vh, qp, qt, qh, qo, 1 if rotate else 0)
+        if rc:
+            _check(rc)
         return q_out
 
     def attend(self, layer, q, scale=None, sinks=None, gate=None, out=None):
         """Attention of the batch's tokens: q [tokens, q_heads, head_dim] -> out of the same shape. scale: 1/sqrt(head_dim)
         by default; sinks [q_heads] f32; gate as q: out = attention * sigmoid(gate)."""
-        import torch
-        qa = _rows(q, self.q_heads, self.head_dim, self.dtype, self.device, "q")
+        h, d, dtype, device = self.q_heads, self.head_dim, self.dtype, self.device
+        qp, qt, qh = _rows(q, h, d, dtype, device, "q")
         rows = q.shape[0]
         if out is None:
-            out = torch.empty((rows, self.q_heads, self.head_dim), dtype=self.dtype, device=self.device)
-        _rows(out, self.q_heads, self.head_dim, self.dtype, self.device, "out")
-        if out.shape[0] != rows or not out.is_contiguous():
-            raise ValueError(f"out must be {rows} contiguous rows")
-        ga, sp = (None, 0, 0), None
+            out = self._empty((rows, h, d), dtype=dtype, device=device)
+            op = out.data_ptr()
+        else:
+            op = self._whole(out, rows, "out")
+        gp, gt, gh, sp = None, 0, 0, None
         if gate is not None:
-            ga = _rows(gate, self.q_heads, self.head_dim, self.dtype, self.device, "gate")
+            gp, gt, gh = _rows(gate, h, d, dtype, device, "gate")
             if gate.shape[0] != rows:
                 raise ValueError("q and gate differ in rows")
         if sinks is not None:
-            if sinks.device != self.device or sinks.dtype != torch.float32 or sinks.shape != (self.q_heads,) \
-                    or not sinks.is_contiguous():
-                raise ValueError(f"sinks must be {self.q_heads} contiguous float32 on {self.device}")
-            sp = ctypes.c_void_p(sinks.data_ptr())
-        if scale is None:
-            scale = self.head_dim ** -0.5
-        _check(lib().mpg_attend(self._h, layer, rows, *qa, scale, sp, *ga, ctypes.c_void_p(out.data_ptr())))
+            if sinks.device != device or sinks.dtype is not self._float32 or sinks.shape != (h,) or not sinks.is_contiguous():
+                raise ValueError(f"sinks must be {h} contiguous float32 on {device}")
+            sp = sinks.data_ptr()
+        rc = self._lib.mpg_attend(self._h, layer, rows, qp, qt, qh, self._scale if scale is None else scale, sp, gp, gt, gh, op)
+        if rc:
+            _check(rc)
         return out

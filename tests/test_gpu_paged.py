@@ -644,5 +644,5 @@ def test_refusals(torch_gpu, pg):
         pg.rotate(x[..., :32], pos, rope)
     # at the C entry: in place with other strides
     lib, P = pg.lib(), ctypes.c_void_p
-    assert lib.mpg_rotate(ctypes.byref(rope.c), 1, 3, 2, 64, P(x.data_ptr()), 128, 64, P(pos.data_ptr()), P(x.data_ptr()), 64,
+    assert lib.mpg_rotate(rope._ptr, 1, 3, 2, 64, P(x.data_ptr()), 128, 64, P(pos.data_ptr()), P(x.data_ptr()), 64,
                           192, None) == -1

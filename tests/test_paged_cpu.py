@@ -107,9 +107,9 @@ def test_null_arguments():
                L.mpg_copy(None, 1, one, one), L.mpg_free(None, 1, one), L.mpg_compact(None, None),
                L.mpg_append(None, 0, 1, None, 0, 0, None, 0, 0, None, 0, 0, None, 0),
                L.mpg_attend(None, 0, 1, None, 0, 0, 1.0, None, None, 0, 0, None), L.mpg_read_rows(None, 0, 0, 0, 0, 1, None),
-               L.mpg_rope_freqs(None, None, None), L.mpg_rotate(None, 0, 1, 1, 64, None, 0, 0, None, None, 0, 0, None)):
+               L.mpg_rope_freqs(None, None, None), L.mpg_rope_turns(None, None), L.mpg_rotate(None, 0, 1, 1, 64, None, 0, 0, None, None, 0, 0, None)):
         assert rc == -1
-    r = paged.Rope(64).c
+    r = paged.Rope(64)._turns
     for args, want in [((0, 1, 1, 32), -1), ((5, 1, 1, 64), -1), ((0, -1, 1, 64), -1), ((0, 1, 70000, 64), -1),
                        ((0, 1, 1, 5000), -1), ((0, 1, 1, 64), -1), ((0, 0, 1, 64), 0)]:
         assert L.mpg_rotate(ctypes.byref(r), *args, None, 64, 64, None, None, 64, 64, None) == want
