@@ -64,7 +64,12 @@ __device__ inline int row_units(int dim, int rot, int layout) {
     if (!WIDE) return rot / 2 + dim - rot;
     return layout == MPG_HALF ? rot / 16 + (dim - rot) / 8 : dim / 8;
 }
-template <typename T, bool WIDE, typename To>
+template <bool STREAM, typename T>
+__device__ inline void put8(T* p, Vec8<T> x) {
+    if constexpr (STREAM) __builtin_nontemporal_store(x, (Vec8<T>*)p);
+    else store8(p, x);
+}
+template <typename T, bool WIDE, bool STREAM = false, typename To>
 __device__ inline void rotate_unit(const T* __restrict__ x, int u, int rot, int layout, const float2* cs, To to) {
     if constexpr (!WIDE) {
         if (u >= rot / 2) {
@@ -85,8 +90,8 @@ __device__ inline void rotate_unit(const T* __restrict__ x, int u, int rot, int 
             a[e] = (T)p;
             b[e] = (T)q;
         }
-        store8(to(8 * u), a);
-        store8(to(rot / 2 + 8 * u), b);
+        put8<STREAM>(to(8 * u), a);
+        put8<STREAM>(to(rot / 2 + 8 * u), b);
     } else {
         const int d = layout == MPG_HALF ? rot / 2 + 8 * u : 8 * u;
         Vec8<T> a = load8(x + d);
@@ -99,7 +104,7 @@ __device__ inline void rotate_unit(const T* __restrict__ x, int u, int rot, int 
                 a[e + 1] = (T)q;
             }
         }
-        store8(to(d), a);
+        put8<STREAM>(to(d), a);
     }
 }
 
@@ -131,21 +136,22 @@ struct Walk {
     }
 };
 
-constexpr int ROT_ROWS = 8;  // rows of a work-group: their angles are shared by the heads
+constexpr int ROT_ROWS = 4;  // rows of a work-group: their angles are shared by the heads
 // n rows of `heads` heads from x (row and head strides) to out, cs: their pairs
-template <typename T, bool WIDE>
+template <typename T, bool WIDE, bool STREAM = false>
 __device__ inline void rotate_rows(const RopeArgs& r, int n, int heads, int dim, const T* x, int64_t x_row, int64_t x_head,
                                    T* out, int64_t o_row, int64_t o_head, const float2* cs, int at, int by) {
     const int half = r.dim / 2;
     for (Walk w(at, by, heads, row_units<T, WIDE>(dim, r.dim, r.layout)); w.row < n; w.next()) {
         T* const o = out + w.row * o_row + w.head * o_head;
-        rotate_unit<T, WIDE>(x + w.row * x_row + w.head * x_head, w.unit, r.dim, r.layout, cs + w.row * half,
+        rotate_unit<T, WIDE, STREAM>(x + w.row * x_row + w.head * x_head, w.unit, r.dim, r.layout, cs + w.row * half,
                              [&](int d) { return o + d; });
     }
 }
 
-// Work-group = ROT_ROWS rows; where those are few, blockIdx.y shares out their heads.
-template <typename T, bool WIDE>
+// Work-group = ROT_ROWS rows; where those are few, blockIdx.y shares out their heads. STREAM: outputs that the L2s cannot
+// hold anyway are stored past them (8,192 rows of 32 heads of 128 in bf16, 134 MB moved: 28.8 -> 22.5 us).
+template <typename T, bool WIDE, bool STREAM>
 __global__ void __launch_bounds__(256) rotate_kernel(RopeArgs r, int rows, int heads, int dim, const T* x, int64_t x_row,
                                                      int64_t x_head, const int* __restrict__ pos, T* out, int64_t o_row,
                                                      int64_t o_head) {
@@ -153,15 +159,16 @@ __global__ void __launch_bounds__(256) rotate_kernel(RopeArgs r, int rows, int h
     const int row0 = blockIdx.x * ROT_ROWS, n = min(ROT_ROWS, rows - row0), half = r.dim / 2;
     for (Walk w(threadIdx.x, 256, 1, half); w.row < n; w.next()) cs[w.row * half + w.unit] = turn(r, pos[row0 + w.row], w.unit);
     __syncthreads();
-    rotate_rows<T, WIDE>(r, n, heads, dim, x + row0 * x_row, x_row, x_head, out + row0 * o_row, o_row, o_head, cs,
+    rotate_rows<T, WIDE, STREAM>(r, n, heads, dim, x + row0 * x_row, x_row, x_head, out + row0 * o_row, o_row, o_head, cs,
                          threadIdx.x + 256 * blockIdx.y, 256 * gridDim.y);
 }
 
 // ---- append ----
-// For a run of new tokens inside one 32-position block of a page: work-groups y = 0 .. 3 rotate the query heads of 8 tokens
-// each; the last one takes the run's K and V. K rows are rotated into LDS and leave in the pages' order, 16 positions side
-// by side. A V block that is all new is turned in registers (8 positions of 8 dims a thread) and written in 16-byte
-// pieces, others element by element.
+// For a run of new tokens inside one 32-position block of a page: work-groups y < kv_heads take a head's K and V, those
+// behind them the query heads of 4 tokens each. K rows are rotated into LDS and leave in the pages' order, 16 positions
+// side by side. A V block that is all new is turned in registers (8 positions of 8 dims a thread) and written in 16-byte
+// pieces, others element by element. Bound by memory: 4,096 + 2,500 + 1,031 + 565 tokens of 32 + 2 x 4 heads of 128 move
+// 168 MB in 35.4 us (44.2 with the K and V of a run in one work-group behind its query heads, 37.5 with K and V apart).
 constexpr int Q_PARTS = KEYS / ROT_ROWS;
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) append_kernel(const Run* __restrict__ runs, const int* __restrict__ nruns,
@@ -176,8 +183,8 @@ __global__ void __launch_bounds__(256) append_kernel(const Run* __restrict__ run
         const Uniform<int> ri = uniform((const int*)(runs + i));
         Run run{ri[0], ri[1], ri[2], ri[3]};
         run.count = min(run.count, rows - run.tok);
-        if (blockIdx.y < gridDim.y - 1) {  // query heads
-            const int t0 = blockIdx.y * ROT_ROWS, n = min(ROT_ROWS, run.count - t0);
+        if ((int)blockIdx.y >= kv_heads) {  // query heads
+            const int t0 = (blockIdx.y - kv_heads) * ROT_ROWS, n = min(ROT_ROWS, run.count - t0);
             if (n <= 0) continue;
             __syncthreads();  // the angles before have been read
             for (Walk w(tid, 256, 1, half); w.row < n; w.next())
@@ -190,48 +197,45 @@ __global__ void __launch_bounds__(256) append_kernel(const Run* __restrict__ run
         }
         if (run.count <= 0) continue;
         const size_t p = uniform(table)[(size_t)run.seq * most_pages + run.pos / page];
-        const int in = run.pos % page, at = in % KEYS, stride = dim + 8;
+        const int in = run.pos % page, at = in % KEYS, chunks = dim / 8, head = blockIdx.y, stride = dim + 8;
+        const size_t base = (p * kv_heads + head) * page * dim + (size_t)(in / KEYS) * KEYS * dim;  // of the 32-position block
         T* const kt = (T*)(cs + KEYS * half);
         __syncthreads();  // what stood in LDS has been read
         if (half > 0)
             for (Walk w(tid, 256, 1, half); w.row < run.count; w.next())
                 cs[w.row * half + w.unit] = turn(r, run.pos + w.row, w.unit);
-        const int units = row_units<T, WIDE>(dim, r.dim, r.layout), chunks = dim / 8;
-        for (int head = 0; head < kv_heads; head++) {
-            __syncthreads();
-            const T* const ks = k + run.tok * k_tok + head * k_head;
-            for (Walk w(tid, 256, 1, units); w.row < run.count; w.next()) {
-                T* const o = kt + w.row * stride;
-                rotate_unit<T, WIDE>(ks + w.row * k_tok, w.unit, r.dim, r.layout, cs + w.row * half, [&](int d) { return o + d; });
+        __syncthreads();
+        const T* const ks = k + run.tok * k_tok + head * k_head;
+        for (Walk w(tid, 256, 1, row_units<T, WIDE>(dim, r.dim, r.layout)); w.row < run.count; w.next()) {
+            T* const o = kt + w.row * stride;
+            rotate_unit<T, WIDE>(ks + w.row * k_tok, w.unit, r.dim, r.layout, cs + w.row * half, [&](int d) { return o + d; });
+        }
+        __syncthreads();
+        T* const kb = kpool + base;
+        for (int j = tid; j < KEYS * chunks; j += 256) {  // 16-byte pieces in the pages' order
+            const int pos = j % 16 + j / (16 * chunks) * 16, t = pos - at;
+            if (t >= 0 && t < run.count) store8(kb + j * 8, load8(kt + t * stride + j / 16 % chunks * 8));
+        }
+        const T* const vs = v + run.tok * v_tok + head * v_head;
+        T* const vb = vpool + base;
+        if (run.count == KEYS) {
+            for (int j = tid; j < dim / 2; j += 256) {  // (group of 8 positions, 8 dims)
+                const int g = j / chunks, d = j % chunks * 8;
+                Vec8<T> x[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = load8(vs + (16 * (e / 4) + 4 * g + e % 4) * v_tok + d);
+#pragma unroll
+                for (int c = 0; c < 8; c++)
+                    store8(vb + (g * dim + d + c) * 8,
+                           Vec8<T>{x[0][c], x[1][c], x[2][c], x[3][c], x[4][c], x[5][c], x[6][c], x[7][c]});
             }
-            __syncthreads();
-            const size_t base = (p * kv_heads + head) * page * dim + (size_t)(in / KEYS) * KEYS * dim;  // of the 32-position block
-            T* const kb = kpool + base;
-            for (int j = tid; j < KEYS * chunks; j += 256) {  // 16-byte pieces in the pages' order
-                const int pos = j % 16 + j / (16 * chunks) * 16, t = pos - at;
-                if (t >= 0 && t < run.count) store8(kb + j * 8, load8(kt + t * stride + j / 16 % chunks * 8));
-            }
-            const T* const vs = v + run.tok * v_tok + head * v_head;
-            T* const vb = vpool + base;
-            if (run.count == KEYS) {
-                for (int j = tid; j < dim / 2; j += 256) {  // (group of 8 positions, 8 dims)
-                    const int g = j / chunks, d = j % chunks * 8;
-                    Vec8<T> x[8];
+        } else {
+            for (Walk w(tid, 256, 1, chunks); w.row < run.count; w.next()) {
+                const int d = w.unit * 8, b = at + w.row;
+                const Vec8<T> x = load8(vs + w.row * v_tok + d);
+                T* const o = vb + (b % 16 / 4 * dim + d) * 8 + b / 16 * 4 + b % 4;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = load8(vs + (16 * (e / 4) + 4 * g + e % 4) * v_tok + d);
-#pragma unroll
-                    for (int c = 0; c < 8; c++)
-                        store8(vb + (g * dim + d + c) * 8,
-                               Vec8<T>{x[0][c], x[1][c], x[2][c], x[3][c], x[4][c], x[5][c], x[6][c], x[7][c]});
-                }
-            } else {
-                for (Walk w(tid, 256, 1, chunks); w.row < run.count; w.next()) {
-                    const int d = w.unit * 8, b = at + w.row;
-                    const Vec8<T> x = load8(vs + w.row * v_tok + d);
-                    T* const o = vb + (b % 16 / 4 * dim + d) * 8 + b / 16 * 4 + b % 4;
-#pragma unroll
-                    for (int c = 0; c < 8; c++) o[c * 8] = x[c];
-                }
+                for (int c = 0; c < 8; c++) o[c * 8] = x[c];
             }
         }
     }
@@ -265,7 +269,7 @@ hipError_t append_as(const Geometry& g, char* pool, int layer, const int* table,
     T* const kp = (T*)pool + (size_t)layer * 2 * g.plane_elems();
     const size_t lds = (size_t)KEYS * (r.dim / 2) * sizeof(float2) + (size_t)KEYS * (g.head_dim + 8) * sizeof(T);
     const auto kernel = r.dim % 16 ? append_kernel<T, false> : append_kernel<T, true>;
-    kernel<<<dim3(grid, q.p ? Q_PARTS + 1 : 1), dim3(256), lds, s>>>(
+    kernel<<<dim3(grid, g.kv_heads + (q.p ? Q_PARTS : 0)), dim3(256), lds, s>>>(
         runs, nruns, table, g.most_pages, g.page, g.head_dim, g.kv_heads, g.q_heads, kp, kp + g.plane_elems(), rows,
         (const T*)k.p, k.tok, k.head, (const T*)v.p, v.tok, v.head, (const T*)q.p, q.tok, q.head, (T*)q_out, r);
     return hipGetLastError();
@@ -277,7 +281,9 @@ hipError_t rotate_as(const RopeArgs& r, int rows, int heads, int dim, const Rows
     const bool wide = r.dim % 16 == 0 && dim % 8 == 0 && x.tok % 8 == 0 && x.head % 8 == 0 && out.tok % 8 == 0 &&
                       out.head % 8 == 0 && (uintptr_t)x.p % 16 == 0 && (uintptr_t)out.p % 16 == 0;
     const size_t lds = (size_t)ROT_ROWS * (r.dim / 2) * sizeof(float2);
-    const auto kernel = wide ? rotate_kernel<T, true> : rotate_kernel<T, false>;
+    constexpr size_t L2 = 32 << 20;  // of the eight dies together
+    const bool stream = (size_t)rows * heads * dim * sizeof(T) > L2;
+    const auto kernel = !wide ? rotate_kernel<T, false, false> : stream ? rotate_kernel<T, true, true> : rotate_kernel<T, true, false>;
     const int groups = (rows + ROT_ROWS - 1) / ROT_ROWS, n = rows < ROT_ROWS ? rows : ROT_ROWS;
     // few rows of many heads: heads shared out, a unit or two a thread
     const int y = groups >= 256 ? 1 : std::max(1, std::min(256 / groups, n * heads * (dim / 16) / 512));
