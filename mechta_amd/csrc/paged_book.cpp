@@ -267,19 +267,29 @@ long long shortest(const std::vector<Tile>& tiles, int kv_heads, int places) {
     return lo;
 }
 
-// Few rows: tiles that are more than the CUs are cut where they are longer than a CU's share, others into as many pieces as
-// stream fastest.
+// Few rows: as many pieces as stream fastest, unless that leaves one much longer than a CU's share of the keys: then, and
+// where the tiles are more than the CUs, pieces of three quarters of a share, dealt out as CUs fall free. (A token each of
+// sequences at 500 .. 8,001 positions, 4 x 128, 64 of them: as many pieces as CUs 85 us, pieces of 1/2, 3/4, 1, 3/2 and 2
+// shares 65 / 63 / 66 / 68 / 76; 50 of them 73 and 56 / 54 / 57 / 59 / 58; 30 of them, where the longest piece is 1.6 shares
+// of 1,147 keys, 32 and 35 for 3/4; 64 at 2,000 .. 4,000, the longest 1.4 of 2,858, 66 and 68.)
 long long few_length(const std::vector<Tile>& tiles, int kv_heads) {
     const long long whole = (long long)tiles.size() * kv_heads;
-    if (whole > CUS) {
-        long long keys = 0;
-        for (const Tile& t : tiles) keys += (long long)(t.k1 - t.k0) * kv_heads;
-        return std::max<long long>(LEAST_KEYS, (keys + CUS - 1) / CUS) / KEYS;
-    }
-    const long long length = shortest(tiles, kv_heads, whole <= STREAMS ? STREAMS : CUS);
-    long long n = 0;
-    for (const Tile& t : tiles) n += (long long)pieces_of(t, length) * kv_heads;
-    return n < STREAMS * 3 / 4 ? shortest(tiles, kv_heads, CUS) : length;
+    long long keys = 0, n = 0, longest = 0;
+    for (const Tile& t : tiles) keys += (long long)(t.k1 - t.k0) * kv_heads;
+    const long long share = (keys + CUS - 1) / CUS, dealt = std::max<long long>(LEAST_KEYS, share * 3 / 4) / KEYS;
+    if (whole > CUS) return dealt;
+    auto count = [&](long long length) {
+        n = longest = 0;
+        for (const Tile& t : tiles) {
+            const int p = pieces_of(t, length);
+            n += (long long)p * kv_heads;
+            longest = std::max<long long>(longest, (t.k1 - t.k0 + p - 1) / p);
+        }
+    };
+    long long length = shortest(tiles, kv_heads, whole <= STREAMS ? STREAMS : CUS);
+    count(length);
+    if (n < STREAMS * 3 / 4) count(length = shortest(tiles, kv_heads, CUS));
+    return longest * 5 > share * 7 + 5 * 512 ? dealt : length;
 }
 
 // Chunks: the cheapest length of a piece by a model of the call in us: a piece's keys, 9 for its beginning and end, the split
