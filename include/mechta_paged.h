@@ -108,6 +108,7 @@ size_t mpg_bytes(const mpg_config* c);
  * stream: a hipStream_t (NULL = the default stream). */
 int mpg_create(mpg_t** out, const mpg_config* c, const int* windows, const mpg_rope* rope, void* stream);
 int mpg_destroy(mpg_t* h);
+/* Calls from here on go to `stream`; that it comes after what the handle has on its stream before is the caller's to see to. */
 int mpg_set_stream(mpg_t* h, void* stream);
 int mpg_sync(mpg_t* h);
 
@@ -144,7 +145,7 @@ int mpg_compact(mpg_t* h, int* moved);
  *   k, v: element (token, kv head, d) at token x *_tok + head x *_head + d (device; 16-byte aligned, strides multiples
  *         of 8 elements, so k and v may be parts of one projection's rows);
  *   q:    the same for the q_heads query heads, or NULL; q_out: [tokens][q_heads][head_dim] (device; it may be q, with
- *         those strides).
+ *         those strides, and overlap the arguments in no other way).
  * rotate != 0: K and q are rotated at their tokens' positions by the handle's rope (refused if it has none); 0: K is
  * stored as it is (rows that are rotated already) and q must be NULL. */
 int mpg_append(mpg_t* h, int layer, int rows, const void* k, int64_t k_tok, int64_t k_head, const void* v, int64_t v_tok,
@@ -155,7 +156,7 @@ int mpg_append(mpg_t* h, int layer, int rows, const void* k, int64_t k_tok, int6
  *   q:     as mpg_append's; scale > 0: scores are scale q.k;
  *   sinks: NULL, or f32 [q_heads] (device): a logit that joins the softmax's sum but no value;
  *   gate:  NULL, or elements as q's with its own strides: out = attention x sigmoid(gate);
- *   out:   [tokens][q_heads][head_dim] (device), 16-byte aligned.
+ *   out:   [tokens][q_heads][head_dim] (device), 16-byte aligned; it overlaps no argument.
  * Sums and softmax in f32; the weights are rounded to the cache's type for the matrix units. What stands in positions a
  * token does not see, NaN and infinities included, has no effect on it. */
 int mpg_attend(mpg_t* h, int layer, int rows, const void* q, int64_t q_tok, int64_t q_head, float scale, const float* sinks,

@@ -362,14 +362,15 @@ void plan_window(const Shape& g, const std::vector<Member>& batch, int window, P
     for (const auto& v : by_kind) tiles.insert(tiles.end(), v.begin(), v.end());
     long long most[KINDS];
     for (int k = 0; k < KINDS; k++) most[k] = length[k] * KEYS;
-    int part = 0;
+    int part = 0, more = 0;  // partials and work items that splits have taken
     for (const Tile& t : tiles) {
         const Member& m = batch[t.member];
         const int rows = m.count * group, count = std::min(TILE_ROWS[t.kind], rows - t.row0);
         const int units = (t.k1 - t.k0 + KEYS - 1) / KEYS;
         int splits = (int)((units + most[t.kind] / KEYS - 1) / (most[t.kind] / KEYS));
-        splits = std::min(splits, (PART_ROWS - part) / (count * g.kv_heads));
+        splits = std::min({splits, (PART_ROWS - part) / (count * g.kv_heads), 1 + (SPLITS_MOST - more) / g.kv_heads});
         if (splits < 2) splits = 1;
+        more += (splits - 1) * g.kv_heads;
         for (int head = 0; head < g.kv_heads; head++) {
             for (int s = 0; s < splits; s++) {
                 const int a = t.k0 + (int)((long long)units * s / splits) * KEYS;

@@ -18,15 +18,15 @@ __global__ void __launch_bounds__(256) apply_kernel(int* __restrict__ dev, const
 
 // ---- page copies: every plane (layer, K|V) of a list of pages. Sources and destinations of a launch are different
 // pages. A work-group moves 4 KB of one plane's page (the least page of the least shape), 16 bytes a thread, past the L2:
-// 256 pages of 1.3 MB in 104 us, 6.4 TB/s; with 2, 4, 8 units in flight a thread 111, 115 and 118 us, through the L2 121.
+// 256 pages of 1.3 MB in 105 us, 6.4 TB/s (with 2, 4, 8 units in flight a thread 112, 116 and 119, through the L2 122).
 constexpr int PAIRS = 256;  // of a launch, in its arguments
 struct PairList {
     Pair p[PAIRS];
 };
 __global__ void __launch_bounds__(256) copy_kernel(char* __restrict__ pool, PairList list, unsigned per_page,
-                                                   unsigned planes, size_t page_bytes, size_t plane_bytes) {
-    const unsigned at = blockIdx.x % per_page, rest = blockIdx.x / per_page, plane = rest % planes, pair = rest / planes;
-    char* const p = pool + plane * plane_bytes + (size_t)at * 4096 + threadIdx.x * 16;
+                                                   size_t page_bytes, size_t plane_bytes) {
+    const unsigned at = blockIdx.x % per_page, pair = blockIdx.x / per_page;
+    char* const p = pool + blockIdx.y * plane_bytes + (size_t)at * 4096 + threadIdx.x * 16;
     const u32x4 x = __builtin_nontemporal_load((const u32x4*)(p + list.p[pair].src * page_bytes));
     __builtin_nontemporal_store(x, (u32x4*)(p + list.p[pair].dst * page_bytes));
 }
@@ -291,16 +291,13 @@ hipError_t launch_apply(int* dev, const unsigned* stage, int segments, hipStream
 
 hipError_t launch_copies(const Geometry& g, char* pool, const Pair* pairs, int n, hipStream_t s) {
     const size_t page = g.page_elems() * 2;
-    const unsigned planes = 2 * g.layers, per_page = (unsigned)(page / 4096);
-    // pairs of a launch: in its arguments, its work-groups counted in 31 bits
-    const int most = (int)std::max<size_t>(1, std::min<size_t>(PAIRS, (1ull << 31) / ((size_t)planes * per_page)));
-    for (int i = 0; i < n; i += most) {
+    const unsigned per_page = (unsigned)(page / 4096);
+    for (int i = 0; i < n; i += PAIRS) {
         PairList list;
-        const int m = std::min(most, n - i);
+        const int m = std::min(PAIRS, n - i);
         std::copy(pairs + i, pairs + i + m, list.p);
         std::fill(list.p + m, list.p + PAIRS, Pair{0, 0});
-        copy_kernel<<<dim3((unsigned)m * planes * per_page), dim3(256), 0, s>>>(pool, list, per_page, planes, page,
-                                                                               g.plane_elems() * 2);
+        copy_kernel<<<dim3(m * per_page, 2 * g.layers), dim3(256), 0, s>>>(pool, list, per_page, page, g.plane_elems() * 2);
         if (const hipError_t e = hipGetLastError()) return e;
     }
     return hipSuccess;
@@ -313,21 +310,36 @@ hipError_t launch_append(const Geometry& g, char* pool, int layer, const int* ta
                             : append_as<__bf16>(g, pool, layer, table, runs, nruns, grid, rows, k, v, q, q_out, rope, s);
 }
 
+// A launch takes less than 2^32 threads: what needs more goes in several.
 hipError_t launch_read(const Geometry& g, const char* pool, int layer, int which, const int* table, int p0, int p1, void* dst,
                        hipStream_t s) {
-    const size_t threads = (size_t)(p1 - p0) * g.kv_heads * g.head_dim / 8;
+    const size_t per = (size_t)g.kv_heads * g.head_dim / 8;  // threads of a position
     const char* const base = pool + ((size_t)layer * 2 + which) * g.plane_elems() * 2;
-    // both types are 16 bits that are only moved
-    read_kernel<_Float16><<<dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s>>>(
-        (const _Float16*)base, table, g.page, g.kv_heads, g.head_dim, which == MKV_V, p0, p1, (_Float16*)dst);
-    return hipGetLastError();
+    const int most = (int)std::min<size_t>((1ull << 31) / per, MPG_CTX_MAX);
+    for (int p = p0; p < p1; p += most) {
+        const int e = std::min(p + most, p1);
+        // both types are 16 bits that are only moved
+        read_kernel<_Float16><<<dim3((unsigned)((per * (e - p) + 255) / 256)), dim3(256), 0, s>>>(
+            (const _Float16*)base, table, g.page, g.kv_heads, g.head_dim, which == MKV_V, p, e,
+            (_Float16*)dst + (size_t)(p - p0) * per * 8);
+        if (const hipError_t err = hipGetLastError()) return err;
+    }
+    return hipSuccess;
 }
 
 hipError_t launch_rotate(const RopeArgs& r, int fmt, int rows, int heads, int dim, const Rows& x, const int* pos,
                          const Rows& out, hipStream_t s) {
-    return fmt == MKV_F16   ? rotate_as<_Float16>(r, rows, heads, dim, x, pos, out, s)
-           : fmt == MKV_F32 ? rotate_as<float>(r, rows, heads, dim, x, pos, out, s)
-                            : rotate_as<__bf16>(r, rows, heads, dim, x, pos, out, s);
+    constexpr int MOST = 1 << 25;  // a work-group of 256 threads for ROT_ROWS of them
+    const int bytes = fmt == MKV_F32 ? 4 : 2;
+    for (int64_t i = 0; i < rows; i += MOST) {
+        const int n = (int)std::min<int64_t>(MOST, rows - i);
+        const Rows xi{(const char*)x.p + i * x.tok * bytes, x.tok, x.head}, oi{(const char*)out.p + i * out.tok * bytes, out.tok, out.head};
+        const hipError_t e = fmt == MKV_F16   ? rotate_as<_Float16>(r, n, heads, dim, xi, pos + i, oi, s)
+                             : fmt == MKV_F32 ? rotate_as<float>(r, n, heads, dim, xi, pos + i, oi, s)
+                                              : rotate_as<__bf16>(r, n, heads, dim, xi, pos + i, oi, s);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace paged

@@ -22,7 +22,8 @@ using namespace mkv::paged;
 
 namespace {
 constexpr int RING = 4;           // staged uploads in flight
-constexpr int GRAPH_GRID = 512;   // work-groups of a captured kernel, which loop over the lists they find
+constexpr int GRAPH_GRID = 512;   // work-groups of a captured kernel; all loop over the lists they find
+constexpr int MOST_GRID = 1 << 20;  // of an eager one: a launch takes less than 2^32 threads
 constexpr unsigned SEG = 2048;    // words of an upload's segment at most: one work-group's share
 }  // namespace
 
@@ -81,6 +82,8 @@ int check_config(const char* who, const mpg_config* c) {
         return fail(MKV_E_ARG, "%s: batches of %d tokens outside [1, %d]", who, c->tokens, MPG_TOKENS_MAX);
     const size_t table = (size_t)c->seqs * ((c->ctx + c->page - 1) / c->page);
     if (table > 1u << 30) return fail(MKV_E_ARG, "%s: page tables of %zu entries", who, table);
+    const double pool = 4. * c->layers * c->pages * c->kv_heads * c->page * c->head_dim;
+    if (pool > 1ll << 48) return fail(MKV_E_NOMEM, "%s: a pool of %g bytes", who, pool);
     return MKV_OK;
 }
 
@@ -380,6 +383,8 @@ static int create(mpg_t** out, const mpg_config* c, const int* windows, const mp
     h->batch_at = s.table + COUNTS + (size_t)c->tokens * (sizeof(Run) / 4);
     h->words = s.words;
     h->book.init(c->pages, c->page, c->seqs, c->ctx);
+    if (const int cap = capturing(h, "mpg_create"))
+        return cap < 0 ? cap : fail(MKV_E_ARG, "mpg_create: the stream is capturing");
     hipError_t e = s.words < 1ull << 32 ? hipGetDevice(&h->device) : hipErrorOutOfMemory;
     if (e == hipSuccess) e = hipMalloc((void**)&h->pool, s.pool);
     if (e == hipSuccess) e = hipMalloc((void**)&h->dev, s.words * 4);
@@ -605,6 +610,7 @@ int mpg_attend(mpg_t* h, int layer, int rows, const void* q, int64_t q_tok, int6
     if (int rc = check_rows("mpg_attend", "out", out, 0, 0)) return rc;
     if (gate)
         if (int rc = check_rows("mpg_attend", "gate", gate, g_tok, g_head)) return rc;
+    if (out == q || out == gate) return fail(MKV_E_ARG, "mpg_attend: out takes the place of an input");
     if (!(scale > 0) || !std::isfinite(scale)) return fail(MKV_E_ARG, "mpg_attend: scale %g", scale);
     if ((uintptr_t)sinks % 4) return fail(MKV_E_ARG, "mpg_attend: misaligned sinks");
     OnDevice on(h->device);
@@ -629,9 +635,9 @@ int mpg_attend(mpg_t* h, int layer, int rows, const void* q, int64_t q_tok, int6
     a.joins = &p.joins;
     a.captured = cap != 0;
     int grid[KINDS];
-    for (int k = 0; k < KINDS; k++) grid[k] = cap ? GRAPH_GRID : (int)p.items[k].size();
+    for (int k = 0; k < KINDS; k++) grid[k] = cap ? GRAPH_GRID : (int)std::min<size_t>(p.items[k].size(), MOST_GRID);
     const hipError_t e = launch_attend(h->g, a, h->dev + h->batch_at + w * h->lists.words, h->lists, grid,
-                                       cap ? GRAPH_GRID : (int)p.joins.size(), h->stream);
+                                       cap ? GRAPH_GRID : (int)std::min<size_t>(p.joins.size(), MOST_GRID), h->stream);
     return e == hipSuccess ? MKV_OK : hip_fail(e, "mpg_attend");
 }
 

@@ -161,7 +161,7 @@ def rotate(x, pos, rope, out=None):
     op, orow, oh = _rows(out, heads, dim, dtype, device, "out")
     if pos.device != device or pos.dtype is not torch.int32 or pos.shape != shape[:1] or not pos.is_contiguous():
         raise ValueError(f"pos must be {rows} contiguous int32 on {device}")
-    stream = torch.cuda.current_stream(device).cuda_stream
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
     if torch.cuda.current_device() == device.index:
         rc = lib().mpg_rotate(rope._ptr, fmt, rows, heads, dim, xp, xr, xh, pos.data_ptr(), op, orow, oh, stream)
     else:
@@ -194,7 +194,7 @@ class PagedKv:
     """The paged cache of `layers` layers: `pages` pages of `page` positions for up to `seqs` sequences of up to `ctx`
     positions; batches of up to `tokens` new tokens. fmt: F16 or BF16 (pages, q, k, v, gate, out). windows: per layer the
     positions a token sees, itself included (0 or None: all). rope: what append() rotates by. Calls are ordered on
-    `stream` (default: torch's current stream).
+    `stream` (default: torch's current stream); where torch works on another one, the caller orders the two.
 
         kv.begin([0, 3], [1, 512])            # one new token for sequence 0, 512 for sequence 3
         for layer in range(layers):
@@ -219,6 +219,7 @@ class PagedKv:
         self.dtype = _dtype(fmt)
         self._views = {}
         self._lib, self._empty, self._float32, self._scale = lib(), torch.empty, torch.float32, head_dim ** -0.5
+        self._raw, self._now = s.cuda_stream, torch._C._cuda_getCurrentRawStream  # (a torch stream object costs 2 us a call)
 
     def close(self):
         """Frees the cache's memory now (tensors that pages() gave must not be used any more); without it, it is freed with
@@ -240,8 +241,8 @@ class PagedKv:
     def set_stream(self, stream):
         if stream.device != self.device:
             raise ValueError(f"the stream is on {stream.device}, the cache on {self.device}")
-        self._stream = stream
         _check(lib().mpg_set_stream(self._h, ctypes.c_void_p(stream.cuda_stream)))
+        self._stream, self._raw = stream, stream.cuda_stream
 
     def sync(self):
         _check(lib().mpg_sync(self._h))
@@ -303,8 +304,9 @@ class PagedKv:
     def pages(self, layer, which):
         """A layer's K or V pages as a tensor over the pool: K [page][kv head][pos/16][d/8][16][8], V [page][kv head]
         [pos/32][4][d][8] (element e of group g of V: position 16 (e/4) + 4 g + e%4 of its 32)."""
-        import torch
-        if (layer, which) not in self._views:
+        view = self._views.get((layer, which))
+        if view is None:
+            import torch
             base = ctypes.c_void_p()
             _check(lib().mpg_pages(self._h, layer, which, ctypes.byref(base)))
             h, p, d = self.kv_heads, self.page, self.head_dim
@@ -314,17 +316,16 @@ class PagedKv:
                 owner = self._owner
                 __cuda_array_interface__ = {"shape": shape, "typestr": "<i2", "data": (base.value, False), "version": 2}
 
-            self._views[layer, which] = torch.as_tensor(_Mem(), device=self.device).view(self.dtype)
-        return self._views[layer, which]
+            view = self._views[layer, which] = torch.as_tensor(_Mem(), device=self.device).view(self.dtype)
+        return view
 
     def read_rows(self, layer, which, seq, p0=0, p1=None, out=None):
         """Positions [p0, p1) of a sequence's K or V, [p1 - p0, kv_heads, head_dim]."""
-        import torch
         if p1 is None:
             p1 = self.length(seq)
         n = max(0, p1 - p0)
         if out is None:
-            out = torch.empty((n, self.kv_heads, self.head_dim), dtype=self.dtype, device=self.device)
+            out = self._new(n, self.kv_heads, self.head_dim)
         _rows(out, self.kv_heads, self.head_dim, self.dtype, self.device, "out")
         if out.shape[0] != n or not out.is_contiguous():
             raise ValueError(f"out must be {n} contiguous rows")
@@ -332,6 +333,18 @@ class PagedKv:
         return out
 
     # ---- the layers' calls ----
+
+    def _new(self, *shape):
+        """An output. Where torch's current stream is another than the cache's, memory that is free on the former may still
+        be in use on the latter, and the other way round: it comes from the cache's stream and is held for both."""
+        if self._now(self.device.index) == self._raw:
+            return self._empty(shape, dtype=self.dtype, device=self.device)
+        import torch
+        now = torch.cuda.current_stream(self.device)
+        with torch.cuda.stream(self._stream):
+            out = self._empty(shape, dtype=self.dtype, device=self.device)
+        out.record_stream(now)
+        return out
 
     def _whole(self, t, rows, what):
         """The address of a contiguous [rows, q_heads, head_dim] tensor that takes an output."""
@@ -352,7 +365,7 @@ class PagedKv:
         if q is not None:
             qp, qt, qh = _rows(q, self.q_heads, d, self.dtype, self.device, "q")
             if q_out is None:
-                q_out = self._empty((rows, self.q_heads, d), dtype=self.dtype, device=self.device)
+                q_out = self._new(rows, self.q_heads, d)
                 qo = q_out.data_ptr()
             else:
                 qo = self._whole(q_out, rows, "q_out")
@@ -370,7 +383,7 @@ class PagedKv:
         qp, qt, qh = _rows(q, h, d, dtype, device, "q")
         rows = q.shape[0]
         if out is None:
-            out = self._empty((rows, h, d), dtype=dtype, device=device)
+            out = self._new(rows, h, d)
             op = out.data_ptr()
         else:
             op = self._whole(out, rows, "out")

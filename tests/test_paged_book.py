@@ -7,6 +7,8 @@ import subprocess
 
 import pytest
 
+from tests.paged_shapes import SHAPES, UNEVEN
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 ARG, POS, NOMEM = -1, -3, -7
 
@@ -272,3 +274,30 @@ def test_a_plan_covers_every_score_once(shim, seed):
     used.sort()
     assert all(a[1] <= b[0] for a, b in zip(used, used[1:]))
     assert not used or (used[0][0] >= 0 and used[-1][1] <= shim.shim_part_rows())
+
+
+@pytest.mark.parametrize("name", SHAPES)
+def test_shapes_go_to_their_kernels(shim, name):
+    dim, kv, group, window, batch, kind, split = SHAPES[name]
+    items, joins = make_plan(shim, kv * group, kv, dim, [(s, *m) for s, m in enumerate(batch)], window)
+    assert items[kind] and any(i[8] >= 0 for i in items[kind]) == split
+
+
+def test_uneven_sequences_are_shared_out(shim):
+    """A piece is never much longer than a CU's share of all keys."""
+    for kv, batch in [(4, UNEVEN), (2, UNEVEN + UNEVEN[:40]), (8, UNEVEN[:20])]:
+        items, _ = make_plan(shim, kv * 4, kv, 128, [(s, *m) for s, m in enumerate(batch)], 0)
+        share = sum(n for _, n in batch) * kv / 256
+        assert max(i[7] - i[6] for i in items[0]) <= 1.4 * share + 512 + 32
+
+
+def test_splits_stay_inside_their_room(shim):
+    """Batches whose splits ask for the most: many long keys behind few rows of many heads."""
+    for kv, group, batch in [(8, 16, [(1, 4000000)] * 3), (64, 1, [(33, 1000000)] * 40), (1, 33, [(1, 4194304)] * 64),
+                             (1, 1, [(33, 100000), (17, 3000000), (1, 2000000)] * 30), (255, 1, [(1, 100 * i) for i in range(1, 9)])]:
+        batch = [(s, *m) for s, m in enumerate(batch)]
+        items, joins = make_plan(shim, kv * group, kv, 64, batch, 0)
+        tokens = sum(c for _, c, _ in batch)
+        assert sum(map(len, items)) <= shim.shim_most_items(kv * group, kv, 64, tokens, len(batch))
+        assert len(joins) <= shim.shim_most_joins(kv * group, kv, 64, tokens, len(batch))
+        assert all(j[4] + j[3] * j[5] <= shim.shim_part_rows() for j in joins)

@@ -113,3 +113,26 @@ def test_null_arguments():
     for args, want in [((0, 1, 1, 32), -1), ((5, 1, 1, 64), -1), ((0, -1, 1, 64), -1), ((0, 1, 70000, 64), -1),
                        ((0, 1, 1, 5000), -1), ((0, 1, 1, 64), -1), ((0, 0, 1, 64), 0)]:
         assert L.mpg_rotate(ctypes.byref(r), *args, None, 64, 64, None, None, 64, 64, None) == want
+
+
+def test_a_pool_past_any_memory_is_refused():
+    L = paged.lib()
+    c = config(layers=4096, q_heads=1024, kv_heads=1024, head_dim=256, page=256, pages=1 << 27)
+    h = ctypes.c_void_p()
+    assert L.mpg_bytes(ctypes.byref(c)) == 0
+    assert L.mpg_create(ctypes.byref(h), ctypes.byref(c), None, None, None) == -7 and not h
+
+
+def test_rotate_refuses_turns_that_are_none():
+    L = paged.lib()
+    for dim, layout in [(0, 0), (3, 0), (514, 0), (-2, 0), (64, 2), (64, -1)]:
+        t = paged._Turns()
+        t.dim, t.layout = dim, layout
+        assert L.mpg_rotate(ctypes.byref(t), 0, 1, 1, 512, 16, 512, 512, 16, 16, 512, 512, None) == -1
+    t = paged._Turns()
+    t.dim = 64
+    for fmt, rows, heads, dim in [(3, 1, 1, 64), (0, -1, 1, 64), (0, 1, -1, 64), (0, 1, 65537, 64), (0, 1, 1, 62), (0, 1, 1, 4098)]:
+        assert L.mpg_rotate(ctypes.byref(t), fmt, rows, heads, dim, 16, 512, 512, 16, 16, 512, 512, None) == -1
+    assert L.mpg_rotate(ctypes.byref(t), 0, 1, 1, 64, 17, 64, 64, 16, 16, 64, 64, None) == -1  # misaligned
+    assert L.mpg_rotate(ctypes.byref(t), 0, 1, 1, 64, 16, 64, 64, 16, 16, 128, 64, None) == -1  # in place, other strides
+    assert L.mpg_rotate(ctypes.byref(t), 0, 0, 1, 64, None, 64, 64, None, None, 64, 64, None) == 0
