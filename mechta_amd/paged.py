@@ -153,7 +153,7 @@ def rotate(x, pos, rope, out=None):
     if len(shape) != 3:
         raise ValueError(f"x has shape {tuple(shape)}, (rows, heads, dim) needed")
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif out.shape[:1] != shape[:1]:
         raise ValueError(f"out has shape {tuple(out.shape)}, x {tuple(shape)}")
     rows, heads, dim = shape
@@ -218,7 +218,8 @@ class PagedKv:
         self._h = self._owner.ptr
         self.dtype = _dtype(fmt)
         self._views = {}
-        self._lib, self._empty, self._float32, self._scale = lib(), torch.empty, torch.float32, head_dim ** -0.5
+        self._lib, self._empty, self._empty_like, self._float32 = lib(), torch.empty, torch.empty_like, torch.float32
+        self._scale = head_dim ** -0.5
         self._raw, self._now = s.cuda_stream, torch._C._cuda_getCurrentRawStream  # (a torch stream object costs 2 us a call)
 
     def close(self):
@@ -325,7 +326,7 @@ class PagedKv:
             p1 = self.length(seq)
         n = max(0, p1 - p0)
         if out is None:
-            out = self._new(n, self.kv_heads, self.head_dim)
+            out = self._new((n, self.kv_heads, self.head_dim))
         _rows(out, self.kv_heads, self.head_dim, self.dtype, self.device, "out")
         if out.shape[0] != n or not out.is_contiguous():
             raise ValueError(f"out must be {n} contiguous rows")
@@ -334,10 +335,13 @@ class PagedKv:
 
     # ---- the layers' calls ----
 
-    def _new(self, *shape):
-        """An output. Where torch's current stream is another than the cache's, memory that is free on the former may still
-        be in use on the latter, and the other way round: it comes from the cache's stream and is held for both."""
+    def _new(self, shape, like=None):
+        """An output (like: a tensor of its shape and type). Where torch's current stream is another than the cache's,
+        memory that is free on the one may still be in use on the other: it comes from the cache's stream and is held for
+        both."""
         if self._now(self.device.index) == self._raw:
+            if like is not None and like.is_contiguous():
+                return self._empty_like(like)
             return self._empty(shape, dtype=self.dtype, device=self.device)
         import torch
         now = torch.cuda.current_stream(self.device)
@@ -365,7 +369,7 @@ class PagedKv:
         if q is not None:
             qp, qt, qh = _rows(q, self.q_heads, d, self.dtype, self.device, "q")
             if q_out is None:
-                q_out = self._new(rows, self.q_heads, d)
+                q_out = self._new((rows, self.q_heads, d), q)
                 qo = q_out.data_ptr()
             else:
                 qo = self._whole(q_out, rows, "q_out")
@@ -383,7 +387,7 @@ class PagedKv:
         qp, qt, qh = _rows(q, h, d, dtype, device, "q")
         rows = q.shape[0]
         if out is None:
-            out = self._new(rows, h, d)
+            out = self._new((rows, h, d), q)
             op = out.data_ptr()
         else:
             op = self._whole(out, rows, "out")
