@@ -24,7 +24,7 @@ namespace {
 constexpr int RING = 4;           // staged uploads in flight
 constexpr int GRAPH_GRID = 512;   // work-groups of a captured kernel; all loop over the lists they find
 constexpr int MOST_GRID = 1 << 20;  // of an eager one: a launch takes less than 2^32 threads
-constexpr unsigned SEG = 2048;    // words of an upload's segment at most: one work-group's share
+constexpr unsigned SEG = 256;     // words of an upload's segment at most: a thread of one work-group each
 }  // namespace
 
 struct mpg_store {
