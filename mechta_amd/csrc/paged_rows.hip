@@ -49,7 +49,7 @@ __device__ inline void rotate_pair(float& a, float& b, float2 cs) {
 
 // One unit of a row's rotation: 8 elements of either side of their pairs (half layout), 8 elements (interleaved), 8
 // elements that are copied; without 8-element alignment a pair or an element. Whoever reads an element writes it, so a
-// row may be rotated in place. cs: the row's pairs. to(d): where element d (and, for units of 8, those behind it) goes.
+// row may be rotated in place. cs(i): the row's pair i. to(d): where element d (and, for units of 8, those behind it) goes.
 template <typename T, bool WIDE>
 __device__ inline int row_units(int dim, int rot, int layout) {
     if (!WIDE) return rot / 2 + dim - rot;
@@ -60,8 +60,8 @@ __device__ inline void put8(T* p, Vec8<T> x) {
     if constexpr (STREAM) __builtin_nontemporal_store(x, (Vec8<T>*)p);
     else store8(p, x);
 }
-template <typename T, bool WIDE, bool STREAM = false, typename To>
-__device__ inline void rotate_unit(const T* __restrict__ x, int u, int rot, int layout, const float2* cs, To to) {
+template <typename T, bool WIDE, bool STREAM = false, typename Pairs, typename To>
+__device__ inline void rotate_unit(const T* __restrict__ x, int u, int rot, int layout, Pairs cs, To to) {
     if constexpr (!WIDE) {
         if (u >= rot / 2) {
             *to(rot / 2 + u) = x[rot / 2 + u];
@@ -69,7 +69,7 @@ __device__ inline void rotate_unit(const T* __restrict__ x, int u, int rot, int 
         }
         const int i = layout == MPG_HALF ? u : 2 * u, j = layout == MPG_HALF ? u + rot / 2 : 2 * u + 1;
         float a = (float)x[i], b = (float)x[j];
-        rotate_pair(a, b, cs[u]);
+        rotate_pair(a, b, cs(u));
         *to(i) = (T)a;
         *to(j) = (T)b;
     } else if (layout == MPG_HALF && u < rot / 16) {
@@ -77,7 +77,7 @@ __device__ inline void rotate_unit(const T* __restrict__ x, int u, int rot, int 
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             float p = (float)a[e], q = (float)b[e];
-            rotate_pair(p, q, cs[8 * u + e]);
+            rotate_pair(p, q, cs(8 * u + e));
             a[e] = (T)p;
             b[e] = (T)q;
         }
@@ -90,7 +90,7 @@ __device__ inline void rotate_unit(const T* __restrict__ x, int u, int rot, int 
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
                 float p = (float)a[e], q = (float)a[e + 1];
-                rotate_pair(p, q, cs[(d + e) / 2]);
+                rotate_pair(p, q, cs((d + e) / 2));
                 a[e] = (T)p;
                 a[e + 1] = (T)q;
             }
@@ -135,8 +135,9 @@ __device__ inline void rotate_rows(const RopeArgs& r, int n, int heads, int dim,
     const int half = r.dim / 2;
     for (Walk w(at, by, heads, row_units<T, WIDE>(dim, r.dim, r.layout)); w.row < n; w.next()) {
         T* const o = out + w.row * o_row + w.head * o_head;
-        rotate_unit<T, WIDE, STREAM>(x + w.row * x_row + w.head * x_head, w.unit, r.dim, r.layout, cs + w.row * half,
-                             [&](int d) { return o + d; });
+        const float2* const pairs = cs + w.row * half;
+        rotate_unit<T, WIDE, STREAM>(x + w.row * x_row + w.head * x_head, w.unit, r.dim, r.layout,
+                                     [&](int i) { return pairs[i]; }, [&](int d) { return o + d; });
     }
 }
 
@@ -168,7 +169,7 @@ __global__ void __launch_bounds__(256) append_kernel(const Run* __restrict__ run
                                                      int rows, const T* __restrict__ k, int64_t k_tok, int64_t k_head,
                                                      const T* __restrict__ v, int64_t v_tok, int64_t v_head, const T* q,
                                                      int64_t q_tok, int64_t q_head, T* q_out, RopeArgs r) {
-    extern __shared__ float2 cs[];  // [tokens][r.dim / 2], behind it K rows [KEYS][dim + 8]
+    extern __shared__ float2 cs[];  // [ROT_ROWS][r.dim / 2]
     const int half = r.dim / 2, tid = threadIdx.x, count = *uniform(nruns);
     for (int i = blockIdx.x; i < count; i += gridDim.x) {
         const Uniform<int> ri = uniform((const int*)(runs + i));
@@ -188,24 +189,15 @@ __global__ void __launch_bounds__(256) append_kernel(const Run* __restrict__ run
         }
         if (run.count <= 0) continue;
         const size_t p = uniform(table)[(size_t)run.seq * most_pages + run.pos / page];
-        const int in = run.pos % page, at = in % KEYS, chunks = dim / 8, head = blockIdx.y, stride = dim + 8;
+        const int in = run.pos % page, at = in % KEYS, chunks = dim / 8, head = blockIdx.y;
         const size_t base = (p * kv_heads + head) * page * dim + (size_t)(in / KEYS) * KEYS * dim;  // of the 32-position block
-        T* const kt = (T*)(cs + KEYS * half);
-        __syncthreads();  // what stood in LDS has been read
-        if (half > 0)
-            for (Walk w(tid, 256, 1, half); w.row < run.count; w.next())
-                cs[w.row * half + w.unit] = turn(r, run.pos + w.row, w.unit);
-        __syncthreads();
         const T* const ks = k + run.tok * k_tok + head * k_head;
-        for (Walk w(tid, 256, 1, row_units<T, WIDE>(dim, r.dim, r.layout)); w.row < run.count; w.next()) {
-            T* const o = kt + w.row * stride;
-            rotate_unit<T, WIDE>(ks + w.row * k_tok, w.unit, r.dim, r.layout, cs + w.row * half, [&](int d) { return o + d; });
-        }
-        __syncthreads();
-        T* const kb = kpool + base;
-        for (int j = tid; j < KEYS * chunks; j += 256) {  // 16-byte pieces in the pages' order
-            const int pos = j % 16 + j / (16 * chunks) * 16, t = pos - at;
-            if (t >= 0 && t < run.count) store8(kb + j * 8, load8(kt + t * stride + j / 16 % chunks * 8));
+        // units of all rows, row by row; neighbours in the pages are of neighbouring rows
+        for (Walk w(tid, 256, row_units<T, WIDE>(dim, r.dim, r.layout), run.count); w.row < 1; w.next()) {
+            const int t = w.unit, b = at + t;
+            T* const o = kpool + base + b / 16 * 16 * dim + b % 16 * 8;
+            rotate_unit<T, WIDE>(ks + t * k_tok, w.head, r.dim, r.layout, [&](int i) { return turn(r, run.pos + t, i); },
+                                 [&](int d) { return o + d / 8 * 128 + d % 8; });
         }
         const T* const vs = v + run.tok * v_tok + head * v_head;
         T* const vb = vpool + base;
@@ -258,7 +250,7 @@ hipError_t append_as(const Geometry& g, char* pool, int layer, const int* table,
     none.layout = MPG_HALF;
     const RopeArgs& r = rope ? *rope : none;
     T* const kp = (T*)pool + (size_t)layer * 2 * g.plane_elems();
-    const size_t lds = (size_t)KEYS * (r.dim / 2) * sizeof(float2) + (size_t)KEYS * (g.head_dim + 8) * sizeof(T);
+    const size_t lds = (size_t)ROT_ROWS * (r.dim / 2) * sizeof(float2);
     const auto kernel = r.dim % 16 ? append_kernel<T, false> : append_kernel<T, true>;
     kernel<<<dim3(grid, g.kv_heads + (q.p ? Q_PARTS : 0)), dim3(256), lds, s>>>(
         runs, nruns, table, g.most_pages, g.page, g.head_dim, g.kv_heads, g.q_heads, kp, kp + g.plane_elems(), rows,
