@@ -127,7 +127,7 @@ struct Walk {
     }
 };
 
-constexpr int ROT_ROWS = 4;  // rows of a work-group: their angles are shared by the heads
+constexpr int ROT_ROWS = 2;  // rows of a work-group: their angles are shared by the heads
 // n rows of `heads` heads from x (row and head strides) to out, cs: their pairs
 template <typename T, bool WIDE, bool STREAM = false>
 __device__ inline void rotate_rows(const RopeArgs& r, int n, int heads, int dim, const T* x, int64_t x_row, int64_t x_head,
@@ -142,7 +142,7 @@ __device__ inline void rotate_rows(const RopeArgs& r, int n, int heads, int dim,
 }
 
 // Work-group = ROT_ROWS rows; where those are few, blockIdx.y shares out their heads. STREAM: outputs that the L2s cannot
-// hold anyway are stored past them (8,192 rows of 32 heads of 128 in bf16, 134 MB moved: 28.8 -> 22.5 us).
+// hold anyway are stored past them (8,192 rows of 32 heads of 128 in bf16, 134 MB moved: 28.8 -> 21.8 us).
 template <typename T, bool WIDE, bool STREAM>
 __global__ void __launch_bounds__(256) rotate_kernel(RopeArgs r, int rows, int heads, int dim, const T* x, int64_t x_row,
                                                      int64_t x_head, const int* __restrict__ pos, T* out, int64_t o_row,
@@ -156,11 +156,12 @@ __global__ void __launch_bounds__(256) rotate_kernel(RopeArgs r, int rows, int h
 }
 
 // ---- append ----
-// For a run of new tokens inside one 32-position block of a page: work-groups y < kv_heads take a head's K and V, those
-// behind them the query heads of 4 tokens each. K rows are rotated into LDS and leave in the pages' order, 16 positions
-// side by side. A V block that is all new is turned in registers (8 positions of 8 dims a thread) and written in 16-byte
-// pieces, others element by element. Bound by memory: 4,096 + 2,500 + 1,031 + 565 tokens of 32 + 2 x 4 heads of 128 move
-// 168 MB in 35.4 us (44.2 with the K and V of a run in one work-group behind its query heads, 37.5 with K and V apart).
+// A run is new tokens inside one 32-position block of a page. The first work-groups take a run's K and V of a head each,
+// those behind them the query heads of 2 tokens each; neighbours have neighbouring rows. K rows go into the pages as they
+// are rotated, neighbouring lanes on neighbouring positions. A V block that is all new is turned in registers (8 positions
+// of 8 dims a thread) and written in 16-byte pieces, others element by element. Bound by memory: 4,096 + 2,500 + 1,031 +
+// 565 tokens of 32 + 2 x 4 heads of 128 move 168 MB in 33.7 us, 5 TB/s (query heads of 4 tokens a work-group 35.4, of 1 and
+// 8 36.9; K and V of all heads in one work-group behind the query heads 44).
 constexpr int Q_PARTS = KEYS / ROT_ROWS;
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) append_kernel(const Run* __restrict__ runs, const int* __restrict__ nruns,
@@ -171,12 +172,15 @@ __global__ void __launch_bounds__(256) append_kernel(const Run* __restrict__ run
                                                      int64_t q_tok, int64_t q_head, T* q_out, RopeArgs r) {
     extern __shared__ float2 cs[];  // [ROT_ROWS][r.dim / 2]
     const int half = r.dim / 2, tid = threadIdx.x, count = *uniform(nruns);
-    for (int i = blockIdx.x; i < count; i += gridDim.x) {
-        const Uniform<int> ri = uniform((const int*)(runs + i));
+    const int kv_items = count * kv_heads, items = q ? kv_items + count * Q_PARTS : kv_items;
+    for (int i = blockIdx.x; i < items; i += gridDim.x) {
+        const bool is_q = i >= kv_items;
+        const int x = is_q ? i - kv_items : i, per = is_q ? Q_PARTS : kv_heads, of = x % per;
+        const Uniform<int> ri = uniform((const int*)(runs + x / per));
         Run run{ri[0], ri[1], ri[2], ri[3]};
         run.count = min(run.count, rows - run.tok);
-        if ((int)blockIdx.y >= kv_heads) {  // query heads
-            const int t0 = (blockIdx.y - kv_heads) * ROT_ROWS, n = min(ROT_ROWS, run.count - t0);
+        if (is_q) {
+            const int t0 = of * ROT_ROWS, n = min(ROT_ROWS, run.count - t0);
             if (n <= 0) continue;
             __syncthreads();  // the angles before have been read
             for (Walk w(tid, 256, 1, half); w.row < n; w.next())
@@ -189,7 +193,7 @@ __global__ void __launch_bounds__(256) append_kernel(const Run* __restrict__ run
         }
         if (run.count <= 0) continue;
         const size_t p = uniform(table)[(size_t)run.seq * most_pages + run.pos / page];
-        const int in = run.pos % page, at = in % KEYS, chunks = dim / 8, head = blockIdx.y;
+        const int in = run.pos % page, at = in % KEYS, chunks = dim / 8, head = of;
         const size_t base = (p * kv_heads + head) * page * dim + (size_t)(in / KEYS) * KEYS * dim;  // of the 32-position block
         const T* const ks = k + run.tok * k_tok + head * k_head;
         // units of all rows, row by row; neighbours in the pages are of neighbouring rows
@@ -244,7 +248,7 @@ __global__ void __launch_bounds__(256) read_kernel(const T* __restrict__ pool, c
 }
 
 template <typename T>
-hipError_t append_as(const Geometry& g, char* pool, int layer, const int* table, const Run* runs, const int* nruns, int grid,
+hipError_t append_as(const Geometry& g, char* pool, int layer, const int* table, const Run* runs, const int* nruns, int most,
                      int rows, const Rows& k, const Rows& v, const Rows& q, void* q_out, const RopeArgs* rope, hipStream_t s) {
     RopeArgs none{};
     none.layout = MPG_HALF;
@@ -252,7 +256,8 @@ hipError_t append_as(const Geometry& g, char* pool, int layer, const int* table,
     T* const kp = (T*)pool + (size_t)layer * 2 * g.plane_elems();
     const size_t lds = (size_t)ROT_ROWS * (r.dim / 2) * sizeof(float2);
     const auto kernel = r.dim % 16 ? append_kernel<T, false> : append_kernel<T, true>;
-    kernel<<<dim3(grid, g.kv_heads + (q.p ? Q_PARTS : 0)), dim3(256), lds, s>>>(
+    const size_t items = (size_t)most * (g.kv_heads + (q.p ? Q_PARTS : 0));
+    kernel<<<dim3((unsigned)std::min<size_t>(items, 1 << 20)), dim3(256), lds, s>>>(
         runs, nruns, table, g.most_pages, g.page, g.head_dim, g.kv_heads, g.q_heads, kp, kp + g.plane_elems(), rows,
         (const T*)k.p, k.tok, k.head, (const T*)v.p, v.tok, v.head, (const T*)q.p, q.tok, q.head, (T*)q_out, r);
     return hipGetLastError();
@@ -297,10 +302,10 @@ hipError_t launch_copies(const Geometry& g, char* pool, const Pair* pairs, int n
 }
 
 hipError_t launch_append(const Geometry& g, char* pool, int layer, const int* table, const Run* runs, const int* nruns,
-                         int grid, int rows, const Rows& k, const Rows& v, const Rows& q, void* q_out, const RopeArgs* rope,
+                         int most, int rows, const Rows& k, const Rows& v, const Rows& q, void* q_out, const RopeArgs* rope,
                          hipStream_t s) {
-    return g.fmt == MKV_F16 ? append_as<_Float16>(g, pool, layer, table, runs, nruns, grid, rows, k, v, q, q_out, rope, s)
-                            : append_as<__bf16>(g, pool, layer, table, runs, nruns, grid, rows, k, v, q, q_out, rope, s);
+    return g.fmt == MKV_F16 ? append_as<_Float16>(g, pool, layer, table, runs, nruns, most, rows, k, v, q, q_out, rope, s)
+                            : append_as<__bf16>(g, pool, layer, table, runs, nruns, most, rows, k, v, q, q_out, rope, s);
 }
 
 // A launch takes less than 2^32 threads: what needs more goes in several.
