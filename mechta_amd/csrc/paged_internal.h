@@ -33,9 +33,10 @@ struct Segment {
 
 hipError_t launch_apply(int* dev, const unsigned* stage, int segments, hipStream_t s);
 hipError_t launch_copies(const Geometry& g, char* pool, const Pair* pairs, int n, hipStream_t s);
+// most: runs that work-groups are launched for (all loop over the list), longest: tokens of the longest run
 hipError_t launch_append(const Geometry& g, char* pool, int layer, const int* table, const Run* runs, const int* nruns,
-                         int most, int rows, const Rows& k, const Rows& v, const Rows& q, void* q_out, const RopeArgs* rope,
-                         hipStream_t s);
+                         int most, int longest, int rows, const Rows& k, const Rows& v, const Rows& q, void* q_out,
+                         const RopeArgs* rope, hipStream_t s);
 hipError_t launch_read(const Geometry& g, const char* pool, int layer, int which, const int* table, int p0, int p1, void* dst,
                        hipStream_t s);
 hipError_t launch_rotate(const RopeArgs& r, int fmt, int rows, int heads, int dim, const Rows& x, const int* pos,

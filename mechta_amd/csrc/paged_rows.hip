@@ -160,22 +160,21 @@ __global__ void __launch_bounds__(256) rotate_kernel(RopeArgs r, int rows, int h
 // those behind them the query heads of 2 tokens each; neighbours have neighbouring rows. K rows go into the pages as they
 // are rotated, neighbouring lanes on neighbouring positions. A V block that is all new is turned in registers (8 positions
 // of 8 dims a thread) and written in 16-byte pieces, others element by element. Bound by memory: 4,096 + 2,500 + 1,031 +
-// 565 tokens of 32 + 2 x 4 heads of 128 move 168 MB in 33.7 us, 5 TB/s (query heads of 4 tokens a work-group 35.4, of 1 and
+// 565 tokens of 32 + 2 x 4 heads of 128 move 168 MB in 32.6 us, 5.2 TB/s (query heads of 4 tokens a work-group 35.4, of 1 and
 // 8 36.9; K and V of all heads in one work-group behind the query heads 44).
-constexpr int Q_PARTS = KEYS / ROT_ROWS;
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) append_kernel(const Run* __restrict__ runs, const int* __restrict__ nruns,
-                                                     const int* __restrict__ table, int most_pages, int page, int dim,
-                                                     int kv_heads, int q_heads, T* __restrict__ kpool, T* __restrict__ vpool,
+                                                     int q_parts, const int* __restrict__ table, int most_pages, int page,
+                                                     int dim, int kv_heads, int q_heads, T* __restrict__ kpool, T* __restrict__ vpool,
                                                      int rows, const T* __restrict__ k, int64_t k_tok, int64_t k_head,
                                                      const T* __restrict__ v, int64_t v_tok, int64_t v_head, const T* q,
                                                      int64_t q_tok, int64_t q_head, T* q_out, RopeArgs r) {
     extern __shared__ float2 cs[];  // [ROT_ROWS][r.dim / 2]
     const int half = r.dim / 2, tid = threadIdx.x, count = *uniform(nruns);
-    const int kv_items = count * kv_heads, items = q ? kv_items + count * Q_PARTS : kv_items;
+    const int kv_items = count * kv_heads, items = kv_items + count * q_parts;
     for (int i = blockIdx.x; i < items; i += gridDim.x) {
         const bool is_q = i >= kv_items;
-        const int x = is_q ? i - kv_items : i, per = is_q ? Q_PARTS : kv_heads, of = x % per;
+        const int x = is_q ? i - kv_items : i, per = is_q ? q_parts : kv_heads, of = x % per;
         const Uniform<int> ri = uniform((const int*)(runs + x / per));
         Run run{ri[0], ri[1], ri[2], ri[3]};
         run.count = min(run.count, rows - run.tok);
@@ -249,16 +248,18 @@ __global__ void __launch_bounds__(256) read_kernel(const T* __restrict__ pool, c
 
 template <typename T>
 hipError_t append_as(const Geometry& g, char* pool, int layer, const int* table, const Run* runs, const int* nruns, int most,
-                     int rows, const Rows& k, const Rows& v, const Rows& q, void* q_out, const RopeArgs* rope, hipStream_t s) {
+                     int longest, int rows, const Rows& k, const Rows& v, const Rows& q, void* q_out, const RopeArgs* rope,
+                     hipStream_t s) {
     RopeArgs none{};
     none.layout = MPG_HALF;
     const RopeArgs& r = rope ? *rope : none;
     T* const kp = (T*)pool + (size_t)layer * 2 * g.plane_elems();
     const size_t lds = (size_t)ROT_ROWS * (r.dim / 2) * sizeof(float2);
     const auto kernel = r.dim % 16 ? append_kernel<T, false> : append_kernel<T, true>;
-    const size_t items = (size_t)most * (g.kv_heads + (q.p ? Q_PARTS : 0));
+    const int q_parts = q.p ? (longest + ROT_ROWS - 1) / ROT_ROWS : 0;
+    const size_t items = (size_t)most * (g.kv_heads + q_parts);
     kernel<<<dim3((unsigned)std::min<size_t>(items, 1 << 20)), dim3(256), lds, s>>>(
-        runs, nruns, table, g.most_pages, g.page, g.head_dim, g.kv_heads, g.q_heads, kp, kp + g.plane_elems(), rows,
+        runs, nruns, q_parts, table, g.most_pages, g.page, g.head_dim, g.kv_heads, g.q_heads, kp, kp + g.plane_elems(), rows,
         (const T*)k.p, k.tok, k.head, (const T*)v.p, v.tok, v.head, (const T*)q.p, q.tok, q.head, (T*)q_out, r);
     return hipGetLastError();
 }
@@ -271,7 +272,9 @@ hipError_t rotate_as(const RopeArgs& r, int rows, int heads, int dim, const Rows
     const size_t lds = (size_t)ROT_ROWS * (r.dim / 2) * sizeof(float2);
     constexpr size_t L2 = 32 << 20;  // of the eight dies together
     const bool stream = (size_t)rows * heads * dim * sizeof(T) > L2;
-    const auto kernel = !wide ? rotate_kernel<T, false, false> : stream ? rotate_kernel<T, true, true> : rotate_kernel<T, true, false>;
+    const auto kernel = !wide    ? rotate_kernel<T, false, false>
+                        : stream ? rotate_kernel<T, true, true>
+                                 : rotate_kernel<T, true, false>;
     const int groups = (rows + ROT_ROWS - 1) / ROT_ROWS, n = rows < ROT_ROWS ? rows : ROT_ROWS;
     // few rows of many heads: heads shared out, a unit or two a thread
     const int y = groups >= 256 ? 1 : std::max(1, std::min(256 / groups, n * heads * (dim / 16) / 512));
@@ -302,10 +305,10 @@ hipError_t launch_copies(const Geometry& g, char* pool, const Pair* pairs, int n
 }
 
 hipError_t launch_append(const Geometry& g, char* pool, int layer, const int* table, const Run* runs, const int* nruns,
-                         int most, int rows, const Rows& k, const Rows& v, const Rows& q, void* q_out, const RopeArgs* rope,
-                         hipStream_t s) {
-    return g.fmt == MKV_F16 ? append_as<_Float16>(g, pool, layer, table, runs, nruns, most, rows, k, v, q, q_out, rope, s)
-                            : append_as<__bf16>(g, pool, layer, table, runs, nruns, most, rows, k, v, q, q_out, rope, s);
+                         int most, int longest, int rows, const Rows& k, const Rows& v, const Rows& q, void* q_out,
+                         const RopeArgs* rope, hipStream_t s) {
+    const auto as = g.fmt == MKV_F16 ? append_as<_Float16> : append_as<__bf16>;
+    return as(g, pool, layer, table, runs, nruns, most, longest, rows, k, v, q, q_out, rope, s);
 }
 
 // A launch takes less than 2^32 threads: what needs more goes in several.
@@ -327,11 +330,12 @@ hipError_t launch_read(const Geometry& g, const char* pool, int layer, int which
 
 hipError_t launch_rotate(const RopeArgs& r, int fmt, int rows, int heads, int dim, const Rows& x, const int* pos,
                          const Rows& out, hipStream_t s) {
-    constexpr int MOST = 1 << 25;  // a work-group of 256 threads for ROT_ROWS of them
+    constexpr int MOST = ROT_ROWS << 23;  // 2^31 threads
     const int bytes = fmt == MKV_F32 ? 4 : 2;
     for (int64_t i = 0; i < rows; i += MOST) {
         const int n = (int)std::min<int64_t>(MOST, rows - i);
-        const Rows xi{(const char*)x.p + i * x.tok * bytes, x.tok, x.head}, oi{(const char*)out.p + i * out.tok * bytes, out.tok, out.head};
+        const Rows xi{(const char*)x.p + i * x.tok * bytes, x.tok, x.head};
+        const Rows oi{(const char*)out.p + i * out.tok * bytes, out.tok, out.head};
         const hipError_t e = fmt == MKV_F16   ? rotate_as<_Float16>(r, n, heads, dim, xi, pos + i, oi, s)
                              : fmt == MKV_F32 ? rotate_as<float>(r, n, heads, dim, xi, pos + i, oi, s)
                                               : rotate_as<__bf16>(r, n, heads, dim, xi, pos + i, oi, s);

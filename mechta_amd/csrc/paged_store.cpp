@@ -48,7 +48,7 @@ struct mpg_store {
     size_t stage_words[RING] = {};
     int turn = 0;
     int tokens = -1;                // of the batch; -1: none stands
-    int nruns = 0;
+    int nruns = 0, longest = 0;     // its runs, and the tokens of the longest
     std::vector<Plan> plans;        // per window, of the batch
 };
 
@@ -485,7 +485,7 @@ int mpg_reserve(mpg_t* h, int n, const int* seq, const int* count) {
 static int lay_out(mpg_t* h, int n, const int* seq, const int* count) {
     std::vector<Member> batch;
     std::vector<Run> runs;
-    int tok = 0;
+    int tok = 0, longest = 0;
     for (int i = 0; i < n; i++) {
         const int len = h->book.len[seq[i]];
         batch.push_back({seq[i], count[i], len});
@@ -494,12 +494,14 @@ static int lay_out(mpg_t* h, int n, const int* seq, const int* count) {
             runs.push_back({seq[i], tok, p, m});
             p += m;
             tok += m;
+            longest = std::max(longest, m);
         }
     }
     for (size_t w = 0; w < h->kinds.size(); w++) plan_window(h->shape, batch, h->kinds[w], h->plans[w]);
     if (int rc = upload(h, &runs, "mpg_begin")) return rc;
     h->tokens = tok;
     h->nruns = (int)runs.size();
+    h->longest = longest;
     return MKV_OK;
 }
 
@@ -595,9 +597,9 @@ int mpg_append(mpg_t* h, int layer, int rows, const void* k, int64_t k_tok, int6
     if (cap < 0) return cap;
     if (!cap && !h->nruns) return MKV_OK;
     const hipError_t e = launch_append(h->g, h->pool, layer, h->dev, (const Run*)(h->dev + h->runs_at + COUNTS),
-                                       h->dev + h->runs_at, cap ? GRAPH_GRID : h->nruns, rows, Rows{k, k_tok, k_head},
-                                       Rows{v, v_tok, v_head}, Rows{q, q_tok, q_head}, q_out, rotate ? &h->rope : nullptr,
-                                       h->stream);
+                                       h->dev + h->runs_at, cap ? GRAPH_GRID : h->nruns, cap ? KEYS : h->longest, rows,
+                                       Rows{k, k_tok, k_head}, Rows{v, v_tok, v_head}, Rows{q, q_tok, q_head}, q_out,
+                                       rotate ? &h->rope : nullptr, h->stream);
     return e == hipSuccess ? MKV_OK : hip_fail(e, "mpg_append");
 }
 
