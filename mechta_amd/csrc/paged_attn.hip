@@ -734,13 +734,15 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
         const float x[4] = {acc[0], acc[1], acc[2], acc[3]};
         store_out<T, D, 4>(a, tok, head, d, x);
     };
-    for (int n = blockIdx.x; n < count; n += gridDim.x) {
+    // work-groups of a join: as many as there are for each
+    const int ways = max(1, (int)gridDim.x / max(1, count)), way = blockIdx.x % ways;
+    for (int n = blockIdx.x / ways; n < count; n += gridDim.x / ways) {
         const Uniform<int> ji = uniform((const int*)(joins + n));
         const Join j{ji[0], ji[1], ji[2], ji[3], ji[4], ji[5], ji[6], 0};
         if (!j.wide) {
             constexpr int LANES = D / 4, GROUPS = 256 / LANES;
             const int d = tid % LANES * 4;
-            for (int r = blockIdx.y * GROUPS + tid / LANES; r < j.count; r += gridDim.y * GROUPS) {
+            for (int r = way * GROUPS + tid / LANES; r < j.count; r += ways * GROUPS) {
                 const int row = j.row0 + r, tok = j.tok0 + row / a.group;
                 if (tok >= a.rows) continue;
                 f32x4 acc = f32x4{};
@@ -782,7 +784,7 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
         }
         constexpr int PER_ROW = D / JOIN_DIMS;
         const int part = tid / 16, lane = tid % 16;
-        for (int u = blockIdx.y; u < j.count * PER_ROW; u += gridDim.y) {
+        for (int u = way; u < j.count * PER_ROW; u += ways) {
             const int r = u / PER_ROW, d = u % PER_ROW * JOIN_DIMS + lane * 4;
             const int row = j.row0 + r, tok = j.tok0 + row / a.group;
             if (tok >= a.rows) continue;
@@ -880,14 +882,14 @@ hipError_t attend_as(const Geometry& g, const AttendArgs& x, const int* batch, c
         e = hipGetLastError();
     }
     if (join_grid && e == hipSuccess) {
-        // work-groups for a join: the most that one of them has rows for
-        int join_rows = 1;
-        for (const Join& j : *x.joins) {
-            const int groups = 1024 / D;
-            join_rows = std::max(join_rows, j.wide ? j.count * (D / JOIN_DIMS) : (j.count + groups - 1) / groups);
-        }
-        if (x.captured) join_rows = 32;
-        join_kernel<T, D><<<dim3(join_grid, join_rows), dim3(256), 0, s>>>(a, (const Join*)(batch + l.joins), batch + KINDS);
+        int ways = 1;  // for a join: the most that one of them has rows for
+        if (!x.captured)
+            for (const Join& j : *x.joins) {
+                const int groups = 1024 / D;
+                ways = std::max(ways, j.wide ? j.count * (D / JOIN_DIMS) : (j.count + groups - 1) / groups);
+            }
+        const int all = std::min(join_grid, MOST_GRID / ways) * ways;
+        join_kernel<T, D><<<dim3(all), dim3(256), 0, s>>>(a, (const Join*)(batch + l.joins), batch + KINDS);
         e = hipGetLastError();
     }
     return e;

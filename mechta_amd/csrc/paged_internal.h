@@ -11,7 +11,7 @@ namespace paged {
 struct Lists {
     size_t items[KINDS], joins, words;  // word offsets of the lists; words of the whole
 };
-constexpr size_t COUNTS = 8;  // words: items of each kind, joins
+constexpr size_t COUNTS = 8;  // words in front of a list: items of each kind, joins; of the runs: how many, the longest
 static_assert(KINDS < COUNTS, "counts");
 
 struct Geometry {
@@ -33,9 +33,11 @@ struct Segment {
 
 hipError_t launch_apply(int* dev, const unsigned* stage, int segments, hipStream_t s);
 hipError_t launch_copies(const Geometry& g, char* pool, const Pair* pairs, int n, hipStream_t s);
-// most: runs that work-groups are launched for (all loop over the list), longest: tokens of the longest run
+constexpr int MOST_GRID = 1 << 20;  // work-groups of a launch, which takes less than 2^32 threads; all loop over their lists
+
+// grid: work-groups, or 0: by the runs (most of them) and the tokens of the longest
 hipError_t launch_append(const Geometry& g, char* pool, int layer, const int* table, const Run* runs, const int* nruns,
-                         int most, int longest, int rows, const Rows& k, const Rows& v, const Rows& q, void* q_out,
+                         int grid, int most, int longest, int rows, const Rows& k, const Rows& v, const Rows& q, void* q_out,
                          const RopeArgs* rope, hipStream_t s);
 hipError_t launch_read(const Geometry& g, const char* pool, int layer, int which, const int* table, int p0, int p1, void* dst,
                        hipStream_t s);

@@ -164,13 +164,14 @@ __global__ void __launch_bounds__(256) rotate_kernel(RopeArgs r, int rows, int h
 // 8 36.9; K and V of all heads in one work-group behind the query heads 44).
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) append_kernel(const Run* __restrict__ runs, const int* __restrict__ nruns,
-                                                     int q_parts, const int* __restrict__ table, int most_pages, int page,
-                                                     int dim, int kv_heads, int q_heads, T* __restrict__ kpool, T* __restrict__ vpool,
+                                                     const int* __restrict__ table, int most_pages, int page, int dim,
+                                                     int kv_heads, int q_heads, T* __restrict__ kpool, T* __restrict__ vpool,
                                                      int rows, const T* __restrict__ k, int64_t k_tok, int64_t k_head,
                                                      const T* __restrict__ v, int64_t v_tok, int64_t v_head, const T* q,
                                                      int64_t q_tok, int64_t q_head, T* q_out, RopeArgs r) {
     extern __shared__ float2 cs[];  // [ROT_ROWS][r.dim / 2]
     const int half = r.dim / 2, tid = threadIdx.x, count = *uniform(nruns);
+    const int q_parts = q ? (uniform(nruns)[1] + ROT_ROWS - 1) / ROT_ROWS : 0;  // by the longest run
     const int kv_items = count * kv_heads, items = kv_items + count * q_parts;
     for (int i = blockIdx.x; i < items; i += gridDim.x) {
         const bool is_q = i >= kv_items;
@@ -247,19 +248,19 @@ __global__ void __launch_bounds__(256) read_kernel(const T* __restrict__ pool, c
 }
 
 template <typename T>
-hipError_t append_as(const Geometry& g, char* pool, int layer, const int* table, const Run* runs, const int* nruns, int most,
-                     int longest, int rows, const Rows& k, const Rows& v, const Rows& q, void* q_out, const RopeArgs* rope,
-                     hipStream_t s) {
+hipError_t append_as(const Geometry& g, char* pool, int layer, const int* table, const Run* runs, const int* nruns, int grid,
+                     int most, int longest, int rows, const Rows& k, const Rows& v, const Rows& q, void* q_out,
+                     const RopeArgs* rope, hipStream_t s) {
     RopeArgs none{};
     none.layout = MPG_HALF;
     const RopeArgs& r = rope ? *rope : none;
     T* const kp = (T*)pool + (size_t)layer * 2 * g.plane_elems();
     const size_t lds = (size_t)ROT_ROWS * (r.dim / 2) * sizeof(float2);
     const auto kernel = r.dim % 16 ? append_kernel<T, false> : append_kernel<T, true>;
-    const int q_parts = q.p ? (longest + ROT_ROWS - 1) / ROT_ROWS : 0;
-    const size_t items = (size_t)most * (g.kv_heads + q_parts);
-    kernel<<<dim3((unsigned)std::min<size_t>(items, 1 << 20)), dim3(256), lds, s>>>(
-        runs, nruns, q_parts, table, g.most_pages, g.page, g.head_dim, g.kv_heads, g.q_heads, kp, kp + g.plane_elems(), rows,
+    const size_t items = (size_t)most * (g.kv_heads + (q.p ? (longest + ROT_ROWS - 1) / ROT_ROWS : 0));
+    if (!grid) grid = (int)std::min<size_t>(items, MOST_GRID);
+    kernel<<<dim3(grid), dim3(256), lds, s>>>(
+        runs, nruns, table, g.most_pages, g.page, g.head_dim, g.kv_heads, g.q_heads, kp, kp + g.plane_elems(), rows,
         (const T*)k.p, k.tok, k.head, (const T*)v.p, v.tok, v.head, (const T*)q.p, q.tok, q.head, (T*)q_out, r);
     return hipGetLastError();
 }
@@ -305,10 +306,10 @@ hipError_t launch_copies(const Geometry& g, char* pool, const Pair* pairs, int n
 }
 
 hipError_t launch_append(const Geometry& g, char* pool, int layer, const int* table, const Run* runs, const int* nruns,
-                         int most, int longest, int rows, const Rows& k, const Rows& v, const Rows& q, void* q_out,
+                         int grid, int most, int longest, int rows, const Rows& k, const Rows& v, const Rows& q, void* q_out,
                          const RopeArgs* rope, hipStream_t s) {
     const auto as = g.fmt == MKV_F16 ? append_as<_Float16> : append_as<__bf16>;
-    return as(g, pool, layer, table, runs, nruns, most, longest, rows, k, v, q, q_out, rope, s);
+    return as(g, pool, layer, table, runs, nruns, grid, most, longest, rows, k, v, q, q_out, rope, s);
 }
 
 // A launch takes less than 2^32 threads: what needs more goes in several.
