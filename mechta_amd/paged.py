@@ -5,6 +5,7 @@ tokens of a batch (rotating K and q) and attends over the pages; rotate() applie
 call goes through the HIP library.
 """
 import ctypes
+from array import array
 
 from mechta_amd import F16, F32, K, V, MkvError, lib as _mkv_lib  # noqa: F401
 
@@ -51,7 +52,7 @@ def lib():
             "mpg_rope_turns": ([R, T], I),
             "mpg_rotate": ([T, I, I, I, I, P, L64, L64, P, P, L64, L64, P], I),
             "mpg_bytes": ([C], S),
-            "mpg_create": ([ctypes.POINTER(P), C, IP, R, P], I),
+            "mpg_create": ([ctypes.POINTER(P), C, P, R, P], I),
             "mpg_destroy": ([P], I),
             "mpg_set_stream": ([P, P], I),
             "mpg_sync": ([P], I),
@@ -59,12 +60,12 @@ def lib():
             "mpg_table": ([P, I, IP, I], I),
             "mpg_free_pages": ([P, IP], I),
             "mpg_pages": ([P, I, I, ctypes.POINTER(P)], I),
-            "mpg_reserve": ([P, I, IP, IP], I),
-            "mpg_begin": ([P, I, IP, IP, IP], I),
+            "mpg_reserve": ([P, I, P, P], I),
+            "mpg_begin": ([P, I, P, P, IP], I),
             "mpg_set_len": ([P, I, I], I),
-            "mpg_fork": ([P, I, IP, IP, IP], I),
-            "mpg_copy": ([P, I, IP, IP], I),
-            "mpg_free": ([P, I, IP], I),
+            "mpg_fork": ([P, I, P, P, P], I),
+            "mpg_copy": ([P, I, P, P], I),
+            "mpg_free": ([P, I, P], I),
             "mpg_compact": ([P, IP], I),
             "mpg_append": ([P, I, I, P, L64, L64, P, L64, L64, P, L64, L64, P, I], I),
             "mpg_attend": ([P, I, I, P, L64, L64, F, P, P, L64, L64, P], I),
@@ -85,10 +86,14 @@ def _check(rc):
 
 
 def _ints(xs, n=None, what="list"):
-    xs = [int(x) for x in xs]
-    if n is not None and len(xs) != n:
-        raise ValueError(f"{what} has {len(xs)} entries, {n} needed")
-    return (ctypes.c_int * max(len(xs), 1))(*xs)
+    """A list of ints as an array and its address; the array is to live as long as that is used."""
+    try:
+        a = array("i", xs)
+    except OverflowError:
+        raise ValueError(f"{what} has entries past 32 bits") from None
+    if n is not None and len(a) != n:
+        raise ValueError(f"{what} has {len(a)} entries, {n} needed")
+    return a, a.buffer_info()[0]
 
 
 def _dtype(fmt):
@@ -211,9 +216,9 @@ class PagedKv:
         self.layers, self.q_heads, self.kv_heads, self.head_dim = layers, q_heads, kv_heads, head_dim
         self.num_pages, self.page, self.seqs, self.ctx, self.fmt, self.rope = pages, page, seqs, ctx, fmt, rope
         self._config = _Config(layers, q_heads, kv_heads, head_dim, fmt, pages, page, seqs, ctx, tokens)
-        w = None if windows is None else _ints([x or 0 for x in windows], layers, "windows")
+        w, wp = (None, None) if windows is None else _ints([x or 0 for x in windows], layers, "windows")
         with torch.cuda.device(self.device):
-            _check(lib().mpg_create(ctypes.byref(self._owner.ptr), ctypes.byref(self._config), w,
+            _check(lib().mpg_create(ctypes.byref(self._owner.ptr), ctypes.byref(self._config), wp,
                                     None if rope is None else ctypes.byref(rope.c), ctypes.c_void_p(s.cuda_stream)))
         self._h = self._owner.ptr
         self.dtype = _dtype(fmt)
@@ -269,37 +274,42 @@ class PagedKv:
 
     def reserve(self, seqs, counts):
         """Lengthens the sequences by `counts` positions that the caller fills in itself (pages())."""
-        _check(lib().mpg_reserve(self._h, len(seqs), _ints(seqs), _ints(counts, len(seqs), "counts")))
+        (a, ap), (b, bp) = _ints(seqs), _ints(counts, len(seqs), "counts")
+        _check(self._lib.mpg_reserve(self._h, len(a), ap, bp))
 
     def begin(self, seqs, counts):
         """Lengthens the sequences by `counts` new tokens and makes them the batch of the appends and attention that
         follow; returns the number of tokens."""
         n = ctypes.c_int()
-        _check(lib().mpg_begin(self._h, len(seqs), _ints(seqs), _ints(counts, len(seqs), "counts"), ctypes.byref(n)))
+        (a, ap), (b, bp) = _ints(seqs), _ints(counts, len(seqs), "counts")
+        _check(self._lib.mpg_begin(self._h, len(a), ap, bp, ctypes.byref(n)))
         return n.value
 
     def set_len(self, seq, n):
         """Shortens a sequence (rollback)."""
-        _check(lib().mpg_set_len(self._h, seq, n))
+        _check(self._lib.mpg_set_len(self._h, seq, n))
 
     def fork(self, src, dst, lens=None):
         """Each empty dst[i] becomes the first lens[i] positions of src[i] (all by default); full pages are shared."""
         n = len(dst)
-        _check(lib().mpg_fork(self._h, n, _ints(src, n, "src"), _ints(dst),
-                              None if lens is None else _ints(lens, n, "lens")))
+        (a, ap), (b, bp) = _ints(src, n, "src"), _ints(dst)
+        c, cp = (None, None) if lens is None else _ints(lens, n, "lens")
+        _check(self._lib.mpg_fork(self._h, n, ap, bp, cp))
 
     def copy(self, src, dst):
         """Each empty dst[i] becomes src[i] on pages of its own."""
         n = len(dst)
-        _check(lib().mpg_copy(self._h, n, _ints(src, n, "src"), _ints(dst)))
+        (a, ap), (b, bp) = _ints(src, n, "src"), _ints(dst)
+        _check(self._lib.mpg_copy(self._h, n, ap, bp))
 
     def free(self, seqs):
-        _check(lib().mpg_free(self._h, len(seqs), _ints(seqs)))
+        a, ap = _ints(seqs)
+        _check(self._lib.mpg_free(self._h, len(a), ap))
 
     def compact(self):
         """Moves pages so that those in use are the lowest; returns how many moved."""
         n = ctypes.c_int()
-        _check(lib().mpg_compact(self._h, ctypes.byref(n)))
+        _check(self._lib.mpg_compact(self._h, ctypes.byref(n)))
         return n.value
 
     def pages(self, layer, which):

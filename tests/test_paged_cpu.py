@@ -136,3 +136,14 @@ def test_rotate_refuses_turns_that_are_none():
     assert L.mpg_rotate(ctypes.byref(t), 0, 1, 1, 64, 17, 64, 64, 16, 16, 64, 64, None) == -1  # misaligned
     assert L.mpg_rotate(ctypes.byref(t), 0, 1, 1, 64, 16, 64, 64, 16, 16, 128, 64, None) == -1  # in place, other strides
     assert L.mpg_rotate(ctypes.byref(t), 0, 0, 1, 64, None, 64, 64, None, None, 64, 64, None) == 0
+
+
+def test_lists_of_ints():
+    a, p = paged._ints([3, 1, 2], 3)
+    assert list(a) == [3, 1, 2] and p
+    assert paged._ints([])[1] == 0
+    with pytest.raises(ValueError, match="4 needed"):
+        paged._ints([1, 2, 3], 4, "counts")
+    for bad in (1 << 32, 1 << 31, -(1 << 31) - 1):
+        with pytest.raises(ValueError, match="32 bits"):
+            paged._ints([0, bad], 2, "seqs")
