@@ -157,7 +157,9 @@ __device__ inline f32x4 add_odd(const T* v, int x, int d, bool seen, f32x4 o) {
 //   softmax of the rows in registers    (the four lane groups of a row hold 8 keys each)
 //   O^T[D][rows] += V^T . P^T           P^T straight from the scores' registers; lane (r, g): row r, dims 4g + i of each 16
 // The next block's K is on its way while the softmax runs, its V while the next scores are computed. The waves' states
-// meet in LDS at the end.
+// meet in LDS at the end. Bound by memory: 64 sequences at 500 .. 8,001 positions of 4 x 128 (359 MB) 61 us, 5.9 TB/s; 4
+// tokens at 65,540 of 2 x 256 (134 MB) 29.5 us, 4.6 TB/s: five blocks a wave, the first one's latency and the meeting of the
+// states stay uncovered. 1 token at 17 positions 5.4 us: a launch and four reads one behind the other.
 template <typename T, int D, int NRT>
 __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, const Item* __restrict__ items,
                                                                        const int* __restrict__ nitems) {
@@ -378,7 +380,9 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
 //   softmax phase  of its row (two lanes a row), in registers
 // Waves 4-7 run one phase behind waves 0-3, so of a SIMD's two waves one feeds the matrix unit while the other computes
 // weights. K and V come by direct loads into rings of SL steps each; barriers hand over what has landed and free what has
-// been read.
+// been read. Bound by the matrix units, which are busy 55% of the cycles, at the 1.7 to 1.9 GHz that the card's power allows
+// then: a prompt of 4,096 tokens, 32 heads of 128 on 4, 131 us, 1.05 PFLOP/s (a library's product of 16,384^3 1.3); 512 tokens
+// at 9,512 positions, 16 heads of 256 on 2, 84 us and 10 for the join.
 template <int D, int KS>
 struct Chunk {
     static constexpr int NW = 8, RW = NW / KS;                   // waves, waves over the rows
@@ -440,8 +444,8 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
         // ONE: a barrier a step; with rings of two steps two, and copies a step further ahead. Copies go out in the softmax
         // phase, which is the shorter one (in the matrix phase they took 430 of its 1,700 cycles): K of step i + SL - 1 + LEAD
         // and V of the step before it in that of step i, into the places of K of step i - 1 + LEAD and of the V before it.
-        // Those have been read by then: ONE, before the barrier in front of waves 0-3's step i, behind waves 4-7's matrix phase
-        // i - 1; else by the wave's own key group, before the barrier in front.
+        // Those have been read by then: ONE, before the barrier in front of waves 0-3's step i, behind waves 4-7's matrix
+        // phase i - 1; else by the wave's own key group, before the barrier in front.
         constexpr bool ONE = SL >= 3;
         constexpr int LEAD = ONE ? 0 : 1;
         __syncthreads();  // the rings and the flag of the item before have been read
@@ -460,7 +464,8 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
         const bool is = row <= last_row && it.tok0 + tok < a.rows;
         const int hi = is ? min(it.pos0 + tok, it.k1 - 1) : -1, lo = a.window ? it.pos0 + tok - a.window + 1 : 0;
         // keys in [tile_lo, tile_hi] are seen by all rows of the work-group, in [all_lo, all_hi] by all of the wave's
-        const int tile_hi = min(it.pos0 + it.row0 / a.group, it.k1 - 1), tile_lo = a.window ? it.pos0 + last_row / a.group - a.window + 1 : 0;
+        const int tile_hi = min(it.pos0 + it.row0 / a.group, it.k1 - 1);
+        const int tile_lo = a.window ? it.pos0 + last_row / a.group - a.window + 1 : 0;
         const int all_hi = min(it.pos0 + (it.row0 + 32 * wr) / a.group, it.k1 - 1);
         const int all_lo = a.window ? it.pos0 + min(it.row0 + 32 * wr + 31, last_row) / a.group - a.window + 1 : 0;
         // infinities and NaN of V in a tile that crosses some row's bounds: each wave looks through the pieces it has copied
@@ -498,7 +503,8 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
             return *(const Vec8<T>*)(kring + i % SL * C::KSTEP + kaddr + x / NS * C::KTILE + x % NS * 512);
         };
         auto v_of = [&](int i, int x) {  // dim block x % NB, tile x / NB / 2, groups 2 (x / NB % 2) + h
-            return *(const Vec8<T>*)(vring + i % SL * C::VSTEP + vaddr + x / NB / 2 * C::TILE + x / NB % 2 * 2 * D * 16 + x % NB * 512);
+            const int at = x / NB / 2 * C::TILE + x / NB % 2 * 2 * D * 16 + x % NB * 512;
+            return *(const Vec8<T>*)(vring + i % SL * C::VSTEP + vaddr + at);
         };
         constexpr int AHEAD = D == 256 ? 3 : 4, NK = NS * SUB, NVO = 2 * NB * SUB;  // operands on their way ahead; of a step
         auto products = [&](int i, auto with_v, auto with_k) INLINE {  // P.V of step i - 1, scores of step i
@@ -615,7 +621,8 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
                     if (!__any(seen)) continue;
 #pragma unroll
                     for (int i = 0; i < 4 * NB; i++) {
-                        f32x4 y = {o[i / 4][i % 4 * 4], o[i / 4][i % 4 * 4 + 1], o[i / 4][i % 4 * 4 + 2], o[i / 4][i % 4 * 4 + 3]};
+                        const f32x16& z = o[i / 4];
+                        f32x4 y = {z[i % 4 * 4], z[i % 4 * 4 + 1], z[i % 4 * 4 + 2], z[i % 4 * 4 + 3]};
                         y = add_odd<T, D>(v, x, 32 * (i / 4) + 8 * (i % 4) + 4 * h, seen, y);
 #pragma unroll
                         for (int c = 0; c < 4; c++) o[i / 4][i % 4 * 4 + c] = y[c];
@@ -629,7 +636,7 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
         constexpr int OB = NB / KS, BLOCKS = D == 64 ? 1 : 2, DW = 32 * BLOCKS, ROW = DW + 4, PER_ROW = DW / 8;
         static_assert(C::NW * 32 * ROW * 4 <= C::LDS, "output rows");
         float* const rows_lds = (float*)ring + w * 32 * ROW;
-        auto put = [&](auto first, float factor) INLINE {  // blocks first .. first + BLOCKS - 1, times the factor of the lane's row
+        auto put = [&](auto first, float factor) INLINE {  // blocks first .. + BLOCKS - 1, times the factor of the lane's row
 #pragma unroll
             for (int b = 0; b < BLOCKS; b++)
 #pragma unroll

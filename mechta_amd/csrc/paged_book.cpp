@@ -190,8 +190,8 @@ struct Tile {
     int member, tok0, row0, k0, k1, kind;
 };
 constexpr int LEAST_KEYS = 128;  // of a piece: a tile for each wave of few rows
-// Pieces of a kind's tiles: about as many as CUs. Few rows stream fastest from 216 work-groups (1 token at 131,072 positions of
-// 2 x 256: 128 / 192 / 216 / 240 / 256 / 512 of them 59.1 / 51.4 / 51.3 / 52.0 / 52.6 / 59.8 us; 64 sequences of 4 x 128 at
+// Pieces of a kind's tiles: about as many as CUs. Few rows stream fastest from 216 work-groups (1 token at 131,072
+// positions of 2 x 256: 128 / 192 / 216 / 240 / 256 / 512 of them 59.1 / 51.4 / 51.3 / 52.0 / 52.6 / 59.8 us; 64 sequences of 4 x 128 at
 // 3,000: 256 / 512 / 768 64.1 / 69.5 / 71.9) -- or from 256 where 216 would leave a quarter of them without work.
 constexpr int CUS = 256, STREAMS = 216;
 constexpr int WIDE_SPLITS = 8, WIDE_ROWS = 512;
@@ -315,7 +315,8 @@ long long chunk_length(const std::vector<Tile>& tiles, const Shape& g, int kind,
             if (p > 1) rows += (long long)p * TILE_ROWS[kind] * g.kv_heads;
         }
         const double busy = (double)sum / ((double)CUS * most);
-        double c = n <= CUS ? most * key * (.65 + .35 * std::min(1., busy)) + 9 : (double)sum / CUS * key + 9. * n / CUS + .5 * sum / n * key;
+        double c = n <= CUS ? most * key * (.65 + .35 * std::min(1., busy)) + 9
+                            : (double)sum / CUS * key + 9. * n / CUS + .5 * sum / n * key;
         if (rows) c += 3 + 8. * g.head_dim * rows / 5e6;
         if (c < cost) {
             cost = c;

@@ -21,7 +21,7 @@ __device__ inline void store8(T* p, Vec8<T> x) {
 
 // What does not change while a kernel runs, read by all lanes alike, in the constant address space: by scalar loads. (By a
 // vector load, as the compiler chose next to the direct loads' inline assembly, the wait for a page number was a wait for
-// every copy on its way: a 4,096-token prompt took 207 us that way, 160 with scalar loads.)
+// every copy on its way: a 4,096-token prompt, then 160 us with scalar loads, took 207 that way.)
 template <typename T>
 using Uniform = const __attribute__((address_space(4))) T*;
 template <typename T>
