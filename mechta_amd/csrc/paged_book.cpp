@@ -194,6 +194,10 @@ constexpr int LEAST_KEYS = 128;  // of a piece: a tile for each wave of few rows
 // positions of 2 x 256: 128 / 192 / 216 / 240 / 256 / 512 of them 59.1 / 51.4 / 51.3 / 52.0 / 52.6 / 59.8 us; 64 sequences of 4 x 128 at
 // 3,000: 256 / 512 / 768 64.1 / 69.5 / 71.9) -- or from 256 where 216 would leave a quarter of them without work.
 constexpr int CUS = 256, STREAMS = 216;
+// Few rows that none of the tiles is worth a join for: 512 keys of 64 or 128 dims, 256 of 256. (Whole / split, us: a token of
+// 4 x 128 at 400 / 513 / 700 positions 5.8, 6.1, 8.9 / 6.9, 6.9, 7.6; of 12 sequences 9.1, 9.2, 11.6 / 9.1, 9.5, 11.0; of
+// 2 x 256 at 200 / 300 / 400 9.1, 10.9, 12.7 / 10.0, 9.7, 9.5; of 12 9.7, 11.8, 13.6 / 11.1, 11.5, 11.8.)
+constexpr int WHOLE = 512 * 128;
 constexpr int WIDE_SPLITS = 8, WIDE_ROWS = 512;
 }  // namespace
 
@@ -267,15 +271,21 @@ long long shortest(const std::vector<Tile>& tiles, int kv_heads, int places) {
     return lo;
 }
 
-// Few rows: as many pieces as stream fastest, unless that leaves one much longer than a CU's share of the keys: then, and
-// where the tiles are more than the CUs, pieces of three quarters of a share, dealt out as CUs fall free. (A token each of
-// sequences at 500 .. 8,001 positions, 4 x 128, 64 of them: as many pieces as CUs 85 us, pieces of 1/2, 3/4, 1, 3/2 and 2
-// shares 65 / 63 / 66 / 68 / 76; 50 of them 73 and 56 / 54 / 57 / 59 / 58; 30 of them, where the longest piece is 1.6 shares
-// of 1,147 keys, 32 and 35 for 3/4; 64 at 2,000 .. 4,000, the longest 1.4 of 2,858, 66 and 68.)
-long long few_length(const std::vector<Tile>& tiles, int kv_heads) {
+// Few rows: whole where they are short; else as many pieces as stream fastest, unless that leaves one much longer than a
+// CU's share of the keys: then, and where the tiles are more than the CUs, pieces of three quarters of a share, dealt out as
+// CUs fall free. (A token each of sequences at 500 .. 8,001 positions, 4 x 128, 64 of them: as many pieces as CUs 85 us,
+// pieces of 1/2, 3/4, 1, 3/2 and 2 shares 65 / 63 / 66 / 68 / 76; 50 of them 73 and 56 / 54 / 57 / 59 / 58; 30 of them,
+// where the longest piece is 1.6 shares of 1,147 keys, 32 and 35 for 3/4; 64 at 2,000 .. 4,000, the longest 1.4 of 2,858,
+// 66 and 68.)
+long long few_length(const std::vector<Tile>& tiles, const Shape& g) {
+    const int kv_heads = g.kv_heads;
     const long long whole = (long long)tiles.size() * kv_heads;
     long long keys = 0, n = 0, longest = 0;
-    for (const Tile& t : tiles) keys += (long long)(t.k1 - t.k0) * kv_heads;
+    for (const Tile& t : tiles) {
+        keys += (long long)(t.k1 - t.k0) * kv_heads;
+        longest = std::max<long long>(longest, t.k1 - t.k0);
+    }
+    if (longest <= WHOLE / std::max(g.head_dim, 128)) return std::max(1ll, (longest + KEYS - 1) / KEYS);
     const long long share = (keys + CUS - 1) / CUS, dealt = std::max<long long>(LEAST_KEYS, share * 3 / 4) / KEYS;
     if (whole > CUS) return dealt;
     auto count = [&](long long length) {
@@ -354,7 +364,7 @@ void plan_window(const Shape& g, const std::vector<Member>& batch, int window, P
         tok0 += batch[i].count;
     }
     long long length[KINDS];
-    for (int k : {FEW, SOME}) length[k] = few_length(by_kind[k], g.kv_heads);
+    for (int k : {FEW, SOME}) length[k] = few_length(by_kind[k], g);
     double half, many;
     length[HALF] = chunk_length(by_kind[HALF], g, HALF, half);
     length[MANY] = chunk_length(by_kind[MANY], g, MANY, many);

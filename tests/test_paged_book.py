@@ -301,3 +301,10 @@ def test_splits_stay_inside_their_room(shim):
         assert sum(map(len, items)) <= shim.shim_most_items(kv * group, kv, 64, tokens, len(batch))
         assert len(joins) <= shim.shim_most_joins(kv * group, kv, 64, tokens, len(batch))
         assert all(j[4] + j[3] * j[5] <= shim.shim_part_rows() for j in joins)
+
+
+def test_short_rows_are_not_split(shim):
+    for dim, most in [(64, 512), (128, 512), (256, 256)]:
+        for n, split in [(1, False), (most, False), (most + 32, True)]:
+            items, joins = make_plan(shim, 8, 2, dim, [(0, 1, n), (1, 1, 7)], 0)
+            assert bool(joins) == split
