@@ -2,6 +2,7 @@
 #include "paged_book.h"
 
 #include <algorithm>
+#include <functional>
 #include <climits>
 
 #include "../../include/mechta_kv.h"
@@ -302,14 +303,14 @@ long long few_length(const std::vector<Tile>& tiles, const Shape& g) {
     return longest * 5 > share * 7 + 5 * 512 ? dealt : length;
 }
 
+// us per key of a work-group: tiles of 128 and 256 rows, heads of 64, 128 and 256
+constexpr double CHUNK_US[2][3] = {{.0107, .0162, .0295}, {.0155, .029, .062}};
 // Chunks: the cheapest length of a piece by a model of the call in us: a piece's keys, 9 for its beginning and end, the split
-// partials written and read back at 5 TB/s and 3 for the launch that joins them. us per key of a work-group: heads of 64 /
-// 128 / 256 in tiles of 256 rows .0155 / .029 / .062, of 128 rows .0107 / .0162 / .0295. (Pieces that are more than the CUs
-// run in rounds; half a mean piece is added for the last one. Where CUs stand idle behind short pieces the card, limited by its
+// partials written and read back at 5 TB/s and 3 for the launch that joins them. (Pieces that are more than the CUs run in
+// rounds; half a mean piece is added for the last one. Where CUs stand idle behind short pieces the card, limited by its
 // power, runs the others faster: up to .65 of the time.)
 long long chunk_length(const std::vector<Tile>& tiles, const Shape& g, int kind, double& cost) {
-    static const double us[2][3] = {{.0107, .0162, .0295}, {.0155, .029, .062}};
-    const double key = us[kind == MANY][g.head_dim / 128];
+    const double key = CHUNK_US[kind == MANY][g.head_dim / 128];
     long long longest = LEAST_KEYS / KEYS, best = longest;
     for (const Tile& t : tiles) longest = std::max(longest, (long long)(t.k1 - t.k0 + KEYS - 1) / KEYS);
     cost = 1e30;
@@ -335,6 +336,39 @@ long long chunk_length(const std::vector<Tile>& tiles, const Shape& g, int kind,
         if (rows > PART_ROWS) break;  // no room for more
     }
     return best;
+}
+// What a launch for few rows adds to one for chunks, us: 3 before its first product, the keys at 5.5 TB/s or the longest
+// piece, 4 where the pieces have to be joined.
+double few_cost(const std::vector<Tile>& tiles, const Shape& g, long long length) {
+    if (tiles.empty()) return 0;
+    long long keys = 0, longest = 0;
+    bool split = false;
+    for (const Tile& t : tiles) {
+        const int p = pieces_of(t, length);
+        keys += (long long)(t.k1 - t.k0) * g.kv_heads;
+        longest = std::max<long long>(longest, (t.k1 - t.k0 + p - 1) / p);
+        split |= p > 1;
+    }
+    return 3 + std::max(keys * g.head_dim * 4 / 5.5e6, longest * g.head_dim * 7e-5) + (split ? 4 : 0);
+}
+
+// The least that tiles of few rows among a chunk's can take, us: their keys through LDS at 3.2 TB/s; where the pieces are
+// more than the CUs, some CU has two of those that are at least the last CU's.
+double mixed_least(const std::vector<Tile>& tiles, const Shape& g, long long length) {
+    long long keys = 0;
+    std::vector<int> pieces;
+    for (const Tile& t : tiles) {
+        const int p = pieces_of(t, length);
+        pieces.insert(pieces.end(), (size_t)p * g.kv_heads, (t.k1 - t.k0 + p - 1) / p);
+        if (t.kind == FEW || t.kind == SOME) keys += (long long)(t.k1 - t.k0) * g.kv_heads;
+    }
+    double least = keys * g.head_dim * 4 / 3.2e6;
+    if ((int)pieces.size() > CUS) {
+        std::nth_element(pieces.begin(), pieces.begin() + CUS, pieces.end(), std::greater<int>());
+        const int next = pieces[CUS], last = *std::min_element(pieces.begin(), pieces.begin() + CUS);
+        least = std::max(least, (next + last) * CHUNK_US[0][g.head_dim / 128] + 18);
+    }
+    return least;
 }
 }  // namespace
 
@@ -368,7 +402,24 @@ void plan_window(const Shape& g, const std::vector<Member>& batch, int window, P
     double half, many;
     length[HALF] = chunk_length(by_kind[HALF], g, HALF, half);
     length[MANY] = chunk_length(by_kind[MANY], g, MANY, many);
-    by_kind[half <= many ? MANY : HALF].clear();
+    // Few rows among a chunk's tiles fill CUs that its last ones leave idle, and spare a launch, often two. (us apart / among:
+    // 512 tokens and 12 decodes at 500 .. 4,000 positions 31.8 / 23.9 of 4 x 128, 40.8 / 30.6 of 2 x 256; 100 and 20 at 100
+    // .. 400 21.9 / 13.9, 31.8 / 19.8. 64 tokens and 60 decodes at 500 .. 8,000 of 4 x 128 92.7 / 114: those stay apart.)
+    std::vector<Tile> both = by_kind[HALF];
+    for (int k : {FEW, SOME}) both.insert(both.end(), by_kind[k].begin(), by_kind[k].end());
+    double together = 1e30;
+    const bool mixed = !by_kind[HALF].empty() && both.size() > by_kind[HALF].size();
+    const long long joint = mixed ? chunk_length(both, g, HALF, together) : 0;
+    if (mixed) together = std::max(together, mixed_least(both, g, joint));
+    const double apart = std::min(half, many) + few_cost(by_kind[FEW], g, length[FEW]) + few_cost(by_kind[SOME], g, length[SOME]);
+    if (mixed && together <= apart) {
+        for (Tile& t : both) t.kind = HALF;
+        by_kind[HALF] = std::move(both);
+        length[HALF] = joint;
+        for (int k : {FEW, SOME, MANY}) by_kind[k].clear();
+    } else {
+        by_kind[half <= many ? MANY : HALF].clear();
+    }
     std::vector<Tile> tiles;
     for (const auto& v : by_kind) tiles.insert(tiles.end(), v.begin(), v.end());
     long long most[KINDS];

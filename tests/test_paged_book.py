@@ -281,6 +281,14 @@ def test_shapes_go_to_their_kernels(shim, name):
     dim, kv, group, window, batch, kind, split = SHAPES[name]
     items, joins = make_plan(shim, kv * group, kv, dim, [(s, *m) for s, m in enumerate(batch)], window)
     assert items[kind] and any(i[8] >= 0 for i in items[kind]) == split
+    assert "among" not in name or not items[0] + items[1] + items[3]
+
+
+def test_long_decodes_stay_apart_from_a_chunk(shim):
+    """Among the chunk's tiles they would stream slower than on their own."""
+    batch = [(0, 64, 1000)] + [(s, 1, 100 * s) for s in range(10, 70)]
+    items, _ = make_plan(shim, 32, 4, 128, batch, 0)
+    assert items[0] and items[2] + items[3]
 
 
 def test_uneven_sequences_are_shared_out(shim):
