@@ -389,11 +389,10 @@ struct Chunk {
     static constexpr int KT = D <= 128 && KS == 1 ? 64 : KEYS;   // keys of a step for a wave
     static constexpr int SUB = KT / KEYS;                        // 32-key tiles of it
     static constexpr int TILE = KEYS * D * 2;                    // bytes of a tile's K, or V
-    static constexpr int KTILE = TILE + 256;                     // in LDS: K's second 16 keys 128 bytes on (banks)
-    static constexpr int KSTEP = KS * SUB * KTILE, VSTEP = KS * SUB * TILE;
+    static constexpr int STEP = KS * SUB * TILE;                 // of a step's
     static constexpr int SL = D == 256 && KS == 2 ? 2 : 4;
     static constexpr int PIECES = SUB * TILE / 1024 / RW;        // 1 KB pieces of K, and of V, a wave copies a step
-    static constexpr int LDS = SL * (KSTEP + VSTEP);
+    static constexpr int LDS = SL * 2 * STEP;
     static_assert(PIECES >= 1 && TILE / 1024 % PIECES == 0 && LDS <= 150 * 1024, "rings");
 };
 
@@ -405,14 +404,15 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
     __shared__ float sm[C::NW][32], sl[C::NW][32];
     __shared__ int odd;
     unsigned char* const kring = ring;
-    unsigned char* const vring = ring + SL * C::KSTEP;
+    unsigned char* const vring = ring + SL * C::STEP;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h = lane >> 5;
     const int wr = w % C::RW, kg = w / C::RW;
     const bool late = w >= 4;  // the SIMD's second wave
     const int count = *uniform(nitems);
-    const unsigned lds_k = (unsigned)(uintptr_t)(lds_void*)ring, lds_v = lds_k + SL * C::KSTEP, voff = lane * 16;
-    // the K row a lane feeds: m = r goes to key 16 (m / 8 % 2) + 8 (m / 16) + m % 8
-    const int kaddr = kg * SUB * C::KTILE + (r >> 3 & 1) * (16 * D * 2 + 128) + ((r >> 4) * 8 + (r & 7)) * 16 + h * 256;
+    const unsigned lds_k = (unsigned)(uintptr_t)(lds_void*)ring, lds_v = lds_k + SL * C::STEP, voff = lane * 16;
+    // the K row a lane feeds: m = r goes to key 16 (m / 8 % 2) + 8 (m / 16) + m % 8. Tiles lie in LDS as in the pages: every 16
+    // lanes that are served at once have 256 bytes of their own (counted: 1% of the cycles conflict).
+    const int kaddr = kg * SUB * C::TILE + (r >> 3 & 1) * 16 * D * 2 + ((r >> 4) * 8 + (r & 7)) * 16 + h * 256;
     const int vaddr = kg * SUB * C::TILE + h * D * 16 + r * 16;
     for (int n = blockIdx.x; n < count; n += gridDim.x) {
         const Item it = load_item(items + n);
@@ -432,12 +432,12 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
         auto page_of = [&](int j) { return table[key_of(j) >> a.page_shift]; };
         auto offset = [&](int j, int page) { return page * page_bytes + (size_t)(key_of(j) & (a.page - 1)) * D * 2 + at0 * 1024; };
         auto issue_k = [&](int j, size_t off) {
-            const unsigned to = lds_k + j % SL * C::KSTEP + (kg * SUB + own) * C::KTILE + at0 * 1024;
+            const unsigned to = lds_k + j % SL * C::STEP + (kg * SUB + own) * C::TILE + at0 * 1024;
 #pragma unroll
-            for (int p = 0; p < C::PIECES; p++) dma16s(kp + off + p * 1024, voff, to + p * 1024 + (at0 + p >= PER / 2 ? 128 : 0));
+            for (int p = 0; p < C::PIECES; p++) dma16s(kp + off + p * 1024, voff, to + p * 1024);
         };
         auto issue_v = [&](int j, size_t off) {
-            const unsigned to = lds_v + j % SL * C::VSTEP + (kg * SUB + own) * C::TILE + at0 * 1024;
+            const unsigned to = lds_v + j % SL * C::STEP + (kg * SUB + own) * C::TILE + at0 * 1024;
 #pragma unroll
             for (int p = 0; p < C::PIECES; p++) dma16s(vp + off + p * 1024, voff, to + p * 1024);
         };
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
             for (int p = 0; p < C::PIECES; p++) {
                 const int at = wr * C::PIECES + p, k0 = it.k0 + KEYS * tile_of(j, own);
                 if (k0 + KEYS - 1 <= tile_hi && k0 >= tile_lo) break;
-                Vec8<T>* const x = (Vec8<T>*)(vring + j % SL * C::VSTEP + kg * SUB * C::TILE + at * 1024 + lane * 16);
+                Vec8<T>* const x = (Vec8<T>*)(vring + j % SL * C::STEP + kg * SUB * C::TILE + at * 1024 + lane * 16);
                 const Vec8<T> v[1] = {*x};
                 if (odd_values(v)) {
                     *x = finite(v[0]);
@@ -500,11 +500,11 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
             if (i > 0) mend(i - 1);
         };
         auto k_of = [&](int i, int x) {  // operand x of step i: tile x / NS, dims 16 (x % NS) ..
-            return *(const Vec8<T>*)(kring + i % SL * C::KSTEP + kaddr + x / NS * C::KTILE + x % NS * 512);
+            return *(const Vec8<T>*)(kring + i % SL * C::STEP + kaddr + x / NS * C::TILE + x % NS * 512);
         };
         auto v_of = [&](int i, int x) {  // dim block x % NB, tile x / NB / 2, groups 2 (x / NB % 2) + h
             const int at = x / NB / 2 * C::TILE + x / NB % 2 * 2 * D * 16 + x % NB * 512;
-            return *(const Vec8<T>*)(vring + i % SL * C::VSTEP + vaddr + at);
+            return *(const Vec8<T>*)(vring + i % SL * C::STEP + vaddr + at);
         };
         constexpr int AHEAD = D == 256 ? 3 : 4, NK = NS * SUB, NVO = 2 * NB * SUB;  // operands on their way ahead; of a step
         auto products = [&](int i, auto with_v, auto with_k) INLINE {  // P.V of step i - 1, scores of step i
