@@ -380,9 +380,10 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
 //   softmax phase  of its row (two lanes a row), in registers
 // Waves 4-7 run one phase behind waves 0-3, so of a SIMD's two waves one feeds the matrix unit while the other computes
 // weights. K and V come by direct loads into rings of SL steps each; barriers hand over what has landed and free what has
-// been read. Bound by the matrix units, which are busy 55% of the cycles, at the 1.7 to 1.9 GHz that the card's power allows
+// been read. Bound by the matrix units, which are busy 56% of the cycles, at the 1.7 to 1.9 GHz that the card's power allows
 // then: a prompt of 4,096 tokens, 32 heads of 128 on 4, 131 us, 1.05 PFLOP/s (a library's product of 16,384^3 1.3); 512 tokens
-// at 9,512 positions, 16 heads of 256 on 2, 84 us and 10 for the join.
+// at 9,512 positions, 16 heads of 256 on 2, 83 us and 10 for the join. By count, 64 keys at heads of 128 are 1,024 cycles of
+// products and about 950 of softmax for each of a SIMD's two waves; a phase takes some 1,600.
 template <int D, int KS>
 struct Chunk {
     static constexpr int NW = 8, RW = NW / KS;                   // waves, waves over the rows
@@ -411,7 +412,7 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
     const int count = *uniform(nitems);
     const unsigned lds_k = (unsigned)(uintptr_t)(lds_void*)ring, lds_v = lds_k + SL * C::STEP, voff = lane * 16;
     // the K row a lane feeds: m = r goes to key 16 (m / 8 % 2) + 8 (m / 16) + m % 8. Tiles lie in LDS as in the pages: every 16
-    // lanes that are served at once have 256 bytes of their own (counted: 1% of the cycles conflict).
+    // lanes that are served at once have 256 bytes of their own (conflicts in 0.4% of the cycles).
     const int kaddr = kg * SUB * C::TILE + (r >> 3 & 1) * 16 * D * 2 + ((r >> 4) * 8 + (r & 7)) * 16 + h * 256;
     const int vaddr = kg * SUB * C::TILE + h * D * 16 + r * 16;
     for (int n = blockIdx.x; n < count; n += gridDim.x) {
