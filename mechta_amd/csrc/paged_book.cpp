@@ -64,7 +64,11 @@ int Book::reserve(const char* who, int n, const int* seq, const int* count) {
         want += need(len[seq[i]] + count[i]) - (int)table[seq[i]].size();
     }
     if (want > free) return fail(MKV_E_NOMEM, "%s: %lld pages needed, %d free", who, want, free);
-    for (int i = 0; i < n; i++) table[seq[i]].reserve(need(len[seq[i]] + count[i]));  // nothing throws behind this
+    for (int i = 0; i < n; i++) {  // nothing throws behind this
+        std::vector<int>& t = table[seq[i]];
+        const size_t m = need(len[seq[i]] + count[i]);
+        if (m > t.capacity()) t.reserve(std::max(m, 2 * t.capacity()));
+    }
     for (int i = 0; i < n; i++) {
         std::vector<int>& t = table[seq[i]];
         len[seq[i]] += count[i];
