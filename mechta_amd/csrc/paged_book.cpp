@@ -374,6 +374,33 @@ double mixed_least(const std::vector<Tile>& tiles, const Shape& g, long long len
     }
     return least;
 }
+
+// Chunks whose tiles are all about as long and some more than the CUs take in whole rounds: those of the last round cut into
+// pieces for all CUs, where the model above makes that cheaper. The number of tiles cut (the first ones; 0: none), and the
+// length of their pieces in KEYS. (1,050 / 1,100 / 1,200 tokens at 8,000 positions of 4 x 128, 264 to 300 tiles: 202 / 201 /
+// 176 us, cut so 152 / 154 / 168; 2,100 at 16,000 of 2 x 256 589 / 468.)
+int last_round(const std::vector<Tile>& tiles, const Shape& g, int kind, double& cost, long long& length) {
+    const int n = (int)tiles.size() * g.kv_heads, rounds = n / CUS, cut = (int)tiles.size() - rounds * CUS / g.kv_heads;
+    if (!rounds || cut <= 0) return 0;
+    long long sum = 0, longest = 0, last = 0;
+    for (const Tile& t : tiles) {
+        sum += t.k1 - t.k0;
+        longest = std::max<long long>(longest, t.k1 - t.k0);
+    }
+    if (longest * (long long)tiles.size() > sum * 5 / 4) return 0;
+    for (int i = 0; i < cut; i++) last = std::max<long long>(last, (tiles[i].k1 - tiles[i].k0 + KEYS - 1) / KEYS);
+    const int p = CUS / (cut * g.kv_heads);
+    if (p < 3) return 0;  // (of two pieces a tile: 1,500 tokens at 8,000 positions 198 us, 184 with all tiles cut alike)
+    const long long piece = std::max<long long>(LEAST_KEYS / KEYS, (last + p - 1) / p);
+    long long pieces = 0;
+    for (int i = 0; i < cut; i++) pieces += (long long)pieces_of(tiles[i], piece) * g.kv_heads;
+    const double key = CHUNK_US[kind == MANY][g.head_dim / 128], rows = (double)pieces * TILE_ROWS[kind];
+    const double c = rounds * (longest * key + 9) + piece * KEYS * key + 9 + 3 + 8. * g.head_dim * rows / 5e6;
+    if (rows > PART_ROWS || c >= .97 * cost) return 0;
+    cost = c;
+    length = piece;
+    return cut;
+}
 }  // namespace
 
 void plan_window(const Shape& g, const std::vector<Member>& batch, int window, Plan& out) {
@@ -406,6 +433,10 @@ void plan_window(const Shape& g, const std::vector<Member>& batch, int window, P
     double half, many;
     length[HALF] = chunk_length(by_kind[HALF], g, HALF, half);
     length[MANY] = chunk_length(by_kind[MANY], g, MANY, many);
+    long long piece[KINDS] = {};
+    int cut[KINDS] = {};
+    cut[HALF] = last_round(by_kind[HALF], g, HALF, half, piece[HALF]);
+    cut[MANY] = last_round(by_kind[MANY], g, MANY, many, piece[MANY]);
     // Few rows among a chunk's tiles fill CUs that its last ones leave idle, and spare a launch, often two. (us apart / among:
     // 512 tokens and 12 decodes at 500 .. 4,000 positions 31.8 / 23.9 of 4 x 128, 40.8 / 30.6 of 2 x 256; 100 and 20 at 100
     // .. 400 21.9 / 13.9, 31.8 / 19.8. 64 tokens and 60 decodes at 500 .. 8,000 of 4 x 128 92.7 / 114: those stay apart.)
@@ -420,20 +451,25 @@ void plan_window(const Shape& g, const std::vector<Member>& batch, int window, P
         for (Tile& t : both) t.kind = HALF;
         by_kind[HALF] = std::move(both);
         length[HALF] = joint;
+        cut[HALF] = 0;
         for (int k : {FEW, SOME, MANY}) by_kind[k].clear();
     } else {
         by_kind[half <= many ? MANY : HALF].clear();
     }
     std::vector<Tile> tiles;
-    for (const auto& v : by_kind) tiles.insert(tiles.end(), v.begin(), v.end());
-    long long most[KINDS];
-    for (int k = 0; k < KINDS; k++) most[k] = length[k] * KEYS;
+    std::vector<long long> most;  // KEYS of a piece of the tile
+    for (int k = 0; k < KINDS; k++)
+        for (int i = 0; i < (int)by_kind[k].size(); i++) {
+            tiles.push_back(by_kind[k][i]);
+            most.push_back(cut[k] ? i < cut[k] ? piece[k] : 1 << 20 : length[k]);
+        }
     int part = 0, more = 0;  // partials and work items that splits have taken
-    for (const Tile& t : tiles) {
+    for (size_t i = 0; i < tiles.size(); i++) {
+        const Tile& t = tiles[i];
         const Member& m = batch[t.member];
         const int rows = m.count * group, count = std::min(TILE_ROWS[t.kind], rows - t.row0);
         const int units = (t.k1 - t.k0 + KEYS - 1) / KEYS;
-        int splits = (int)((units + most[t.kind] / KEYS - 1) / (most[t.kind] / KEYS));
+        int splits = pieces_of(t, most[i]);
         splits = std::min({splits, (PART_ROWS - part) / (count * g.kv_heads), 1 + (SPLITS_MOST - more) / g.kv_heads});
         if (splits < 2) splits = 1;
         more += (splits - 1) * g.kv_heads;

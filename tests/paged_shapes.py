@@ -16,6 +16,7 @@ SHAPES = {
     "decodes among chunks": (128, 4, 8, 513, [(700, 700), (256, 3001), (33, 97)] + [(1, 400 * i + 5) for i in range(10)], 2, False),
     "decodes among chunks, split": (256, 2, 8, 0, [(1, 1003), (300, 2000), (4, 1001), (300, 2011), (1, 5), (2, 999)], 2, True),
     "decodes among a short chunk": (64, 4, 8, 0, [(1, 30), (100, 300)] + [(1, 37 * i + 1) for i in range(10)], 2, False),
+    "last round of chunks cut": (128, 4, 8, 0, [(1050, 8000)], 2, True),
     "prompt of small tiles": (256, 2, 8, 700, [(1037, 1037)], 2, False),
     "prompts of large tiles, 64": (64, 8, 16, 4096, [(163, 164), (185, 185)], 3, False),
     "prompts of large tiles, 128": (128, 8, 16, 100, [(107, 107), (95, 111), (159, 159), (73, 73)], 3, False),

@@ -316,3 +316,14 @@ def test_short_rows_are_not_split(shim):
         for n, split in [(1, False), (most, False), (most + 32, True)]:
             items, joins = make_plan(shim, 8, 2, dim, [(0, 1, n), (1, 1, 7)], 0)
             assert bool(joins) == split
+
+
+def test_the_last_round_of_chunks_is_cut(shim):
+    """A few tiles more than the CUs: those are cut into pieces for all CUs, the others stay whole."""
+    for kv, group, dim, batch in [(4, 8, 128, [(0, 1050, 8000)]), (4, 8, 128, [(0, 1100, 8000)]), (2, 8, 256, [(0, 2100, 16000)])]:
+        items, joins = make_plan(shim, kv * group, kv, dim, batch, 0)
+        for kind in (2, 3):
+            whole = [i for i in items[kind] if i[8] < 0]
+            pieces = [i for i in items[kind] if i[8] >= 0]
+            if items[kind]:
+                assert len(whole) == 256 and 128 <= len(pieces) <= 256 and max(i[7] - i[6] for i in pieces) <= batch[0][2] / 3 + 32
