@@ -727,6 +727,8 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
 }
 
 // ---- splits of a tile's rows put together ----
+// The sum of a split counts whatever its reference: it is 0 where the row sees nothing of the split, and NaN beside a
+// reference of -inf where the one key that it sees there has a NaN score, which no maximum takes.
 // D / 4 lanes hold a row, four dims each, and read its splits four at a time; a work-group takes 1024 / D rows. Wide: a
 // work-group takes 64 dims of a row; 16 lanes hold them, and each 16 lanes add up every 16th split, with the
 // splits' factors in LDS. (A row whole in a work-group, 32 rows of 121 splits: 7.9 us; by 64 dims 5.2.)
@@ -768,7 +770,10 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
                     const float was = top;
 #pragma unroll
                     for (int s = 0; s < 4; s++) {
-                        if (s0 + s >= j.splits) m[s] = NEG_INF;
+                        if (s0 + s >= j.splits) {
+                            m[s] = NEG_INF;
+                            l[s] = 0.f;
+                        }
                         top = fmaxf(top, m[s]);
                     }
                     if (s0) {
@@ -781,7 +786,7 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
                         const float f = m[s] == NEG_INF ? 0.f : fast_exp2(m[s] - top);
 #pragma unroll
                         for (int i = 0; i < 4; i++) acc[i] += f == 0.f ? 0.f : f * x[s][i];
-                        total += f == 0.f ? 0.f : f * l[s];
+                        total += f * l[s];
                     }
                 };
                 four(0);
@@ -816,7 +821,7 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
             for (int s = tid; s < j.splits; s += 256) {
                 const float m = a.pm[first + (size_t)s * j.count], f = m == NEG_INF ? 0.f : fast_exp2(m - top);
                 factor[s] = f;
-                total += f == 0.f ? 0.f : f * a.pl[first + (size_t)s * j.count];
+                total += f * a.pl[first + (size_t)s * j.count];
             }
 #pragma unroll
             for (int i = 1; i < 64; i *= 2) total += __shfl_xor(total, i);
