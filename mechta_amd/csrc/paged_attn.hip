@@ -314,7 +314,8 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
                 }
             }
         }
-        // the four waves' states of 16 rows at a time: 16 threads a row, 8 dims each and again
+        // the four waves' states of 16 rows at a time: 16 threads a row, 8 dims each and again (a wave that saw nothing of a
+        // row has zeros)
 #pragma unroll
         for (int t = 0; t < NRT; t++) {
             const float sum = add_xor32(add_xor16(l[t]));
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
                     for (int y = 0; y < 2; y++) {
                         const f32x4 z = *(const f32x4*)&so[x][rr][d + 4 * y];
 #pragma unroll
-                        for (int i = 0; i < 4; i++) acc[y][i] += f[x] == 0.f ? 0.f : f[x] * z[i];
+                        for (int i = 0; i < 4; i++) acc[y][i] += f[x] * z[i];
                     }
                 acc[0] *= factor;
                 acc[1] *= factor;
@@ -694,8 +695,7 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
             const f32x4* const take = (const f32x4*)ring + (w ^ C::RW) * (NB / 2 * 256) + lane;
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                if (m == NEG_INF) o[b] = f32x16{};
-                else o[b] *= f;
+                o[b] *= f;
                 if (b / (NB / 2) != kg) {
 #pragma unroll
                     for (int c = 0; c < 4; c++)
@@ -727,8 +727,9 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
 }
 
 // ---- splits of a tile's rows put together ----
-// The sum of a split counts whatever its reference: it is 0 where the row sees nothing of the split, and NaN beside a
-// reference of -inf where the one key that it sees there has a NaN score, which no maximum takes.
+// A split with no weight for a row counts all the same: it is zeros where the row sees nothing of it, and NaN or infinities
+// where the row does see them, which reach it however small their weights (m = -inf beside l = NaN: the one key that the
+// row sees there has a NaN score, which no maximum takes).
 // D / 4 lanes hold a row, four dims each, and read its splits four at a time; a work-group takes 1024 / D rows. Wide: a
 // work-group takes 64 dims of a row; 16 lanes hold them, and each 16 lanes add up every 16th split, with the
 // splits' factors in LDS. (A row whole in a work-group, 32 rows of 121 splits: 7.9 us; by 64 dims 5.2.)
@@ -773,6 +774,7 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
                         if (s0 + s >= j.splits) {
                             m[s] = NEG_INF;
                             l[s] = 0.f;
+                            x[s] = f32x4{};
                         }
                         top = fmaxf(top, m[s]);
                     }
@@ -785,7 +787,7 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
                     for (int s = 0; s < 4; s++) {
                         const float f = m[s] == NEG_INF ? 0.f : fast_exp2(m[s] - top);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) acc[i] += f == 0.f ? 0.f : f * x[s][i];
+                        for (int i = 0; i < 4; i++) acc[i] += f * x[s][i];
                         total += f * l[s];
                     }
                 };
@@ -832,7 +834,7 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
             auto add = [&](int s, f32x4 y) INLINE {
                 const float f = factor[s];
 #pragma unroll
-                for (int c = 0; c < 4; c++) acc[c] += f == 0.f ? 0.f : f * y[c];
+                for (int c = 0; c < 4; c++) acc[c] += f * y[c];
             };
 #pragma unroll
             for (int i = 0; i < EARLY; i++)

@@ -1,5 +1,5 @@
-"""NaN that a row sees only in a part of its keys with no weight of its own, a piece whose only key for the row has a NaN
-score, reaches the row all the same."""
+"""NaN and infinities that a row sees only in a part of its keys with no weight of its own: a piece whose only key for the row
+has a NaN score, pieces and waves whose weights are all too small for 32 bits. They reach the row all the same."""
 import math
 
 import pytest
@@ -57,3 +57,48 @@ def test_a_nan_score_alone_in_a_piece(torch_gpu, pg, typ, dim, kv_heads, window,
             hit[:, -1] = ((pos >= x) & ((pos - window < x) if window else (pos >= 0)))[:, None]
             assert torch.isnan(out[hit]).all(), x
             assert torch.equal(out[~hit], clean[~hit]), x
+
+
+# dim, kv_heads, group, new tokens, length, kind of tile, split over the keys
+FAINT = [(64, 1, 4, 1, 300, 0, False), (128, 2, 8, 1, 3000, 0, True), (128, 1, 8, 1, 40000, 0, True), (256, 2, 8, 4, 200, 1, False),
+         (256, 2, 8, 4, 9000, 1, True), (64, 8, 16, 400, 600, 3, False), (64, 8, 4, 300, 4000, 3, True), (128, 2, 8, 40, 9001, 2, True), (256, 2, 8, 300, 400, 2, False),
+         (64, 1, 16, 200, 9001, 2, True), (256, 2, 8, 512, 9512, 2, True)]
+
+
+def test_faint_batches_go_to_their_kernels(shim):
+    for dim, kv, group, count, n, kind, split in FAINT:
+        items, joins = make_plan(shim, kv * group, kv, dim, [(0, count, n)], 0)
+        assert items[kind] and bool(joins) == split, (dim, count, n, [len(i) for i in items], len(joins))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("typ", ["f16", "bf16"])
+@pytest.mark.parametrize("dim,kv_heads,group,count,n,kind,split", FAINT)
+def test_odd_values_of_weights_too_small(torch_gpu, pg, typ, dim, kv_heads, group, count, n, kind, split):
+    """Every earlier position has a score 4 dim below the new ones' 0: e^-256 at most, zero in 32 bits, and zero times NaN or
+    an infinity is NaN. A weight of exactly e^-256 would make an infinity infinite: one or the other, and never a finite row."""
+    torch = torch_gpu
+    fmt, t = types(torch, pg)[typ]
+    with pg.PagedKv(1, kv_heads * group, kv_heads, dim, n // 64 + 1, page=64, seqs=1, ctx=n, fmt=fmt, tokens=n) as kv:
+        k = torch.zeros(n, kv_heads, dim, dtype=t, device="cuda")
+        k[:n - count] = -4
+        v = rnd(torch, 2, n, kv_heads, dim, dtype=t)
+        for at, c in ((0, n - count), (n - count, count)):
+            kv.begin([0], [c])
+            kv.append(0, k[at:at + c], v[at:at + c])
+        q = torch.ones(count, kv_heads * group, dim, dtype=t, device="cuda")
+        clean = kv.attend(0, q, scale=1.0)
+        close(clean, *attention(q, k, v, n - count, 1.0))
+        old = n - count
+        for x in sorted({0, 31, old // 3, old // 2, old - 70, old - 33, old - 1} & set(range(old))):
+            for value in (math.nan, math.inf):
+                e = element(kv, 1, 0, x, kv_heads - 1, 7)
+                e.fill_(value)
+                out = kv.attend(0, q, scale=1.0)
+                e.copy_(v[x, kv_heads - 1, 7])
+                hit = torch.zeros_like(out, dtype=torch.bool)
+                hit[:, (kv_heads - 1) * group:, 7] = True
+                assert not torch.isfinite(out[hit]).any(), (x, value)
+                if math.isnan(value):
+                    assert torch.isnan(out[hit]).all(), x
+                assert torch.equal(out[~hit], clean[~hit]), (x, value)
