@@ -2,7 +2,6 @@
 #include "paged_book.h"
 
 #include <algorithm>
-#include <functional>
 #include <climits>
 
 #include "../../include/mechta_kv.h"
@@ -113,18 +112,36 @@ int Book::fork(const char* who, int n, const int* src, const int* dst, const int
     return MKV_OK;
 }
 
-int Book::release(const char* who, int n, const int* seq) {
-    if (int rc = distinct(who, n, seq)) return rc;
+void Book::undo_reserve(int n, const int* seq, const int* count) {
+    for (int i = 0; i < n; i++) {  // (the new pages belong to these sequences alone)
+        std::vector<int>& t = table[seq[i]];
+        len[seq[i]] -= count[i];
+        while ((int)t.size() > need(len[seq[i]])) {
+            drop(t.back());
+            t.pop_back();
+        }
+        stale(seq[i], (int)t.size());
+    }
+}
+
+void Book::clear(int n, const int* seq) {
     for (int i = 0; i < n; i++) {
         for (int p : table[seq[i]]) drop(p);
         table[seq[i]].clear();
         len[seq[i]] = 0;
         fresh[seq[i]] = 0;
     }
+}
+
+int Book::release(const char* who, int n, const int* seq, const std::function<int()>& before) {
+    if (int rc = distinct(who, n, seq)) return rc;
+    if (before)
+        if (int rc = before()) return rc;
+    clear(n, seq);
     return MKV_OK;
 }
 
-int Book::set_len(const char* who, int seq, int n, std::vector<Pair>& copies) {
+int Book::set_len(const char* who, int seq, int n, std::vector<Pair>& copies, Cut* cut) {
     if (int rc = distinct(who, 1, &seq)) return rc;
     if (n < 0 || n > len[seq])
         return fail(MKV_E_POS, "%s: length %d of sequence %d, which has %d", who, n, seq, len[seq]);
@@ -136,8 +153,12 @@ int Book::set_len(const char* who, int seq, int n, std::vector<Pair>& copies) {
         for (int k = keep; k < (int)t.size(); k++) given |= owners[t[k]] == 1;
         if (!free && !given) return fail(MKV_E_NOMEM, "%s: no free page for a copy of a shared one", who);
     }
-    if (shared) copies.reserve(1);  // nothing throws behind this
-    while ((int)t.size() > keep) {
+    if (shared) copies.reserve(1);
+    if (cut) {
+        const int from = shared ? keep - 1 : keep;
+        *cut = Cut{len[seq], from, shared, std::vector<int>(t.begin() + from, t.end())};
+    }
+    while ((int)t.size() > keep) {  // nothing throws from here on
         drop(t.back());
         t.pop_back();
     }
@@ -151,6 +172,23 @@ int Book::set_len(const char* who, int seq, int n, std::vector<Pair>& copies) {
     stale(seq, keep);
     len[seq] = n;
     return MKV_OK;
+}
+
+void Book::undo_set_len(int seq, const Cut& cut) {
+    std::vector<int>& t = table[seq];
+    if (cut.copied) {
+        drop(t.back());
+        t.pop_back();
+    }
+    for (int p : cut.pages) {  // the table has room for what it had
+        if (!owners[p]++) {
+            open[p / 64] &= ~(1ull << (p % 64));
+            free--;
+        }
+        t.push_back(p);
+    }
+    len[seq] = cut.len;
+    stale(seq, cut.from);
 }
 
 int Book::compact(std::vector<Pair>& copies) {
@@ -173,11 +211,31 @@ int Book::compact(std::vector<Pair>& copies) {
                 stale(s, k);
                 table[s][k] = to[table[s][k]];
             }
-    for (size_t w = 0; w < open.size(); w++) open[w] = 0;
-    for (int p = used; p < pages; p++) open[p / 64] |= 1ull << (p % 64);
-    low = (size_t)used / 64;
-    if (low >= open.size()) low = open.size() - 1;
+    reopen();
     return (int)copies.size();
+}
+
+void Book::undo_compact(const std::vector<Pair>& copies) {
+    for (const Pair& c : copies) {
+        owners[c.src] = owners[c.dst];
+        owners[c.dst] = 0;
+    }
+    for (int s = 0; s < seqs; s++)
+        for (int k = 0; k < (int)table[s].size(); k++) {  // the holes are in order
+            const auto c = std::lower_bound(copies.begin(), copies.end(), table[s][k],
+                                            [](const Pair& a, int page) { return a.dst < page; });
+            if (c == copies.end() || c->dst != table[s][k]) continue;
+            stale(s, k);
+            table[s][k] = c->src;
+        }
+    reopen();
+}
+
+void Book::reopen() {  // the free pages, by their owners
+    std::fill(open.begin(), open.end(), 0);
+    for (int p = 0; p < pages; p++)
+        if (!owners[p]) open[p / 64] |= 1ull << (p % 64);
+    low = 0;
 }
 
 // ---- plans ----

@@ -3,6 +3,7 @@
 #pragma once
 #include <cstddef>
 #include <cstdint>
+#include <functional>
 #include <vector>
 
 namespace mkv {
@@ -17,7 +18,15 @@ struct Pair {
     int src, dst;
 };
 
-// Which pages belong to whom. Pure host state. Each call checks everything first; a refused one changes nothing.
+// What set_len gave up: the sequence's length and its pages from `from` on; copied: page `from` was replaced by a copy.
+struct Cut {
+    int len, from;
+    bool copied;
+    std::vector<int> pages;
+};
+
+// Which pages belong to whom. Pure host state. Each call checks everything first; a refused one changes nothing. What the
+// device is then told can fail: undo_* put the book back to what it was before the call right before, and never fail.
 struct Book {
     int pages = 0, page = 0, seqs = 0, ctx = 0, free = 0;
     std::vector<int> owners;              // per page
@@ -29,14 +38,21 @@ struct Book {
     void init(int pages, int page, int seqs, int ctx);
     int reserve(const char* who, int n, const int* seq, const int* count);
     int fork(const char* who, int n, const int* src, const int* dst, const int* len, bool own, std::vector<Pair>& copies);
-    int release(const char* who, int n, const int* seq);
-    int set_len(const char* who, int seq, int len, std::vector<Pair>& copies);
+    // before: called when all is checked, before anything changes; where it fails, so does the call
+    int release(const char* who, int n, const int* seq, const std::function<int()>& before = nullptr);
+    int set_len(const char* who, int seq, int len, std::vector<Pair>& copies, Cut* cut = nullptr);
     int compact(std::vector<Pair>& copies);
+    void undo_reserve(int n, const int* seq, const int* count);
+    void undo_fork(int n, const int* dst) { clear(n, dst); }
+    void undo_set_len(int seq, const Cut& cut);
+    void undo_compact(const std::vector<Pair>& copies);
     int need(int len) const { return (len + page - 1) / page; }
 
    private:
     int take();
     void drop(int p);
+    void clear(int n, const int* seq);
+    void reopen();
     void stale(int seq, int from) {
         if (fresh[seq] > from) fresh[seq] = from;
     }

@@ -293,6 +293,22 @@ int end_batch(mpg_store* h, const char* who) {
     return upload(h, &none, who);
 }
 
+// What the device has to do for a call that has changed the book: the batch ends, pages are copied. Where it cannot be told,
+// the book is put back.
+template <typename U>
+int settle(mpg_store* h, const std::vector<Pair>& copies, const char* who, U undo) {
+    int rc;
+    try {
+        rc = end_batch(h, who);
+        if (!rc) rc = copy_pages(h, copies, who);
+    } catch (...) {
+        undo();
+        throw;
+    }
+    if (rc) undo();
+    return rc;
+}
+
 int check_batch(const mpg_store* h, int rows, const char* who) {
     if (h->tokens < 0) return fail(MKV_E_ARG, "%s: no batch stands (mpg_begin)", who);
     if (rows < h->tokens) return fail(MKV_E_SIZE, "%s: %d rows, the batch has %d tokens", who, rows, h->tokens);
@@ -480,7 +496,7 @@ int mpg_reserve(mpg_t* h, int n, const int* seq, const int* count) {
     MPG_HOST_CALL(h, "mpg_reserve");
     return guarded("mpg_reserve", [&] {
         if (int rc = h->book.reserve("mpg_reserve", n, seq, count)) return rc;
-        return end_batch(h, "mpg_reserve");
+        return settle(h, {}, "mpg_reserve", [&] { h->book.undo_reserve(n, seq, count); });
     });
 }
 
@@ -513,19 +529,15 @@ static int begin(mpg_t* h, int n, const int* seq, const int* count, int* tokens)
     for (int i = 0; i < n && seq && count; i++) sum += std::max(count[i], 0);
     if (sum > h->c.tokens)
         return fail(MKV_E_ARG, "mpg_begin: %lld tokens, the handle's batches have at most %d", sum, h->c.tokens);
-    std::vector<Pair> none;
     if (int rc = h->book.reserve("mpg_begin", n, seq, count)) return rc;
     h->tokens = -1;  // until the new one is on its way
-    auto back = [&] {  // (the last pages belong to these sequences alone: nothing to copy)
-        for (int i = 0; i < n; i++) (void)h->book.set_len("mpg_begin", seq[i], h->book.len[seq[i]] - count[i], none);
-    };
     try {
         const int rc = lay_out(h, n, seq, count);
-        if (rc) back();
+        if (rc) h->book.undo_reserve(n, seq, count);
         else if (tokens) *tokens = h->tokens;
         return rc;
     } catch (...) {
-        back();
+        h->book.undo_reserve(n, seq, count);
         throw;
     }
 }
@@ -538,9 +550,9 @@ int mpg_set_len(mpg_t* h, int seq, int len) {
     MPG_HOST_CALL(h, "mpg_set_len");
     return guarded("mpg_set_len", [&] {
         std::vector<Pair> copies;
-        if (int rc = h->book.set_len("mpg_set_len", seq, len, copies)) return rc;
-        if (int rc = end_batch(h, "mpg_set_len")) return rc;
-        return copy_pages(h, copies, "mpg_set_len");
+        Cut cut;
+        if (int rc = h->book.set_len("mpg_set_len", seq, len, copies, &cut)) return rc;
+        return settle(h, copies, "mpg_set_len", [&] { h->book.undo_set_len(seq, cut); });
     });
 }
 
@@ -549,8 +561,7 @@ static int fork_pages(mpg_t* h, int n, const int* src, const int* dst, const int
     return guarded(who, [&] {
         std::vector<Pair> copies;
         if (int rc = h->book.fork(who, n, src, dst, len, own, copies)) return rc;
-        if (int rc = end_batch(h, who)) return rc;
-        return copy_pages(h, copies, who);
+        return settle(h, copies, who, [&] { h->book.undo_fork(n, dst); });
     });
 }
 
@@ -564,8 +575,7 @@ int mpg_copy(mpg_t* h, int n, const int* src, const int* dst) {
 int mpg_free(mpg_t* h, int n, const int* seq) {
     MPG_HOST_CALL(h, "mpg_free");
     return guarded("mpg_free", [&] {
-        if (int rc = h->book.release("mpg_free", n, seq)) return rc;
-        return end_batch(h, "mpg_free");
+        return h->book.release("mpg_free", n, seq, [&] { return end_batch(h, "mpg_free"); });
     });
 }
 
@@ -574,9 +584,9 @@ int mpg_compact(mpg_t* h, int* moved) {
     return guarded("mpg_compact", [&] {
         std::vector<Pair> copies;
         const int n = h->book.compact(copies);
+        if (int rc = settle(h, copies, "mpg_compact", [&] { h->book.undo_compact(copies); })) return rc;
         if (moved) *moved = n;
-        if (int rc = end_batch(h, "mpg_compact")) return rc;
-        return copy_pages(h, copies, "mpg_compact");
+        return MKV_OK;
     });
 }
 
