@@ -1,7 +1,8 @@
 /* mechta_paged.h -- many sequences on one paged K/V cache on one MI355X, in the same library as mechta_kv.h
  * (libmechta_kv.so). Error codes are the MKV_E_* of mechta_kv.h and the message of a failed call is in
  * mkv_last_error(); a refused call changes nothing and enqueues nothing, and one that fails on its way to the device (MKV_E_HIP,
- * or MKV_E_NOMEM of the host) leaves every sequence as it was, so that it can be made again.
+ * or MKV_E_NOMEM of the host) leaves every sequence as it was, so that it can be made again, and the batch too, unless it
+ * was the copying of pages that failed: then no batch stands.
  *
  * A handle owns a pool of `pages` pages. A page holds `page` consecutive positions of one sequence, K and V of every
  * layer. Sequences are numbered 0 .. seqs - 1; a sequence is the list of its pages and a length, both kept on the host

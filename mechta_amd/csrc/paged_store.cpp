@@ -51,7 +51,8 @@ struct mpg_store {
     int turn = 0;
     int tokens = -1;                // of the batch; -1: none stands
     int nruns = 0, longest = 0;     // its runs, and the tokens of the longest
-    std::vector<Plan> plans;        // per window, of the batch
+    bool listed = false;            // the lists on the device are a batch's: replays would do it
+    std::vector<Plan> plans, next;  // per window, of the batch and of the one that is being laid out
 };
 
 namespace {
@@ -208,8 +209,9 @@ int copy_pages(mpg_store* h, const std::vector<Pair>& copies, const char* who) {
     return e == hipSuccess ? MKV_OK : hip_fail(e, who);
 }
 
-// The new entries of the page tables, and with `batch` its runs and lists, to the device.
-int upload(mpg_store* h, const std::vector<Run>* runs, const char* who) {
+// The new entries of the page tables to the device, and with `runs` the lists of a batch: its runs and plans, or (plans NULL)
+// none. A call that fails has sent nothing.
+int upload(mpg_store* h, const std::vector<Run>* runs, const std::vector<Plan>* plans, const char* who) {
     std::vector<Segment> segs;
     size_t at = 0;  // words of payload so far
     auto add = [&](size_t dst, size_t words) {
@@ -239,11 +241,14 @@ int upload(mpg_store* h, const std::vector<Run>* runs, const char* who) {
         for (const Run& r : *runs) run_count[1] = std::max(run_count[1], r.count);
         put(h->runs_at, run_count, COUNTS);
         put(h->runs_at + COUNTS, runs->data(), runs->size() * (sizeof(Run) / 4));
-        counts.resize(h->plans.size());
-        for (size_t w = 0; w < h->plans.size(); w++) {
-            const Plan& p = h->plans[w];
+        counts.assign(h->kinds.size(), std::vector<int>(COUNTS, 0));
+        for (size_t w = 0; w < h->kinds.size(); w++) {
             const size_t base = h->batch_at + w * h->lists.words;
-            counts[w].assign(COUNTS, 0);
+            if (!plans) {
+                put(base, counts[w].data(), COUNTS);
+                continue;
+            }
+            const Plan& p = (*plans)[w];
             for (int k = 0; k < KINDS; k++) counts[w][k] = (int)p.items[k].size();
             counts[w][KINDS] = (int)p.joins.size();
             put(base, counts[w].data(), COUNTS);
@@ -277,20 +282,27 @@ int upload(mpg_store* h, const std::vector<Run>* runs, const char* who) {
         to += p.words;
     }
     e = launch_apply(h->dev, h->stage[slot], (int)segs.size(), h->stream);
-    if (e == hipSuccess) e = hipEventRecord(h->done[slot], h->stream);
     if (e != hipSuccess) return hip_fail(e, who);
+    if (hipEventRecord(h->done[slot], h->stream) != hipSuccess) {
+        // on its way all the same, but nothing will tell when the buffer has been read: it is neither written nor freed again
+        (void)hipGetLastError();
+        h->stage[slot] = nullptr;
+        h->stage_words[slot] = 0;
+    }
     h->turn = (slot + 1) % RING;
     for (int s = 0; s < b.seqs; s++) b.fresh[s] = (int)b.table[s].size();
     return MKV_OK;
 }
 
-// What replays of captured calls do once pages have changed hands and no batch stands: nothing.
+// What replays of captured calls do once pages have changed hands and no batch stands: nothing. The batch stands until the
+// empty lists are on their way.
 int end_batch(mpg_store* h, const char* who) {
-    if (h->tokens < 0) return MKV_OK;
-    h->tokens = -1;
-    for (Plan& p : h->plans) p = Plan{};
+    if (!h->listed) return MKV_OK;
     const std::vector<Run> none;
-    return upload(h, &none, who);
+    if (const int rc = upload(h, &none, nullptr, who)) return rc;
+    h->listed = false;
+    h->tokens = -1;
+    return MKV_OK;
 }
 
 // What the device has to do for a call that has changed the book: the batch ends, pages are copied. Where it cannot be told,
@@ -394,6 +406,7 @@ static int create(mpg_t** out, const mpg_config* c, const int* windows, const mp
     h->windows = per_layer;
     h->kinds = kinds;
     h->plans.resize(kinds.size());
+    h->next.resize(kinds.size());
     h->has_rope = rope != nullptr;
     if (rope) h->rope = rope_args(*rope);
     h->stream = (hipStream_t)stream;
@@ -500,7 +513,8 @@ int mpg_reserve(mpg_t* h, int n, const int* seq, const int* count) {
     });
 }
 
-// The batch of sequences that have been lengthened already: its runs, its plans, and both on their way to the device.
+// The batch of sequences that have been lengthened already: its runs, its plans, and both on their way to the device. Where
+// that fails the batch before stands.
 static int lay_out(mpg_t* h, int n, const int* seq, const int* count) {
     std::vector<Member> batch;
     std::vector<Run> runs;
@@ -516,8 +530,10 @@ static int lay_out(mpg_t* h, int n, const int* seq, const int* count) {
             longest = std::max(longest, m);
         }
     }
-    for (size_t w = 0; w < h->kinds.size(); w++) plan_window(h->shape, batch, h->kinds[w], h->plans[w]);
-    if (int rc = upload(h, &runs, "mpg_begin")) return rc;
+    for (size_t w = 0; w < h->kinds.size(); w++) plan_window(h->shape, batch, h->kinds[w], h->next[w]);
+    if (int rc = upload(h, &runs, &h->next, "mpg_begin")) return rc;
+    h->listed = true;
+    h->plans.swap(h->next);
     h->tokens = tok;
     h->nruns = (int)runs.size();
     h->longest = longest;
@@ -530,7 +546,6 @@ static int begin(mpg_t* h, int n, const int* seq, const int* count, int* tokens)
     if (sum > h->c.tokens)
         return fail(MKV_E_ARG, "mpg_begin: %lld tokens, the handle's batches have at most %d", sum, h->c.tokens);
     if (int rc = h->book.reserve("mpg_begin", n, seq, count)) return rc;
-    h->tokens = -1;  // until the new one is on its way
     try {
         const int rc = lay_out(h, n, seq, count);
         if (rc) h->book.undo_reserve(n, seq, count);
@@ -672,7 +687,7 @@ int mpg_read_rows(mpg_t* h, int layer, int which, int seq, int p0, int p1, void*
     if (cap && b.fresh[seq] < (int)b.table[seq].size())
         return fail(MKV_E_ARG, "mpg_read_rows: the device does not have the sequence's pages yet; read once before capturing");
     if (!cap)
-        if (int rc = guarded("mpg_read_rows", [&] { return upload(h, nullptr, "mpg_read_rows"); })) return rc;
+        if (int rc = guarded("mpg_read_rows", [&] { return upload(h, nullptr, nullptr, "mpg_read_rows"); })) return rc;
     const hipError_t e = launch_read(h->g, h->pool, layer, which, h->dev + (size_t)seq * h->g.most_pages, p0, p1, dst, h->stream);
     return e == hipSuccess ? MKV_OK : hip_fail(e, "mpg_read_rows");
 }

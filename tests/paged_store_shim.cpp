@@ -24,7 +24,7 @@ void operator delete(void* p) noexcept { free(p); }
 void operator delete(void* p, size_t) noexcept { free(p); }
 
 static char message[512];
-static int capturing_now = 0, copied = 0, appended = 0, attended = 0;
+static int record_fails = 0, capturing_now = 0, copied = 0, appended = 0, attended = 0;
 namespace mkv {
 int fail(int code, const char* fmt, ...) {
     va_list ap;
@@ -103,7 +103,7 @@ hipError_t hipEventDestroy(hipEvent_t e) {
     free(e);
     return hipSuccess;
 }
-hipError_t hipEventRecord(hipEvent_t, hipStream_t) { return step(hipErrorUnknown); }
+hipError_t hipEventRecord(hipEvent_t, hipStream_t) { return record_fails ? hipErrorUnknown : step(hipErrorUnknown); }
 hipError_t hipEventSynchronize(hipEvent_t) { return step(hipErrorUnknown); }
 hipError_t hipStreamSynchronize(hipStream_t) { return hipSuccess; }
 hipError_t hipStreamIsCapturing(hipStream_t, hipStreamCaptureStatus* st) {
@@ -117,6 +117,7 @@ void shim_fail_after(long n) {  // the fallible step after the next n fails; -1:
     steps = 0;
 }
 long shim_steps() { return steps; }
+void shim_fail_records(int on) { record_fails = on; }
 int shim_copied() { return copied; }
 int shim_launches() { return appended + attended; }
 int shim_owners(const mpg_t* h, int page) { return h->book.owners[page]; }

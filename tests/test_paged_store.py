@@ -234,10 +234,48 @@ def test_random_histories_with_failures(shim, seed):
                 s.content[x] = s.content[src][:m]
             s.write()
         assert all(s.holds(x, s.content[x]) for x in range(s.SEQS)), op
+        s.check_device()
         owned = sum((s.table(x) for x in range(s.SEQS)), [])
         assert s.state()[3] == [owned.count(p) for p in range(s.PAGES)] and s.state()[2] == s.PAGES - len(set(owned))
         for x in range(s.SEQS):  # what the device has of the tables, but for what it will be sent
             sent = min(shim.shim_fresh(s.h, x), len(s.table(x)))
             assert [shim.shim_device_table(s.h, x, k) for k in range(sent)] == s.table(x)[:sent]
     assert failed > 30 and done > 100
+    s.close()
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_a_failed_page_call_leaves_no_stale_batch(shim, name):
+    """Whatever fails: replays do the batch that stands, or nothing; a page call that succeeds then ends it."""
+    failed = 0
+    for s, ok in each_failure(shim, CALLS[name]):
+        s.check_device()
+        stands = shim.shim_tokens(s.h) >= 0
+        assert s.eager() == ((0, 0) if stands else (-1, -1)) and not (ok and stands)
+        assert shim.mpg_free(s.h, 1, ints([3])) == 0
+        assert shim.shim_tokens(s.h) == -1 and not s.runs() and not shim.shim_work(s.h, 0) and not shim.shim_work(s.h, 1)
+        failed += not ok
+    assert failed > 4
+
+
+def test_a_failed_begin_leaves_the_batch_before(shim):
+    failed = 0
+    for s, ok in each_failure(shim, lambda s: s.begin([2, 4, 0], [60, 3, 20])):
+        s.check_device()
+        assert shim.shim_tokens(s.h) == (83 if ok else 10) and s.eager() == (0, 0)
+        assert shim.mpg_free(s.h, 1, ints([3])) == 0 and not s.runs()
+        assert s.begin([2, 4], [1, 1]) == 0
+        s.check_device()
+        failed += not ok
+    assert failed > 4
+
+
+def test_uploads_go_on_behind_an_event_that_was_not_recorded(shim):
+    """The lists went out: the call has succeeded."""
+    s = filled(shim)
+    for i in range(12):
+        shim.shim_fail_records(i % 3 != 0)
+        assert s.begin([2], [1]) == 0, shim.shim_message()
+        shim.shim_fail_records(0)
+        s.check_device()
     s.close()
