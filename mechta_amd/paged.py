@@ -228,8 +228,9 @@ class PagedKv:
         self._raw, self._now = s.cuda_stream, torch._C._cuda_getCurrentRawStream  # (a torch stream object costs 2 us a call)
 
     def close(self):
-        """Frees the cache's memory now (tensors that pages() gave must not be used any more); without it, it is freed with
-        the last of the cache and those tensors."""
+        """Frees the cache's memory now (tensors that pages() gave must not be used any more; every call is refused from here
+        on); without it, it is freed with the last of the cache and those tensors."""
+        self._views.clear()
         self._owner.close()
         self._h = self._owner.ptr
 

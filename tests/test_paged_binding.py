@@ -1,0 +1,24 @@
+"""The paged cache's Python binding: what it keeps, and what it refuses by itself."""
+import pytest
+
+from mechta_amd import paged
+
+
+def test_pages_are_refused_after_close():
+    """The tensors over the pool given before are of memory that is free now: none is given again."""
+    kv = paged.PagedKv.__new__(paged.PagedKv)  # (as after close() on a device)
+    kv._owner = paged._Handle()
+    kv._views = {(0, paged.K): "a tensor over the pool"}
+    kv.close()
+    with pytest.raises(paged.MkvError, match="NULL handle"):
+        kv.pages(0, paged.K)
+
+
+@pytest.mark.gpu
+def test_pages_are_refused_after_close_on_the_device(torch_gpu):
+    kv = paged.PagedKv(1, 2, 1, 64, 4, page=32, seqs=1)
+    assert kv.pages(0, paged.V).shape[0] == 4 and kv.pages(0, paged.K) is kv.pages(0, paged.K)
+    kv.close()
+    for which in (paged.K, paged.V):
+        with pytest.raises(paged.MkvError, match="NULL handle"):
+            kv.pages(0, which)
