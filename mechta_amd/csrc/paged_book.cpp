@@ -461,6 +461,10 @@ int last_round(const std::vector<Tile>& tiles, const Shape& g, int kind, double&
 }
 }  // namespace
 
+int splits_room(int rows, int kv_heads, int part, int more) {
+    return std::min({SPLITS_MOST, (PART_ROWS - part) / (rows * kv_heads), 1 + (SPLITS_MOST - more) / kv_heads});
+}
+
 void plan_window(const Shape& g, const std::vector<Member>& batch, int window, Plan& out) {
     for (auto& v : out.items) v.clear();
     out.joins.clear();
@@ -527,8 +531,7 @@ void plan_window(const Shape& g, const std::vector<Member>& batch, int window, P
         const Member& m = batch[t.member];
         const int rows = m.count * group, count = std::min(TILE_ROWS[t.kind], rows - t.row0);
         const int units = (t.k1 - t.k0 + KEYS - 1) / KEYS;
-        int splits = pieces_of(t, most[i]);
-        splits = std::min({splits, (PART_ROWS - part) / (count * g.kv_heads), 1 + (SPLITS_MOST - more) / g.kv_heads});
+        int splits = std::min(pieces_of(t, most[i]), splits_room(count, g.kv_heads, part, more));
         if (splits < 2) splits = 1;
         more += (splits - 1) * g.kv_heads;
         for (int head = 0; head < g.kv_heads; head++) {

@@ -81,6 +81,8 @@ struct Run {
 enum { FEW, SOME, HALF, MANY, KINDS };  // Item lists by the rows of a tile: 16, 32, 128, 256
 constexpr int TILE_ROWS[KINDS] = {16, 32, 128, 256};
 constexpr int SPLITS_MOST = 1024;  // splits of a tile at most; work-groups that splits add to a plan at most
+// Splits that a tile of so many rows can have at most, behind `part` rows of partials and `more` work items of splits.
+int splits_room(int rows, int kv_heads, int part, int more);
 struct Plan {
     std::vector<Item> items[KINDS];
     std::vector<Join> joins;

@@ -118,6 +118,8 @@ void shim_fail_after(long n) {  // the fallible step after the next n fails; -1:
 }
 long shim_steps() { return steps; }
 void shim_fail_records(int on) { record_fails = on; }
+int shim_splits_room(int rows, int kv_heads, int part, int more) { return splits_room(rows, kv_heads, part, more); }
+int shim_splits_most() { return SPLITS_MOST; }
 int shim_copied() { return copied; }
 int shim_launches() { return appended + attended; }
 int shim_owners(const mpg_t* h, int page) { return h->book.owners[page]; }

@@ -279,3 +279,15 @@ def test_uploads_go_on_behind_an_event_that_was_not_recorded(shim):
         shim.shim_fail_records(0)
         s.check_device()
     s.close()
+
+
+def test_splits_fit_the_join(shim):
+    """The join holds the factors of SPLITS_MOST splits of a row; what all splits add to a plan stays below that too."""
+    most = shim.shim_splits_most()
+    for kv in (1, 2, 3, 8, 64, 1023, 1024):
+        for rows in (1, 16, 33, 256):
+            for part in (0, 65536 - rows * kv, 65536):
+                for more in (0, most // 2, most - 1, most):
+                    n = shim.shim_splits_room(rows, kv, max(part, 0), more)
+                    assert n <= most and (n < 2 or (n - 1) * kv + more <= most and max(part, 0) + n * rows * kv <= 65536)
+    assert shim.shim_splits_room(1, 1, 0, 0) == most
