@@ -119,6 +119,10 @@ class Rope:
         _check(lib().mpg_rope_turns(ctypes.byref(self.c), ctypes.byref(self._turns)))
         self._ptr = ctypes.addressof(self._turns)
 
+    def __setstate__(self, state):  # copies and pickles go by the turns of their own
+        self.__dict__.update(state)
+        self._ptr = ctypes.addressof(self._turns)
+
     def freqs(self):
         """(turning speed of each pair in radians per position, amplitude)."""
         th, amp = (ctypes.c_double * max(self.dim // 2, 1))(), ctypes.c_double()

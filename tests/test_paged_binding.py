@@ -1,4 +1,8 @@
 """The paged cache's Python binding: what it keeps, and what it refuses by itself."""
+import copy
+import ctypes
+import pickle
+
 import pytest
 
 from mechta_amd import paged
@@ -22,3 +26,10 @@ def test_pages_are_refused_after_close_on_the_device(torch_gpu):
     for which in (paged.K, paged.V):
         with pytest.raises(paged.MkvError, match="NULL handle"):
             kv.pages(0, which)
+
+def test_a_copied_rope_goes_by_its_own_turns():
+    """Copies and pickles (a model's configuration on its way to another process) hold no address of another object."""
+    rope = paged.Rope(64, layout="interleaved", base=5e5, scaling="yarn", factor=4.0, original=4096)
+    for other in (copy.copy(rope), copy.deepcopy(rope), pickle.loads(pickle.dumps(rope))):
+        assert other._ptr == ctypes.addressof(other._turns)
+        assert bytes(other._turns) == bytes(rope._turns) and other.freqs() == rope.freqs() and other.dim == 64
