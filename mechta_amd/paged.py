@@ -96,6 +96,21 @@ def _ints(xs, n=None, what="list"):
     return a, a.buffer_info()[0]
 
 
+def _int(x, what):
+    """x, refused where the C ABI's int does not hold it (ctypes would pass on its low 32 bits)."""
+    if not -1 << 31 <= x < 1 << 31:
+        raise ValueError(f"{what} {x} is past 32 bits")
+    return x
+
+
+def _config(layers, q_heads, kv_heads, head_dim, pages, page, seqs, ctx, fmt, tokens):
+    c = _Config()
+    for name, x in dict(layers=layers, q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim, fmt=fmt, pages=pages, page=page,
+                        seqs=seqs, ctx=ctx, tokens=tokens).items():
+        setattr(c, name, _int(x, name))
+    return c
+
+
 def _dtype(fmt):
     import torch
     return {F16: torch.float16, F32: torch.float32, BF16: torch.bfloat16}[fmt]
@@ -112,7 +127,7 @@ class Rope:
             raise ValueError(f"layout {layout!r}: one of {', '.join(LAYOUTS)}")
         if scaling not in SCALINGS:
             raise ValueError(f"scaling {scaling!r}: one of {', '.join(SCALINGS)}")
-        self.c = _Rope(dim, LAYOUTS[layout], SCALINGS[scaling], int(original), base, factor, beta_fast, beta_slow, low,
+        self.c = _Rope(_int(dim, "dim"), LAYOUTS[layout], SCALINGS[scaling], _int(int(original), "original"), base, factor, beta_fast, beta_slow, low,
                        high, amplitude)
         self.dim = dim
         self._turns = _Turns()
@@ -157,10 +172,12 @@ def rotate(x, pos, rope, out=None):
         fmt = _FORMATS.get(dtype)
         if fmt is None:
             raise ValueError(f"x is {dtype}: float16, bfloat16 or float32 needed")
-    if device.type != "cuda":
-        raise ValueError("x must be a device tensor")
     if len(shape) != 3:
         raise ValueError(f"x has shape {tuple(shape)}, (rows, heads, dim) needed")
+    if max(shape) >= 1 << 31:
+        raise ValueError(f"x of shape {tuple(shape)} is past 32 bits")
+    if device.type != "cuda":
+        raise ValueError("x must be a device tensor")
     if out is None:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif out.shape[:1] != shape[:1]:
@@ -219,7 +236,7 @@ class PagedKv:
         self._stream, self.device = s, s.device
         self.layers, self.q_heads, self.kv_heads, self.head_dim = layers, q_heads, kv_heads, head_dim
         self.num_pages, self.page, self.seqs, self.ctx, self.fmt, self.rope = pages, page, seqs, ctx, fmt, rope
-        self._config = _Config(layers, q_heads, kv_heads, head_dim, fmt, pages, page, seqs, ctx, tokens)
+        self._config = _config(layers, q_heads, kv_heads, head_dim, pages, page, seqs, ctx, fmt, tokens)
         w, wp = (None, None) if windows is None else _ints([x or 0 for x in windows], layers, "windows")
         with torch.cuda.device(self.device):
             _check(lib().mpg_create(ctypes.byref(self._owner.ptr), ctypes.byref(self._config), wp,
@@ -262,12 +279,12 @@ class PagedKv:
 
     def length(self, seq):
         n = ctypes.c_int()
-        _check(lib().mpg_len(self._h, seq, ctypes.byref(n)))
+        _check(lib().mpg_len(self._h, _int(seq, "sequence"), ctypes.byref(n)))
         return n.value
 
     def table(self, seq):
         """The sequence's pages, in order."""
-        n = _check(lib().mpg_table(self._h, seq, None, 0))
+        n = _check(lib().mpg_table(self._h, _int(seq, "sequence"), None, 0))
         t = (ctypes.c_int * max(n, 1))()
         _check(lib().mpg_table(self._h, seq, t, n))
         return list(t)[:n]
@@ -292,7 +309,7 @@ class PagedKv:
 
     def set_len(self, seq, n):
         """Shortens a sequence (rollback)."""
-        _check(self._lib.mpg_set_len(self._h, seq, n))
+        _check(self._lib.mpg_set_len(self._h, _int(seq, "sequence"), _int(n, "length")))
 
     def fork(self, src, dst, lens=None):
         """Each empty dst[i] becomes the first lens[i] positions of src[i] (all by default); full pages are shared."""
@@ -324,7 +341,7 @@ class PagedKv:
         if view is None:
             import torch
             base = ctypes.c_void_p()
-            _check(lib().mpg_pages(self._h, layer, which, ctypes.byref(base)))
+            _check(lib().mpg_pages(self._h, _int(layer, "layer"), _int(which, "which"), ctypes.byref(base)))
             h, p, d = self.kv_heads, self.page, self.head_dim
             shape = (self.num_pages, h, p // 16, d // 8, 16, 8) if which == K else (self.num_pages, h, p // 32, 4, d, 8)
 
@@ -345,7 +362,8 @@ class PagedKv:
         _rows(out, self.kv_heads, self.head_dim, self.dtype, self.device, "out")
         if out.shape[0] != n or not out.is_contiguous():
             raise ValueError(f"out must be {n} contiguous rows")
-        _check(lib().mpg_read_rows(self._h, layer, which, seq, p0, p1, ctypes.c_void_p(out.data_ptr())))
+        _check(lib().mpg_read_rows(self._h, _int(layer, "layer"), _int(which, "which"), _int(seq, "sequence"),
+                                   _int(p0, "position"), _int(p1, "position"), ctypes.c_void_p(out.data_ptr())))
         return out
 
     # ---- the layers' calls ----
@@ -375,6 +393,7 @@ class PagedKv:
     def append(self, layer, k, v, q=None, q_out=None, rotate=None):
         """Writes the batch's k and v [tokens, kv_heads, head_dim] into the pages, k rotated (rotate=False: it is already;
         default: if the cache has a rope). With q [tokens, q_heads, head_dim]: returns it rotated, in q_out (may be q)."""
+        _int(layer, "layer")
         rows, h, d = k.shape[0], self.kv_heads, self.head_dim
         kp, kt, kh = _rows(k, h, d, self.dtype, self.device, "k")
         vp, vt, vh = _rows(v, h, d, self.dtype, self.device, "v")
@@ -398,6 +417,7 @@ class PagedKv:
     def attend(self, layer, q, scale=None, sinks=None, gate=None, out=None):
         """Attention of the batch's tokens: q [tokens, q_heads, head_dim] -> out of the same shape. scale: 1/sqrt(head_dim)
         by default; sinks [q_heads] f32; gate as q: out = attention * sigmoid(gate)."""
+        _int(layer, "layer")
         h, d, dtype, device = self.q_heads, self.head_dim, self.dtype, self.device
         qp, qt, qh = _rows(q, h, d, dtype, device, "q")
         rows = q.shape[0]

@@ -4,6 +4,7 @@ import ctypes
 import pickle
 
 import pytest
+import torch
 
 from mechta_amd import paged
 
@@ -33,3 +34,37 @@ def test_a_copied_rope_goes_by_its_own_turns():
     for other in (copy.copy(rope), copy.deepcopy(rope), pickle.loads(pickle.dumps(rope))):
         assert other._ptr == ctypes.addressof(other._turns)
         assert bytes(other._turns) == bytes(rope._turns) and other.freqs() == rope.freqs() and other.dim == 64
+
+
+@pytest.mark.parametrize("past", [1 << 31, 1 << 32, (1 << 32) + 64, -(1 << 31) - 1])
+def test_numbers_past_32_bits_are_refused(past, monkeypatch):
+    """The C ABI's ints would hold their low 32 bits: another layer, sequence or length."""
+    class Library:  # none of these calls may get as far
+        def __getattr__(self, name):
+            return lambda *a: pytest.fail(f"reached {name}")
+
+    kv = paged.PagedKv.__new__(paged.PagedKv)
+    kv._owner, kv._views = paged._Handle(), {}
+    kv._h, kv._lib = kv._owner.ptr, Library()
+    kv.kv_heads = kv.q_heads = 1
+    kv.head_dim, kv.device = 64, torch.device("cpu")
+    kv.dtype = torch.float16
+    k = torch.zeros(1, 1, 64, dtype=torch.float16)
+    monkeypatch.setattr(paged, "lib", Library)
+    for call in (lambda: kv.length(past), lambda: kv.table(past), lambda: kv.set_len(past, 0), lambda: kv.set_len(0, past),
+                 lambda: kv.pages(past, 0), lambda: kv.pages(0, past), lambda: kv.read_rows(past, 0, 0, 0, 1, k),
+                 lambda: kv.read_rows(0, past, 0, 0, 1, k), lambda: kv.read_rows(0, 0, past, 0, 1, k),
+                 lambda: kv.read_rows(0, 0, 0, past, past + 1, k), lambda: kv.append(past, k, k),
+                 lambda: kv.attend(past, k, out=k.clone()), lambda: paged.Rope(past),
+                 lambda: paged.Rope(64, scaling="yarn", factor=2.0, original=past),
+                 lambda: paged._config(1, 2, 1, 64, 8, 32, past, 200, paged.F16, 64),
+                 lambda: paged._config(1, 2, 1, 64, 8, 32, 3, past, paged.F16, 64)):
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
+
+
+@pytest.mark.parametrize("shape", [((1 << 32) + 1, 1, 64), (1, (1 << 32) + 1, 64), (1, 1, (1 << 32) + 64)])
+def test_rows_past_32_bits_are_refused(shape):
+    x = torch.zeros(1, 1, 1, device="meta").expand(shape)
+    with pytest.raises(ValueError, match="32 bits"):
+        paged.rotate(x, torch.empty(0, dtype=torch.int32, device="meta"), paged.Rope(64), out=x)
