@@ -145,7 +145,7 @@ int mpg_compact(mpg_t* h, int* moved);
 /* Writes the batch's K and V rows of one layer into its pages and, with q, rotates the query heads beside.
  *   rows: rows that the arguments hold, the batch's tokens at least (a replay leaves out tokens behind them);
  *   k, v: element (token, kv head, d) at token x *_tok + head x *_head + d (device; 16-byte aligned, strides multiples
- *         of 8 elements, so k and v may be parts of one projection's rows);
+ *         of 8 elements, so k and v may be parts of one projection's rows; any where there is one row, one head);
  *   q:    the same for the q_heads query heads, or NULL; q_out: [tokens][q_heads][head_dim] (device; it may be q, with
  *         those strides, and overlap the arguments in no other way).
  * rotate != 0: K and q are rotated at their tokens' positions by the handle's rope (refused if it has none); 0: K is

@@ -327,9 +327,9 @@ int check_batch(const mpg_store* h, int rows, const char* who) {
     return MKV_OK;
 }
 
-int check_rows(const char* who, const char* what, const void* p, int64_t tok, int64_t head) {
+int check_rows(const char* who, const char* what, const void* p, int rows, int64_t tok, int heads, int64_t head) {
     if (!p) return fail(MKV_E_ARG, "%s: NULL %s", who, what);
-    if ((uintptr_t)p % 16 || tok % 8 || head % 8)
+    if ((uintptr_t)p % 16 || (rows > 1 && tok % 8) || (heads > 1 && head % 8))
         return fail(MKV_E_ARG, "%s: %s must be 16-byte aligned, its strides multiples of 8 elements", who, what);
     return MKV_OK;
 }
@@ -610,14 +610,15 @@ int mpg_append(mpg_t* h, int layer, int rows, const void* k, int64_t k_tok, int6
     if (int rc = check_layer(h, layer, "mpg_append")) return rc;
     if (int rc = check_batch(h, rows, "mpg_append")) return rc;
     if (!rows) return MKV_OK;
-    if (int rc = check_rows("mpg_append", "k", k, k_tok, k_head)) return rc;
-    if (int rc = check_rows("mpg_append", "v", v, v_tok, v_head)) return rc;
+    if (int rc = check_rows("mpg_append", "k", k, rows, k_tok, h->c.kv_heads, k_head)) return rc;
+    if (int rc = check_rows("mpg_append", "v", v, rows, v_tok, h->c.kv_heads, v_head)) return rc;
     if (rotate && !h->has_rope) return fail(MKV_E_ARG, "mpg_append: the handle has no rotary positions");
     if (q) {
         if (!rotate) return fail(MKV_E_ARG, "mpg_append: q without rotation");
-        if (int rc = check_rows("mpg_append", "q", q, q_tok, q_head)) return rc;
-        if (int rc = check_rows("mpg_append", "q_out", q_out, 0, 0)) return rc;
-        if (q == q_out && (q_head != h->c.head_dim || q_tok != (int64_t)h->c.q_heads * h->c.head_dim))
+        if (int rc = check_rows("mpg_append", "q", q, rows, q_tok, h->c.q_heads, q_head)) return rc;
+        if (int rc = check_rows("mpg_append", "q_out", q_out, 1, 0, 1, 0)) return rc;
+        if (q == q_out && ((h->c.q_heads > 1 && q_head != h->c.head_dim) ||
+                           (rows > 1 && q_tok != (int64_t)h->c.q_heads * h->c.head_dim)))
             return fail(MKV_E_ARG, "mpg_append: in place needs q in one piece");
     }
     OnDevice on(h->device);
@@ -636,10 +637,10 @@ int mpg_attend(mpg_t* h, int layer, int rows, const void* q, int64_t q_tok, int6
     if (int rc = check_layer(h, layer, "mpg_attend")) return rc;
     if (int rc = check_batch(h, rows, "mpg_attend")) return rc;
     if (!rows) return MKV_OK;
-    if (int rc = check_rows("mpg_attend", "q", q, q_tok, q_head)) return rc;
-    if (int rc = check_rows("mpg_attend", "out", out, 0, 0)) return rc;
+    if (int rc = check_rows("mpg_attend", "q", q, rows, q_tok, h->c.q_heads, q_head)) return rc;
+    if (int rc = check_rows("mpg_attend", "out", out, 1, 0, 1, 0)) return rc;
     if (gate)
-        if (int rc = check_rows("mpg_attend", "gate", gate, g_tok, g_head)) return rc;
+        if (int rc = check_rows("mpg_attend", "gate", gate, rows, g_tok, h->c.q_heads, g_head)) return rc;
     if (out == q || out == gate) return fail(MKV_E_ARG, "mpg_attend: out takes the place of an input");
     if (!(scale > 0) || !std::isfinite(scale)) return fail(MKV_E_ARG, "mpg_attend: scale %g", scale);
     if ((uintptr_t)sinks % 4) return fail(MKV_E_ARG, "mpg_attend: misaligned sinks");

@@ -68,3 +68,27 @@ def test_rows_past_32_bits_are_refused(shape):
     x = torch.zeros(1, 1, 1, device="meta").expand(shape)
     with pytest.raises(ValueError, match="32 bits"):
         paged.rotate(x, torch.empty(0, dtype=torch.int32, device="meta"), paged.Rope(64), out=x)
+
+
+@pytest.mark.gpu
+def test_one_token_of_odd_strides(torch_gpu):
+    """A token cut from a row of another width is as good as one that was not; q may be rotated in place."""
+    heads, group, dim = 2, 3, 64
+    with paged.PagedKv(1, heads * group, heads, dim, 4, page=32, seqs=2, rope=paged.Rope(dim)) as kv:
+        x = torch.randn(1, heads * (group + 2) * dim + 3, device="cuda").half()
+        assert x.stride(0) % 8
+
+        def parts(x):
+            a = x[:, :heads * (group + 2) * dim].unflatten(1, (-1, dim))
+            return a[:, :heads], a[:, heads:2 * heads], a[:, 2 * heads:]
+
+        ones, got = torch.ones(80, heads, dim, device="cuda").half(), []
+        kv.begin([0, 1], [40, 40])
+        kv.append(0, ones, ones)
+        for seq, y in enumerate((x, x[:, :-3].clone())):
+            kv.begin([seq], [1])
+            k, v, q = parts(y)
+            r = kv.append(0, k, v, q)
+            got.append((r, kv.attend(0, r, gate=q), kv.attend(0, q), kv.read_rows(0, 0, seq), kv.read_rows(0, 1, seq)))
+            assert kv.append(0, k, v, q, q_out=q) is q and torch.equal(q, r)
+        assert all(torch.equal(a, b) for a, b in zip(*got))

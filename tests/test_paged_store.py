@@ -7,6 +7,7 @@ import subprocess
 
 import pytest
 
+from mechta_amd import paged
 from mechta_amd.build import HIPCC
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -32,6 +33,10 @@ def shim(tmp_path_factory):
 
 def ints(xs):
     return (ctypes.c_int * max(len(xs), 1))(*xs)
+
+
+def rope(dim):
+    return ctypes.byref(paged.Rope(dim).c)
 
 
 class Store:
@@ -291,3 +296,24 @@ def test_splits_fit_the_join(shim):
                     n = shim.shim_splits_room(rows, kv, max(part, 0), more)
                     assert n <= most and (n < 2 or (n - 1) * kv + more <= most and max(part, 0) + n * rows * kv <= 65536)
     assert shim.shim_splits_room(1, 1, 0, 0) == most
+
+
+def test_strides_of_one_entry_do_not_matter(shim):
+    """torch gives an axis of one entry whatever stride it was cut with. A second entry's has to fit."""
+    h = P()
+    assert shim.mpg_create(ctypes.byref(h), ints([1, 1, 1, 64, 0, 8, 32, 2, 200, 10]), None, rope(64), None) == 0
+    x, y = P(64), P(128)
+    for n, tok, head, want in [(1, 131, 67, 0), (1, 128, 1, 0), (2, 128, 67, 0), (2, 131, 64, -1)]:
+        assert shim.mpg_begin(h, 1, ints([0]), ints([n]), None) == 0
+        assert shim.mpg_append(h, 0, n, x, tok, head, x, tok, head, x, tok, head, y, 1) == want, (n, tok, head)
+        assert shim.mpg_attend(h, 0, n, x, tok, head, 1.0, None, x, tok, head, y) == want
+        # in place: q in one piece, as far as it has more than one piece
+        assert shim.mpg_append(h, 0, n, x, 64, 64, x, 64, 64, x, tok, head, x, 1) == (0 if n == 1 else -1)
+    assert shim.mpg_append(h, 0, 2, x, 64, 64, x, 64, 64, x, 64, 7, x, 1) == 0
+    assert shim.mpg_destroy(h) == 0
+    s = Store(shim)  # several heads, one token
+    assert s.begin([0], [1]) == 0
+    for head, want in [(64, 0), (65, -1)]:
+        assert shim.mpg_append(s.h, 0, 1, x, 3, head, x, 5, head, None, 0, 0, None, 0) == want
+        assert shim.mpg_attend(s.h, 0, 1, x, 3, head, 1.0, None, None, 0, 0, y) == want
+    s.close()
