@@ -98,8 +98,9 @@ int mpg_rope_turns(const mpg_rope* r, mpg_turns* turns);
 int mpg_rope_freqs(const mpg_rope* r, double* freqs, double* amplitude);
 /* Rotates rows x heads vectors of dim elements at the positions pos[row] (device, int32): out = x rotated, its elements
  * behind r->dim copied. fmt: MKV_F16, MKV_F32 or MPG_BF16. x and out (device): element (row, head, d) at
- * row x *_row + head x *_head + d; out may be x with x's strides, and overlap it in no other way. On the current device,
- * enqueued on `stream`. Products and sums in f32, rounded once. */
+ * row x *_row + head x *_head + d; out may be x with x's strides, and overlap it in no other way; the rows and heads
+ * of out lie apart (strides shorter than a head, or the same for both, are refused). On the current device, enqueued on
+ * `stream`. Products and sums in f32, rounded once. */
 int mpg_rotate(const mpg_turns* r, int fmt, int rows, int heads, int dim, const void* x, int64_t x_row, int64_t x_head,
                const int* pos, void* out, int64_t o_row, int64_t o_head, void* stream);
 

@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <cstring>
 #include <exception>
 #include <memory>
@@ -364,6 +365,9 @@ int mpg_rotate(const mpg_turns* r, int fmt, int rows, int heads, int dim, const 
     if (!x || !pos || !out) return fail(MKV_E_ARG, "mpg_rotate: NULL argument");
     if (x == out && (x_row != o_row || x_head != o_head))
         return fail(MKV_E_ARG, "mpg_rotate: in place needs the same strides");
+    const int64_t row = std::llabs(o_row), head = std::llabs(o_head);
+    if ((rows > 1 && row < dim) || (heads > 1 && head < dim) || (rows > 1 && heads > 1 && row == head))
+        return fail(MKV_E_ARG, "mpg_rotate: rows or heads of out lie on each other (strides %lld, %lld)", (long long)o_row, (long long)o_head);
     const size_t bytes = fmt == MKV_F32 ? 4 : 2;
     if ((uintptr_t)x % bytes || (uintptr_t)out % bytes || (uintptr_t)pos % 4)
         return fail(MKV_E_ARG, "mpg_rotate: misaligned pointer");

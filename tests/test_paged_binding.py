@@ -92,3 +92,14 @@ def test_one_token_of_odd_strides(torch_gpu):
             got.append((r, kv.attend(0, r, gate=q), kv.attend(0, q), kv.read_rows(0, 0, seq), kv.read_rows(0, 1, seq)))
             assert kv.append(0, k, v, q, q_out=q) is q and torch.equal(q, r)
         assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_rotate_refuses_rows_that_lie_on_each_other():
+    """Two threads would write one place, or rotate it twice."""
+    lib, turns = paged.lib(), paged.Rope(64)._ptr
+    # rows, heads, strides of out; x elsewhere and in place
+    for rows, heads, row, head in [(2, 1, 0, 64), (1, 2, 64, 0), (2, 3, 192, 63), (2, 3, -63, 64), (2, 2, 64, 64), (2, 2, 64, -64),
+                                   (5, 1, 1, 0)]:
+        for x in (64, 1 << 20):
+            assert lib.mpg_rotate(turns, 0, rows, heads, 64, x, row, head, 64, 64, row, head, None) == -1, (rows, heads, row, head)
+            assert b"on each other" in lib.mkv_last_error()
