@@ -174,7 +174,8 @@ def rotate(x, pos, rope, out=None):
             raise ValueError(f"x is {dtype}: float16, bfloat16 or float32 needed")
     if len(shape) != 3:
         raise ValueError(f"x has shape {tuple(shape)}, (rows, heads, dim) needed")
-    if max(shape) >= 1 << 31:
+    rows, heads, dim = shape
+    if (rows | heads | dim) >> 31:
         raise ValueError(f"x of shape {tuple(shape)} is past 32 bits")
     if device.type != "cuda":
         raise ValueError("x must be a device tensor")
@@ -182,7 +183,6 @@ def rotate(x, pos, rope, out=None):
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif out.shape[:1] != shape[:1]:
         raise ValueError(f"out has shape {tuple(out.shape)}, x {tuple(shape)}")
-    rows, heads, dim = shape
     xp, xr, xh = _rows(x, heads, dim, dtype, device, "x")
     op, orow, oh = _rows(out, heads, dim, dtype, device, "out")
     if pos.device != device or pos.dtype is not torch.int32 or pos.shape != shape[:1] or not pos.is_contiguous():
@@ -393,7 +393,8 @@ class PagedKv:
     def append(self, layer, k, v, q=None, q_out=None, rotate=None):
         """Writes the batch's k and v [tokens, kv_heads, head_dim] into the pages, k rotated (rotate=False: it is already;
         default: if the cache has a rope). With q [tokens, q_heads, head_dim]: returns it rotated, in q_out (may be q)."""
-        _int(layer, "layer")
+        if not -0x80000000 <= layer < 0x80000000:
+            _int(layer, "layer")
         rows, h, d = k.shape[0], self.kv_heads, self.head_dim
         kp, kt, kh = _rows(k, h, d, self.dtype, self.device, "k")
         vp, vt, vh = _rows(v, h, d, self.dtype, self.device, "v")
@@ -417,7 +418,8 @@ class PagedKv:
     def attend(self, layer, q, scale=None, sinks=None, gate=None, out=None):
         """Attention of the batch's tokens: q [tokens, q_heads, head_dim] -> out of the same shape. scale: 1/sqrt(head_dim)
         by default; sinks [q_heads] f32; gate as q: out = attention * sigmoid(gate)."""
-        _int(layer, "layer")
+        if not -0x80000000 <= layer < 0x80000000:
+            _int(layer, "layer")
         h, d, dtype, device = self.q_heads, self.head_dim, self.dtype, self.device
         qp, qt, qh = _rows(q, h, d, dtype, device, "q")
         rows = q.shape[0]
