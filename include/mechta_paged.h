@@ -16,8 +16,10 @@
  * or until pages change hands (mpg_fork, mpg_copy, mpg_free, mpg_compact, mpg_set_len, mpg_reserve): then appends and
  * attention are refused until a new mpg_begin.
  *
- * Ordering: every call is enqueued on the handle's HIP stream; none waits, except mpg_sync and mpg_destroy (and
- * mpg_begin, where the stream is four of its calls behind). Calls of one handle come from one thread at a time and run
+ * Ordering: every call is enqueued on the handle's HIP stream; none waits, except mpg_create, mpg_sync and mpg_destroy.
+ * What goes up to the device (mpg_begin; the page calls that end a batch; mpg_read_rows, uncaptured, where pages are new)
+ * goes through four pinned buffers: such a call waits where the stream is four of them behind, and for a larger buffer
+ * when it needs one. Calls of one handle come from one thread at a time and run
  * on one stream at a time: the handle's workspaces are shared by all its calls. A call makes the handle's device
  * current while it runs.
  *

@@ -27,7 +27,8 @@ EXTRA = {"kv_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-fno-honor-na
                             "-amdgpu-sched-strategy=max-ilp"], "kv_decode.hip": ["-fno-honor-nans", "-mllvm", "-amdgpu-sched-strategy=max-ilp"],
          "kv_attn32.hip": ["-fno-honor-nans"], "flint_kv.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-fno-honor-nans"],
          "kv_produce.hip": ["-ffp-contract=off"],
-         # accumulators in VGPRs: few_rows of heads of 256 and 32 rows fits its registers (with AGPRs it spilled 35)
+         # accumulators in VGPRs: few_rows of heads of 256 and 32 rows fits its registers (with AGPRs it spilled 35);
+         # chunk_rows of heads of 256 keeps 8 bytes a lane in memory
          "paged_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 # measurement aid of bench.py (a plain HBM read of a given size), its own library: not part of the KV-cache ABI
 PROBE_SRC, PROBE_LIB = "hbm_probe.hip", os.path.join(OUTDIR, "libmkv_probe.so")

@@ -32,7 +32,7 @@ __device__ inline f32x16 mfma32(Vec8<__bf16> a, Vec8<__bf16> b, f32x16 c) {
 }
 
 // The weights 2^(s - ref) of a row are rounded to the cache's type for the matrix units (half a step: 2^-11 of a weight
-// in f16, 2^-8 in bf16; the sum takes them unrounded). ref is the largest score of the first tile, and moves up, with the
+// in f16, 2^-8 in bf16); their sum, in f32, is of the rounded ones, so that a row's weights still add up to one. ref is the largest score of the first tile, and moves up, with the
 // sums rescaled, only where a score exceeds it by more than LAZY. f16 has no room below 2^-14: its weights are taken
 // 2^LIFT times as large, so that a score 24 below the largest still keeps all its bits, and stay below
 // 2^(LIFT + LAZY) = 2^15.
@@ -158,8 +158,8 @@ __device__ inline f32x4 add_odd(const T* v, int x, int d, bool seen, f32x4 o) {
 //   O^T[D][rows] += V^T . P^T           P^T straight from the scores' registers; lane (r, g): row r, dims 4g + i of each 16
 // The next block's K is on its way while the softmax runs, its V while the next scores are computed. The waves' states
 // meet in LDS at the end. Bound by memory: 64 sequences at 500 .. 8,001 positions of 4 x 128 (359 MB) 61 us, 5.9 TB/s; 4
-// tokens at 65,540 of 2 x 256 (134 MB) 29.5 us, 4.6 TB/s: five blocks a wave, the first one's latency and the meeting of the
-// states stay uncovered. 1 token at 17 positions 5.4 us: a launch and four reads one behind the other.
+// tokens at 65,540 of 2 x 256 (134 MB) 29 us, 4.6 TB/s: five blocks a wave, the first one's latency and the meeting of the
+// states stay uncovered. 1 token at 17 positions 5.3 us: a launch and four reads one behind the other.
 template <typename T, int D, int NRT>
 __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, const Item* __restrict__ items,
                                                                        const int* __restrict__ nitems) {
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
 // Waves 4-7 run one phase behind waves 0-3, so of a SIMD's two waves one feeds the matrix unit while the other computes
 // weights. K and V come by direct loads into rings of SL steps each; barriers hand over what has landed and free what has
 // been read. Bound by the matrix units, which are busy 56% of the cycles, at the 1.7 to 1.9 GHz that the card's power allows
-// then: a prompt of 4,096 tokens, 32 heads of 128 on 4, 131 us, 1.05 PFLOP/s (a library's product of 16,384^3 1.3); 512 tokens
+// then: a prompt of 4,096 tokens, 32 heads of 128 on 4, 128 us, 1.07 PFLOP/s (a library's product of 16,384^3 1.3); 512 tokens
 // at 9,512 positions, 16 heads of 256 on 2, 83 us and 10 for the join. By count, 64 keys at heads of 128 are 1,024 cycles of
 // products and about 950 of softmax for each of a SIMD's two waves; a phase takes some 1,600.
 template <int D, int KS>

@@ -7,8 +7,6 @@ namespace paged {
 
 template <typename T>
 using Vec8 = T __attribute__((ext_vector_type(8)));
-template <typename T>
-using Vec4 = T __attribute__((ext_vector_type(4)));
 
 template <typename T>  // 16-byte aligned
 __device__ inline Vec8<T> load8(const T* p) {
