@@ -131,6 +131,10 @@ int mpg_reserve(mpg_t* h, int n, const int* seq, const int* count);
 /* mpg_reserve, and makes them the batch: sequence seq[i]'s last count[i] positions are its new tokens. *tokens: their
  * sum. */
 int mpg_begin(mpg_t* h, int n, const int* seq, const int* count, int* tokens);
+/* mpg_begin for sequences that were forked off one prompt, or off each other: what several of them have in common (whole pages,
+ * each of the same positions) is attended once for all that have it, where the batch's plan finds that to be worth it. Appends
+ * and attention follow as ever, in the batch's order; results differ from mpg_begin's by the rounding of sums in another order. */
+int mpg_begin_shared(mpg_t* h, int n, const int* seq, const int* count, int* tokens);
 /* Shortens a sequence to len positions and gives back the pages behind them (rollback of rejected drafts). A page that
  * becomes partly filled while others own it is copied first. */
 int mpg_set_len(mpg_t* h, int seq, int len);

@@ -62,11 +62,21 @@ struct Args {
     void* out;
     float scale2;  // scale * log2 e
     float *pm, *pl, *pacc;
+    const Place* order;  // tokens of tiles that several sequences share
 };
 
 __device__ inline Item load_item(const Item* p) {
     const Uniform<int> x = uniform((const int*)p);
-    return Item{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], x[8], 0, {0, 0}};
+    return Item{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], x[8], 0, x[10], 0};
+}
+// Token and position of a tile's row (last_row: the tile's last; rows behind it are nobody's).
+__device__ inline Place place_of(const Args& a, const Item& it, int row, int last_row) {
+    if (it.top) return a.order[it.tok0 + min(row, last_row) / a.group];
+    return Place{it.tok0 + row / a.group, it.pos0 + row / a.group};
+}
+// The position of the furthest of rows up to `row`.
+__device__ inline int furthest(const Args& a, const Item& it, int row) {
+    return it.top ? it.top - 1 : it.pos0 + row / a.group;
 }
 
 // The factor of a finished row's sums: 1 / l, with the sink (m: the reference of acc and l, in log2 units).
@@ -181,7 +191,7 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
         const int last_row = min(it.row0 + 16 * NRT, it.rows) - 1;
         // blocks with every key in [all_lo, all_hi] are seen by all rows whole
         const int all_hi = it.pos0 + it.row0 / a.group;
-        const int all_lo = a.window ? it.pos0 + last_row / a.group - a.window + 1 : 0;
+        const int all_lo = a.window ? furthest(a, it, last_row) - a.window + 1 : 0;
         const int blocks = (it.k1 - it.k0 + KEYS - 1) / KEYS;
         auto key_of = [&](int j) { return it.k0 + KEYS * j; };
         auto page_of = [&](int j) { return table[key_of(min(j, blocks - 1)) >> a.page_shift]; };
@@ -213,11 +223,12 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
         int lo[NRT], hi[NRT];  // keys the lane's row sees
 #pragma unroll
         for (int t = 0; t < NRT; t++) {
-            const int row = it.row0 + 16 * t + r, tok = row / a.group, head = it.head * a.group + row % a.group;
-            const bool is = row <= last_row && it.tok0 + tok < a.rows;
-            hi[t] = is ? it.pos0 + tok : -1;
-            lo[t] = a.window ? it.pos0 + tok - a.window + 1 : 0;
-            const T* const src = (const T*)a.q + (int64_t)(it.tok0 + tok) * a.q_tok + head * a.q_head + 8 * g;
+            const int row = it.row0 + 16 * t + r, head = it.head * a.group + row % a.group;
+            const Place at = place_of(a, it, row, last_row);
+            const bool is = row <= last_row && at.tok < a.rows;
+            hi[t] = is ? at.pos : -1;
+            lo[t] = a.window ? at.pos - a.window + 1 : 0;
+            const T* const src = (const T*)a.q + (int64_t)at.tok * a.q_tok + head * a.q_head + 8 * g;
             if constexpr (QLDS) {
                 // each wave brings a quarter of the rows' dims
 #pragma unroll
@@ -328,7 +339,7 @@ __global__ void __launch_bounds__(256, NRT* D <= 256 ? 2 : 1) few_rows(Args a, c
             for (int i = 0; i < NV; i++) *(f32x4*)&so[w][r][16 * i + 4 * g] = o[t][i];
             lds_barrier();
             const int rr = threadIdx.x >> 4, row = it.row0 + 16 * t + rr, tok = it.tok0 + row / a.group;
-            if (row > last_row || tok >= a.rows) continue;
+            if (row > last_row || (it.part < 0 && tok >= a.rows)) continue;
             const int head = it.head * a.group + row % a.group;
             const float top = fmaxf(fmaxf(sm[0][rr], sm[1][rr]), fmaxf(sm[2][rr], sm[3][rr]));
             float f[4], total = 0.f;
@@ -462,14 +473,15 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
         size_t v_next = offset(SL - 2 + LEAD, page_of(SL - 2 + LEAD)), k_next = offset(SL - 1 + LEAD, page_of(SL - 1 + LEAD));
 
         const int row = it.row0 + 32 * wr + r, last_row = min(it.row0 + 32 * C::RW, it.rows) - 1;
-        const int tok = row / a.group, head = it.head * a.group + row % a.group;
-        const bool is = row <= last_row && it.tok0 + tok < a.rows;
-        const int hi = is ? min(it.pos0 + tok, it.k1 - 1) : -1, lo = a.window ? it.pos0 + tok - a.window + 1 : 0;
+        const int head = it.head * a.group + row % a.group;
+        const Place at = place_of(a, it, row, last_row);
+        const bool is = row <= last_row && at.tok < a.rows;
+        const int hi = is ? min(at.pos, it.k1 - 1) : -1, lo = a.window ? at.pos - a.window + 1 : 0;
         // keys in [tile_lo, tile_hi] are seen by all rows of the work-group, in [all_lo, all_hi] by all of the wave's
         const int tile_hi = min(it.pos0 + it.row0 / a.group, it.k1 - 1);
-        const int tile_lo = a.window ? it.pos0 + last_row / a.group - a.window + 1 : 0;
+        const int tile_lo = a.window ? furthest(a, it, last_row) - a.window + 1 : 0;
         const int all_hi = min(it.pos0 + (it.row0 + 32 * wr) / a.group, it.k1 - 1);
-        const int all_lo = a.window ? it.pos0 + min(it.row0 + 32 * wr + 31, last_row) / a.group - a.window + 1 : 0;
+        const int all_lo = a.window ? furthest(a, it, min(it.row0 + 32 * wr + 31, last_row)) - a.window + 1 : 0;
         // infinities and NaN of V in a tile that crosses some row's bounds: each wave looks through the pieces it has copied
         // and puts zeros there before the others read them (add_odd brings them in after the loop)
         auto mend = [&](int j) INLINE {
@@ -486,7 +498,7 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
             }
         };
         Vec8<T> q[NS];
-        const T* const src = (const T*)a.q + (int64_t)(it.tok0 + tok) * a.q_tok + head * a.q_head + 8 * h;
+        const T* const src = (const T*)a.q + (int64_t)at.tok * a.q_tok + head * a.q_head + 8 * h;
 #pragma unroll
         for (int s = 0; s < NS; s++) q[s] = is ? load8(src + 16 * s) : Vec8<T>{};
         f32x16 o[NB], s[SUB];
@@ -653,7 +665,7 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
             for (int i = lane; i < 32 * PER_ROW; i += 64) {
                 const int x = i / PER_ROW, d = i % PER_ROW * 8, row = it.row0 + 32 * wr + x;
                 const int tok = it.tok0 + row / a.group, head = it.head * a.group + row % a.group;
-                if (row > last_row || tok >= a.rows) continue;
+                if (row > last_row || (it.part < 0 && tok >= a.rows)) continue;
                 const f32x4 lo = *(const f32x4*)(rows_lds + x * ROW + d), hi = *(const f32x4*)(rows_lds + x * ROW + d + 4);
                 const int dim = 32 * first + d;
                 if (it.part >= 0) {
@@ -719,7 +731,7 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
             if (kg == 0) finish_rows(low);
             else finish_rows(high);
         }
-        if (it.part >= 0 && kg == 0 && h == 0 && is) {
+        if (it.part >= 0 && kg == 0 && h == 0 && row <= last_row) {
             a.pm[it.part + 32 * wr + r] = m;
             a.pl[it.part + 32 * wr + r] = l;
         }
@@ -734,8 +746,37 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
 // work-group takes 64 dims of a row; 16 lanes hold them, and each 16 lanes add up every 16th split, with the
 // splits' factors in LDS. (A row whole in a work-group, 32 rows of 121 splits: 7.9 us; by 64 dims 5.2.)
 constexpr int JOIN_DIMS = 64;
+//
+// Rows of sequences that share keys have more splits, those of the shared tiles they are in: Seg by Seg behind their own.
+struct Segs {  // of a join; one that it does not have has no splits
+    Seg x[LEVELS];
+    int splits = 0;
+    __device__ Segs(const Seg* p, int n) {
+#pragma unroll
+        for (int i = 0; i < LEVELS; i++) {
+            x[i] = Seg{0, 0, 0, 0};
+            if (i < n) {
+                const Uniform<int> u = uniform((const int*)(p + i));
+                x[i] = Seg{u[0], u[1], u[2], 0};
+                splits += u[2];
+            }
+        }
+    }
+    // the partial of row r of the join in split s of them
+    __device__ size_t row(int s, int r) const {
+        int part = x[0].part, stride = x[0].stride;
+#pragma unroll
+        for (int i = 1, before = x[0].splits; i < LEVELS; before += x[i++].splits)
+            if (s >= before) {
+                part = x[i].part - before * x[i].stride;
+                stride = x[i].stride;
+            }
+        return (size_t)(part + s * stride + r);
+    }
+};
 template <typename T, int D>
-__global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restrict__ joins, const int* __restrict__ njoins) {
+__global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restrict__ joins, const int* __restrict__ njoins,
+                                                   const Seg* __restrict__ segs) {
     __shared__ float factor[SPLITS_MOST];
     __shared__ __attribute__((aligned(16))) f32x4 sa[16][16];
     __shared__ float red[2][4];
@@ -749,7 +790,8 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
     const int ways = max(1, (int)gridDim.x / max(1, count)), way = blockIdx.x % ways;
     for (int n = blockIdx.x / ways; n < count; n += gridDim.x / ways) {
         const Uniform<int> ji = uniform((const int*)(joins + n));
-        const Join j{ji[0], ji[1], ji[2], ji[3], ji[4], ji[5], ji[6], 0};
+        const Join j{ji[0], ji[1], ji[2], ji[3], ji[4], ji[5], ji[6], ji[7]};
+        const Segs shared(segs + (size_t)n * LEVELS, j.segs);
         if (!j.wide) {
             constexpr int LANES = D / 4, GROUPS = 256 / LANES;
             const int d = tid % LANES * 4;
@@ -758,12 +800,13 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
                 if (tok >= a.rows) continue;
                 f32x4 acc = f32x4{};
                 float top = NEG_INF, total = 0.f;
-                auto four = [&](int s0) INLINE {  // splits s0 .. s0 + 3; those behind the last: the last again, not counted
+                // splits s0 .. s0 + 3 of those at `part`; behind the last: the last again, not counted
+                auto four = [&](int part, int stride, int splits, int s0, bool begun) INLINE {
                     float m[4], l[4];
                     f32x4 x[4];
 #pragma unroll
                     for (int s = 0; s < 4; s++) {
-                        const size_t at = j.part + r + (size_t)min(s0 + s, j.splits - 1) * j.count;
+                        const size_t at = part + r + (size_t)min(s0 + s, splits - 1) * stride;
                         m[s] = a.pm[at];
                         l[s] = a.pl[at];
                         x[s] = *(const f32x4*)(a.pacc + at * D + d);
@@ -771,14 +814,14 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
                     const float was = top;
 #pragma unroll
                     for (int s = 0; s < 4; s++) {
-                        if (s0 + s >= j.splits) {
+                        if (s0 + s >= splits) {
                             m[s] = NEG_INF;
                             l[s] = 0.f;
                             x[s] = f32x4{};
                         }
                         top = fmaxf(top, m[s]);
                     }
-                    if (s0) {
+                    if (begun) {
                         const float f = was == NEG_INF ? 0.f : fast_exp2(was - top);
                         acc *= f;
                         total *= f;
@@ -791,8 +834,11 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
                         total += f * l[s];
                     }
                 };
-                four(0);
-                for (int s = 4; s < j.splits; s += 4) four(s);
+                four(j.part, j.count, j.splits, 0, false);
+                for (int s = 4; s < j.splits; s += 4) four(j.part, j.count, j.splits, s, true);
+#pragma unroll
+                for (int i = 0; i < LEVELS; i++)
+                    for (int s = 0; s < shared.x[i].splits; s += 4) four(shared.x[i].part, shared.x[i].stride, shared.x[i].splits, s, true);
                 finish(tok, j.head * a.group + row % a.group, d, acc, top, total);
             }
             continue;
@@ -804,15 +850,15 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
             const int row = j.row0 + r, tok = j.tok0 + row / a.group;
             if (tok >= a.rows) continue;
             const size_t first = j.part + r;
+            const int splits = j.splits + shared.splits;
+            auto partial = [&](int s) INLINE { return s < j.splits ? first + (size_t)s * j.count : shared.row(s - j.splits, r); };
             float top = NEG_INF;
-            for (int s = tid; s < j.splits; s += 256) top = fmaxf(top, a.pm[first + (size_t)s * j.count]);
+            for (int s = tid; s < splits; s += 256) top = fmaxf(top, a.pm[partial(s)]);
             // the first splits' values are on their way meanwhile
             constexpr int EARLY = 8;
-            const float* const src = a.pacc + first * D + d;
-            const size_t step = (size_t)j.count * D;
             f32x4 x[EARLY];
 #pragma unroll
-            for (int i = 0; i < EARLY; i++) x[i] = *(const f32x4*)(src + min(part + 16 * i, j.splits - 1) * step);
+            for (int i = 0; i < EARLY; i++) x[i] = *(const f32x4*)(a.pacc + partial(min(part + 16 * i, splits - 1)) * D + d);
 #pragma unroll
             for (int i = 1; i < 64; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
             __syncthreads();  // the row before has been read
@@ -820,10 +866,11 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
             lds_barrier();
             top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
             float total = 0.f;
-            for (int s = tid; s < j.splits; s += 256) {
-                const float m = a.pm[first + (size_t)s * j.count], f = m == NEG_INF ? 0.f : fast_exp2(m - top);
+            for (int s = tid; s < splits; s += 256) {
+                const size_t at = partial(s);
+                const float m = a.pm[at], f = m == NEG_INF ? 0.f : fast_exp2(m - top);
                 factor[s] = f;
-                total += f * a.pl[first + (size_t)s * j.count];
+                total += f * a.pl[at];
             }
 #pragma unroll
             for (int i = 1; i < 64; i *= 2) total += __shfl_xor(total, i);
@@ -838,9 +885,9 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
             };
 #pragma unroll
             for (int i = 0; i < EARLY; i++)
-                if (part + 16 * i < j.splits) add(part + 16 * i, x[i]);
+                if (part + 16 * i < splits) add(part + 16 * i, x[i]);
 #pragma unroll 4
-            for (int s = part + 16 * EARLY; s < j.splits; s += 16) add(s, *(const f32x4*)(src + s * step));
+            for (int s = part + 16 * EARLY; s < splits; s += 16) add(s, *(const f32x4*)(a.pacc + partial(s) * D + d));
             sa[part][lane] = acc;
             lds_barrier();
             if (part) continue;
@@ -879,6 +926,7 @@ hipError_t attend_as(const Geometry& g, const AttendArgs& x, const int* batch, c
     a.pm = x.pm;
     a.pl = x.pl;
     a.pacc = x.pacc;
+    a.order = x.order;
     hipError_t e = hipSuccess;
     if (grid[FEW]) {
         few_rows<T, D, 1><<<dim3(grid[FEW]), dim3(256), 0, s>>>(a, (const Item*)(batch + l.items[FEW]), batch + FEW);
@@ -904,7 +952,7 @@ hipError_t attend_as(const Geometry& g, const AttendArgs& x, const int* batch, c
                 ways = std::max(ways, j.wide ? j.count * (D / JOIN_DIMS) : (j.count + groups - 1) / groups);
             }
         const int all = std::min(join_grid, MOST_GRID / ways) * ways;
-        join_kernel<T, D><<<dim3(all), dim3(256), 0, s>>>(a, (const Join*)(batch + l.joins), batch + KINDS);
+        join_kernel<T, D><<<dim3(all), dim3(256), 0, s>>>(a, (const Join*)(batch + l.joins), batch + KINDS, (const Seg*)(batch + l.segs));
         e = hipGetLastError();
     }
     return e;

@@ -251,6 +251,7 @@ size_t most_joins(const Shape& g, int tokens, int seqs) { return most_items(g, t
 namespace {
 struct Tile {
     int member, tok0, row0, k0, k1, kind;
+    int range;  // of a shared range, -1: of the member
 };
 constexpr int LEAST_KEYS = 128;  // of a piece: a tile for each wave of few rows
 // Pieces of a kind's tiles: about as many as CUs. Few rows stream fastest from 216 work-groups (1 token at 131,072
@@ -465,20 +466,103 @@ int splits_room(int rows, int kv_heads, int part, int more) {
     return std::min({SPLITS_MOST, (PART_ROWS - part) / (rows * kv_heads), 1 + (SPLITS_MOST - more) / kv_heads});
 }
 
-void plan_window(const Shape& g, const std::vector<Member>& batch, int window, Plan& out) {
+namespace {
+// Which of a batch's common positions are attended once for all that have them. Apart they are read once for each (though the
+// later readings may find them in a cache); together they cost a launch more, or tiles among those there, and their partials.
+struct Sharer {
+    static constexpr int LEAST = 128;         // positions of a range
+    static constexpr int LEAST_SPARED = 512;  // positions that a range spares its sequences, in all
+    static constexpr int ROWS = 256;          // of a sequence with more rows no tile is worth sharing
+    static constexpr int DEEP = 64;           // forks of forks that are looked through
+    const Book& b;
+    const std::vector<Member>& batch;
+    Share& out;
+    const std::vector<int>& table(int i) const { return b.table[batch[i].seq]; }
+    int whole(int i) const { return (batch[i].len - batch[i].count) / b.page; }  // pages before the new tokens
+    // pages that i and j have in common
+    int common(int i, int j) const {
+        const std::vector<int>&x = table(i), &y = table(j);
+        int lo = 0, hi = std::min(whole(i), whole(j));
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (x[mid - 1] == y[mid - 1]) lo = mid;
+            else hi = mid - 1;
+        }
+        return lo;
+    }
+    void leaf(int i, int start, int range) {
+        out.from[i] = start * b.page;
+        out.range[i] = range;
+        out.members.push_back(i);
+    }
+    // who: sequences that have pages [0, probe) in common, of which those before `start` are done by `range` and what it is in
+    void split(std::vector<int>& who, int start, int probe, int range, int level, int deep) {
+        auto page = [&](int i) { return whole(i) > probe ? table(i)[probe] : -1 - i; };
+        if (level == LEVELS || deep == DEEP) {
+            for (int i : who) leaf(i, start, range);
+            return;
+        }
+        std::stable_sort(who.begin(), who.end(), [&](int i, int j) { return page(i) < page(j); });
+        for (size_t x = 0; x < who.size();) {
+            size_t y = x + 1;
+            int end = whole(who[x]);
+            for (; y < who.size() && page(who[y]) == page(who[x]); y++) end = std::min(end, common(who[x], who[y]));
+            if (y - x == 1) {
+                leaf(who[x], start, range);
+            } else {
+                std::vector<int> group(who.begin() + x, who.begin() + y);
+                const long long span = (long long)(end - start) * b.page;
+                const bool pays = span >= LEAST && span * (long long)(group.size() - 1) >= LEAST_SPARED;
+                if (pays) out.ranges.push_back({start * b.page, end * b.page, (int)out.members.size(), (int)group.size(), range});
+                if (pays) split(group, end, end, (int)out.ranges.size() - 1, level + 1, deep + 1);
+                else split(group, start, end, range, level, deep + 1);
+            }
+            x = y;
+        }
+    }
+};
+}  // namespace
+
+void share(const Book& b, const Shape& g, const std::vector<Member>& batch, Share& out) {
+    const int n = (int)batch.size(), group = g.q_heads / g.kv_heads;
+    out = Share{};
+    out.from.assign(n, 0);
+    out.range.assign(n, -1);
+    out.at.assign(n, 0);
+    std::vector<int> who;
+    for (int i = 0; i < n; i++)
+        if (batch[i].count > 0 && (long long)batch[i].count * group <= Sharer::ROWS) who.push_back(i);
+    Sharer s{b, batch, out};
+    s.split(who, 0, 0, -1, 0, 0);
+    if (out.ranges.empty()) return;
+    std::vector<int> tok(n);
+    for (int i = 0, t = 0; i < n; t += batch[i++].count) tok[i] = t;
+    for (int i : out.members) {
+        out.at[i] = (int)out.order.size();
+        for (int t = 0; t < batch[i].count; t++) out.order.push_back({tok[i] + t, batch[i].len - batch[i].count + t});
+    }
+}
+
+static void plan(const Shape& g, const std::vector<Member>& batch, const Share* share, int window, Plan& out) {
     for (auto& v : out.items) v.clear();
     out.joins.clear();
+    out.segs.clear();
     const int group = g.q_heads / g.kv_heads;
     std::vector<Tile> by_kind[KINDS];
     auto add = [&](int i, int tok0, int kind) {
         const Member& m = batch[i];
-        const int rows = m.count * group, pos0 = m.len - m.count;
+        const int rows = m.count * group, pos0 = m.len - m.count, from = share ? share->from[i] : 0;
         for (int r = 0; r < rows; r += TILE_ROWS[kind]) {
             const int last = (std::min(r + TILE_ROWS[kind], rows) - 1) / group;
             const int lo = window ? std::max(0, pos0 + r / group - window + 1) : 0;
-            by_kind[kind].push_back({i, tok0, r, lo / KEYS * KEYS, pos0 + last + 1, kind});
+            by_kind[kind].push_back({i, tok0, r, std::max(from, lo / KEYS * KEYS), pos0 + last + 1, kind, -1});
         }
     };
+    // A shared range in this window: its rows, the keys that any of them sees, where its partials are.
+    struct Common {
+        int rows = 0, tok0 = 0, k0 = 0, part = 0, splits = 0;
+    };
+    std::vector<Common> common(share ? share->ranges.size() : 0);
     int tok0 = 0;
     for (int i = 0; i < (int)batch.size(); i++) {
         const int rows = batch[i].count * group;
@@ -490,6 +574,40 @@ void plan_window(const Shape& g, const std::vector<Member>& batch, int window, P
         }
         tok0 += batch[i].count;
     }
+    for (size_t x = 0; x < common.size(); x++) {
+        const Range& r = share->ranges[x];
+        Common& c = common[x];
+        c.tok0 = share->at[share->members[r.first]];
+        int lo = r.k1;
+        for (int i = r.first; i < r.first + r.count; i++) {
+            const Member& m = batch[share->members[i]];
+            c.rows += m.count * group;
+            lo = std::min(lo, window ? std::max(0, m.len - m.count - window + 1) : 0);
+        }
+        c.k0 = std::max(r.k0, lo / KEYS * KEYS);
+        if (c.k0 >= r.k1) {  // no row sees any of it
+            c.rows = 0;
+            continue;
+        }
+        auto tiles = [&](int kind) {
+            for (int row = 0; row < c.rows; row += TILE_ROWS[kind]) by_kind[kind].push_back({share->members[r.first], c.tok0, row, c.k0, r.k1, kind, (int)x});
+        };
+        if (c.rows <= TILE_ROWS[SOME]) {
+            tiles(c.rows <= TILE_ROWS[FEW] ? FEW : SOME);
+        } else {
+            tiles(HALF);
+            tiles(MANY);
+        }
+    }
+    // the shared ranges that a member's rows have keys in, the outermost first
+    auto chain = [&](int i) {
+        std::vector<int> c;
+        for (int x = share ? share->range[i] : -1; x >= 0; x = share->ranges[x].parent)
+            if (common[x].rows) c.insert(c.begin(), x);
+        return c;
+    };
+    bool any = false;
+    for (const Common& c : common) any |= c.rows > 0;
     long long length[KINDS];
     for (int k : {FEW, SOME}) length[k] = few_length(by_kind[k], g);
     double half, many;
@@ -497,8 +615,10 @@ void plan_window(const Shape& g, const std::vector<Member>& batch, int window, P
     length[MANY] = chunk_length(by_kind[MANY], g, MANY, many);
     long long piece[KINDS] = {};
     int cut[KINDS] = {};
-    cut[HALF] = last_round(by_kind[HALF], g, HALF, half, piece[HALF]);
-    cut[MANY] = last_round(by_kind[MANY], g, MANY, many, piece[MANY]);
+    if (!any) {  // (the tiles of a shared range are split alike)
+        cut[HALF] = last_round(by_kind[HALF], g, HALF, half, piece[HALF]);
+        cut[MANY] = last_round(by_kind[MANY], g, MANY, many, piece[MANY]);
+    }
     // Few rows among a chunk's tiles fill CUs that its last ones leave idle, and spare a launch, often two. (us apart / among:
     // 512 tokens and 12 decodes at 500 .. 4,000 positions 31.8 / 23.9 of 4 x 128, 40.8 / 30.6 of 2 x 256; 100 and 20 at 100
     // .. 400 21.9 / 13.9, 31.8 / 19.8. 64 tokens and 60 decodes at 500 .. 8,000 of 4 x 128 92.7 / 114: those stay apart.)
@@ -526,24 +646,78 @@ void plan_window(const Shape& g, const std::vector<Member>& batch, int window, P
             most.push_back(cut[k] ? i < cut[k] ? piece[k] : 1 << 20 : length[k]);
         }
     int part = 0, more = 0;  // partials and work items that splits have taken
+    // What shared ranges and the rows in them cannot do without: a split's partials each, and the ranges' work items.
+    long long least = 0, items = 0;
+    if (any) {
+        for (const Common& c : common) least += (long long)c.rows * g.kv_heads;
+        for (const Tile& t : tiles) {
+            if (t.range >= 0) items += g.kv_heads;
+            else if (!chain(t.member).empty())
+                least += (long long)std::min(TILE_ROWS[t.kind], batch[t.member].count * group - t.row0) * g.kv_heads;
+        }
+        if (least > PART_ROWS || items > SPLITS_MOST / 2) {
+            plan(g, batch, nullptr, window, out);
+            return;
+        }
+        more = (int)items;
+        for (size_t i = 0; i < tiles.size(); i++) {
+            const Tile& t = tiles[i];
+            if (t.range < 0) continue;
+            Common& c = common[t.range];
+            if (!c.splits) {  // its first tile
+                const int count = (c.rows + TILE_ROWS[t.kind] - 1) / TILE_ROWS[t.kind];
+                least -= (long long)c.rows * g.kv_heads;
+                c.splits = std::min({pieces_of(t, most[i]), splits_room(c.rows, g.kv_heads, part + (int)least, more), SPLITS_MOST / (LEVELS + 1),
+                                     1 + (SPLITS_MOST - more) / (g.kv_heads * count)});
+                c.splits = std::max(c.splits, 1);
+                more += (c.splits - 1) * g.kv_heads * count;
+                c.part = part;
+                part += c.splits * c.rows * g.kv_heads;
+            }
+            const Range& r = share->ranges[t.range];
+            const int units = (t.k1 - t.k0 + KEYS - 1) / KEYS, last = std::min(t.row0 + TILE_ROWS[t.kind], c.rows) - 1;
+            int top = 0;
+            for (int x = t.row0 / group; x <= last / group; x++) top = std::max(top, share->order[c.tok0 + x].pos + 1);
+            for (int head = 0; head < g.kv_heads; head++)
+                for (int s = 0; s < c.splits; s++)
+                    out.items[t.kind].push_back({batch[t.member].seq, head, c.tok0, t.row0, c.rows, r.k1,
+                                                 t.k0 + (int)((long long)units * s / c.splits) * KEYS,
+                                                 s + 1 < c.splits ? t.k0 + (int)((long long)units * (s + 1) / c.splits) * KEYS : t.k1,
+                                                 c.part + (head * c.splits + s) * c.rows + t.row0, s, top, 0});
+        }
+    }
     for (size_t i = 0; i < tiles.size(); i++) {
         const Tile& t = tiles[i];
+        if (t.range >= 0) continue;
         const Member& m = batch[t.member];
         const int rows = m.count * group, count = std::min(TILE_ROWS[t.kind], rows - t.row0);
         const int units = (t.k1 - t.k0 + KEYS - 1) / KEYS;
-        int splits = std::min(pieces_of(t, most[i]), splits_room(count, g.kv_heads, part, more));
+        const std::vector<int> in = any ? chain(t.member) : std::vector<int>();
+        if (!in.empty()) least -= (long long)count * g.kv_heads;
+        int splits = std::min(pieces_of(t, most[i]), splits_room(count, g.kv_heads, part + (int)least, more));
+        if (!in.empty()) splits = std::min(splits, SPLITS_MOST / (LEVELS + 1));
         if (splits < 2) splits = 1;
         more += (splits - 1) * g.kv_heads;
+        const bool joined = splits > 1 || !in.empty();
         for (int head = 0; head < g.kv_heads; head++) {
             for (int s = 0; s < splits; s++) {
                 const int a = t.k0 + (int)((long long)units * s / splits) * KEYS;
                 const int b = s + 1 < splits ? t.k0 + (int)((long long)units * (s + 1) / splits) * KEYS : t.k1;
                 out.items[t.kind].push_back({m.seq, head, t.tok0, t.row0, rows, m.len - m.count, a, b,
-                                             splits > 1 ? part + s * count : -1, s, {0, 0}});
+                                             joined ? part + s * count : -1, s, 0, 0});
             }
-            if (splits > 1) {
-                out.joins.push_back({head, t.tok0, t.row0, count, part, splits, 0, 0});
+            if (joined) {
+                out.joins.push_back({head, t.tok0, t.row0, count, part, splits, 0, (int)in.size()});
                 part += splits * count;
+                for (int x = 0; any && x < LEVELS; x++) {
+                    Seg seg{0, 0, 0, 0};
+                    if (x < (int)in.size()) {
+                        const Common& c = common[in[x]];
+                        const int row = (share->at[t.member] - c.tok0) * group + t.row0;
+                        seg = {c.part + head * c.splits * c.rows + row, c.rows, c.splits, 0};
+                    }
+                    out.segs.push_back(seg);
+                }
             }
         }
     }
@@ -551,13 +725,23 @@ void plan_window(const Shape& g, const std::vector<Member>& batch, int window, P
     // splits by 64 dims each: 45 us, row by row 14).
     long long rows = 0;
     for (const Join& j : out.joins) rows += j.count;
-    for (Join& j : out.joins) j.wide = j.splits > WIDE_SPLITS && rows <= WIDE_ROWS;
+    for (size_t n = 0; n < out.joins.size(); n++) {
+        Join& j = out.joins[n];
+        int splits = j.splits;
+        for (int x = 0; x < j.segs; x++) splits += out.segs[n * LEVELS + x].splits;
+        j.wide = splits > WIDE_SPLITS && rows <= WIDE_ROWS;
+    }
     for (auto& list : out.items) {
         std::stable_sort(list.begin(), list.end(), [](const Item& a, const Item& b) {
             return a.seq != b.seq ? a.seq < b.seq : a.head != b.head ? a.head < b.head : a.split < b.split;
         });
         deal(list);
     }
+}
+
+void plan_window(const Shape& g, const std::vector<Member>& batch, int window, Plan& out) { plan(g, batch, nullptr, window, out); }
+void plan_shared(const Shape& g, const std::vector<Member>& batch, const Share& s, int window, Plan& out) {
+    plan(g, batch, s.ranges.empty() ? nullptr : &s, window, out);
 }
 
 }  // namespace paged

@@ -68,11 +68,24 @@ struct Item {
     int pos0;        // position of the sequence's first new token
     int k0, k1;      // k0 a multiple of KEYS
     int part;        // first row of the split partials it writes, -1: it writes the output
-    int split, pad[2];
+    int split;
+    int top;         // 0, or the tile is of keys that several sequences have (seq is one of them): its tokens are entries tok0 ..
+                     // of the batch's order, all behind the keys, the furthest at position top - 1; pos0: the end of the keys, k1 or behind it
+    int pad;
 };
-// Join of a tile's splits: split s of row r at part + s * count + r. wide: a work-group for every 64 dims of a row.
+// Join of a tile's splits: split s of row r at part + s * count + r, and those of the shared tiles that its rows are in, Seg
+// `segs` of them. wide: a work-group for every 64 dims of a row.
 struct Join {
-    int head, tok0, row0, count, part, splits, wide, pad;
+    int head, tok0, row0, count, part, splits, wide, segs;
+};
+// Splits of shared keys: split s of a join's row r at part + s * stride + r. Join n's are entries LEVELS n ..
+struct Seg {
+    int part, stride, splits, pad;
+};
+constexpr int LEVELS = 3;  // shared ranges that a sequence's tokens are in at most
+// An entry of a batch's order: a token and its position.
+struct Place {
+    int tok, pos;
 };
 // A run of at most KEYS new tokens inside one KEYS-aligned run of positions.
 struct Run {
@@ -86,6 +99,7 @@ int splits_room(int rows, int kv_heads, int part, int more);
 struct Plan {
     std::vector<Item> items[KINDS];
     std::vector<Join> joins;
+    std::vector<Seg> segs;  // none: no join has any
 };
 struct Shape {  // what a plan depends on besides the batch
     int q_heads, kv_heads, head_dim;
@@ -94,6 +108,24 @@ struct Member {
     int seq, count, len;
 };
 void plan_window(const Shape& g, const std::vector<Member>& batch, int window, Plan& out);
+
+// What sequences of a batch have in common. Pages come to be shared by forks alone, so two sequences that have a page have
+// all pages before it: the page lists make a tree.
+struct Range {  // positions [k0, k1), on the same pages for the sequences members[first .. first + count)
+    int k0, k1, first, count, parent;
+};
+struct Share {
+    std::vector<Range> ranges;   // parents before children
+    std::vector<int> members;    // places in the batch, in an order in which those of every range lie together
+    std::vector<int> from;       // per place in the batch: the first position that is attended for it alone
+    std::vector<int> range;      // per place in the batch: the innermost range it is in, -1: none
+    std::vector<Place> order;    // the tokens of `members`, one sequence behind the other
+    std::vector<int> at;         // per place in the batch: its first token's entry in `order`
+};
+void share(const Book& b, const Shape& g, const std::vector<Member>& batch, Share& out);
+// plan_window with the keys that several sequences have taken once for all of them; plan_window's plan where the split
+// partials of that find no room.
+void plan_shared(const Shape& g, const std::vector<Member>& batch, const Share& s, int window, Plan& out);
 // Entries a plan of `tokens` tokens of `seqs` sequences can have at most.
 size_t most_items(const Shape& g, int tokens, int seqs);
 size_t most_joins(const Shape& g, int tokens, int seqs);

@@ -9,7 +9,7 @@ namespace paged {
 
 // The batch as it lies on the device, in 4-byte words from `base`: counts of each list, then the lists.
 struct Lists {
-    size_t items[KINDS], joins, words;  // word offsets of the lists; words of the whole
+    size_t items[KINDS], joins, segs, words;  // word offsets of the lists; words of the whole
 };
 constexpr size_t COUNTS = 8;  // words in front of a list: items of each kind, joins; of the runs: how many, the longest
 static_assert(KINDS < COUNTS, "counts");
@@ -53,6 +53,7 @@ struct AttendArgs {
     void* out;
     float scale;
     float *pm, *pl, *pacc;  // split partials: reference maximum, sum, accumulator rows
+    const Place* order;              // the tokens of shared tiles
     const std::vector<Join>* joins;  // the plan's, for the launch's shape
     bool captured;                   // a captured launch serves any plan
 };

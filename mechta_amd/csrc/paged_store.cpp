@@ -4,71 +4,20 @@
 // into work with its lengths in hand. What the kernels need of that (new entries of the page tables, the batch's runs of
 // new tokens, the lists of work per window) goes to the device once per batch: the host writes it into pinned memory, one
 // kernel puts it in place. The kernels of the layers read it there, so captured calls follow the batch.
-#include <hip/hip_runtime.h>
-
 #include <algorithm>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
-#include <exception>
-#include <memory>
 #include <vector>
 
-#include "mkv_store.h"
-#include "paged_internal.h"
+#include "paged_handle.h"
 
 using mkv::fail;
 using mkv::hip_fail;
 using namespace mkv::paged;
 
 namespace {
-constexpr int RING = 4;           // staged uploads in flight
-// Work-groups of a captured kernel, of whatever batch it finds (all loop over their lists): not many more than run at once,
-// since those that find nothing are in the way too. 1 token at 100 positions, 4 at 20,000, 64 at 3,000 of 4 x 128: attention
-// 10.3 / 21.1 / 65.8 us; with 512 of each kind and 16,384 for the joins 13.1 / 28.8 / 68.6.
-constexpr int GRAPH_GRID = 1024, GRAPH_CHUNKS = 256, GRAPH_ROWS = 1024;
-constexpr unsigned SEG = 256;     // words of an upload's segment at most: a thread of one work-group each
-}  // namespace
-
-struct mpg_store {
-    mpg_config c;
-    Geometry g;
-    Shape shape;
-    Book book;
-    std::vector<int> windows;       // per layer
-    std::vector<int> kinds;         // the different windows
-    bool has_rope = false;
-    RopeArgs rope;
-    int device = 0;
-    hipStream_t stream = nullptr;
-    char* pool = nullptr;           // [layer][K|V][page]
-    int* dev = nullptr;             // page tables, runs, one batch of lists per window
-    size_t runs_at = 0, batch_at = 0, words = 0;  // word offsets in dev; its size
-    Lists lists;
-    float* part = nullptr;          // split partials
-    unsigned* stage[RING] = {};     // pinned
-    hipEvent_t done[RING] = {};
-    size_t stage_words[RING] = {};
-    int turn = 0;
-    int tokens = -1;                // of the batch; -1: none stands
-    int nruns = 0, longest = 0;     // its runs, and the tokens of the longest
-    bool listed = false;            // the lists on the device are a batch's: replays would do it
-    std::vector<Plan> plans, next;  // per window, of the batch and of the one that is being laid out
-};
-
-namespace {
-
-struct OnDevice {  // makes a handle's device current, and the caller's again
-    int was = -1;
-    explicit OnDevice(int device) {
-        int now = 0;
-        if (hipGetDevice(&now) == hipSuccess && now != device && hipSetDevice(device) == hipSuccess) was = now;
-    }
-    ~OnDevice() {
-        if (was >= 0) (void)hipSetDevice(was);
-    }
-};
-
+constexpr unsigned SEG = 256;  // words of an upload's segment at most: a thread of one work-group each
 int check_config(const char* who, const mpg_config* c) {
     if (!c) return fail(MKV_E_ARG, "%s: NULL argument", who);
     if (c->layers < 1 || c->layers > 4096) return fail(MKV_E_ARG, "%s: %d layers", who, c->layers);
@@ -108,9 +57,11 @@ Sizes sizes(const mpg_config& c, int kinds) {
     }
     s.l.joins = at;
     at += most_joins(g, c.tokens, c.seqs) * (sizeof(Join) / 4);
+    s.l.segs = at = (at + 3) / 4 * 4;
+    at += most_joins(g, c.tokens, c.seqs) * LEVELS * (sizeof(Seg) / 4);
     s.l.words = (at + 3) / 4 * 4;
     s.table = (s.table + 3) / 4 * 4;
-    s.words = s.table + COUNTS + (size_t)c.tokens * (sizeof(Run) / 4) + s.l.words * kinds;
+    s.words = s.table + COUNTS + (size_t)c.tokens * (sizeof(Run) / 4) + s.l.words * kinds + (size_t)c.tokens * (sizeof(Place) / 4);
     s.part = (size_t)PART_ROWS * (2 + c.head_dim);
     return s;
 }
@@ -171,48 +122,15 @@ RopeArgs rope_args(const mpg_rope& r) {
     return a;
 }
 
-int check_layer(const mpg_store* h, int layer, const char* who) {
-    if (!h) return fail(MKV_E_ARG, "%s: NULL handle", who);
-    if (layer < 0 || layer >= h->c.layers) return fail(MKV_E_LAYER, "%s: layer %d outside [0, %d)", who, layer, h->c.layers);
-    return MKV_OK;
-}
-
-// 0: not capturing, 1: capturing, < 0: an error that has been noted
-int capturing(const mpg_store* h, const char* who) {
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    const hipError_t e = hipStreamIsCapturing(h->stream, &st);
-    if (e != hipSuccess) {
-        (void)hipGetLastError();
-        return hip_fail(e, who);
-    }
-    return st == hipStreamCaptureStatusNone ? 0 : 1;
-}
-
-template <typename F>
-int guarded(const char* who, F f) {  // no exception crosses the C boundary
-    try {
-        return f();
-    } catch (const std::exception&) {
-        return fail(MKV_E_NOMEM, "%s: host allocation", who);
-    }
-}
-
-// A call that changes the host's book: with the handle's device current, refused while the stream captures.
-#define MPG_HOST_CALL(h, who)                                                                                \
-    if (!(h)) return fail(MKV_E_ARG, "%s: NULL handle", who);                                                \
-    OnDevice on((h)->device);                                                                                \
-    if (const int cap = capturing(h, who))                                                                   \
-        return cap < 0 ? cap : fail(MKV_E_ARG, "%s: the stream is capturing; page calls run outside a graph", who)
-
 int copy_pages(mpg_store* h, const std::vector<Pair>& copies, const char* who) {
     if (copies.empty()) return MKV_OK;
     const hipError_t e = launch_copies(h->g, h->pool, copies.data(), (int)copies.size(), h->stream);
     return e == hipSuccess ? MKV_OK : hip_fail(e, who);
 }
 
-// The new entries of the page tables to the device, and with `runs` the lists of a batch: its runs and plans, or (plans NULL)
-// none. A call that fails has sent nothing.
-int upload(mpg_store* h, const std::vector<Run>* runs, const std::vector<Plan>* plans, const char* who) {
+// The new entries of the page tables to the device, and with `runs` the lists of a batch: its runs, its plans and the order of
+// its tokens in shared tiles, or (plans NULL) none. A call that fails has sent nothing.
+int upload(mpg_store* h, const std::vector<Run>* runs, const std::vector<Plan>* plans, const std::vector<Place>* order, const char* who) {
     std::vector<Segment> segs;
     size_t at = 0;  // words of payload so far
     auto add = [&](size_t dst, size_t words) {
@@ -256,7 +174,9 @@ int upload(mpg_store* h, const std::vector<Run>* runs, const std::vector<Plan>* 
             for (int k = 0; k < KINDS; k++)
                 put(base + h->lists.items[k], p.items[k].data(), p.items[k].size() * (sizeof(Item) / 4));
             put(base + h->lists.joins, p.joins.data(), p.joins.size() * (sizeof(Join) / 4));
+            put(base + h->lists.segs, p.segs.data(), p.segs.size() * (sizeof(Seg) / 4));
         }
+        if (order) put(h->order_at, order->data(), order->size() * (sizeof(Place) / 4));
     }
     if (segs.empty()) return MKV_OK;
     const size_t head = segs.size() * (sizeof(Segment) / 4), all = head + at;
@@ -300,7 +220,7 @@ int upload(mpg_store* h, const std::vector<Run>* runs, const std::vector<Plan>* 
 int end_batch(mpg_store* h, const char* who) {
     if (!h->listed) return MKV_OK;
     const std::vector<Run> none;
-    if (const int rc = upload(h, &none, nullptr, who)) return rc;
+    if (const int rc = upload(h, &none, nullptr, nullptr, who)) return rc;
     h->listed = false;
     h->tokens = -1;
     return MKV_OK;
@@ -320,19 +240,6 @@ int settle(mpg_store* h, const std::vector<Pair>& copies, const char* who, U und
     }
     if (rc) undo();
     return rc;
-}
-
-int check_batch(const mpg_store* h, int rows, const char* who) {
-    if (h->tokens < 0) return fail(MKV_E_ARG, "%s: no batch stands (mpg_begin)", who);
-    if (rows < h->tokens) return fail(MKV_E_SIZE, "%s: %d rows, the batch has %d tokens", who, rows, h->tokens);
-    return MKV_OK;
-}
-
-int check_rows(const char* who, const char* what, const void* p, int rows, int64_t tok, int heads, int64_t head) {
-    if (!p) return fail(MKV_E_ARG, "%s: NULL %s", who, what);
-    if ((uintptr_t)p % 16 || (rows > 1 && tok % 8) || (heads > 1 && head % 8))
-        return fail(MKV_E_ARG, "%s: %s must be 16-byte aligned, its strides multiples of 8 elements", who, what);
-    return MKV_OK;
 }
 
 }  // namespace
@@ -417,6 +324,7 @@ static int create(mpg_t** out, const mpg_config* c, const int* windows, const mp
     h->lists = s.l;
     h->runs_at = s.table;
     h->batch_at = s.table + COUNTS + (size_t)c->tokens * (sizeof(Run) / 4);
+    h->order_at = h->batch_at + s.l.words * MPG_WINDOWS_MAX;
     h->words = s.words;
     h->book.init(c->pages, c->page, c->seqs, c->ctx);
     if (const int cap = capturing(h, "mpg_create"))
@@ -519,7 +427,7 @@ int mpg_reserve(mpg_t* h, int n, const int* seq, const int* count) {
 
 // The batch of sequences that have been lengthened already: its runs, its plans, and both on their way to the device. Where
 // that fails the batch before stands.
-static int lay_out(mpg_t* h, int n, const int* seq, const int* count) {
+static int lay_out(mpg_t* h, int n, const int* seq, const int* count, bool shared, const char* who) {
     std::vector<Member> batch;
     std::vector<Run> runs;
     int tok = 0, longest = 0;
@@ -534,8 +442,13 @@ static int lay_out(mpg_t* h, int n, const int* seq, const int* count) {
             longest = std::max(longest, m);
         }
     }
-    for (size_t w = 0; w < h->kinds.size(); w++) plan_window(h->shape, batch, h->kinds[w], h->next[w]);
-    if (int rc = upload(h, &runs, &h->next, "mpg_begin")) return rc;
+    Share common;
+    if (shared) share(h->book, h->shape, batch, common);
+    for (size_t w = 0; w < h->kinds.size(); w++) {
+        if (shared) plan_shared(h->shape, batch, common, h->kinds[w], h->next[w]);
+        else plan_window(h->shape, batch, h->kinds[w], h->next[w]);
+    }
+    if (int rc = upload(h, &runs, &h->next, &common.order, who)) return rc;
     h->listed = true;
     h->plans.swap(h->next);
     h->tokens = tok;
@@ -544,27 +457,33 @@ static int lay_out(mpg_t* h, int n, const int* seq, const int* count) {
     return MKV_OK;
 }
 
-static int begin(mpg_t* h, int n, const int* seq, const int* count, int* tokens) {
-    long long sum = 0;
-    for (int i = 0; i < n && seq && count; i++) sum += std::max(count[i], 0);
-    if (sum > h->c.tokens)
-        return fail(MKV_E_ARG, "mpg_begin: %lld tokens, the handle's batches have at most %d", sum, h->c.tokens);
-    if (int rc = h->book.reserve("mpg_begin", n, seq, count)) return rc;
-    try {
-        const int rc = lay_out(h, n, seq, count);
-        if (rc) h->book.undo_reserve(n, seq, count);
-        else if (tokens) *tokens = h->tokens;
-        return rc;
-    } catch (...) {
-        h->book.undo_reserve(n, seq, count);
-        throw;
-    }
+static int begin(mpg_t* h, int n, const int* seq, const int* count, int* tokens, bool shared, const char* who) {
+    MPG_HOST_CALL(h, who);
+    return guarded(who, [&] {
+        long long sum = 0;
+        for (int i = 0; i < n && seq && count; i++) sum += std::max(count[i], 0);
+        if (sum > h->c.tokens)
+            return fail(MKV_E_ARG, "%s: %lld tokens, the handle's batches have at most %d", who, sum, h->c.tokens);
+        if (int rc = h->book.reserve(who, n, seq, count)) return rc;
+        try {
+            const int rc = lay_out(h, n, seq, count, shared, who);
+            if (rc) h->book.undo_reserve(n, seq, count);
+            else if (tokens) *tokens = h->tokens;
+            return rc;
+        } catch (...) {
+            h->book.undo_reserve(n, seq, count);
+            throw;
+        }
+    });
 }
 
 int mpg_begin(mpg_t* h, int n, const int* seq, const int* count, int* tokens) {
-    MPG_HOST_CALL(h, "mpg_begin");
-    return guarded("mpg_begin", [&] { return begin(h, n, seq, count, tokens); });
+    return begin(h, n, seq, count, tokens, false, "mpg_begin");
 }
+int mpg_begin_shared(mpg_t* h, int n, const int* seq, const int* count, int* tokens) {
+    return begin(h, n, seq, count, tokens, true, "mpg_begin_shared");
+}
+
 int mpg_set_len(mpg_t* h, int seq, int len) {
     MPG_HOST_CALL(h, "mpg_set_len");
     return guarded("mpg_set_len", [&] {
@@ -667,6 +586,7 @@ int mpg_attend(mpg_t* h, int layer, int rows, const void* q, int64_t q_tok, int6
     a.pm = h->part;
     a.pl = h->part + PART_ROWS;
     a.pacc = h->part + 2 * (size_t)PART_ROWS;
+    a.order = (const Place*)(h->dev + h->order_at);
     a.joins = &p.joins;
     a.captured = cap != 0;
     int grid[KINDS];
@@ -692,7 +612,7 @@ int mpg_read_rows(mpg_t* h, int layer, int which, int seq, int p0, int p1, void*
     if (cap && b.fresh[seq] < (int)b.table[seq].size())
         return fail(MKV_E_ARG, "mpg_read_rows: the device does not have the sequence's pages yet; read once before capturing");
     if (!cap)
-        if (int rc = guarded("mpg_read_rows", [&] { return upload(h, nullptr, nullptr, "mpg_read_rows"); })) return rc;
+        if (int rc = guarded("mpg_read_rows", [&] { return upload(h, nullptr, nullptr, nullptr, "mpg_read_rows"); })) return rc;
     const hipError_t e = launch_read(h->g, h->pool, layer, which, h->dev + (size_t)seq * h->g.most_pages, p0, p1, dst, h->stream);
     return e == hipSuccess ? MKV_OK : hip_fail(e, "mpg_read_rows");
 }

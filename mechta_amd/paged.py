@@ -13,7 +13,7 @@ BF16 = 2
 
 # every symbol include/mechta_paged.h declares
 SYMBOLS = ["mpg_rope_freqs", "mpg_rope_turns", "mpg_rotate", "mpg_bytes", "mpg_create", "mpg_destroy", "mpg_set_stream", "mpg_sync",
-           "mpg_len", "mpg_table", "mpg_free_pages", "mpg_pages", "mpg_reserve", "mpg_begin", "mpg_set_len", "mpg_fork",
+           "mpg_len", "mpg_table", "mpg_free_pages", "mpg_pages", "mpg_reserve", "mpg_begin", "mpg_begin_shared", "mpg_set_len", "mpg_fork",
            "mpg_copy", "mpg_free", "mpg_compact", "mpg_append", "mpg_attend", "mpg_read_rows"]
 
 LAYOUTS = {"half": 0, "interleaved": 1}
@@ -62,6 +62,7 @@ def lib():
             "mpg_pages": ([P, I, I, ctypes.POINTER(P)], I),
             "mpg_reserve": ([P, I, P, P], I),
             "mpg_begin": ([P, I, P, P, IP], I),
+            "mpg_begin_shared": ([P, I, P, P, IP], I),
             "mpg_set_len": ([P, I, I], I),
             "mpg_fork": ([P, I, P, P, P], I),
             "mpg_copy": ([P, I, P, P], I),
@@ -299,12 +300,14 @@ class PagedKv:
         (a, ap), (b, bp) = _ints(seqs), _ints(counts, len(seqs), "counts")
         _check(self._lib.mpg_reserve(self._h, len(a), ap, bp))
 
-    def begin(self, seqs, counts):
+    def begin(self, seqs, counts, shared=False):
         """Lengthens the sequences by `counts` new tokens and makes them the batch of the appends and attention that
-        follow; returns the number of tokens."""
+        follow; returns the number of tokens. shared: pages that several of the sequences have in common (forks of one prompt)
+        are attended once for all of them, where that is worth it."""
         n = ctypes.c_int()
         (a, ap), (b, bp) = _ints(seqs), _ints(counts, len(seqs), "counts")
-        _check(self._lib.mpg_begin(self._h, len(a), ap, bp, ctypes.byref(n)))
+        call = self._lib.mpg_begin_shared if shared else self._lib.mpg_begin
+        _check(call(self._h, len(a), ap, bp, ctypes.byref(n)))
         return n.value
 
     def set_len(self, seq, n):
