@@ -13,7 +13,7 @@
  * lays out the work of every layer; then, layer by layer, mpg_append writes the new rows (rotating K, and q beside) and
  * mpg_attend attends. The tokens of a batch are packed: those of the first sequence, then those of the second, and so
  * on; rows of the arguments behind the last token are neither read nor written. A batch stands until the next mpg_begin,
- * or until pages change hands (mpg_fork, mpg_copy, mpg_free, mpg_compact, mpg_set_len, mpg_reserve): then appends and
+ * or until pages change hands (mpg_fork, mpg_copy, mpg_free, mpg_compact, mpg_set_len, mpg_reserve, mpg_evict): then appends and
  * attention are refused until a new mpg_begin.
  *
  * Ordering: every call is enqueued on the handle's HIP stream; none waits, except mpg_create, mpg_sync and mpg_destroy.
@@ -23,7 +23,7 @@
  * on one stream at a time: the handle's workspaces are shared by all its calls. A call makes the handle's device
  * current while it runs.
  *
- * Graphs: mpg_append, mpg_attend and mpg_read_rows may be captured, the others are refused on a stream that is
+ * Graphs: mpg_append, mpg_attend, mpg_weigh and mpg_read_rows may be captured, the others are refused on a stream that is
  * capturing. What a captured call works on is read on the device when the graph runs: after another mpg_begin a replay
  * of the same graph does that batch, of any sequences, counts and lengths; tokens behind the rows that
  * were captured are left out. Replays are ordered with the handle's other calls like any call.
@@ -170,6 +170,39 @@ int mpg_append(mpg_t* h, int layer, int rows, const void* k, int64_t k_tok, int6
  * token does not see, NaN and infinities included, has no effect on it. */
 int mpg_attend(mpg_t* h, int layer, int rows, const void* q, int64_t q_tok, int64_t q_head, float scale, const float* sinks,
                const void* gate, int64_t g_tok, int64_t g_head, void* out);
+/* ---- what positions are looked at, and eviction by it ----
+ * A handle may keep a weight (f32) for each position of each sequence, layer and kv head: the attention weights that tokens have
+ * given it, accumulated by mpg_weigh. New positions (mpg_begin, mpg_reserve) weigh nothing; forks and copies take the weights
+ * along; what lies behind a sequence's length is undefined. mpg_evict keeps a sequence's positions of the largest weights.
+ *
+ * An evicted sequence keeps counting: mpg_position is where its next token stands, its length plus all positions evicted, and
+ * mpg_append rotates there. Each layer and kv head keeps positions of its own, so a sequence cannot be cut back (mpg_set_len,
+ * mpg_fork) to less than eviction has left, but for nothing at all. */
+
+/* Device bytes that mpg_keep_weights allocates for a handle of this configuration (0 if it would refuse). */
+size_t mpg_weights_bytes(const mpg_config* c, int last);
+/* From here on the handle keeps weights: of each sequence of a batch, mpg_weigh counts the `last` last new tokens (0: all).
+ * Before the handle's first positions and its first batch; it waits for the stream. */
+int mpg_keep_weights(mpg_t* h, int last);
+/* Device address of a layer's weights: of (sequence, kv head, position) at sequence x *seq_stride + head x *head_stride +
+ * position. A caller may write those of a sequence's positions, in order with the handle's stream. */
+int mpg_weights(const mpg_t* h, int layer, float** base, int64_t* seq_stride, int64_t* head_stride);
+/* For each sequence of the batch with new tokens, each kv head and each of its positions j: weight = decay x weight + the sum,
+ * over the counted tokens and the query heads of the kv head, of the attention weights of j (mpg_attend's softmax, with its
+ * scale, window and sinks; after the layer's mpg_append). Other sequences' weights are left as they are. decay >= 0: 1
+ * accumulates, 0 starts afresh whatever was there. q, rows: mpg_attend's, rotated. All in f32. A score that is NaN or plus infinity makes
+ * all that its row sees NaN. */
+int mpg_weigh(mpg_t* h, int layer, int rows, const void* q, int64_t q_tok, int64_t q_head, float scale, const float* sinks,
+              float decay);
+/* Cuts each of n different sequences of more than keep[i] positions to keep[i] >= 1: its first `first` and last `recent` ones
+ * and, for each layer and kv head by itself, those of the largest weights between them (of equal ones the lowest positions; NaN
+ * weighs most). K, V and weights stay in order, on new pages: the pool needs as many free pages as keep[i] positions of each
+ * take, before the old ones are given back (MKV_E_NOMEM). Layers with a window need `recent` to be no less than it. A batch ends,
+ * as with every call that changes pages. */
+int mpg_evict(mpg_t* h, int n, const int* seq, const int* keep, int first, int recent);
+/* The position of a sequence's next token: its length, and what has been evicted of it. */
+int mpg_position(const mpg_t* h, int seq, int* position);
+
 /* Positions [p0, p1) of a sequence's K or V: dst [p1 - p0][kv_heads][head_dim] of the cache's type (device). When captured,
  * a replay reads the pages the sequence has then as far as the device knows: as of the last mpg_begin or mpg_read_rows. */
 int mpg_read_rows(mpg_t* h, int layer, int which, int seq, int p0, int p1, void* dst);

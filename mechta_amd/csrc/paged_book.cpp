@@ -21,6 +21,9 @@ void Book::init(int pages_, int page_, int seqs_, int ctx_) {
     table.assign(seqs, {});
     len.assign(seqs, 0);
     fresh.assign(seqs, 0);
+    shift.assign(seqs, 0);
+    floor.assign(seqs, 0);
+    moved.assign(seqs, 0);
 }
 
 int Book::take() {  // the free page of the lowest number; one is free
@@ -60,6 +63,9 @@ int Book::reserve(const char* who, int n, const int* seq, const int* count) {
         if (count[i] > ctx - len[seq[i]])
             return fail(MKV_E_POS, "%s: sequence %d of %d positions plus %d: more than the context %d", who, seq[i],
                         len[seq[i]], count[i], ctx);
+        if (count[i] > INT_MAX - len[seq[i]] - shift[seq[i]])
+            return fail(MKV_E_POS, "%s: sequence %d at position %lld plus %d: past 32 bits", who, seq[i],
+                        (long long)len[seq[i]] + shift[seq[i]], count[i]);
         want += need(len[seq[i]] + count[i]) - (int)table[seq[i]].size();
     }
     if (want > free) return fail(MKV_E_NOMEM, "%s: %lld pages needed, %d free", who, want, free);
@@ -91,6 +97,8 @@ int Book::fork(const char* who, int n, const int* src, const int* dst, const int
         const int m = upto ? upto[i] : len[src[i]];
         if (m < 0 || m > len[src[i]])
             return fail(MKV_E_POS, "%s: %d positions of sequence %d, which has %d", who, m, src[i], len[src[i]]);
+        if (m && m < floor[src[i]])
+            return fail(MKV_E_POS, "%s: %d positions of sequence %d, of which eviction has left %d", who, m, src[i], floor[src[i]]);
         want += own ? need(m) : m % page ? 1 : 0;
     }
     if (want > free) return fail(MKV_E_NOMEM, "%s: %lld pages needed, %d free", who, want, free);
@@ -108,6 +116,7 @@ int Book::fork(const char* who, int n, const int* src, const int* dst, const int
         }
         len[dst[i]] = m;
         stale(dst[i], 0);
+        if (m) move(dst[i], shift[src[i]], floor[src[i]]);
     }
     return MKV_OK;
 }
@@ -130,6 +139,7 @@ void Book::clear(int n, const int* seq) {
         table[seq[i]].clear();
         len[seq[i]] = 0;
         fresh[seq[i]] = 0;
+        move(seq[i], 0, 0);
     }
 }
 
@@ -145,6 +155,8 @@ int Book::set_len(const char* who, int seq, int n, std::vector<Pair>& copies, Cu
     if (int rc = distinct(who, 1, &seq)) return rc;
     if (n < 0 || n > len[seq])
         return fail(MKV_E_POS, "%s: length %d of sequence %d, which has %d", who, n, seq, len[seq]);
+    if (n && n < floor[seq])
+        return fail(MKV_E_POS, "%s: length %d of sequence %d, of which eviction has left %d", who, n, seq, floor[seq]);
     std::vector<int>& t = table[seq];
     const int keep = need(n);
     const bool shared = n % page && owners[t[keep - 1]] > 1;
@@ -156,7 +168,7 @@ int Book::set_len(const char* who, int seq, int n, std::vector<Pair>& copies, Cu
     if (shared) copies.reserve(1);
     if (cut) {
         const int from = shared ? keep - 1 : keep;
-        *cut = Cut{len[seq], from, shared, std::vector<int>(t.begin() + from, t.end())};
+        *cut = Cut{len[seq], from, shared, std::vector<int>(t.begin() + from, t.end()), shift[seq], floor[seq]};
     }
     while ((int)t.size() > keep) {  // nothing throws from here on
         drop(t.back());
@@ -171,6 +183,7 @@ int Book::set_len(const char* who, int seq, int n, std::vector<Pair>& copies, Cu
     }
     stale(seq, keep);
     len[seq] = n;
+    if (!n) move(seq, 0, 0);
     return MKV_OK;
 }
 
@@ -181,14 +194,63 @@ void Book::undo_set_len(int seq, const Cut& cut) {
         t.pop_back();
     }
     for (int p : cut.pages) {  // the table has room for what it had
-        if (!owners[p]++) {
-            open[p / 64] &= ~(1ull << (p % 64));
-            free--;
-        }
+        own_again(p);
         t.push_back(p);
     }
     len[seq] = cut.len;
     stale(seq, cut.from);
+    move(seq, cut.shift, cut.floor);
+}
+
+void Book::own_again(int p) {  // a page that has been given back, or that others own
+    if (owners[p]++) return;
+    open[p / 64] &= ~(1ull << (p % 64));
+    free--;
+}
+
+int Book::can_evict(const char* who, int n, const int* seq, const int* keep) const {
+    if (int rc = distinct(who, n, seq)) return rc;
+    if (n && !keep) return fail(MKV_E_ARG, "%s: NULL argument", who);
+    long long want = 0;
+    for (int i = 0; i < n; i++) {
+        if (keep[i] < 1) return fail(MKV_E_ARG, "%s: %d positions kept of sequence %d", who, keep[i], seq[i]);
+        if (len[seq[i]] > keep[i]) want += need(keep[i]);
+    }
+    return want > free ? fail(MKV_E_NOMEM, "%s: %lld pages needed, %d free", who, want, free) : (int)MKV_OK;
+}
+
+int Book::evict(const char* who, int n, const int* seq, const int* keep, std::vector<Evicted>& cut) {
+    if (int rc = can_evict(who, n, seq, keep)) return rc;
+    std::vector<std::vector<int>> fresh_pages(n);  // nothing throws behind these
+    cut.reserve(n);
+    for (int i = 0; i < n; i++)
+        if (len[seq[i]] > keep[i]) fresh_pages[i].reserve(need(keep[i]));
+    for (int i = 0; i < n; i++) {
+        const int s = seq[i];
+        if (len[s] <= keep[i]) continue;
+        for (int k = 0; k < need(keep[i]); k++) fresh_pages[i].push_back(take());
+        cut.push_back({s, len[s], shift[s], floor[s], {}});
+        cut.back().pages.swap(table[s]);
+        table[s].swap(fresh_pages[i]);
+        fresh[s] = 0;
+        move(s, shift[s] + len[s] - keep[i], keep[i]);
+        len[s] = keep[i];
+    }
+    for (const Evicted& e : cut)  // only now: what is taken is never what is given back
+        for (int p : e.pages) drop(p);
+    return MKV_OK;
+}
+
+void Book::undo_evict(std::vector<Evicted>& cut) {
+    for (Evicted& e : cut)
+        for (int p : e.pages) own_again(p);
+    for (Evicted& e : cut) {
+        for (int p : table[e.seq]) drop(p);
+        table[e.seq].swap(e.pages);
+        fresh[e.seq] = 0;
+        move(e.seq, e.shift, e.floor);
+        len[e.seq] = e.len;
+    }
 }
 
 int Book::compact(std::vector<Pair>& copies) {
@@ -742,6 +804,145 @@ static void plan(const Shape& g, const std::vector<Member>& batch, const Share* 
 void plan_window(const Shape& g, const std::vector<Member>& batch, int window, Plan& out) { plan(g, batch, nullptr, window, out); }
 void plan_shared(const Shape& g, const std::vector<Member>& batch, const Share& s, int window, Plan& out) {
     plan(g, batch, s.ranges.empty() ? nullptr : &s, window, out);
+}
+
+// ---- accumulated attention weights ----
+
+size_t weigh_entries(const Shape& g, int tokens, int seqs) {
+    const size_t group = g.q_heads / g.kv_heads;
+    return ((size_t)tokens * group / SCORE_ROWS + 2 * (size_t)std::min(seqs, tokens)) * g.kv_heads + WEIGH_MOST;
+}
+
+void plan_weigh(const Shape& g, const std::vector<Member>& batch, int window, int last, const WeighRoom& room, WeighPlan& out) {
+    for (auto& v : out.scores) v.clear();
+    for (auto& v : out.sums) v.clear();
+    out.fades.clear();
+    const int group = g.q_heads / g.kv_heads, heads = g.kv_heads;
+    struct Weighed {  // a sequence with counted tokens
+        int seq, tok0, rows, pos0, k0, len, scores;
+    };
+    std::vector<Weighed> few, many;
+    long long stats = 0, work = 0, few_keys = 0, few_rows = 0, tile_keys = 0, rows_left = 0;
+    int tok = 0;
+    for (const Member& m : batch) {
+        const int n = last ? std::min(last, m.count) : m.count, tok0 = tok + m.count - n;
+        tok += m.count;
+        if (!n) continue;
+        const int pos0 = m.len - n, k0 = (window ? std::max(0, pos0 - window + 1) : 0) / KEYS * KEYS, rows = n * group;
+        const long long blocks = (m.len - k0 + KEYS - 1) / KEYS, kept = blocks * KEYS * rows * heads;
+        rows_left += (long long)rows * heads;
+        Weighed w{m.seq, tok0, rows, pos0, k0, m.len, -1};
+        if (rows <= TILE_ROWS[SOME] && work + kept <= room.work) {
+            w.scores = (int)work;
+            work += kept;
+            few_keys += (long long)(m.len - k0) * heads;
+            few_rows += heads;
+            few.push_back(w);
+        } else {
+            tile_keys += (long long)((rows + SCORE_ROWS - 1) / SCORE_ROWS) * (m.len - k0) * heads;
+            many.push_back(w);
+        }
+        if (k0 > 0)
+            for (int h = 0; h < heads; h++) out.fades.push_back({m.seq, h, 0, k0, 0, 0, 0, 0});
+    }
+    // rows x pieces of statistics, at least one piece for all that is left
+    auto pieces_in = [&](int rows, long long units, long long length) {
+        const long long p = (units + length - 1) / length, most = (room.stats - stats - rows_left) / rows;
+        return (int)std::max(1ll, std::min(p, most));
+    };
+    int more = 0;
+    // Few rows: bound by the keys' stream, cut as those of the attention.
+    const long long few_share = (few_keys + STREAMS - 1) / STREAMS;
+    const long long few_length = std::max<long long>(LEAST_KEYS, few_rows > STREAMS / 2 ? few_share * 3 / 4 : few_share) / KEYS;
+    for (const Weighed& w : few) {
+        const int units = (w.len - w.k0 + KEYS - 1) / KEYS;
+        for (int h = 0; h < heads; h++) {
+            rows_left -= w.rows;
+            int pieces = pieces_in(w.rows, units, few_length);
+            pieces = std::min(pieces, 1 + (WEIGH_MOST / 2 - std::min(more, WEIGH_MOST / 2)));
+            more += pieces - 1;
+            const int scores = w.scores + h * units * KEYS * w.rows, stat = (int)stats;
+            stats += (long long)pieces * w.rows;
+            for (int p = 0; p < pieces; p++) {
+                const int a = (int)((long long)units * p / pieces), b = (int)((long long)units * (p + 1) / pieces);
+                out.scores[w.rows <= TILE_ROWS[FEW] ? SCORE_FEW : SCORE_SOME].push_back(
+                    {w.seq, h, w.tok0, w.rows, 0, w.pos0, w.k0 + a * KEYS, std::min(w.len, w.k0 + b * KEYS), stat + p * w.rows,
+                     scores + a * KEYS * w.rows, {0, 0}});
+            }
+            out.sums[0].push_back({w.seq, h, w.tok0, w.rows, w.pos0, w.k0, w.len, 0, w.rows, stat, pieces, scores, w.k0, -1, {0, 0}});
+        }
+    }
+    // their sums by ranges of keys
+    {
+        std::vector<Sum> whole;
+        whole.swap(out.sums[0]);
+        const long long keys = std::min(1ll << 30, std::max<long long>(512, (few_keys / (WEIGH_MOST / 4) + 255) / 256 * 256));
+        for (Sum s : whole) {
+            const int end = s.k1;
+            for (int k = s.k0; k < end; k += (int)keys) {
+                s.k0 = k;
+                s.k1 = (int)std::min<long long>(end, k + keys);
+                out.sums[0].push_back(s);
+            }
+        }
+    }
+    // Many rows: bound by the matrix units and the exponentials. Tiles of rows against all their keys, split where they are few.
+    more = 0;
+    constexpr int PLACES = 2 * CUS;
+    const long long many_length = std::max<long long>(LEAST_KEYS, (tile_keys + PLACES - 1) / PLACES) / KEYS;
+    long long key_tiles = 0, row_tiles = 0;
+    for (const Weighed& w : many) {
+        key_tiles += (long long)((w.len - w.k0 + SUM_KEYS - 1) / SUM_KEYS) * heads;
+        for (int k = w.k0; k < w.len; k += SUM_KEYS) {
+            const int r0 = (int)std::max(0ll, (long long)(k - w.pos0) * group);
+            row_tiles += (long long)(w.rows - r0 + KEYS - 1) / KEYS * heads;
+        }
+    }
+    const int per = (int)std::max(1ll, (key_tiles + WEIGH_MOST / 2 - 1) / (WEIGH_MOST / 2));  // key tiles of a work-group
+    const long long chunk = per > 1 ? 1ll << 40 : std::max<long long>(8, (row_tiles + 4 * CUS - 1) / (4 * CUS)) * KEYS;  // rows of one
+    for (const Weighed& w : many) {
+        const int units = (w.len - w.k0 + KEYS - 1) / KEYS;
+        int pieces = 0;
+        for (int h = 0; h < heads; h++) {
+            rows_left -= w.rows;
+            const int tiles = (w.rows + SCORE_ROWS - 1) / SCORE_ROWS;
+            if (!h) {
+                rows_left -= (long long)w.rows * (heads - 1);
+                pieces = pieces_in(w.rows * heads, units, many_length);
+                rows_left += (long long)w.rows * (heads - 1);
+                pieces = std::min(pieces, 1 + std::max(0, WEIGH_MOST - more) / (tiles * heads));
+                more += (pieces - 1) * tiles * heads;
+            }
+            const int stat = (int)stats;
+            stats += (long long)pieces * w.rows;
+            for (int r = 0; r < w.rows; r += SCORE_ROWS) {
+                const int end = std::min(w.len, w.pos0 + (std::min(r + SCORE_ROWS, w.rows) - 1) / group + 1);
+                const int lo = window ? std::max(0, w.pos0 + r / group - window + 1) / KEYS * KEYS : 0;
+                for (int p = 0; p < pieces; p++) {  // (a piece without keys leaves its rows' statistics empty)
+                    const int a = std::max(lo, w.k0 + (int)((long long)units * p / pieces) * KEYS);
+                    const int b = std::min(end, w.k0 + (int)((long long)units * (p + 1) / pieces) * KEYS);
+                    out.scores[SCORE_MANY].push_back({w.seq, h, w.tok0, w.rows, r, w.pos0, a, std::max(a, b), stat + p * w.rows + r, -1, {0, 0}});
+                }
+            }
+            for (int k = w.k0; k < w.len; k += SUM_KEYS * per) {
+                const int end = std::min(w.len, k + SUM_KEYS * per);
+                const int r0 = (int)std::min<long long>(w.rows, std::max(0ll, (long long)(k - w.pos0) * group)) / KEYS * KEYS;
+                const int r1 = window ? (int)std::min<long long>(w.rows, std::max(0ll, ((long long)end - 1 + window - w.pos0) * group)) : w.rows;
+                int sums = (int)std::max(1ll, (std::max(0, r1 - r0) + chunk - 1) / chunk);
+                if (sums > 1 && work + (long long)sums * SUM_KEYS > room.work) sums = 1;
+                for (int x = 0; x < sums; x++) {
+                    const int units_of = (std::max(0, r1 - r0) + KEYS - 1) / KEYS;
+                    const int a = r0 + (int)((long long)units_of * x / sums) * KEYS;
+                    const int b = std::min(std::max(r0, r1), r0 + (int)((long long)units_of * (x + 1) / sums) * KEYS);
+                    out.sums[1].push_back({w.seq, h, w.tok0, w.rows, w.pos0, k, end, a, b, stat, pieces, -1, 0, sums > 1 ? (int)work + x * SUM_KEYS : -1, {0, 0}});
+                }
+                if (sums > 1) {
+                    out.fades.push_back({w.seq, h, k, end, (int)work, sums, SUM_KEYS, 0});
+                    work += (long long)sums * SUM_KEYS;
+                }
+            }
+        }
+    }
 }
 
 }  // namespace paged

@@ -23,6 +23,12 @@ struct Cut {
     int len, from;
     bool copied;
     std::vector<int> pages;
+    int shift = 0, floor = 0;
+};
+// What evict took from a sequence.
+struct Evicted {
+    int seq, len, shift, floor;
+    std::vector<int> pages;
 };
 
 // Which pages belong to whom. Pure host state. Each call checks everything first; a refused one changes nothing. What the
@@ -35,6 +41,9 @@ struct Book {
     std::vector<std::vector<int>> table;  // per sequence
     std::vector<int> len;
     std::vector<int> fresh;               // per sequence: entries of its table from here on are not on the device yet
+    std::vector<int> shift;               // per sequence: positions evicted; position i of what is left, from `floor` - 1 on, was
+    std::vector<int> floor;               //   i + shift once (below that, each layer and head has kept others)
+    std::vector<char> moved;              // per sequence: its shift is not on the device yet
     void init(int pages, int page, int seqs, int ctx);
     int reserve(const char* who, int n, const int* seq, const int* count);
     int fork(const char* who, int n, const int* src, const int* dst, const int* len, bool own, std::vector<Pair>& copies);
@@ -42,6 +51,10 @@ struct Book {
     int release(const char* who, int n, const int* seq, const std::function<int()>& before = nullptr);
     int set_len(const char* who, int seq, int len, std::vector<Pair>& copies, Cut* cut = nullptr);
     int compact(std::vector<Pair>& copies);
+    // Cuts each sequence of more than keep[i] positions to keep[i], on new pages in place of its own.
+    int can_evict(const char* who, int n, const int* seq, const int* keep) const;
+    int evict(const char* who, int n, const int* seq, const int* keep, std::vector<Evicted>& cut);
+    void undo_evict(std::vector<Evicted>& cut);
     void undo_reserve(int n, const int* seq, const int* count);
     void undo_fork(int n, const int* dst) { clear(n, dst); }
     void undo_set_len(int seq, const Cut& cut);
@@ -53,8 +66,14 @@ struct Book {
     void drop(int p);
     void clear(int n, const int* seq);
     void reopen();
+    void own_again(int page);
     void stale(int seq, int from) {
         if (fresh[seq] > from) fresh[seq] = from;
+    }
+    void move(int seq, int by, int from) {
+        moved[seq] |= shift[seq] != by;
+        shift[seq] = by;
+        floor[seq] = from;
     }
     int distinct(const char* who, int n, const int* seq) const;
 };
@@ -129,6 +148,41 @@ void plan_shared(const Shape& g, const std::vector<Member>& batch, const Share& 
 // Entries a plan of `tokens` tokens of `seqs` sequences can have at most.
 size_t most_items(const Shape& g, int tokens, int seqs);
 size_t most_joins(const Shape& g, int tokens, int seqs);
+
+
+// ---- accumulated attention weights ----
+// Per window, the work of weighing a batch: what each position is given by the sequences' counted tokens (rows = counted
+// tokens x group). First the statistics of the rows, for few rows with their scores, then the sums over them.
+struct Score {  // rows row0 .. of one kv head against keys [k0, k1): the reference and the sum of each to stats[stat ..]
+    int seq, head, tok0, rows, row0, pos0;  // tok0, pos0: the first counted token and its position
+    int k0, k1, stat;
+    int keep;        // where the scores go in the work space, by blocks of KEYS keys [row][key], -1: nowhere
+    int pad[2];
+};
+struct Sum {  // keys [k0, k1) from rows [r0, r1)
+    int seq, head, tok0, rows, pos0, k0, k1;
+    int r0, r1;
+    int stat, pieces;  // statistics of piece p of row r at stats[stat + p * rows + r]
+    int scores, s0;    // kept scores, the first of key s0; -1: none
+    int part;          // where the sums go in the work space, -1: to the position's weight
+    int pad[2];
+};
+struct Fade {  // weights of keys [k0, k1), faded, plus `sums` partial sums, of key k0 + i at part + s * stride + i
+    int seq, head, k0, k1, part, sums, stride, pad;
+};
+enum { SCORE_FEW, SCORE_SOME, SCORE_MANY, SUM_FEW, SUM_MANY, FADES, WEIGH_LISTS };  // few: up to 16 rows, some: up to 32
+struct WeighPlan {
+    std::vector<Score> scores[SCORE_MANY + 1];
+    std::vector<Sum> sums[2];
+    std::vector<Fade> fades;
+};
+struct WeighRoom {
+    long long stats, work;  // pairs, floats
+};
+constexpr int SCORE_ROWS = 128, SUM_KEYS = 256;  // of a tile: rows of SCORE_MANY, keys of SUM_MANY
+constexpr int WEIGH_MOST = 4096;                 // entries of a list at most, besides one for each tile of SCORE_ROWS or sequence, and head
+size_t weigh_entries(const Shape& g, int tokens, int seqs);
+void plan_weigh(const Shape& g, const std::vector<Member>& batch, int window, int last, const WeighRoom& room, WeighPlan& out);
 
 }  // namespace paged
 }  // namespace mkv

@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <exception>
+#include <functional>
 #include <memory>
 #include <vector>
 
@@ -12,6 +13,21 @@
 namespace mkv {
 namespace paged {
 constexpr int RING = 4;           // staged uploads in flight
+
+// What a handle that keeps attention weights has to do when its sequences change (paged_weights.cpp).
+struct Weights {
+    virtual ~Weights() = default;
+    // Positions [from, from + count) of the sequences are new: they weigh nothing. (What lies behind a sequence's length may
+    // be anything, so it does not matter if the call that is about to lengthen it fails.)
+    virtual int clear(int n, const int* seq, const int* from, const int* count, const char* who) = 0;
+    // The first len[i] positions of dst[i], which is empty, weigh what those of src[i] do.
+    virtual int copy(int n, const int* src, const int* dst, const int* len, const char* who) = 0;
+    // The work of a batch, its lists for the device (none: no batch), and that it stands.
+    virtual void lay_out(const std::vector<Member>& batch) = 0;
+    virtual void lists(bool none, const std::function<void(size_t, const void*, size_t)>& put) = 0;
+    virtual void stands() = 0;
+};
+
 // Work-groups of a captured kernel, of whatever batch it finds (all loop over their lists): not many more than run at once,
 // since those that find nothing are in the way too. 1 token at 100 positions, 4 at 20,000, 64 at 3,000 of 4 x 128: attention
 // 10.3 / 21.1 / 65.8 us; with 512 of each kind and 16,384 for the joins 13.1 / 28.8 / 68.6.
@@ -43,6 +59,9 @@ struct mpg_store {
     int nruns = 0, longest = 0;     // its runs, and the tokens of the longest
     bool listed = false;            // the lists on the device are a batch's: replays would do it
     std::vector<mkv::paged::Plan> plans, next;  // per window, of the batch and of the one that is being laid out
+    bool begun = false;             // a batch has stood: captured calls may hold the handle's addresses
+    size_t shift_at = 0;            // word offset in dev of the sequences' evicted positions; 0: nothing is ever evicted
+    std::unique_ptr<mkv::paged::Weights> weights;  // none: the handle keeps no weights
 };
 
 namespace mkv {
@@ -104,6 +123,10 @@ int guarded(const char* who, F f) {  // no exception crosses the C boundary
     OnDevice on((h)->device);                                                                                \
     if (const int cap = capturing(h, who))                                                                   \
         return cap < 0 ? cap : fail(MKV_E_ARG, "%s: the stream is capturing; page calls run outside a graph", who)
+
+// paged_store.cpp: the batch that stands ends; what the device does not know of the page tables and shifts goes up.
+int end_batch(mpg_store* h, const char* who);
+int upload_tables(mpg_store* h, const char* who);
 
 }  // namespace paged
 }  // namespace mkv

@@ -16,6 +16,7 @@ static_assert(KINDS < COUNTS, "counts");
 
 struct Geometry {
     int layers, q_heads, kv_heads, head_dim, fmt, pages, page, most_pages;  // most_pages: of a sequence
+    const int* shift = nullptr;  // device: positions evicted from each sequence, where any may be
     size_t page_elems() const { return (size_t)kv_heads * page * head_dim; }
     size_t plane_elems() const { return page_elems() * pages; }
 };
@@ -60,6 +61,51 @@ struct AttendArgs {
 // grid[kind] work-groups for each kind of item (0: not launched), joins likewise; lists and counts on the device.
 hipError_t launch_attend(const Geometry& g, const AttendArgs& a, const int* batch, const Lists& l, const int* grid,
                          int join_grid, hipStream_t s);
+
+// Accumulated attention weights: of (layer, sequence, kv head), `stride` floats.
+struct WeightsAt {
+    float* p;
+    int layers, seqs, kv_heads;
+    size_t stride;
+    __host__ __device__ size_t at(int layer, int seq, int head) const {
+        return (((size_t)layer * seqs + seq) * kv_heads + head) * stride;
+    }
+};
+struct Change {  // positions [a, a + count) of a sequence; a copy's source is `other`
+    int seq, a, count, other;
+};
+hipError_t launch_clear(const WeightsAt& w, const Change* c, int n, hipStream_t s);
+hipError_t launch_weights_copy(const WeightsAt& w, const Change* c, int n, hipStream_t s);
+
+struct WeighLists {  // word offsets in a batch's lists, behind COUNTS of their lengths
+    size_t at[WEIGH_LISTS], words;
+};
+struct WeighArgs {
+    const char* pool;
+    int layer, window, rows;
+    const int* table;
+    Rows q;
+    const float* sinks;
+    float scale, decay;
+    float* stats;  // pairs
+    float* work;
+};
+// grid: work-groups for each list, 0: not launched
+hipError_t launch_weigh(const Geometry& g, const WeightsAt& w, const WeighArgs& a, const int* batch, const WeighLists& l,
+                        const int* grid, hipStream_t s);
+
+struct Eviction {  // `keep` of a sequence's `len` positions; their indexes at `off` of each layer and head's
+    int seq, len, keep, off;
+};
+struct NewPage {  // page `nth` of a sequence (entry of the evictions) is `page` now
+    int entry, nth, page;
+};
+// Which positions stay: to picks[(layer * kv_heads + head) * stride + off ..], in order; `entries` keeps the list for the others.
+hipError_t launch_pick(const Geometry& g, const WeightsAt& w, const Eviction* e, int n, int first, int recent, Eviction* entries,
+                       int* picks, size_t stride, hipStream_t s);
+hipError_t launch_gather(const Geometry& g, char* pool, const int* table, const Eviction* entries, const int* picks, size_t stride,
+                         const NewPage* pages, int n, hipStream_t s);
+hipError_t launch_pack(const WeightsAt& w, const Eviction* entries, int n, const int* picks, size_t stride, hipStream_t s);
 
 }  // namespace paged
 }  // namespace mkv

@@ -168,7 +168,8 @@ __global__ void __launch_bounds__(256) append_kernel(const Run* __restrict__ run
                                                      int kv_heads, int q_heads, T* __restrict__ kpool, T* __restrict__ vpool,
                                                      int rows, const T* __restrict__ k, int64_t k_tok, int64_t k_head,
                                                      const T* __restrict__ v, int64_t v_tok, int64_t v_head, const T* q,
-                                                     int64_t q_tok, int64_t q_head, T* q_out, RopeArgs r) {
+                                                     int64_t q_tok, int64_t q_head, T* q_out, RopeArgs r,
+                                                     const int* __restrict__ shift) {
     extern __shared__ float2 cs[];  // [ROT_ROWS][r.dim / 2]
     const int half = r.dim / 2, tid = threadIdx.x, count = *uniform(nruns);
     const int q_parts = q ? (uniform(nruns)[1] + ROT_ROWS - 1) / ROT_ROWS : 0;  // by the longest run
@@ -179,12 +180,13 @@ __global__ void __launch_bounds__(256) append_kernel(const Run* __restrict__ run
         const Uniform<int> ri = uniform((const int*)(runs + x / per));
         Run run{ri[0], ri[1], ri[2], ri[3]};
         run.count = min(run.count, rows - run.tok);
+        const int pos = run.pos + (shift ? uniform(shift)[run.seq] : 0);  // what eviction has taken lies in front
         if (is_q) {
             const int t0 = of * ROT_ROWS, n = min(ROT_ROWS, run.count - t0);
             if (n <= 0) continue;
             __syncthreads();  // the angles before have been read
             for (Walk w(tid, 256, 1, half); w.row < n; w.next())
-                cs[w.row * half + w.unit] = turn(r, run.pos + t0 + w.row, w.unit);
+                cs[w.row * half + w.unit] = turn(r, pos + t0 + w.row, w.unit);
             __syncthreads();
             const int64_t tok = run.tok + t0;
             rotate_rows<T, WIDE>(r, n, q_heads, dim, q + tok * q_tok, q_tok, q_head, q_out + tok * q_heads * dim,
@@ -200,7 +202,7 @@ __global__ void __launch_bounds__(256) append_kernel(const Run* __restrict__ run
         for (Walk w(tid, 256, row_units<T, WIDE>(dim, r.dim, r.layout), run.count); w.row < 1; w.next()) {
             const int t = w.unit, b = at + t;
             T* const o = kpool + base + b / 16 * 16 * dim + b % 16 * 8;
-            rotate_unit<T, WIDE>(ks + t * k_tok, w.head, r.dim, r.layout, [&](int i) { return turn(r, run.pos + t, i); },
+            rotate_unit<T, WIDE>(ks + t * k_tok, w.head, r.dim, r.layout, [&](int i) { return turn(r, pos + t, i); },
                                  [&](int d) { return o + d / 8 * 128 + d % 8; });
         }
         const T* const vs = v + run.tok * v_tok + head * v_head;
@@ -261,7 +263,7 @@ hipError_t append_as(const Geometry& g, char* pool, int layer, const int* table,
     if (!grid) grid = (int)std::min<size_t>(items, MOST_GRID);
     kernel<<<dim3(grid), dim3(256), lds, s>>>(
         runs, nruns, table, g.most_pages, g.page, g.head_dim, g.kv_heads, g.q_heads, kp, kp + g.plane_elems(), rows,
-        (const T*)k.p, k.tok, k.head, (const T*)v.p, v.tok, v.head, (const T*)q.p, q.tok, q.head, (T*)q_out, r);
+        (const T*)k.p, k.tok, k.head, (const T*)v.p, v.tok, v.head, (const T*)q.p, q.tok, q.head, (T*)q_out, r, g.shift);
     return hipGetLastError();
 }
 

@@ -152,6 +152,7 @@ int upload(mpg_store* h, const std::vector<Run>* runs, const std::vector<Plan>* 
     for (int s = 0; s < b.seqs; s++) {
         const int n = (int)b.table[s].size();
         if (b.fresh[s] < n) put((size_t)s * h->g.most_pages + b.fresh[s], b.table[s].data() + b.fresh[s], n - b.fresh[s]);
+        if (h->shift_at && b.moved[s]) put(h->shift_at + s, &b.shift[s], 1);
     }
     int run_count[COUNTS] = {};
     std::vector<std::vector<int>> counts;
@@ -177,6 +178,7 @@ int upload(mpg_store* h, const std::vector<Run>* runs, const std::vector<Plan>* 
             put(base + h->lists.segs, p.segs.data(), p.segs.size() * (sizeof(Seg) / 4));
         }
         if (order) put(h->order_at, order->data(), order->size() * (sizeof(Place) / 4));
+        if (h->weights) h->weights->lists(!plans, put);
     }
     if (segs.empty()) return MKV_OK;
     const size_t head = segs.size() * (sizeof(Segment) / 4), all = head + at;
@@ -212,12 +214,17 @@ int upload(mpg_store* h, const std::vector<Run>* runs, const std::vector<Plan>* 
     }
     h->turn = (slot + 1) % RING;
     for (int s = 0; s < b.seqs; s++) b.fresh[s] = (int)b.table[s].size();
+    std::fill(b.moved.begin(), b.moved.end(), 0);
     return MKV_OK;
 }
 
+}  // namespace
+
+int mkv::paged::upload_tables(mpg_store* h, const char* who) { return upload(h, nullptr, nullptr, nullptr, who); }
+
 // What replays of captured calls do once pages have changed hands and no batch stands: nothing. The batch stands until the
 // empty lists are on their way.
-int end_batch(mpg_store* h, const char* who) {
+int mkv::paged::end_batch(mpg_store* h, const char* who) {
     if (!h->listed) return MKV_OK;
     const std::vector<Run> none;
     if (const int rc = upload(h, &none, nullptr, nullptr, who)) return rc;
@@ -226,13 +233,16 @@ int end_batch(mpg_store* h, const char* who) {
     return MKV_OK;
 }
 
-// What the device has to do for a call that has changed the book: the batch ends, pages are copied. Where it cannot be told,
-// the book is put back.
-template <typename U>
-int settle(mpg_store* h, const std::vector<Pair>& copies, const char* who, U undo) {
+namespace {
+
+// What the device has to do for a call that has changed the book: the weights follow, the batch ends, pages are copied. Where it
+// cannot be told, the book is put back.
+template <typename U, typename W>
+int settle(mpg_store* h, const std::vector<Pair>& copies, const char* who, U undo, W weights) {
     int rc;
     try {
-        rc = end_batch(h, who);
+        rc = h->weights ? weights() : MKV_OK;
+        if (!rc) rc = end_batch(h, who);
         if (!rc) rc = copy_pages(h, copies, who);
     } catch (...) {
         undo();
@@ -417,11 +427,19 @@ int mpg_pages(const mpg_t* h, int layer, int which, void** base) {
     return MKV_OK;
 }
 
+// The last count[i] positions of sequences that have just been lengthened weigh nothing yet.
+static int clear_new(mpg_t* h, int n, const int* seq, const int* count, const char* who) {
+    std::vector<int> from(n);
+    for (int i = 0; i < n; i++) from[i] = h->book.len[seq[i]] - count[i];
+    return h->weights->clear(n, seq, from.data(), count, who);
+}
+
 int mpg_reserve(mpg_t* h, int n, const int* seq, const int* count) {
     MPG_HOST_CALL(h, "mpg_reserve");
     return guarded("mpg_reserve", [&] {
         if (int rc = h->book.reserve("mpg_reserve", n, seq, count)) return rc;
-        return settle(h, {}, "mpg_reserve", [&] { h->book.undo_reserve(n, seq, count); });
+        return settle(
+            h, {}, "mpg_reserve", [&] { h->book.undo_reserve(n, seq, count); }, [&] { return clear_new(h, n, seq, count, "mpg_reserve"); });
     });
 }
 
@@ -448,7 +466,13 @@ static int lay_out(mpg_t* h, int n, const int* seq, const int* count, bool share
         if (shared) plan_shared(h->shape, batch, common, h->kinds[w], h->next[w]);
         else plan_window(h->shape, batch, h->kinds[w], h->next[w]);
     }
+    if (h->weights) {
+        h->weights->lay_out(batch);
+        if (int rc = clear_new(h, n, seq, count, who)) return rc;
+    }
     if (int rc = upload(h, &runs, &h->next, &common.order, who)) return rc;
+    if (h->weights) h->weights->stands();
+    h->begun = true;
     h->listed = true;
     h->plans.swap(h->next);
     h->tokens = tok;
@@ -490,7 +514,8 @@ int mpg_set_len(mpg_t* h, int seq, int len) {
         std::vector<Pair> copies;
         Cut cut;
         if (int rc = h->book.set_len("mpg_set_len", seq, len, copies, &cut)) return rc;
-        return settle(h, copies, "mpg_set_len", [&] { h->book.undo_set_len(seq, cut); });
+        return settle(
+            h, copies, "mpg_set_len", [&] { h->book.undo_set_len(seq, cut); }, [] { return MKV_OK; });
     });
 }
 
@@ -499,7 +524,13 @@ static int fork_pages(mpg_t* h, int n, const int* src, const int* dst, const int
     return guarded(who, [&] {
         std::vector<Pair> copies;
         if (int rc = h->book.fork(who, n, src, dst, len, own, copies)) return rc;
-        return settle(h, copies, who, [&] { h->book.undo_fork(n, dst); });
+        return settle(
+            h, copies, who, [&] { h->book.undo_fork(n, dst); },
+            [&] {
+                std::vector<int> upto(n);
+                for (int i = 0; i < n; i++) upto[i] = h->book.len[dst[i]];
+                return h->weights->copy(n, src, dst, upto.data(), who);
+            });
     });
 }
 
@@ -522,7 +553,7 @@ int mpg_compact(mpg_t* h, int* moved) {
     return guarded("mpg_compact", [&] {
         std::vector<Pair> copies;
         const int n = h->book.compact(copies);
-        if (int rc = settle(h, copies, "mpg_compact", [&] { h->book.undo_compact(copies); })) return rc;
+        if (int rc = settle(h, copies, "mpg_compact", [&] { h->book.undo_compact(copies); }, [] { return MKV_OK; })) return rc;
         if (moved) *moved = n;
         return MKV_OK;
     });

@@ -1,0 +1,732 @@
+// paged_weigh.hip -- attention weights accumulated position by position, and eviction by them.
+//
+// What the counted tokens t of a batch give to position j of kv head g, over the query heads h of its group:
+//   w_j = sum over t, h of exp(s_thj - m_th) / l_th,   l_th = sum over j of exp(s_thj - m_th) [+ exp(sink_h - m_th)]
+// so it takes two readings of the scores: of every row's m and l (score_few, score_rows), then of every position's sum over
+// the rows (sum_few, sum_rows). Few rows keep their scores between the two, 4 bytes a score against 2 x head_dim of K; many
+// rows' scores are computed again. Everything behind the products is in f32, nothing is rounded in between, and sums are taken
+// in an order that does not depend on timing.
+#include <algorithm>
+
+#include "mkv_device.h"
+#include "paged_device.h"
+
+namespace mkv {
+namespace paged {
+namespace {
+
+#define INLINE __attribute__((always_inline))
+
+__device__ inline f32x4 mfma16(Vec8<_Float16> a, Vec8<_Float16> b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ inline f32x4 mfma16(Vec8<__bf16> a, Vec8<__bf16> b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ inline f32x16 mfma32(Vec8<_Float16> a, Vec8<_Float16> b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ inline f32x16 mfma32(Vec8<__bf16> a, Vec8<__bf16> b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+struct Args {
+    const int* table;
+    int most_pages, page, page_shift;
+    int kv_heads, group, window, rows;
+    const void* kpool;  // the layer's K pages
+    const void* q;
+    int64_t q_tok, q_head;
+    const float* sinks;
+    float scale2, decay;  // scale * log2 e
+    float2* stats;        // a row's reference (log2 units) and sum, piece by piece of its keys
+    float* work;
+    float* weights;       // of the layer
+    size_t stride, seq_stride;
+};
+
+// K of a sequence: where the 32 positions from `key` on lie.
+template <int D>
+struct Keys {
+    const char* p;
+    Uniform<int> table;
+    size_t page_bytes;
+    int shift, mask;
+    __device__ Keys(const Args& a, int seq, int head)
+        : p((const char*)a.kpool + (size_t)head * a.page * D * 2), table(uniform(a.table) + (size_t)seq * a.most_pages),
+          page_bytes((size_t)a.kv_heads * a.page * D * 2), shift(a.page_shift), mask(a.page - 1) {}
+    __device__ const char* block(int key) const { return p + table[key >> shift] * page_bytes + (size_t)(key & mask) * D * 2; }
+};
+
+// (m, l) of the same row put together; m = -inf: nothing but what l says (NaN of a score that no maximum takes).
+__device__ inline float2 merge(float2 x, float2 y) {
+    const float m = fmaxf(x.x, y.x);
+    const float f = x.x == NEG_INF ? 0.f : fast_exp2(x.x - m), g = y.x == NEG_INF ? 0.f : fast_exp2(y.x - m);
+    return make_float2(m, x.y * f + y.y * g);
+}
+__device__ inline float2 shuffled(float2 x, int by) { return make_float2(__shfl_xor(x.x, by), __shfl_xor(x.y, by)); }
+// What turns a row's scores into weights: exp2(score - m) * r.
+__device__ inline float2 factor_of(const Args& a, float2 s, int head) {
+    if (a.sinks) s = merge(s, make_float2(a.sinks[head] * LOG2E, 1.f));
+    return make_float2(s.x, 1.f / s.y);
+}
+// One more score of a row (log2 units) in its (m, l).
+template <int N>
+__device__ inline void add_scores(float2& ml, const float (&s)[N]) {
+    float top = ml.x;
+#pragma unroll
+    for (int i = 0; i < N; i++) top = fmaxf(top, s[i]);
+    const float ref = top == NEG_INF ? 0.f : top;
+    float sum = ml.x == NEG_INF ? ml.y : ml.y * fast_exp2(ml.x - ref);
+#pragma unroll
+    for (int i = 0; i < N; i++) sum += fast_exp2(s[i] - ref);
+    ml = make_float2(top, sum);
+}
+
+__device__ inline Score load_score(const Score* p) {
+    const Uniform<int> x = uniform((const int*)p);
+    return Score{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], x[8], x[9], {0, 0}};
+}
+__device__ inline Sum load_sum(const Sum* p) {
+    const Uniform<int> x = uniform((const int*)p);
+    return Sum{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], x[8], x[9], x[10], x[11], x[12], x[13], {0, 0}};
+}
+
+// ---- statistics of few rows, NRT x 16 of them, with their scores ----
+// 4 waves, each with every fourth block of 32 keys, its K straight from memory into the operands of the 16x16x32 products, the
+// next block's on its way meanwhile. Lane (r, g): row r, keys 4g + i and 16 + 4g + i of the block; each lane has an m and l of
+// its own until the end. Bound by memory.
+template <typename T, int D, int NRT>
+__global__ void __launch_bounds__(256) score_few(Args a, const Score* __restrict__ items, const int* __restrict__ nitems) {
+    constexpr int NS = D / 32;
+    __shared__ float2 sml[4][16 * NRT];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const int count = *uniform(nitems);
+    for (int n = blockIdx.x; n < count; n += gridDim.x) {
+        const Score it = load_score(items + n);
+        const Keys<D> keys(a, it.seq, it.head);
+        const int blocks = (it.k1 - it.k0 + KEYS - 1) / KEYS;
+        Vec8<T> kf[2][NS];
+        auto load_k = [&](int j) INLINE {
+            const char* const p = keys.block(it.k0 + KEYS * min(j, blocks - 1));
+#pragma unroll
+            for (int s = 0; s < NS; s++)
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+                    kf[b][s] = __builtin_nontemporal_load((const Vec8<T>*)(p + b * 16 * D * 2 + s * 1024 + lane * 16));
+        };
+        if (w < blocks) load_k(w);
+        Vec8<T> q[NRT][NS];
+        int lo[NRT], hi[NRT];
+        float2 ml[NRT];
+#pragma unroll
+        for (int t = 0; t < NRT; t++) {
+            const int row = 16 * t + r, tok = row / a.group, head = it.head * a.group + row % a.group;
+            const bool is = row < it.rows && it.tok0 + tok < a.rows;
+            hi[t] = is ? it.pos0 + tok : -1;
+            lo[t] = a.window ? it.pos0 + tok - a.window + 1 : 0;
+            const T* const src = (const T*)a.q + (int64_t)(it.tok0 + tok) * a.q_tok + head * a.q_head + 8 * g;
+#pragma unroll
+            for (int s = 0; s < NS; s++) q[t][s] = is ? load8(src + 32 * s) : Vec8<T>{};
+            ml[t] = make_float2(NEG_INF, 0.f);
+        }
+        const int all_hi = it.pos0, all_lo = a.window ? it.pos0 + (it.rows - 1) / a.group - a.window + 1 : 0;
+        for (int j = w; j < blocks; j += 4) {
+            f32x4 s[NRT][2];
+#pragma unroll
+            for (int t = 0; t < NRT; t++) s[t][0] = s[t][1] = f32x4{};
+#pragma unroll
+            for (int i = 0; i < NS; i++)
+#pragma unroll
+                for (int t = 0; t < NRT; t++)
+#pragma unroll
+                    for (int b = 0; b < 2; b++) s[t][b] = mfma16(kf[b][i], q[t][i], s[t][b]);
+            load_k(j + 4);
+            const int k0 = it.k0 + KEYS * j;
+            const bool edge = k0 + KEYS - 1 > all_hi || k0 < all_lo;
+            float* const to = a.work + it.keep + (size_t)j * KEYS * it.rows;
+#pragma unroll
+            for (int t = 0; t < NRT; t++) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    x[e] = s[t][e / 4][e % 4] * a.scale2;
+                    const int key = k0 + e / 4 * 16 + 4 * g + e % 4;
+                    if (edge && (key > hi[t] || key < lo[t])) x[e] = NEG_INF;
+                }
+                add_scores(ml[t], x);
+                const int row = 16 * t + r;
+                if (row < it.rows) {
+                    *(f32x4*)(to + row * KEYS + 4 * g) = f32x4{x[0], x[1], x[2], x[3]};
+                    *(f32x4*)(to + row * KEYS + 16 + 4 * g) = f32x4{x[4], x[5], x[6], x[7]};
+                }
+            }
+        }
+        __syncthreads();  // the item before has been read
+#pragma unroll
+        for (int t = 0; t < NRT; t++) {
+            ml[t] = merge(ml[t], shuffled(ml[t], 16));
+            ml[t] = merge(ml[t], shuffled(ml[t], 32));
+            if (g == 0) sml[w][16 * t + r] = ml[t];
+        }
+        __syncthreads();
+        const int row = threadIdx.x;
+        if (row < 16 * NRT && row < it.rows) a.stats[it.stat + row] = merge(merge(sml[0][row], sml[1][row]), merge(sml[2][row], sml[3][row]));
+    }
+}
+
+// ---- statistics of many rows: 4 waves of 32 rows against the same keys ----
+// S^T[32 keys][32 rows] = K . Q^T (32x32x16): lane (r, h) has row r, keys 8c + 4h + i.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) score_rows(Args a, const Score* __restrict__ items, const int* __restrict__ nitems) {
+    constexpr int NS = D / 16;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h = lane >> 5;
+    const int count = *uniform(nitems);
+    for (int n = blockIdx.x; n < count; n += gridDim.x) {
+        const Score it = load_score(items + n);
+        const Keys<D> keys(a, it.seq, it.head);
+        const int first = it.row0 + 32 * w, row = first + r, last = min(first + 31, it.rows - 1);
+        if (first >= it.rows) continue;
+        const int tok = row / a.group, head = it.head * a.group + row % a.group;
+        const bool is = row < it.rows && it.tok0 + tok < a.rows;
+        const int hi = is ? it.pos0 + tok : -1, lo = a.window ? it.pos0 + tok - a.window + 1 : 0;
+        const int all_hi = it.pos0 + first / a.group, all_lo = a.window ? it.pos0 + last / a.group - a.window + 1 : 0;
+        Vec8<T> q[NS], k[NS];
+        const T* const src = (const T*)a.q + (int64_t)(it.tok0 + tok) * a.q_tok + head * a.q_head + 8 * h;
+#pragma unroll
+        for (int s = 0; s < NS; s++) q[s] = is ? load8(src + 16 * s) : Vec8<T>{};
+        const int blocks = (it.k1 - it.k0 + KEYS - 1) / KEYS;
+        const unsigned at = (r >> 4) * 16 * D * 2 + h * 256 + (r & 15) * 16;
+        auto load_k = [&](int j) INLINE {
+            const char* const p = keys.block(it.k0 + KEYS * min(j, blocks - 1)) + at;
+#pragma unroll
+            for (int s = 0; s < NS; s++) k[s] = load8((const T*)(p + s * 512));
+        };
+        float2 ml = make_float2(NEG_INF, 0.f);
+        if (blocks > 0) load_k(0);
+        for (int j = 0; j < blocks; j++) {
+            f32x16 s = f32x16{};
+#pragma unroll
+            for (int i = 0; i < NS; i++) s = mfma32(k[i], q[i], s);
+            load_k(j + 1);
+            const int k0 = it.k0 + KEYS * j;
+            const bool edge = k0 + KEYS - 1 > all_hi || k0 < all_lo;
+            float x[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                x[i] = s[i] * a.scale2;
+                const int key = k0 + i / 4 * 8 + 4 * h + i % 4;
+                if (edge && (key > hi || key < lo)) x[i] = NEG_INF;
+            }
+            add_scores(ml, x);
+        }
+        ml = merge(ml, shuffled(ml, 32));
+        if (h == 0 && row < it.rows) a.stats[it.stat + 32 * w + r] = ml;
+    }
+}
+
+// ---- sums over few rows' kept scores: a thread a key ----
+__global__ void __launch_bounds__(256) sum_few(Args a, const Sum* __restrict__ items, const int* __restrict__ nitems) {
+    __shared__ float2 f[32];
+    __shared__ int odd;  // a row whose weights are no numbers where it sees, and nothing all the same where it does not
+    const int count = *uniform(nitems), tid = threadIdx.x;
+    for (int n = blockIdx.x; n < count; n += gridDim.x) {
+        const Sum it = load_sum(items + n);
+        const int rows = min(it.rows, (a.rows - it.tok0) * a.group);  // that the call has
+        __syncthreads();  // the item before has been read
+        if (tid == 0) odd = 0;
+        __syncthreads();
+        {  // 8 lanes a row
+            const int row = tid / 8;
+            float2 s = make_float2(NEG_INF, 0.f);
+            if (row < rows)
+                for (int p = tid % 8; p < it.pieces; p += 8) s = merge(s, a.stats[it.stat + p * it.rows + row]);
+#pragma unroll
+            for (int i = 1; i < 8; i *= 2) s = merge(s, shuffled(s, i));
+            if (tid % 8 == 0 && row < rows) {
+                f[row] = s = factor_of(a, s, it.head * a.group + row % a.group);
+                if (!(s.y < -NEG_INF)) odd = 1;
+            }
+        }
+        __syncthreads();
+        float* const weights = a.weights + it.seq * a.seq_stride + it.head * a.stride;
+        for (int key = it.k0 + tid; key < it.k1; key += 256) {
+            const int i = key - it.s0;
+            const float* const s = a.work + it.scores + (size_t)(i / KEYS) * KEYS * it.rows + i % KEYS;
+            float sum = 0.f;
+#pragma unroll 8
+            for (int r = 0; r < rows; r++) sum += fast_exp2(s[r * KEYS] - f[r].x) * f[r].y;
+            if (odd) {
+                sum = 0.f;
+                for (int r = 0; r < rows; r++) {
+                    const int pos = it.pos0 + r / a.group;
+                    if (key <= pos && (!a.window || key > pos - a.window)) sum += fast_exp2(s[r * KEYS] - f[r].x) * f[r].y;
+                }
+            }
+            weights[key] = (a.decay == 0.f ? 0.f : a.decay * weights[key]) + sum;
+        }
+    }
+}
+
+// ---- sums over many rows: 4 waves of 64 keys against the same rows, 32 at a time through LDS ----
+// S[32 rows][32 keys] = Q . K^T (32x32x16), K in registers: lane (x, h) has key x, rows 8c + 4h + i, so a key's sum over the
+// rows stays in its lane.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) sum_rows(Args a, const Sum* __restrict__ items, const int* __restrict__ nitems) {
+    constexpr int NS = D / 16, PER = D / 64;  // 16-byte pieces of a row tile that a thread brings
+    __shared__ __attribute__((aligned(16))) T sq[2][32][D + 8];
+    __shared__ __attribute__((aligned(16))) float sm[2][32], sr[2][32];
+    __shared__ __attribute__((aligned(16))) int sp[2][32];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), x = lane & 31, h = lane >> 5;
+    const int count = *uniform(nitems);
+    for (int n = blockIdx.x; n < count; n += gridDim.x) {
+        const Sum it = load_sum(items + n);
+        const Keys<D> keys(a, it.seq, it.head);
+        float* const weights = a.weights + it.seq * a.seq_stride + it.head * a.stride;
+        for (int k0 = it.k0; k0 < it.k1; k0 += SUM_KEYS) {
+            const int first = k0 + 64 * w;  // the wave's keys; behind the last the last block again, not counted
+            Vec8<T> k[2][NS];
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                const char* const p = keys.block(min(first + 32 * b, (it.k1 - 1) / KEYS * KEYS)) + (x >> 4) * 16 * D * 2 + h * 256 + (x & 15) * 16;
+#pragma unroll
+                for (int s = 0; s < NS; s++) k[b][s] = load8((const T*)(p + s * 512));
+            }
+            float sum[2] = {0.f, 0.f};
+            Vec8<T> next[PER];
+            float2 stat;
+            int pos;
+            auto bring = [&](int r0) INLINE {  // rows r0 .. r0 + 31 and their statistics, 8 lanes a row
+#pragma unroll
+                for (int i = 0; i < PER; i++) {
+                    const int c = tid + 256 * i, row = r0 + c / (D / 8), tok = it.tok0 + row / a.group;
+                    const bool is = row < it.r1 && tok < a.rows;
+                    next[i] = is ? load8((const T*)a.q + (int64_t)tok * a.q_tok + (it.head * a.group + row % a.group) * a.q_head + c % (D / 8) * 8)
+                                 : Vec8<T>{};
+                }
+                const int row = r0 + tid / 8;
+                stat = make_float2(NEG_INF, 0.f);
+                if (row < it.r1)
+                    for (int p = tid % 8; p < it.pieces; p += 8) stat = merge(stat, a.stats[it.stat + p * it.rows + row]);
+                pos = it.pos0 + row / a.group;
+            };
+            auto put = [&](int r0, int to) INLINE {
+#pragma unroll
+                for (int i = 0; i < PER; i++) {
+                    const int c = tid + 256 * i;
+                    *(Vec8<T>*)&sq[to][c / (D / 8)][c % (D / 8) * 8] = next[i];
+                }
+#pragma unroll
+                for (int i = 1; i < 8; i *= 2) stat = merge(stat, shuffled(stat, i));
+                if (tid % 8 == 0) {
+                    const int row = r0 + tid / 8;
+                    const bool is = row < it.r1 && it.tok0 + row / a.group < a.rows;
+                    // a row that is none weighs nothing: exp2(0 - inf) * 0
+                    const float2 f = is ? factor_of(a, stat, it.head * a.group + row % a.group) : make_float2(-NEG_INF, 0.f);
+                    sm[to][tid / 8] = f.x;
+                    sr[to][tid / 8] = f.y;
+                    sp[to][tid / 8] = is ? pos : -1;
+                }
+            };
+            const long long there = min((long long)it.r1, (long long)(a.rows - it.tok0) * a.group);  // rows that the call has
+            // the first rows that see any of these keys
+            int r0 = max(it.r0, (int)(min((long long)(k0 - it.pos0) * a.group, (long long)it.rows)) / KEYS * KEYS);
+            __syncthreads();  // the rows before have been read
+            if (r0 < it.r1) {
+                bring(r0);
+                put(r0, 0);
+            }
+            __syncthreads();
+            for (int at = 0; r0 < it.r1; r0 += 32, at ^= 1) {
+                const bool more = r0 + 32 < it.r1;
+                if (more) bring(r0 + 32);
+                f32x16 s[2] = {f32x16{}, f32x16{}};
+#pragma unroll
+                for (int i = 0; i < NS; i++) {
+                    const Vec8<T> q = *(const Vec8<T>*)&sq[at][x][16 * i + 8 * h];
+#pragma unroll
+                    for (int b = 0; b < 2; b++) s[b] = mfma32(q, k[b][i], s[b]);
+                }
+                // rows from r0 on at it.pos0 + r0 / group and behind
+                const int low = it.pos0 + r0 / a.group, high = it.pos0 + (r0 + 31) / a.group;
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    const int key = first + 32 * b + x;
+                    const bool edge = r0 + 32 > there || first + 32 * b + 31 > low || (a.window && first + 32 * b < high - a.window + 1);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const f32x4 m = *(const f32x4*)&sm[at][8 * c + 4 * h], f = *(const f32x4*)&sr[at][8 * c + 4 * h];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            float y = __builtin_fmaf(s[b][4 * c + i], a.scale2, -m[i]);
+                            y = fast_exp2(y) * f[i];
+                            if (edge) {
+                                const int p = sp[at][8 * c + 4 * h + i];
+                                if (key > p || (a.window && key < p - a.window + 1)) y = 0.f;
+                            }
+                            sum[b] += y;
+                        }
+                    }
+                }
+                if (more) put(r0 + 32, at ^ 1);
+                __syncthreads();
+            }
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                const float y = sum[b] + __shfl_xor(sum[b], 32);
+                const int key = first + 32 * b + x;
+                if (h || key >= it.k1) continue;
+                if (it.part >= 0) a.work[it.part + key - it.k0] = y;
+                else weights[key] = (a.decay == 0.f ? 0.f : a.decay * weights[key]) + y;
+            }
+        }
+    }
+}
+
+// ---- weights that fade, and partial sums that join them ----
+__global__ void __launch_bounds__(256) fade_kernel(Args a, const Fade* __restrict__ items, const int* __restrict__ nitems) {
+    const int count = *uniform(nitems);
+    for (int n = blockIdx.x; n < count; n += gridDim.x) {
+        const Uniform<int> u = uniform((const int*)(items + n));
+        const Fade it{u[0], u[1], u[2], u[3], u[4], u[5], u[6], 0};
+        if (!it.sums && a.decay == 1.f) continue;
+        float* const weights = a.weights + it.seq * a.seq_stride + it.head * a.stride;
+        for (int key = it.k0 + threadIdx.x; key < it.k1; key += 256) {
+            const float* const p = a.work + it.part + key - it.k0;
+            float sum = 0.f;
+            for (int s = 0; s < it.sums; s++) sum += p[(size_t)s * it.stride];
+            weights[key] = (a.decay == 0.f ? 0.f : a.decay * weights[key]) + sum;
+        }
+    }
+}
+
+// ---- weights of positions that are new, or another sequence's ----
+constexpr int CHANGES = 128;  // of a launch, in its arguments
+struct ChangeList {
+    Change c[CHANGES];
+};
+constexpr int SPAN = 4096;  // positions of a work-group
+template <bool COPY>
+__global__ void __launch_bounds__(256) change_kernel(WeightsAt w, ChangeList list, int n, int spans, size_t all) {
+    for (size_t i = blockIdx.x; i < all; i += gridDim.x) {  // (layer and head, change, span)
+        const int span = (int)(i % spans), c = (int)(i / spans % n);
+        const size_t unit = i / spans / n;
+        const int layer = (int)(unit / w.kv_heads), head = (int)(unit % w.kv_heads);
+        const Change x = list.c[c];
+        float* const p = w.p + w.at(layer, x.seq, head) + x.a;
+        const float* const from = COPY ? w.p + w.at(layer, x.other, head) + x.a : nullptr;
+        const int end = min(x.count, (span + 1) * SPAN);
+        for (int j = span * SPAN + threadIdx.x; j < end; j += 256) p[j] = COPY ? from[j] : 0.f;
+    }
+}
+
+// ---- eviction ----
+constexpr int EVICTIONS = 128, NEW_PAGES = 256;
+struct EvictionList {
+    Eviction e[EVICTIONS];
+};
+struct PageList {
+    NewPage p[NEW_PAGES];
+};
+
+// Weights in an order of whole numbers; NaN weighs most, both zeros the same.
+__device__ inline unsigned order_of(float x) {
+    if (x != x) return ~0u;
+    const unsigned u = __float_as_uint(x == 0.f ? 0.f : x);
+    return u >> 31 ? ~u : u | 0x80000000u;
+}
+
+// The picks of one sequence, layer and head by a work-group: the least weight that stays, by four digits of eight bits from the
+// highest on, then the positions in order; of those with just that weight the first ones.
+__global__ void __launch_bounds__(1024) pick_kernel(WeightsAt w, EvictionList list, int n, int entry0, int first, int recent,
+                                                    Eviction* __restrict__ entries, int* __restrict__ picks, size_t stride, int units) {
+    // (at most EVICTIONS x 2^22 pairs of a sequence and a layer's head)
+    __shared__ int hist[256];
+    __shared__ int waves[16];
+    __shared__ int found[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    for (int b = blockIdx.x; b < n * units; b += gridDim.x) {
+        const int c = b / units, unit = b % units;
+        const Eviction e = list.e[c];
+        if (unit == 0 && tid == 0) entries[entry0 + c] = e;
+        int* const to = picks + (size_t)unit * stride + e.off;
+        const float* const src = w.p + w.at(unit / w.kv_heads, e.seq, unit % w.kv_heads);
+        const int lo = first, hi = e.len - recent, want = e.keep - first - recent;
+        for (int i = tid; i < first; i += 1024) to[i] = i;
+        for (int i = tid; i < recent; i += 1024) to[e.keep - recent + i] = hi + i;
+        unsigned known = 0, mask = 0;  // the digits of the least weight that stays
+        int left = want;               // of those that have them
+        for (int digit = 24; digit >= 0 && want; digit -= 8) {
+            __syncthreads();
+            if (tid < 256) hist[tid] = 0;
+            __syncthreads();
+            for (int i = lo + tid; i < hi; i += 1024) {
+                const unsigned k = order_of(src[i]);
+                if ((k & mask) == known) atomicAdd(&hist[k >> digit & 255], 1);
+            }
+            __syncthreads();
+            if (tid < 64) {  // from the highest digit down: lane l has digits 255 - 4 l .. 252 - 4 l
+                int mine[4], sum = 0;
+#pragma unroll
+                for (int x = 0; x < 4; x++) sum += mine[x] = hist[255 - 4 * lane - x];
+                int before = sum;
+#pragma unroll
+                for (int x = 1; x < 64; x *= 2) {
+                    const int y = __shfl_up(before, x);
+                    if (lane >= x) before += y;
+                }
+                before -= sum;
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    if (before < left && before + mine[x] >= left) {
+                        found[0] = 255 - 4 * lane - x;
+                        found[1] = left - before;
+                    }
+                    before += mine[x];
+                }
+            }
+            __syncthreads();
+            known |= (unsigned)found[0] << digit;
+            mask |= 255u << digit;
+            left = found[1];
+        }
+        // left: how many of those with just the least weight stay
+        int more = 0, same = 0;  // before the tile: heavier ones, ones of the least weight
+        for (int i0 = lo; i0 < hi && want; i0 += 4096) {
+            unsigned k[4];
+            int mine = 0;  // (heavier) + (same) << 16
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int i = i0 + 4 * tid + x;
+                k[x] = i < hi ? order_of(src[i]) : 0;
+                if (i < hi) mine += k[x] > known ? 1 : k[x] == known ? 1 << 16 : 0;
+            }
+            int before = mine;
+#pragma unroll
+            for (int x = 1; x < 64; x *= 2) {
+                const int y = __shfl_up(before, x);
+                if (lane >= x) before += y;
+            }
+            __syncthreads();
+            if (lane == 63) waves[wave] = before;
+            __syncthreads();
+            int all = 0;
+            before -= mine;
+#pragma unroll
+            for (int x = 0; x < 16; x++) {
+                if (x < wave) before += waves[x];
+                all += waves[x];
+            }
+            int m = more + (before & 0xFFFF), s = same + (before >> 16);
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int i = i0 + 4 * tid + x;
+                if (i >= hi) break;
+                if (k[x] > known) to[first + m++ + min(s, left)] = i;
+                else if (k[x] == known) {
+                    if (s < left) to[first + m + s] = i;
+                    s++;
+                }
+            }
+            more += all & 0xFFFF;
+            same += all >> 16;
+        }
+        __syncthreads();
+    }
+}
+
+// A new page's block of 32 positions of a head and layer, K or V: 16 bytes of K a thread (8 dims of a position), 16 bytes of V
+// (a dim of 8 positions, which come from 8 places). Positions behind the last that stays are left as they were.
+template <int D>
+__global__ void __launch_bounds__(256) gather_kernel(unsigned short* __restrict__ pool, const int* __restrict__ table, int most_pages,
+                                                     int page, int kv_heads, int units, size_t plane,
+                                                     const Eviction* __restrict__ entries, const int* __restrict__ picks,
+                                                     size_t stride, PageList list) {
+    __shared__ size_t from[KEYS];
+    __shared__ int in[KEYS];
+    typedef Vec8<unsigned short> Unit;
+    const int tid = threadIdx.x, blocks = page / KEYS;
+    const NewPage np = list.p[blockIdx.x / blocks];
+    const int block = blockIdx.x % blocks;
+    const bool is_v = blockIdx.z;
+    const Eviction e = entries[np.entry];
+    const int p0 = np.nth * page + block * KEYS, count = min(KEYS, e.keep - p0);
+    if (count <= 0) return;
+    for (int unit = blockIdx.y; unit < units; unit += gridDim.y) {
+        const int head = unit % kv_heads, layer = unit / kv_heads;
+        unsigned short* const base = pool + ((size_t)layer * 2 + is_v) * plane;
+        __syncthreads();  // the places before have been read
+        if (tid < count) {
+            const int p = picks[(size_t)unit * stride + e.off + p0 + tid];
+            from[tid] = ((size_t)table[(size_t)e.seq * most_pages + p / page] * kv_heads + head) * page * D + (size_t)(p % page / KEYS) * KEYS * D;
+            in[tid] = p % KEYS;
+        }
+        __syncthreads();
+        unsigned short* const to = base + ((size_t)np.page * kv_heads + head) * page * D + (size_t)block * KEYS * D;
+        if (!is_v) {
+            for (int i = tid; i < KEYS * D / 8; i += 256) {
+                const int x = i % KEYS, c = i / KEYS;
+                if (x >= count) continue;
+                const int y = in[x];
+                *(Unit*)(to + x / 16 * 16 * D + c * 128 + x % 16 * 8) = *(const Unit*)(base + from[x] + y / 16 * 16 * D + c * 128 + y % 16 * 8);
+            }
+            continue;
+        }
+        for (int i = tid; i < 4 * D; i += 256) {
+            const int g = i / D, d = i % D;
+            Unit u;
+            bool whole = true;
+#pragma unroll
+            for (int z = 0; z < 8; z++) {
+                const int x = 16 * (z / 4) + 4 * g + z % 4;
+                if (x < count) {
+                    const int y = in[x];
+                    u[z] = base[from[x] + (y % 16 / 4 * D + d) * 8 + y / 16 * 4 + y % 4];
+                } else {
+                    whole = false;
+                }
+            }
+            unsigned short* const o = to + i * 8;
+            if (whole) {
+                *(Unit*)o = u;
+            } else {
+#pragma unroll
+                for (int z = 0; z < 8; z++)
+                    if (16 * (z / 4) + 4 * g + z % 4 < count) o[z] = u[z];
+            }
+        }
+    }
+}
+
+// The weights that stay, in place: a position's goes to one that is not behind it, tile by tile.
+__global__ void __launch_bounds__(1024) pack_kernel(WeightsAt w, const Eviction* __restrict__ entries, const int* __restrict__ picks,
+                                                    size_t stride, int n, int units) {
+    for (size_t b = blockIdx.x; b < (size_t)n * units; b += gridDim.x) {
+        const int unit = (int)(b % units);
+        const Eviction e = entries[b / units];
+        float* const p = w.p + w.at(unit / w.kv_heads, e.seq, unit % w.kv_heads);
+        const int* const from = picks + (size_t)unit * stride + e.off;
+        for (int i0 = 0; i0 < e.keep; i0 += 4096) {
+            float x[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int i = i0 + threadIdx.x + 1024 * j;
+                x[j] = i < e.keep ? p[from[i]] : 0.f;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int i = i0 + threadIdx.x + 1024 * j;
+                if (i < e.keep) p[i] = x[j];
+            }
+            __syncthreads();
+        }
+    }
+}
+
+template <typename T, int D>
+hipError_t weigh_as(const Args& a, const int* batch, const WeighLists& l, const int* grid, hipStream_t s) {
+    hipError_t e = hipSuccess;
+    auto go = [&](auto kernel, int list, auto* items) {
+        if (!grid[list] || e != hipSuccess) return;
+        kernel<<<dim3(grid[list]), dim3(256), 0, s>>>(a, items, batch + list);
+        e = hipGetLastError();
+    };
+    go(score_few<T, D, 1>, SCORE_FEW, (const Score*)(batch + l.at[SCORE_FEW]));
+    go(score_few<T, D, 2>, SCORE_SOME, (const Score*)(batch + l.at[SCORE_SOME]));
+    go(score_rows<T, D>, SCORE_MANY, (const Score*)(batch + l.at[SCORE_MANY]));
+    go(sum_few, SUM_FEW, (const Sum*)(batch + l.at[SUM_FEW]));
+    go(sum_rows<T, D>, SUM_MANY, (const Sum*)(batch + l.at[SUM_MANY]));
+    go(fade_kernel, FADES, (const Fade*)(batch + l.at[FADES]));
+    return e;
+}
+
+template <typename T>
+hipError_t weigh_dim(int dim, const Args& a, const int* batch, const WeighLists& l, const int* grid, hipStream_t s) {
+    return dim == 64 ? weigh_as<T, 64>(a, batch, l, grid, s) : dim == 128 ? weigh_as<T, 128>(a, batch, l, grid, s) : weigh_as<T, 256>(a, batch, l, grid, s);
+}
+
+template <bool COPY>
+hipError_t change(const WeightsAt& w, const Change* c, int n, hipStream_t s) {
+    for (int i = 0; i < n; i += CHANGES) {
+        ChangeList list;
+        const int m = std::min(CHANGES, n - i);
+        int most = 0;
+        for (int j = 0; j < CHANGES; j++) list.c[j] = j < m ? c[i + j] : Change{0, 0, 0, 0};
+        for (int j = 0; j < m; j++) most = std::max(most, c[i + j].count);
+        const int spans = (most + SPAN - 1) / SPAN;
+        const size_t all = (size_t)w.layers * w.kv_heads * m * spans;
+        change_kernel<COPY><<<dim3((unsigned)std::min<size_t>(all, MOST_GRID)), dim3(256), 0, s>>>(w, list, m, spans, all);
+        if (const hipError_t e = hipGetLastError()) return e;
+    }
+    return hipSuccess;
+}
+
+}  // namespace
+
+hipError_t launch_clear(const WeightsAt& w, const Change* c, int n, hipStream_t s) { return change<false>(w, c, n, s); }
+hipError_t launch_weights_copy(const WeightsAt& w, const Change* c, int n, hipStream_t s) { return change<true>(w, c, n, s); }
+
+hipError_t launch_weigh(const Geometry& g, const WeightsAt& w, const WeighArgs& x, const int* batch, const WeighLists& l,
+                        const int* grid, hipStream_t s) {
+    Args a;
+    a.table = x.table;
+    a.most_pages = g.most_pages;
+    a.page = g.page;
+    a.page_shift = __builtin_ctz(g.page);
+    a.kv_heads = g.kv_heads;
+    a.group = g.q_heads / g.kv_heads;
+    a.window = x.window;
+    a.rows = x.rows;
+    a.kpool = x.pool + (size_t)x.layer * 2 * g.plane_elems() * 2;
+    a.q = x.q.p;
+    a.q_tok = x.q.tok;
+    a.q_head = x.q.head;
+    a.sinks = x.sinks;
+    a.scale2 = x.scale * LOG2E;
+    a.decay = x.decay;
+    a.stats = (float2*)x.stats;
+    a.work = x.work;
+    a.weights = w.p + w.at(x.layer, 0, 0);
+    a.stride = w.stride;
+    a.seq_stride = w.stride * w.kv_heads;
+    return g.fmt == MKV_F16 ? weigh_dim<_Float16>(g.head_dim, a, batch, l, grid, s) : weigh_dim<__bf16>(g.head_dim, a, batch, l, grid, s);
+}
+
+hipError_t launch_pick(const Geometry& g, const WeightsAt& w, const Eviction* e, int n, int first, int recent, Eviction* entries,
+                       int* picks, size_t stride, hipStream_t s) {
+    const int units = g.layers * g.kv_heads;
+    for (int i = 0; i < n; i += EVICTIONS) {
+        EvictionList list;
+        const int m = std::min(EVICTIONS, n - i);
+        for (int j = 0; j < EVICTIONS; j++) list.e[j] = j < m ? e[i + j] : Eviction{0, 0, 0, 0};
+        pick_kernel<<<dim3((unsigned)std::min<long long>((long long)m * units, MOST_GRID)), dim3(1024), 0, s>>>(w, list, m, i, first, recent, entries,
+                                                                                                    picks, stride, units);
+        if (const hipError_t err = hipGetLastError()) return err;
+    }
+    return hipSuccess;
+}
+
+hipError_t launch_gather(const Geometry& g, char* pool, const int* table, const Eviction* entries, const int* picks, size_t stride,
+                         const NewPage* pages, int n, hipStream_t s) {
+    const auto kernel = g.head_dim == 64 ? gather_kernel<64> : g.head_dim == 128 ? gather_kernel<128> : gather_kernel<256>;
+    for (int i = 0; i < n; i += NEW_PAGES) {
+        PageList list;
+        const int m = std::min(NEW_PAGES, n - i);
+        for (int j = 0; j < NEW_PAGES; j++) list.p[j] = j < m ? pages[i + j] : NewPage{0, 0, 0};
+        const int units = g.layers * g.kv_heads;
+        kernel<<<dim3(m * (g.page / KEYS), std::min(units, 1024), 2), dim3(256), 0, s>>>(
+            (unsigned short*)pool, table, g.most_pages, g.page, g.kv_heads, units, g.plane_elems(), entries, picks, stride, list);
+        if (const hipError_t err = hipGetLastError()) return err;
+    }
+    return hipSuccess;
+}
+
+hipError_t launch_pack(const WeightsAt& w, const Eviction* entries, int n, const int* picks, size_t stride, hipStream_t s) {
+    const int units = w.layers * w.kv_heads;
+    pack_kernel<<<dim3((unsigned)std::min<long long>((long long)n * units, MOST_GRID / 4)), dim3(1024), 0, s>>>(w, entries, picks, stride, n, units);
+    return hipGetLastError();
+}
+
+}  // namespace paged
+}  // namespace mkv

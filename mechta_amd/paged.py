@@ -14,7 +14,8 @@ BF16 = 2
 # every symbol include/mechta_paged.h declares
 SYMBOLS = ["mpg_rope_freqs", "mpg_rope_turns", "mpg_rotate", "mpg_bytes", "mpg_create", "mpg_destroy", "mpg_set_stream", "mpg_sync",
            "mpg_len", "mpg_table", "mpg_free_pages", "mpg_pages", "mpg_reserve", "mpg_begin", "mpg_begin_shared", "mpg_set_len", "mpg_fork",
-           "mpg_copy", "mpg_free", "mpg_compact", "mpg_append", "mpg_attend", "mpg_read_rows"]
+           "mpg_copy", "mpg_free", "mpg_compact", "mpg_append", "mpg_attend", "mpg_read_rows",
+           "mpg_weights_bytes", "mpg_keep_weights", "mpg_weights", "mpg_weigh", "mpg_evict", "mpg_position"]
 
 LAYOUTS = {"half": 0, "interleaved": 1}
 SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
@@ -71,6 +72,12 @@ def lib():
             "mpg_append": ([P, I, I, P, L64, L64, P, L64, L64, P, L64, L64, P, I], I),
             "mpg_attend": ([P, I, I, P, L64, L64, F, P, P, L64, L64, P], I),
             "mpg_read_rows": ([P, I, I, I, I, I, P], I),
+            "mpg_weights_bytes": ([C, I], S),
+            "mpg_keep_weights": ([P, I], I),
+            "mpg_weights": ([P, I, ctypes.POINTER(P), ctypes.POINTER(L64), ctypes.POINTER(L64)], I),
+            "mpg_weigh": ([P, I, I, P, L64, L64, F, P, F], I),
+            "mpg_evict": ([P, I, P, P, I, I], I),
+            "mpg_position": ([P, I, IP], I),
         }
         for name, (args, res) in sig.items():
             f = getattr(L, name)
@@ -220,7 +227,9 @@ class _Handle:
 class PagedKv:
     """The paged cache of `layers` layers: `pages` pages of `page` positions for up to `seqs` sequences of up to `ctx`
     positions; batches of up to `tokens` new tokens. fmt: F16 or BF16 (pages, q, k, v, gate, out). windows: per layer the
-    positions a token sees, itself included (0 or None: all). rope: what append() rotates by. Calls are ordered on
+    positions a token sees, itself included (0 or None: all). rope: what append() rotates by. weigh_last: the cache keeps
+    attention weights, by which it can evict(): of each sequence of a batch weigh() counts so many of the last new tokens (0:
+    all; None: no weights are kept). Calls are ordered on
     `stream` (default: torch's current stream); where torch works on another one, the caller orders the two.
 
         kv.begin([0, 3], [1, 512])            # one new token for sequence 0, 512 for sequence 3
@@ -230,7 +239,7 @@ class PagedKv:
     """
 
     def __init__(self, layers, q_heads, kv_heads, head_dim, pages, page=64, seqs=64, ctx=262144, fmt=F16, tokens=8192,
-                 windows=None, rope=None, stream=None):
+                 windows=None, rope=None, stream=None, weigh_last=None):
         import torch
         self._owner = _Handle()
         s = stream if stream is not None else torch.cuda.current_stream()
@@ -242,6 +251,8 @@ class PagedKv:
         with torch.cuda.device(self.device):
             _check(lib().mpg_create(ctypes.byref(self._owner.ptr), ctypes.byref(self._config), wp,
                                     None if rope is None else ctypes.byref(rope.c), ctypes.c_void_p(s.cuda_stream)))
+            if weigh_last is not None:
+                _check(lib().mpg_keep_weights(self._owner.ptr, _int(weigh_last, "weigh_last")))
         self._h = self._owner.ptr
         self.dtype = _dtype(fmt)
         self._views = {}
@@ -281,6 +292,12 @@ class PagedKv:
     def length(self, seq):
         n = ctypes.c_int()
         _check(lib().mpg_len(self._h, _int(seq, "sequence"), ctypes.byref(n)))
+        return n.value
+
+    def position(self, seq):
+        """Where the sequence's next token stands: its length, and the positions evicted of it."""
+        n = ctypes.c_int()
+        _check(lib().mpg_position(self._h, _int(seq, "sequence"), ctypes.byref(n)))
         return n.value
 
     def table(self, seq):
@@ -336,6 +353,30 @@ class PagedKv:
         n = ctypes.c_int()
         _check(self._lib.mpg_compact(self._h, ctypes.byref(n)))
         return n.value
+
+    def evict(self, seqs, keep, first=0, recent=0):
+        """Cuts each of the sequences that is longer to `keep` positions (a number, or one for each): its `first` first and
+        `recent` last ones and, for each layer and K/V head by itself, those of the largest weights between them."""
+        a, ap = _ints(seqs)
+        b, bp = _ints([keep] * len(a) if isinstance(keep, int) else keep, len(a), "keep")
+        _check(self._lib.mpg_evict(self._h, len(a), ap, bp, _int(first, "first"), _int(recent, "recent")))
+
+    def weights(self, layer):
+        """A layer's accumulated attention weights, [sequence, K/V head, position] (f32); those behind a sequence's length are
+        undefined."""
+        view = self._views.get((layer, "weights"))
+        if view is None:
+            import torch
+            base, by_seq, by_head = ctypes.c_void_p(), ctypes.c_int64(), ctypes.c_int64()
+            _check(lib().mpg_weights(self._h, _int(layer, "layer"), ctypes.byref(base), ctypes.byref(by_seq), ctypes.byref(by_head)))
+
+            class _Mem:  # the tensor keeps the memory
+                owner = self._owner
+                __cuda_array_interface__ = {"shape": (self.seqs, self.kv_heads, self.ctx), "typestr": "<f4", "version": 2,
+                                            "strides": (4 * by_seq.value, 4 * by_head.value, 4), "data": (base.value, False)}
+
+            view = self._views[layer, "weights"] = torch.as_tensor(_Mem(), device=self.device)
+        return view
 
     def pages(self, layer, which):
         """A layer's K or V pages as a tensor over the pool: K [page][kv head][pos/16][d/8][16][8], V [page][kv head]
@@ -393,6 +434,11 @@ class PagedKv:
             raise ValueError(f"{what} must be {rows} contiguous rows")
         return p
 
+    def _sinks(self, sinks):
+        if sinks.device != self.device or sinks.dtype is not self._float32 or sinks.shape != (self.q_heads,) or not sinks.is_contiguous():
+            raise ValueError(f"sinks must be {self.q_heads} contiguous float32 on {self.device}")
+        return sinks.data_ptr()
+
     def append(self, layer, k, v, q=None, q_out=None, rotate=None):
         """Writes the batch's k and v [tokens, kv_heads, head_dim] into the pages, k rotated (rotate=False: it is already;
         default: if the cache has a rope). With q [tokens, q_heads, head_dim]: returns it rotated, in q_out (may be q)."""
@@ -437,10 +483,19 @@ class PagedKv:
             if gate.shape[0] != rows:
                 raise ValueError("q and gate differ in rows")
         if sinks is not None:
-            if sinks.device != device or sinks.dtype is not self._float32 or sinks.shape != (h,) or not sinks.is_contiguous():
-                raise ValueError(f"sinks must be {h} contiguous float32 on {device}")
-            sp = sinks.data_ptr()
+            sp = self._sinks(sinks)
         rc = self._lib.mpg_attend(self._h, layer, rows, qp, qt, qh, self._scale if scale is None else scale, sp, gp, gt, gh, op)
         if rc:
             _check(rc)
         return out
+
+    def weigh(self, layer, q, scale=None, sinks=None, decay=1.0):
+        """Adds the attention weights that the batch's counted tokens (weigh_last) give to each position, as attend(layer, q)
+        has them, summed over the tokens and the query heads of a K/V head, to `decay` times the position's weight."""
+        if not -0x80000000 <= layer < 0x80000000:
+            _int(layer, "layer")
+        qp, qt, qh = _rows(q, self.q_heads, self.head_dim, self.dtype, self.device, "q")
+        sp = None if sinks is None else self._sinks(sinks)
+        rc = self._lib.mpg_weigh(self._h, layer, q.shape[0], qp, qt, qh, self._scale if scale is None else scale, sp, decay)
+        if rc:
+            _check(rc)
