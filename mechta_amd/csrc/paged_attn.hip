@@ -744,7 +744,8 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
 // row sees there has a NaN score, which no maximum takes).
 // D / 4 lanes hold a row, four dims each, and read its splits four at a time; a work-group takes 1024 / D rows. Wide: a
 // work-group takes 64 dims of a row; 16 lanes hold them, and each 16 lanes add up every 16th split, with the
-// splits' factors in LDS. (A row whole in a work-group, 32 rows of 121 splits: 7.9 us; by 64 dims 5.2.)
+// splits' factors in LDS. (A row whole in a work-group, 32 rows of 121 splits: 7.9 us; by 64 dims 5.2.) ROW_WIDE, many splits of many
+// rows: a work-group takes a row, each D / 4 lanes four splits of it at a time.
 constexpr int JOIN_DIMS = 64;
 //
 // Rows of sequences that share keys have more splits, those of the shared tiles they are in: Seg by Seg behind their own.
@@ -843,6 +844,73 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
             }
             continue;
         }
+        const int splits = j.splits + shared.splits;
+        if (j.wide == ROW_WIDE) {
+            constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+            const int group = tid / LANES, lane = tid % LANES;
+            for (int r = way; r < j.count; r += ways) {
+                const int row = j.row0 + r, tok = j.tok0 + row / a.group;
+                if (tok >= a.rows) continue;
+                f32x4 acc = f32x4{};
+                float top = NEG_INF, total = 0.f;
+                for (int s0 = 4 * group; s0 < splits; s0 += 4 * GROUPS) {  // behind the last the last again, not counted
+                    float m[4], l[4];
+                    f32x4 x[4];
+#pragma unroll
+                    for (int s = 0; s < 4; s++) {
+                        const int at = min(s0 + s, splits - 1);
+                        const size_t p = at < j.splits ? j.part + r + (size_t)at * j.count : shared.row(at - j.splits, r);
+                        m[s] = a.pm[p];
+                        l[s] = a.pl[p];
+                        x[s] = *(const f32x4*)(a.pacc + p * D + lane * 4);
+                    }
+                    const float was = top;
+#pragma unroll
+                    for (int s = 0; s < 4; s++) {
+                        if (s0 + s >= splits) {
+                            m[s] = NEG_INF;
+                            l[s] = 0.f;
+                            x[s] = f32x4{};
+                        }
+                        top = fmaxf(top, m[s]);
+                    }
+                    const float f = was == NEG_INF ? 0.f : fast_exp2(was - top);
+                    acc *= f;
+                    total *= f;
+#pragma unroll
+                    for (int s = 0; s < 4; s++) {
+                        const float f = m[s] == NEG_INF ? 0.f : fast_exp2(m[s] - top);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[i] += f * x[s][i];
+                        total += f * l[s];
+                    }
+                }
+                __syncthreads();  // the row before has been read
+                (&sa[0][0])[tid] = acc;
+                if (lane == 0) {
+                    factor[group] = top;
+                    factor[16 + group] = total;
+                }
+                lds_barrier();
+                if (group) continue;
+                float all = top;
+#pragma unroll
+                for (int x = 1; x < GROUPS; x++) all = fmaxf(all, factor[x]);
+                const float f = top == NEG_INF ? 0.f : fast_exp2(top - all);
+                acc *= f;
+                total *= f;
+#pragma unroll
+                for (int x = 1; x < GROUPS; x++) {
+                    const float f = factor[x] == NEG_INF ? 0.f : fast_exp2(factor[x] - all);
+                    const f32x4 y = (&sa[0][0])[x * LANES + lane];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[i] += f * y[i];
+                    total += f * factor[16 + x];
+                }
+                finish(tok, j.head * a.group + row % a.group, lane * 4, acc, all, total);
+            }
+            continue;
+        }
         constexpr int PER_ROW = D / JOIN_DIMS;
         const int part = tid / 16, lane = tid % 16;
         for (int u = way; u < j.count * PER_ROW; u += ways) {
@@ -850,7 +918,6 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
             const int row = j.row0 + r, tok = j.tok0 + row / a.group;
             if (tok >= a.rows) continue;
             const size_t first = j.part + r;
-            const int splits = j.splits + shared.splits;
             auto partial = [&](int s) INLINE { return s < j.splits ? first + (size_t)s * j.count : shared.row(s - j.splits, r); };
             float top = NEG_INF;
             for (int s = tid; s < splits; s += 256) top = fmaxf(top, a.pm[partial(s)]);
@@ -949,7 +1016,7 @@ hipError_t attend_as(const Geometry& g, const AttendArgs& x, const int* batch, c
         if (!x.captured)
             for (const Join& j : *x.joins) {
                 const int groups = 1024 / D;
-                ways = std::max(ways, j.wide ? j.count * (D / JOIN_DIMS) : (j.count + groups - 1) / groups);
+                ways = std::max(ways, j.wide == ROW_WIDE ? j.count : j.wide ? j.count * (D / JOIN_DIMS) : (j.count + groups - 1) / groups);
             }
         const int all = std::min(join_grid, MOST_GRID / ways) * ways;
         join_kernel<T, D><<<dim3(all), dim3(256), 0, s>>>(a, (const Join*)(batch + l.joins), batch + KINDS, (const Seg*)(batch + l.segs));

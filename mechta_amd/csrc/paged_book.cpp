@@ -325,6 +325,14 @@ constexpr int CUS = 256, STREAMS = 216;
 // 2 x 256 at 200 / 300 / 400 9.1, 10.9, 12.7 / 10.0, 9.7, 9.5; of 12 9.7, 11.8, 13.6 / 11.1, 11.5, 11.8.)
 constexpr int WHOLE = 512 * 128;
 constexpr int WIDE_SPLITS = 8, WIDE_ROWS = 512;
+// Rows of a shared batch, times their dims, that are joined by 64 dims a work-group. (Whole calls, us, by 64 dims / row by row,
+// sequences of a token on a prompt of 4,096 of 4 x 128: 4 12.2 / 14.7, 8 13.4 / 14.6, 16 18.0 / 14.7; 8 and 16 of 2 x 256 15.8 / 17.9,
+// 20.1 / 18.9.)
+constexpr int WIDE_SHARED = 512 * 64;
+// Rows and splits of a shared batch that are joined a row a work-group. (Whole calls, us, so / D / 4 lanes a row: 8 verifies of 4 tokens at
+// 65,536, 2 x 256, 512 rows of 54 splits 61.2 / 66; 16 tokens on 16,384 of 4 x 128 23.9 / 26.9; 64 tokens, 2,048 rows of up to 40 42.5 / 39.6,
+// of 8 x 64 35.7 / 31.)
+constexpr int ROW_SPLITS = 16, ROW_ROWS = 1024;
 }  // namespace
 
 // Dies take the items of a list in turn (position i: die i % 8). The tiles of one (sequence, head, split) stream the same
@@ -433,27 +441,37 @@ constexpr double CHUNK_US[2][3] = {{.0107, .0162, .0295}, {.0155, .029, .062}};
 // Chunks: the cheapest length of a piece by a model of the call in us: a piece's keys, 9 for its beginning and end, the split
 // partials written and read back at 5 TB/s and 3 for the launch that joins them. (Pieces that are more than the CUs run in
 // rounds; half a mean piece is added for the last one. Where CUs stand idle behind short pieces the card, limited by its
-// power, runs the others faster: up to .65 of the time.)
-long long chunk_length(const std::vector<Tile>& tiles, const Shape& g, int kind, double& cost) {
+// power, runs the others faster: up to .65 of the time.) Tiles of shared ranges are much longer than the others: with them
+// the call may be as long as its longest piece.
+// (The call's cost for one length; returns the split partials' rows.)
+long long chunk_cost(const std::vector<Tile>& tiles, const Shape& g, int kind, long long length, double& c) {
     const double key = CHUNK_US[kind == MANY][g.head_dim / 128];
+    long long n = 0, sum = 0, rows = 0, most = 0;
+    bool shared = false;
+    for (const Tile& t : tiles) {
+        const int p = pieces_of(t, length);
+        const long long keys = t.k1 - t.k0;
+        n += (long long)p * g.kv_heads;
+        sum += keys * g.kv_heads;
+        most = std::max(most, (keys + p - 1) / p);
+        shared |= t.range >= 0;
+        if (p > 1 || t.range >= 0) rows += (long long)p * TILE_ROWS[kind] * g.kv_heads;
+    }
+    const double busy = (double)sum / ((double)CUS * most);
+    c = n <= CUS ? most * key * (.65 + .35 * std::min(1., busy)) + 9
+                 : (double)sum / CUS * key + 9. * n / CUS + .5 * sum / n * key;
+    if (shared) c = std::max(c, most * key + 9);
+    if (rows) c += 3 + 8. * g.head_dim * rows / 5e6;
+    return rows;
+}
+long long chunk_length(const std::vector<Tile>& tiles, const Shape& g, int kind, double& cost) {
     long long longest = LEAST_KEYS / KEYS, best = longest;
     for (const Tile& t : tiles) longest = std::max(longest, (long long)(t.k1 - t.k0 + KEYS - 1) / KEYS);
     cost = 1e30;
     for (long long length = longest;; length = length * 7 / 8) {  // from whole tiles down
         if (length < LEAST_KEYS / KEYS) break;
-        long long n = 0, sum = 0, rows = 0, most = 0;
-        for (const Tile& t : tiles) {
-            const int p = pieces_of(t, length);
-            const long long keys = t.k1 - t.k0;
-            n += (long long)p * g.kv_heads;
-            sum += keys * g.kv_heads;
-            most = std::max(most, (keys + p - 1) / p);
-            if (p > 1) rows += (long long)p * TILE_ROWS[kind] * g.kv_heads;
-        }
-        const double busy = (double)sum / ((double)CUS * most);
-        double c = n <= CUS ? most * key * (.65 + .35 * std::min(1., busy)) + 9
-                            : (double)sum / CUS * key + 9. * n / CUS + .5 * sum / n * key;
-        if (rows) c += 3 + 8. * g.head_dim * rows / 5e6;
+        double c;
+        const long long rows = chunk_cost(tiles, g, kind, length, c);
         if (c < cost) {
             cost = c;
             best = length;
@@ -605,12 +623,45 @@ void share(const Book& b, const Shape& g, const std::vector<Member>& batch, Shar
     }
 }
 
-static void plan(const Shape& g, const std::vector<Member>& batch, const Share* share, int window, Plan& out) {
-    for (auto& v : out.items) v.clear();
-    out.joins.clear();
-    out.segs.clear();
+namespace {
+// A shared range in a window: its rows, their first entry in the order, the first key that any of them sees (rows 0: none sees
+// any); its splits and partials.
+struct Common {
+    int rows = 0, tok0 = 0, k0 = 0, splits = 0, part = 0;
+};
+// How a batch's work may be cut. APART: every sequence by itself. STREAMED: what they share in tiles of 32 rows beside their own, all by
+// few_rows. TILED: what they share in a chunk's tiles where it has more than 32 rows.
+enum Way { APART, STREAMED, TILED };
+struct Draft {
+    std::vector<Tile> tiles[KINDS];
+    long long length[KINDS], piece[KINDS] = {};  // of a piece of each kind's tiles; of those in the last round of CUs
+    int cut[KINDS] = {};                         // tiles of that round
+    std::vector<Common> common;
+    double cost = 0;  // us, of a batch with pages in common
+};
+
+// What a launch for few rows takes where sequences have keys in common: `distinct` bytes from memory, all of them from the L2s, or
+// the longest piece of a work-group alone on its CU (several share it where there are more), and 9 for its beginning, its
+// end and the join (5 without one).
+double stream_cost(const std::vector<Tile>& tiles, const Shape& g, int kind, long long length, double distinct, bool joined) {
+    if (tiles.empty()) return 0;
+    double keys = 0, n = 0, longest = 0;
+    for (const Tile& t : tiles) {
+        const int p = pieces_of(t, length);
+        n += (double)p * g.kv_heads;
+        keys += (double)(t.k1 - t.k0) * g.kv_heads;
+        longest = std::max<double>(longest, (t.k1 - t.k0 + p - 1) / p);
+        joined |= p > 1;
+    }
+    const double bytes = 4. * g.head_dim, us = g.head_dim * (kind == SOME ? 1.25e-4 : 7e-5);  // of a key
+    const double work = n <= CUS ? longest * us : (keys / CUS * (g.head_dim <= 128 ? .7 : 1.) + .5 * longest) * us;
+    return (joined ? 9 : 5) + std::max({distinct * bytes / 5.5e6, keys * bytes / 17e6, work});
+}
+
+void draft(const Shape& g, const std::vector<Member>& batch, const Share* share, int window, Way way, Draft& out) {
     const int group = g.q_heads / g.kv_heads;
-    std::vector<Tile> by_kind[KINDS];
+    std::vector<Tile>(&by_kind)[KINDS] = out.tiles;
+    if (way == APART) share = nullptr;
     auto add = [&](int i, int tok0, int kind) {
         const Member& m = batch[i];
         const int rows = m.count * group, pos0 = m.len - m.count, from = share ? share->from[i] : 0;
@@ -620,25 +671,22 @@ static void plan(const Shape& g, const std::vector<Member>& batch, const Share* 
             by_kind[kind].push_back({i, tok0, r, std::max(from, lo / KEYS * KEYS), pos0 + last + 1, kind, -1});
         }
     };
-    // A shared range in this window: its rows, the keys that any of them sees, where its partials are.
-    struct Common {
-        int rows = 0, tok0 = 0, k0 = 0, part = 0, splits = 0;
-    };
-    std::vector<Common> common(share ? share->ranges.size() : 0);
     int tok0 = 0;
     for (int i = 0; i < (int)batch.size(); i++) {
         const int rows = batch[i].count * group;
         if (rows <= TILE_ROWS[SOME]) {
-            add(i, tok0, rows <= TILE_ROWS[FEW] ? FEW : SOME);
+            add(i, tok0, rows <= TILE_ROWS[FEW] && way != STREAMED ? FEW : SOME);
         } else {  // either size of tile is a candidate
             add(i, tok0, HALF);
             add(i, tok0, MANY);
         }
         tok0 += batch[i].count;
     }
-    for (size_t x = 0; x < common.size(); x++) {
+    out.common.resize(share ? share->ranges.size() : 0);
+    bool any = false;
+    for (size_t x = 0; x < out.common.size(); x++) {
         const Range& r = share->ranges[x];
-        Common& c = common[x];
+        Common& c = out.common[x];
         c.tok0 = share->at[share->members[r.first]];
         int lo = r.k1;
         for (int i = r.first; i < r.first + r.count; i++) {
@@ -647,39 +695,29 @@ static void plan(const Shape& g, const std::vector<Member>& batch, const Share* 
             lo = std::min(lo, window ? std::max(0, m.len - m.count - window + 1) : 0);
         }
         c.k0 = std::max(r.k0, lo / KEYS * KEYS);
-        if (c.k0 >= r.k1) {  // no row sees any of it
+        if (c.k0 >= r.k1) {
             c.rows = 0;
             continue;
         }
+        any = true;
         auto tiles = [&](int kind) {
             for (int row = 0; row < c.rows; row += TILE_ROWS[kind]) by_kind[kind].push_back({share->members[r.first], c.tok0, row, c.k0, r.k1, kind, (int)x});
         };
-        if (c.rows <= TILE_ROWS[SOME]) {
-            tiles(c.rows <= TILE_ROWS[FEW] ? FEW : SOME);
+        if (c.rows <= TILE_ROWS[SOME] || way == STREAMED) {
+            tiles(c.rows <= TILE_ROWS[FEW] && way != STREAMED ? FEW : SOME);
         } else {
             tiles(HALF);
             tiles(MANY);
         }
     }
-    // the shared ranges that a member's rows have keys in, the outermost first
-    auto chain = [&](int i) {
-        std::vector<int> c;
-        for (int x = share ? share->range[i] : -1; x >= 0; x = share->ranges[x].parent)
-            if (common[x].rows) c.insert(c.begin(), x);
-        return c;
-    };
-    bool any = false;
-    for (const Common& c : common) any |= c.rows > 0;
-    long long length[KINDS];
+    long long(&length)[KINDS] = out.length;
     for (int k : {FEW, SOME}) length[k] = few_length(by_kind[k], g);
     double half, many;
     length[HALF] = chunk_length(by_kind[HALF], g, HALF, half);
     length[MANY] = chunk_length(by_kind[MANY], g, MANY, many);
-    long long piece[KINDS] = {};
-    int cut[KINDS] = {};
     if (!any) {  // (the tiles of a shared range are split alike)
-        cut[HALF] = last_round(by_kind[HALF], g, HALF, half, piece[HALF]);
-        cut[MANY] = last_round(by_kind[MANY], g, MANY, many, piece[MANY]);
+        out.cut[HALF] = last_round(by_kind[HALF], g, HALF, half, out.piece[HALF]);
+        out.cut[MANY] = last_round(by_kind[MANY], g, MANY, many, out.piece[MANY]);
     }
     // Few rows among a chunk's tiles fill CUs that its last ones leave idle, and spare a launch, often two. (us apart / among:
     // 512 tokens and 12 decodes at 500 .. 4,000 positions 31.8 / 23.9 of 4 x 128, 40.8 / 30.6 of 2 x 256; 100 and 20 at 100
@@ -695,17 +733,75 @@ static void plan(const Shape& g, const std::vector<Member>& batch, const Share* 
         for (Tile& t : both) t.kind = HALF;
         by_kind[HALF] = std::move(both);
         length[HALF] = joint;
-        cut[HALF] = 0;
+        out.cut[HALF] = 0;
         for (int k : {FEW, SOME, MANY}) by_kind[k].clear();
     } else {
         by_kind[half <= many ? MANY : HALF].clear();
     }
+}
+
+// What a draft takes, where sequences have keys in common.
+double cost_of(const Shape& g, const Share& share, int window, const std::vector<Member>& batch, const Draft& d) {
+    double distinct[KINDS] = {};  // keys of the lists for few rows, what several tiles have counted once
+    for (int k : {FEW, SOME}) {
+        std::vector<char> seen(share.ranges.size(), 0);
+        for (const Tile& t : d.tiles[k]) {
+            if (t.range >= 0) {
+                if (t.row0 == 0) distinct[k] += (double)(t.k1 - t.k0) * g.kv_heads;
+                continue;
+            }
+            distinct[k] += (double)(t.k1 - t.k0) * g.kv_heads;
+            for (int x = share.range[t.member]; x >= 0; x = share.ranges[x].parent) {  // of ranges that it takes by itself
+                const int have = std::min(t.k1, share.ranges[x].k1) - std::max(t.k0, share.ranges[x].k0);
+                if (have <= 0) continue;
+                if (seen[x]) distinct[k] -= (double)have * g.kv_heads;
+                seen[x] = 1;
+            }
+        }
+    }
+    bool joined = false;
+    for (const Common& c : d.common) joined |= c.rows > 0;
+    double chunks = 0;
+    for (int k : {HALF, MANY})
+        if (!d.tiles[k].empty()) chunk_cost(d.tiles[k], g, k, d.length[k], chunks);
+    const double few = stream_cost(d.tiles[FEW], g, FEW, d.length[FEW], distinct[FEW], joined);
+    const double some = stream_cost(d.tiles[SOME], g, SOME, d.length[SOME], distinct[SOME], joined);
+    return chunks + few + some - (chunks > 0 && few + some > 0 ? 4 : 0) - (few > 0 && some > 0 ? 4 : 0);
+}
+}  // namespace
+
+static void plan(const Shape& g, const std::vector<Member>& batch, const Share* share, int window, Plan& out) {
+    for (auto& v : out.items) v.clear();
+    out.joins.clear();
+    out.segs.clear();
+    const int group = g.q_heads / g.kv_heads;
+    Draft best;
+    draft(g, batch, share, window, APART, best);
+    if (share) {
+        best.cost = cost_of(g, *share, window, batch, best);
+        for (Way way : {STREAMED, TILED}) {
+            Draft d;
+            draft(g, batch, share, window, way, d);
+            d.cost = cost_of(g, *share, window, batch, d);
+            if (d.cost < best.cost) best = std::move(d);
+        }
+    }
+    std::vector<Common>& common = best.common;
+    // the shared ranges that a member's rows have keys in, the outermost first
+    auto chain = [&](int i) {
+        std::vector<int> c;
+        for (int x = common.empty() ? -1 : share->range[i]; x >= 0; x = share->ranges[x].parent)
+            if (common[x].rows) c.insert(c.begin(), x);
+        return c;
+    };
+    bool any = false;
+    for (const Common& c : common) any |= c.rows > 0;
     std::vector<Tile> tiles;
     std::vector<long long> most;  // KEYS of a piece of the tile
     for (int k = 0; k < KINDS; k++)
-        for (int i = 0; i < (int)by_kind[k].size(); i++) {
-            tiles.push_back(by_kind[k][i]);
-            most.push_back(cut[k] ? i < cut[k] ? piece[k] : 1 << 20 : length[k]);
+        for (int i = 0; i < (int)best.tiles[k].size(); i++) {
+            tiles.push_back(best.tiles[k][i]);
+            most.push_back(best.cut[k] ? i < best.cut[k] ? best.piece[k] : 1 << 20 : best.length[k]);
         }
     int part = 0, more = 0;  // partials and work items that splits have taken
     // What shared ranges and the rows in them cannot do without: a split's partials each, and the ranges' work items.
@@ -791,7 +887,8 @@ static void plan(const Shape& g, const std::vector<Member>& batch, const Share* 
         Join& j = out.joins[n];
         int splits = j.splits;
         for (int x = 0; x < j.segs; x++) splits += out.segs[n * LEVELS + x].splits;
-        j.wide = splits > WIDE_SPLITS && rows <= WIDE_ROWS;
+        j.wide = splits > WIDE_SPLITS && (any ? rows * g.head_dim <= WIDE_SHARED : rows <= WIDE_ROWS);
+        if (any && !j.wide && splits > ROW_SPLITS && rows <= ROW_ROWS) j.wide = ROW_WIDE;
     }
     for (auto& list : out.items) {
         std::stable_sort(list.begin(), list.end(), [](const Item& a, const Item& b) {

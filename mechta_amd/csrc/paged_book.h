@@ -93,7 +93,7 @@ struct Item {
     int pad;
 };
 // Join of a tile's splits: split s of row r at part + s * count + r, and those of the shared tiles that its rows are in, Seg
-// `segs` of them. wide: a work-group for every 64 dims of a row.
+// `segs` of them. wide: a work-group for every 64 dims of a row, or (ROW_WIDE) for a row.
 struct Join {
     int head, tok0, row0, count, part, splits, wide, segs;
 };
@@ -101,6 +101,7 @@ struct Join {
 struct Seg {
     int part, stride, splits, pad;
 };
+constexpr int ROW_WIDE = 2;
 constexpr int LEVELS = 3;  // shared ranges that a sequence's tokens are in at most
 // An entry of a batch's order: a token and its position.
 struct Place {

@@ -5,6 +5,7 @@ import random
 
 import pytest
 
+from tests.paged_forests import FORESTS
 from tests.paged_reference import attention, close
 
 pytestmark = pytest.mark.gpu
@@ -72,28 +73,14 @@ class Forest:
         return out
 
 
-# kv_heads, group, page, prompt, forks, own part up to, tokens, window
-SHAPES = {
-    "samples of a prompt, tiles of 16": (2, 4, 64, 700, 4, 40, [1], 0),
-    "tiles of 32": (1, 8, 32, 900, 4, 300, [1], 0),
-    "tiles of 128": (2, 8, 64, 1500, 13, 90, [1], 0),
-    "tiles of 256 and splits": (1, 8, 64, 5000, 60, 200, [1], 0),
-    "some verify, some generate": (2, 5, 128, 2000, 11, 150, [1, 4, 2], 0),
-    "a sliding window inside the prompt": (2, 8, 32, 1500, 9, 300, [1, 3], 700),
-    "a window's edge inside the tile": (1, 2, 64, 640, 20, 400, [1], 513),
-    "chunks beside generation": (2, 4, 64, 1200, 6, 100, [1, 130, 1], 0),
-    "one query head a head": (3, 1, 256, 1100, 7, 300, [1], 0),
-    "sixteen query heads a head": (1, 16, 32, 1030, 5, 64, [2], 0),
-}
-
-
-@pytest.mark.parametrize("typ,dim", [("f16", 64), ("bf16", 128), ("f16", 256), ("bf16", 256)])
-@pytest.mark.parametrize("name", SHAPES)
-def test_forks_of_a_prompt(torch_gpu, pg, name, typ, dim):
+@pytest.mark.parametrize("typ", ["f16", "bf16"])
+@pytest.mark.parametrize("name", FORESTS)
+def test_forks_of_a_prompt(torch_gpu, pg, name, typ):
     torch = torch_gpu
-    heads, group, page, prompt, forks, own, tokens, window = SHAPES[name]
-    f = Forest(torch, pg, heads, group, dim, typ, page, window=window)
-    f.grow([0], [prompt])
+    heads, group, dim, page, prompt, forks, own, tokens, window, _ = FORESTS[name]
+    f = Forest(torch, pg, heads, group, dim, typ, page, pages=(prompt + forks * (own + 600)) // page + 100, window=window)
+    for at in range(0, prompt, 8000):
+        f.grow([0], [min(8000, prompt - at)])
     f.fork([0] * (forks - 1), list(range(1, forks)))
     r = random.Random(3)
     f.grow(list(range(forks)), [r.randint(1, own) for _ in range(forks)])
@@ -104,15 +91,15 @@ def test_forks_of_a_prompt(torch_gpu, pg, name, typ, dim):
     f.check(sinks=sinks, gate=True, what=name)
 
 
-@pytest.mark.parametrize("typ,dim,page,window", [("f16", 128, 32, 0), ("bf16", 64, 64, 900), ("f16", 256, 32, 0)])
+@pytest.mark.parametrize("typ,dim,page,window", [("f16", 128, 32, 0), ("bf16", 64, 64, 3900), ("f16", 256, 32, 0)])
 def test_a_tree_of_forks(torch_gpu, pg, typ, dim, page, window):
-    f = Forest(torch_gpu, pg, 2, 4, dim, typ, page, pages=900, window=window)
-    f.grow([0], [1100])
+    f = Forest(torch_gpu, pg, 2, 8, dim, typ, page, pages=1800, window=window)
+    f.grow([0], [7100])
     f.fork([0] * 3, [1, 2, 3])
-    f.grow([0, 1, 2, 3], [500, 700, 33, 640])
+    f.grow([0, 1, 2, 3], [2500, 2700, 33, 1640])
     f.fork([s % 4 for s in range(4, 16)], list(range(4, 16)))
     f.grow(list(range(16)), [300 + s for s in range(16)])
-    f.fork([s % 16 for s in range(16, 40)], list(range(16, 40)), [1200 + 5 * s for s in range(16, 40)])
+    f.fork([s % 16 for s in range(16, 40)], list(range(16, 40)), [7200 + 5 * s for s in range(16, 40)])
     r = random.Random(1)
     for step in range(3):
         seqs = r.sample(range(40), 30)
@@ -121,25 +108,30 @@ def test_a_tree_of_forks(torch_gpu, pg, typ, dim, page, window):
 
 
 @pytest.mark.parametrize("typ", ["f16", "bf16"])
-def test_odd_values_behind_a_shared_window(torch_gpu, pg, typ):
+@pytest.mark.parametrize("forks", [24, 60])  # in tiles of 32 rows, of 128
+def test_odd_values_behind_a_shared_window(torch_gpu, pg, typ, forks):
     """Infinities and NaN of the prompt in front of a row's window do not reach it; those inside reach the rows that see them."""
     torch = torch_gpu
-    f = Forest(torch, pg, 1, 8, 64, typ, 32, window=200)
-    f.grow([0], [320])
-    f.fork([0] * 5, list(range(1, 6)))
-    f.grow(list(range(6)), [10, 30, 50, 70, 90, 20])
-    seqs = [3, 0, 4, 5, 1, 2]
-    f.begin(seqs, [1] * 6, True)
-    assert f.kv.table(0)[:10] == f.kv.table(4)[:10]
-    page, at = f.kv.table(0)[6], 6 * 32 + 3  # position 195: seen by rows at positions up to 394
-    v = f.kv.pages(0, pg.V).view(-1, 1, 1, 4, 64, 2, 4)
-    v[page, 0, 0, 0, :, 0, 3] = math.nan
-    q = f.rnd(6, 8, 64)
-    out = f.kv.attend(0, q)
-    for i, s in enumerate(seqs):
-        sees = f.kv.length(s) - 1 - 200 < at
-        assert torch.isnan(out[i]).all() if sees else torch.isfinite(out[i]).all(), s
-    assert {f.kv.length(s) - 1 - 200 < at for s in seqs} == {True, False}
+    f = Forest(torch, pg, 4, 8, 64, typ, 32, pages=1500, window=5000)
+    f.grow([0], [6400])
+    f.fork([0] * (forks - 1), list(range(1, forks)))
+    f.grow(list(range(forks)), [10 + 20 * (i % 7) for i in range(forks)])
+    seqs = list(range(forks))
+    random.Random(2).shuffle(seqs)
+    f.begin(seqs, [1] * forks, True)
+    assert f.kv.table(0)[:200] == f.kv.table(4)[:200]
+    at = 1472  # seen by rows at positions up to 6,471
+    page = f.kv.table(0)[at // 32]
+    v = f.kv.pages(0, pg.V).view(-1, 4, 1, 4, 64, 2, 4)
+    for value in (math.nan, math.inf):
+        v[page, 1, 0, 0, :, 0, 0] = value
+        q = f.rnd(forks, 32, 64)
+        out = f.kv.attend(0, q)
+        sees = [f.kv.length(s) - 1 - 5000 < at for s in seqs]
+        assert set(sees) == {True, False}
+        for i in range(forks):
+            assert torch.isfinite(out[i, :8]).all() and torch.isfinite(out[i, 16:]).all()
+            assert not torch.isfinite(out[i, 8:16]).any() if sees[i] else torch.isfinite(out[i, 8:16]).all(), i
 
 
 def test_captured_attention_follows_shared_batches(torch_gpu, pg):
@@ -147,10 +139,10 @@ def test_captured_attention_follows_shared_batches(torch_gpu, pg):
     torch = torch_gpu
     for first_shared in (False, True):
         stream = torch.cuda.Stream()
-        f = Forest(torch, pg, 2, 8, 128, "bf16", 64, stream=torch.cuda.current_stream(), tokens=512)
-        f.grow([0], [512] if first_shared else [500])
+        f = Forest(torch, pg, 2, 8, 128, "bf16", 64, stream=torch.cuda.current_stream(), tokens=8192)
+        f.grow([0], [8000] if first_shared else [7900])
         f.grow([0], [512])
-        f.fork([0] * 15, list(range(1, 16)))
+        f.fork([0] * 39, list(range(1, 40)))
         rows = 64
         q, out = f.rnd(rows, 16, 128), torch.zeros(rows, 16, 128, dtype=f.type, device="cuda")
         f.begin(list(range(8)), [1] * 8, first_shared)
@@ -160,8 +152,8 @@ def test_captured_attention_follows_shared_batches(torch_gpu, pg):
         with torch.cuda.graph(graph, stream=stream):
             f.kv.attend(0, q, out=out)
         f.kv.set_stream(torch.cuda.current_stream())
-        for seqs, counts, shared in [(list(range(16)), [1] * 16, True), ([3, 1], [4, 1], False), (list(range(15, -1, -1)), [3] * 16, True),
-                                     (list(range(16)), [2] * 16, False), ([5], [1], True)]:
+        for seqs, counts, shared in [(list(range(20)), [1] * 20, True), ([3, 1], [4, 1], False), (list(range(39, -1, -1)), [1] * 40, True),
+                                     (list(range(16)), [2] * 16, False), ([5], [1], True), (list(range(16)), [4] * 16, True)]:
             n = f.begin(seqs, counts, shared)
             eager = f.kv.attend(0, q[:n].contiguous())
             out.fill_(7)
@@ -174,13 +166,13 @@ def test_captured_attention_follows_shared_batches(torch_gpu, pg):
 def test_shared_batches_are_repeatable_and_near_the_plain_ones(torch_gpu, pg):
     torch = torch_gpu
     f = Forest(torch, pg, 2, 8, 128, "f16", 64)
-    f.grow([0], [2100])
-    f.fork([0] * 9, list(range(1, 10)))
-    f.begin(list(range(10)), [1] * 10, True)
-    q = f.rnd(10, 16, 128)
+    f.grow([0], [8100])
+    f.fork([0] * 29, list(range(1, 30)))
+    f.begin(list(range(30)), [1] * 30, True)
+    q = f.rnd(30, 16, 128)
     a, b = f.kv.attend(0, q), f.kv.attend(0, q)
     assert torch.equal(a, b)
-    f.kv.begin(list(range(10)), [0] * 10, shared=True)  # nothing new: nothing to attend
+    f.kv.begin(list(range(30)), [0] * 30, shared=True)  # nothing new: nothing to attend
     assert f.kv.attend(0, q[:0]).shape == (0, 16, 128)
 
 

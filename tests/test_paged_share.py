@@ -7,6 +7,8 @@ import subprocess
 
 import pytest
 
+from tests.paged_forests import FORESTS
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 TILE = {0: 16, 1: 32, 2: 128, 3: 256}
 
@@ -68,7 +70,7 @@ def planned(f, kv, group, dim, seqs, counts, window):
 
 
 def check(f, kv, group, dim, seqs, counts, window):
-    """Returns the ranges, and how many scores the shared tiles have."""
+    """Returns the ranges, how many scores the shared tiles have, and of which kinds they are."""
     L = f.L
     ranges, items, joins, segs, order = planned(f, kv, group, dim, seqs, counts, window)
     tokens = sum(counts)
@@ -136,7 +138,7 @@ def check(f, kv, group, dim, seqs, counts, window):
         spans = sorted(s for s in spans if s[0] < s[1])
         assert spans[0][0] == (max(0, pos - window + 1) if window else 0) and spans[-1][1] == pos + 1
         assert all(a[1] == b[0] for a, b in zip(spans, spans[1:])), "keys that are left out, or taken twice"
-    return ranges, shared
+    return ranges, shared, tuple(k for k, list_ in enumerate(items) if any(i[10] for i in list_))
 
 
 @pytest.mark.parametrize("seed", range(60))
@@ -160,36 +162,43 @@ def test_a_shared_plan_covers_every_score_once(shim, seed):
     f.close()
 
 
-@pytest.mark.parametrize("group,dim,tokens", [(8, 128, 1), (8, 256, 4), (4, 64, 1), (1, 64, 1), (5, 128, 3)])
-def test_forks_of_a_prompt_share_it(shim, group, dim, tokens):
-    f = Forest(shim, 64)
-    f.grow([0], [8000])
-    f.fork([0] * 31, list(range(1, 32)))
-    ranges, shared = check(f, 2, group, dim, list(range(31, -1, -1)), [tokens] * 32, 0)
-    assert ranges == 1 and shared == 8000 // 64 * 64 * 32 * tokens * 2 * group
+@pytest.mark.parametrize("name", FORESTS)
+def test_forks_of_a_prompt(shim, name):
+    kv, group, dim, page, prompt, forks, own, tokens, window, kinds = FORESTS[name]
+    f = Forest(shim, page)
+    f.grow([0], [prompt])
+    f.fork([0] * (forks - 1), list(range(1, forks)))
+    r = random.Random(3)
+    f.grow(list(range(forks)), [r.randint(1, own) for _ in range(forks)])
+    seqs = r.sample(range(forks), forks)
+    counts = [tokens[i % len(tokens)] for i in range(forks)]
+    ranges, shared, got = check(f, kv, group, dim, seqs, counts, window)
+    assert ranges == 1 and got == kinds
+    if kinds and not window:  # all whole pages of the prompt, for all that are not chunks
+        assert shared == prompt // page * page * kv * group * sum(c for c in counts if c * group <= 256)
     f.close()
 
 
 def test_a_tree_of_forks(shim):
     """Three levels and no more; a level that is not worth a tile of its own goes to the ones below it."""
     f = Forest(shim, 32)
-    f.grow([0], [1024])
+    f.grow([0], [8192])
     f.fork([0] * 3, [1, 2, 3])
-    f.grow([0, 1, 2, 3], [640] * 4)
+    f.grow([0, 1, 2, 3], [4096] * 4)
     f.fork([s % 4 for s in range(4, 16)], list(range(4, 16)))
-    f.grow(list(range(16)), [512] * 16)
+    f.grow(list(range(16)), [2048] * 16)
     f.fork([s % 16 for s in range(16, 48)], list(range(16, 48)))
     f.grow(list(range(48)), [33] * 48)
-    ranges, shared = check(f, 1, 4, 128, list(range(48)), [1] * 48, 0)
-    assert ranges == 1 + 4 + 16 and shared == 48 * 4 * (1024 + 640 + 512)
+    ranges, shared, kinds = check(f, 2, 8, 128, list(range(48)), [1] * 48, 0)
+    assert ranges == 1 + 4 + 16 and shared == 48 * 16 * (8192 + 4096 + 2048) and kinds
     f.close()
     f = Forest(shim, 32)
     f.grow([0], [64])  # too short to be worth it: the two prompts behind it take it with them
     f.fork([0], [1])
-    f.grow([0, 1], [2000, 3000])
-    f.fork([0, 0, 1, 1], [2, 3, 4, 5])
-    ranges, shared = check(f, 1, 4, 128, [3, 5, 0, 1, 4, 2], [1] * 6, 0)
-    assert ranges == 2 and shared == 4 * 3 * (2064 // 32 * 32 + 3064 // 32 * 32)
+    f.grow([0, 1], [20000, 30000])
+    f.fork([0] * 7 + [1] * 7, list(range(2, 16)))
+    ranges, shared, kinds = check(f, 4, 8, 128, list(range(15, -1, -1)), [1] * 16, 0)
+    assert ranges == 2 and shared == 32 * 8 * (20064 // 32 * 32 + 30064 // 32 * 32)
     f.close()
 
 
@@ -207,7 +216,7 @@ def test_without_anything_in_common_the_plan_is_the_plain_one(shim):
     f = Forest(shim, 64)
     f.grow([0, 1, 2], [5000, 100, 3000])
     f.fork([1], [3])  # 100 positions: one page
-    ranges, shared = check(f, 2, 8, 128, [2, 3, 1, 0], [1, 2, 1, 300], 0)
+    ranges, shared, _ = check(f, 2, 8, 128, [2, 3, 1, 0], [1, 2, 1, 300], 0)
     assert ranges == 0 and shared == 0 and shim.shim_plain(16, 2, 128, 0) == 1
     f.close()
 
@@ -217,7 +226,7 @@ def test_a_window_past_the_prompt_leaves_it_out(shim):
     f.grow([0], [4000])
     f.fork([0] * 7, list(range(1, 8)))
     f.grow(list(range(8)), [600] * 8)
-    ranges, shared = check(f, 2, 8, 128, list(range(8)), [1] * 8, 513)
+    ranges, shared, _ = check(f, 2, 8, 128, list(range(8)), [1] * 8, 513)
     assert ranges == 1 and shared == 0 and shim.shim_plain(16, 2, 128, 513) == 1
     f.close()
 
@@ -226,6 +235,6 @@ def test_more_rows_than_partials_fit_are_attended_apart(shim):
     f = Forest(shim, 32, seqs=600, pages=2000)
     f.grow([0], [2000])
     f.fork([0] * 599, list(range(1, 600)))
-    ranges, shared = check(f, 8, 16, 64, list(range(600)), [1] * 600, 0)  # 76,800 rows
+    ranges, shared, _ = check(f, 8, 16, 64, list(range(600)), [1] * 600, 0)  # 76,800 rows
     assert ranges == 1 and shared == 0 and shim.shim_plain(128, 8, 64, 0) == 1
     f.close()
