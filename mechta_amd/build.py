@@ -29,7 +29,9 @@ EXTRA = {"kv_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-fno-honor-na
          "kv_produce.hip": ["-ffp-contract=off"],
          # accumulators in VGPRs: few_rows of heads of 256 and 32 rows fits its registers (with AGPRs it spilled 35);
          # chunk_rows of heads of 256 keeps 8 bytes a lane in memory
-         "paged_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+         "paged_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+         # scores are read by vector instructions right behind their products
+         "paged_weigh.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 # measurement aid of bench.py (a plain HBM read of a given size), its own library: not part of the KV-cache ABI
 PROBE_SRC, PROBE_LIB = "hbm_probe.hip", os.path.join(OUTDIR, "libmkv_probe.so")
 ARCH = os.environ.get("MKV_OFFLOAD_ARCH", "gfx950")

@@ -913,13 +913,14 @@ size_t weigh_entries(const Shape& g, int tokens, int seqs) {
 void plan_weigh(const Shape& g, const std::vector<Member>& batch, int window, int last, const WeighRoom& room, WeighPlan& out) {
     for (auto& v : out.scores) v.clear();
     for (auto& v : out.sums) v.clear();
+    out.merges.clear();
     out.fades.clear();
     const int group = g.q_heads / g.kv_heads, heads = g.kv_heads;
     struct Weighed {  // a sequence with counted tokens
         int seq, tok0, rows, pos0, k0, len, scores;
     };
     std::vector<Weighed> few, many;
-    long long stats = 0, work = 0, few_keys = 0, few_rows = 0, tile_keys = 0, rows_left = 0;
+    long long stats = 0, work = 0, few_keys = 0, tile_keys = 0, rows_left = 0;
     int tok = 0;
     for (const Member& m : batch) {
         const int n = last ? std::min(last, m.count) : m.count, tok0 = tok + m.count - n;
@@ -933,7 +934,6 @@ void plan_weigh(const Shape& g, const std::vector<Member>& batch, int window, in
             w.scores = (int)work;
             work += kept;
             few_keys += (long long)(m.len - k0) * heads;
-            few_rows += heads;
             few.push_back(w);
         } else {
             tile_keys += (long long)((rows + SCORE_ROWS - 1) / SCORE_ROWS) * (m.len - k0) * heads;
@@ -948,14 +948,16 @@ void plan_weigh(const Shape& g, const std::vector<Member>& batch, int window, in
         return (int)std::max(1ll, std::min(p, most));
     };
     int more = 0;
-    // Few rows: bound by the keys' stream, cut as those of the attention.
-    const long long few_share = (few_keys + STREAMS - 1) / STREAMS;
-    const long long few_length = std::max<long long>(LEAST_KEYS, few_rows > STREAMS / 2 ? few_share * 3 / 4 : few_share) / KEYS;
+    // Few rows: bound by the keys' stream. Whole where they are short, which spares the launch for their sums (a token at 300 positions of
+    // 2 x 256 6.2 us, in three pieces 8.4; 12 windows of 545 keys of 4 x 128 9.3 and 9.2); else in about four pieces a CU. (The statistics of 64 sequences at 500 .. 8,001 positions of 4 x 128 in 428 / 640 / 1,160 / 2,300 work-groups: 45.5 / 44.1 / 42.3 /
+    // 41.5 us.)
+    constexpr int WHOLE_FEW = 512;
+    const long long few_length = std::max<long long>(LEAST_KEYS, (few_keys + 4 * CUS - 1) / (4 * CUS)) / KEYS;
     for (const Weighed& w : few) {
         const int units = (w.len - w.k0 + KEYS - 1) / KEYS;
         for (int h = 0; h < heads; h++) {
             rows_left -= w.rows;
-            int pieces = pieces_in(w.rows, units, few_length);
+            int pieces = units * KEYS <= WHOLE_FEW ? 1 : pieces_in(w.rows, units, few_length);
             pieces = std::min(pieces, 1 + (WEIGH_MOST / 2 - std::min(more, WEIGH_MOST / 2)));
             more += pieces - 1;
             const int scores = w.scores + h * units * KEYS * w.rows, stat = (int)stats;
@@ -964,9 +966,9 @@ void plan_weigh(const Shape& g, const std::vector<Member>& batch, int window, in
                 const int a = (int)((long long)units * p / pieces), b = (int)((long long)units * (p + 1) / pieces);
                 out.scores[w.rows <= TILE_ROWS[FEW] ? SCORE_FEW : SCORE_SOME].push_back(
                     {w.seq, h, w.tok0, w.rows, 0, w.pos0, w.k0 + a * KEYS, std::min(w.len, w.k0 + b * KEYS), stat + p * w.rows,
-                     scores + a * KEYS * w.rows, {0, 0}});
+                     scores + a * KEYS * w.rows, pieces == 1, 0});
             }
-            out.sums[0].push_back({w.seq, h, w.tok0, w.rows, w.pos0, w.k0, w.len, 0, w.rows, stat, pieces, scores, w.k0, -1, {0, 0}});
+            if (pieces > 1) out.sums[0].push_back({w.seq, h, w.tok0, w.rows, w.pos0, w.k0, w.len, 0, w.rows, stat, pieces, scores, w.k0, -1, {0, 0}});
         }
     }
     // their sums by ranges of keys
@@ -986,6 +988,7 @@ void plan_weigh(const Shape& g, const std::vector<Member>& batch, int window, in
     // Many rows: bound by the matrix units and the exponentials. Tiles of rows against all their keys, split where they are few.
     more = 0;
     constexpr int PLACES = 2 * CUS;
+    constexpr int SUM_PLACES = 6 * CUS - 64;
     const long long many_length = std::max<long long>(LEAST_KEYS, (tile_keys + PLACES - 1) / PLACES) / KEYS;
     long long key_tiles = 0, row_tiles = 0;
     for (const Weighed& w : many) {
@@ -996,7 +999,7 @@ void plan_weigh(const Shape& g, const std::vector<Member>& batch, int window, in
         }
     }
     const int per = (int)std::max(1ll, (key_tiles + WEIGH_MOST / 2 - 1) / (WEIGH_MOST / 2));  // key tiles of a work-group
-    const long long chunk = per > 1 ? 1ll << 40 : std::max<long long>(8, (row_tiles + 4 * CUS - 1) / (4 * CUS)) * KEYS;  // rows of one
+    const long long chunk = per > 1 ? 1ll << 40 : std::max<long long>(4, (row_tiles + SUM_PLACES - 1) / SUM_PLACES) * KEYS;  // rows of one
     for (const Weighed& w : many) {
         const int units = (w.len - w.k0 + KEYS - 1) / KEYS;
         int pieces = 0;
@@ -1012,13 +1015,15 @@ void plan_weigh(const Shape& g, const std::vector<Member>& batch, int window, in
             }
             const int stat = (int)stats;
             stats += (long long)pieces * w.rows;
+            for (int r = 0; pieces > 1 && r < w.rows; r += SCORE_ROWS)
+                out.merges.push_back({h, w.tok0, w.rows, r, std::min(r + SCORE_ROWS, w.rows), stat, pieces, 0});
             for (int r = 0; r < w.rows; r += SCORE_ROWS) {
                 const int end = std::min(w.len, w.pos0 + (std::min(r + SCORE_ROWS, w.rows) - 1) / group + 1);
                 const int lo = window ? std::max(0, w.pos0 + r / group - window + 1) / KEYS * KEYS : 0;
                 for (int p = 0; p < pieces; p++) {  // (a piece without keys leaves its rows' statistics empty)
                     const int a = std::max(lo, w.k0 + (int)((long long)units * p / pieces) * KEYS);
                     const int b = std::min(end, w.k0 + (int)((long long)units * (p + 1) / pieces) * KEYS);
-                    out.scores[SCORE_MANY].push_back({w.seq, h, w.tok0, w.rows, r, w.pos0, a, std::max(a, b), stat + p * w.rows + r, -1, {0, 0}});
+                    out.scores[SCORE_MANY].push_back({w.seq, h, w.tok0, w.rows, r, w.pos0, a, std::max(a, b), stat + p * w.rows + r, -1, pieces == 1, 0});
                 }
             }
             for (int k = w.k0; k < w.len; k += SUM_KEYS * per) {
@@ -1040,6 +1045,10 @@ void plan_weigh(const Shape& g, const std::vector<Member>& batch, int window, in
             }
         }
     }
+    // All tiles of rows run at once, several on a CU, which takes every CUS-th of them: the longest beside the shortest.
+    auto& tiles = out.scores[SCORE_MANY];
+    std::stable_sort(tiles.begin(), tiles.end(), [](const Score& x, const Score& y) { return x.k1 - x.k0 > y.k1 - y.k0; });
+    for (size_t i = CUS; i < tiles.size(); i += 2 * CUS) std::reverse(tiles.begin() + i, tiles.begin() + std::min(tiles.size(), i + CUS));
 }
 
 }  // namespace paged

@@ -157,23 +157,29 @@ size_t most_joins(const Shape& g, int tokens, int seqs);
 struct Score {  // rows row0 .. of one kv head against keys [k0, k1): the reference and the sum of each to stats[stat ..]
     int seq, head, tok0, rows, row0, pos0;  // tok0, pos0: the first counted token and its position
     int k0, k1, stat;
-    int keep;        // where the scores go in the work space, by blocks of KEYS keys [row][key], -1: nowhere
-    int pad[2];
+    int keep;        // few rows: where the scores go in the work space, by blocks of KEYS keys [row][key]
+    int whole;       // there is no other piece: many rows: what goes to stats is final; few: the sums are taken at once
+    int pad;
+};
+struct Merge {  // rows r0 .. r1 of several pieces: the final statistics to the first piece's place
+    int head, tok0, rows, r0, r1, stat, pieces, pad;
 };
 struct Sum {  // keys [k0, k1) from rows [r0, r1)
     int seq, head, tok0, rows, pos0, k0, k1;
     int r0, r1;
-    int stat, pieces;  // statistics of piece p of row r at stats[stat + p * rows + r]
-    int scores, s0;    // kept scores, the first of key s0; -1: none
+    int stat, pieces;  // few rows: statistics of piece p of row r at stats[stat + p * rows + r]; many: the final ones at stats[stat + r]
+    int scores, s0;    // few rows: kept scores, the first of key s0
     int part;          // where the sums go in the work space, -1: to the position's weight
     int pad[2];
 };
 struct Fade {  // weights of keys [k0, k1), faded, plus `sums` partial sums, of key k0 + i at part + s * stride + i
     int seq, head, k0, k1, part, sums, stride, pad;
 };
-enum { SCORE_FEW, SCORE_SOME, SCORE_MANY, SUM_FEW, SUM_MANY, FADES, WEIGH_LISTS };  // few: up to 16 rows, some: up to 32
+// few: up to 16 rows, some: up to 32, many: tiles of 128
+enum { SCORE_FEW, SCORE_SOME, SCORE_MANY, MERGES, SUM_FEW, SUM_MANY, FADES, WEIGH_LISTS };
 struct WeighPlan {
     std::vector<Score> scores[SCORE_MANY + 1];
+    std::vector<Merge> merges;
     std::vector<Sum> sums[2];
     std::vector<Fade> fades;
 };

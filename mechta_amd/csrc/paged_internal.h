@@ -12,7 +12,7 @@ struct Lists {
     size_t items[KINDS], joins, segs, words;  // word offsets of the lists; words of the whole
 };
 constexpr size_t COUNTS = 8;  // words in front of a list: items of each kind, joins; of the runs: how many, the longest
-static_assert(KINDS < COUNTS, "counts");
+static_assert(KINDS < COUNTS && WEIGH_LISTS <= COUNTS, "counts");
 
 struct Geometry {
     int layers, q_heads, kv_heads, head_dim, fmt, pages, page, most_pages;  // most_pages: of a sequence

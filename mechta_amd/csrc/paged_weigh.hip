@@ -70,12 +70,16 @@ __device__ inline float2 factor_of(const Args& a, float2 s, int head) {
     if (a.sinks) s = merge(s, make_float2(a.sinks[head] * LOG2E, 1.f));
     return make_float2(s.x, 1.f / s.y);
 }
-// One more score of a row (log2 units) in its (m, l).
+// The same for row `row` of a sequence's kv head; a row that the call does not have weighs nothing, exp2(score - inf) * 0.
+__device__ inline float2 final_of(const Args& a, float2 s, int tok0, int head, int row) {
+    return tok0 + row / a.group < a.rows ? factor_of(a, s, head * a.group + row % a.group) : make_float2(-NEG_INF, 0.f);
+}
+// Scores of a row (log2 units) in its (m, l).
 template <int N>
 __device__ inline void add_scores(float2& ml, const float (&s)[N]) {
     float top = ml.x;
 #pragma unroll
-    for (int i = 0; i < N; i++) top = fmaxf(top, s[i]);
+    for (int i = 0; i < N; i += 2) top = vmax3(top, s[i], s[i + 1]);
     const float ref = top == NEG_INF ? 0.f : top;
     float sum = ml.x == NEG_INF ? ml.y : ml.y * fast_exp2(ml.x - ref);
 #pragma unroll
@@ -85,21 +89,49 @@ __device__ inline void add_scores(float2& ml, const float (&s)[N]) {
 
 __device__ inline Score load_score(const Score* p) {
     const Uniform<int> x = uniform((const int*)p);
-    return Score{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], x[8], x[9], {0, 0}};
+    return Score{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], x[8], x[9], x[10], 0};
 }
 __device__ inline Sum load_sum(const Sum* p) {
     const Uniform<int> x = uniform((const int*)p);
     return Sum{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], x[8], x[9], x[10], x[11], x[12], x[13], {0, 0}};
 }
 
+// ---- few rows' kept scores summed up: a thread a key ----
+__device__ inline void put_factor(const Args& a, float2 s, int head, int row, float2* f, int& odd) {
+    f[row] = s = factor_of(a, s, head * a.group + row % a.group);
+    if (!(s.y < -NEG_INF)) odd = 1;  // its weights are no numbers where it sees, and nothing all the same where it does not
+}
+// rows: of the sequence, there: of them in the call; f: their factors
+__device__ inline void sum_kept(const Args& a, int seq, int head, int pos0, int k0, int k1, int rows, int there, int scores, int s0,
+                                const float2* f, int odd) {
+    float* const weights = a.weights + seq * a.seq_stride + head * a.stride;
+    for (int key = k0 + (int)threadIdx.x; key < k1; key += 256) {
+        const int i = key - s0;
+        const float* const s = a.work + scores + (size_t)(i / KEYS) * KEYS * rows + i % KEYS;
+        const float was = a.decay == 0.f ? 0.f : a.decay * weights[key];
+        float sum = 0.f;
+#pragma unroll 8
+        for (int r = 0; r < there; r++) sum += fast_exp2(s[r * KEYS] - f[r].x) * f[r].y;
+        if (odd) {
+            sum = 0.f;
+            for (int r = 0; r < there; r++) {
+                const int pos = pos0 + r / a.group;
+                if (key <= pos && (!a.window || key > pos - a.window)) sum += fast_exp2(s[r * KEYS] - f[r].x) * f[r].y;
+            }
+        }
+        weights[key] = was + sum;
+    }
+}
+
 // ---- statistics of few rows, NRT x 16 of them, with their scores ----
 // 4 waves, each with every fourth block of 32 keys, its K straight from memory into the operands of the 16x16x32 products, the
 // next block's on its way meanwhile. Lane (r, g): row r, keys 4g + i and 16 + 4g + i of the block; each lane has an m and l of
-// its own until the end. Bound by memory.
+// its own until the end. Where there is no other piece, the sums are taken at once. Bound by memory.
 template <typename T, int D, int NRT>
 __global__ void __launch_bounds__(256) score_few(Args a, const Score* __restrict__ items, const int* __restrict__ nitems) {
     constexpr int NS = D / 32;
-    __shared__ float2 sml[4][16 * NRT];
+    __shared__ float2 sml[4][16 * NRT], f[16 * NRT];
+    __shared__ int odd;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     const int count = *uniform(nitems);
     for (int n = blockIdx.x; n < count; n += gridDim.x) {
@@ -169,213 +201,273 @@ __global__ void __launch_bounds__(256) score_few(Args a, const Score* __restrict
             ml[t] = merge(ml[t], shuffled(ml[t], 32));
             if (g == 0) sml[w][16 * t + r] = ml[t];
         }
+        if (threadIdx.x == 0) odd = 0;
         __syncthreads();
-        const int row = threadIdx.x;
-        if (row < 16 * NRT && row < it.rows) a.stats[it.stat + row] = merge(merge(sml[0][row], sml[1][row]), merge(sml[2][row], sml[3][row]));
+        const int row = threadIdx.x, there = min(it.rows, (a.rows - it.tok0) * a.group);
+        if (row < 16 * NRT && row < it.rows) {
+            const float2 all = merge(merge(sml[0][row], sml[1][row]), merge(sml[2][row], sml[3][row]));
+            if (!it.whole) a.stats[it.stat + row] = all;
+            else if (row < there) put_factor(a, all, it.head, row, f, odd);
+        }
+        if (!it.whole) continue;
+        __syncthreads();  // (and the scores, from whichever wave)
+        sum_kept(a, it.seq, it.head, it.pos0, it.k0, it.k1, it.rows, there, it.keep, it.k0, f, odd);
     }
 }
 
-// ---- statistics of many rows: 4 waves of 32 rows against the same keys ----
-// S^T[32 keys][32 rows] = K . Q^T (32x32x16): lane (r, h) has row r, keys 8c + 4h + i.
+// ---- many rows ----
+// Both readings compute S^T[32 keys][32 rows] = K . Q^T (32x32x16): lane (r, h) has row r, keys 8c + 4h + i, so a row's statistics,
+// and what turns its scores into weights, are its lane's. One side stays in registers, 32 rows or 32 keys a wave; the other comes
+// by direct loads into a ring in LDS that the work-group's waves share, tiles of 32, one barrier a tile: what lands is
+// waited for by each wave before the barrier, and what is overwritten behind it has been read before it. Bound by the vector units (an
+// exponential and two to three others a score, in either reading) and the products beside them.
+constexpr int RING_TILES = 4;
+// 64 lanes x 16 or 4 bytes from addresses of their own, to `lds` and behind
+__device__ inline void dma16v(const void* src, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory", "m0");
+}
+__device__ inline void dma4v(const void* src, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory", "m0");
+}
+template <int N>
+__device__ inline void landed() {  // but for the wave's last N direct loads
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Operands that have been loaded: the compiler waits for them here. (Where they are used, in the loop, its wait for them is one for every
+// direct load on its way.)
+template <typename T, int N>
+__device__ inline void arrived(Vec8<T> (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+        u32x4 x = __builtin_bit_cast(u32x4, v[i]);
+        asm volatile("" : "+v"(x));
+        v[i] = __builtin_bit_cast(Vec8<T>, x);
+    }
+}
+
+// Work-group: 128 rows, 32 a wave.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) score_rows(Args a, const Score* __restrict__ items, const int* __restrict__ nitems) {
-    constexpr int NS = D / 16;
+    constexpr int NS = D / 16, TILE = KEYS * D * 2, PER = D / 64;  // bytes of a tile; KB of it that a wave brings
+    __shared__ __attribute__((aligned(1024))) unsigned char ring[RING_TILES * TILE];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h = lane >> 5;
+    const unsigned lds = (unsigned)(uintptr_t)(lds_void*)ring, voff = lane * 16;
+    const int kaddr = (r >> 4) * 16 * D * 2 + h * 256 + (r & 15) * 16;
     const int count = *uniform(nitems);
     for (int n = blockIdx.x; n < count; n += gridDim.x) {
         const Score it = load_score(items + n);
         const Keys<D> keys(a, it.seq, it.head);
-        const int first = it.row0 + 32 * w, row = first + r, last = min(first + 31, it.rows - 1);
-        if (first >= it.rows) continue;
+        const int first = it.row0 + 32 * w, row = first + r, last = min(first + 32, it.rows) - 1;
+        const int blocks = (it.k1 - it.k0 + KEYS - 1) / KEYS;
+        auto block = [&](int j) INLINE { return keys.block(it.k0 + KEYS * min(j, blocks - 1)); };
+        auto issue = [&](int j, const char* p) INLINE {
+            const unsigned to = lds + j % RING_TILES * TILE + w * PER * 1024;
+#pragma unroll
+            for (int i = 0; i < PER; i++) dma16s(p + (w * PER + i) * 1024, voff, to + i * 1024);
+        };
+        const char* next = nullptr;  // where the next block is, looked up a step ahead
+        __syncthreads();  // the ring of the item before has been read
+        if (blocks > 0) {
+#pragma unroll
+            for (int j = 0; j < RING_TILES - 1; j++) issue(j, block(j));
+            next = block(RING_TILES - 1);
+        }
+        Vec8<T> q[NS];
         const int tok = row / a.group, head = it.head * a.group + row % a.group;
         const bool is = row < it.rows && it.tok0 + tok < a.rows;
         const int hi = is ? it.pos0 + tok : -1, lo = a.window ? it.pos0 + tok - a.window + 1 : 0;
-        const int all_hi = it.pos0 + first / a.group, all_lo = a.window ? it.pos0 + last / a.group - a.window + 1 : 0;
-        Vec8<T> q[NS], k[NS];
         const T* const src = (const T*)a.q + (int64_t)(it.tok0 + tok) * a.q_tok + head * a.q_head + 8 * h;
 #pragma unroll
         for (int s = 0; s < NS; s++) q[s] = is ? load8(src + 16 * s) : Vec8<T>{};
-        const int blocks = (it.k1 - it.k0 + KEYS - 1) / KEYS;
-        const unsigned at = (r >> 4) * 16 * D * 2 + h * 256 + (r & 15) * 16;
-        auto load_k = [&](int j) INLINE {
-            const char* const p = keys.block(it.k0 + KEYS * min(j, blocks - 1)) + at;
-#pragma unroll
-            for (int s = 0; s < NS; s++) k[s] = load8((const T*)(p + s * 512));
-        };
+        arrived(q);
         float2 ml = make_float2(NEG_INF, 0.f);
-        if (blocks > 0) load_k(0);
+        const int all_hi = it.pos0 + first / a.group, all_lo = a.window ? it.pos0 + last / a.group - a.window + 1 : 0;
         for (int j = 0; j < blocks; j++) {
+            landed<(RING_TILES - 2) * PER>();
+            lds_barrier();
+            issue(j + RING_TILES - 1, next);
+            next = block(j + RING_TILES);
+            const unsigned char* const k = ring + j % RING_TILES * TILE + kaddr;
             f32x16 s = f32x16{};
 #pragma unroll
-            for (int i = 0; i < NS; i++) s = mfma32(k[i], q[i], s);
-            load_k(j + 1);
-            const int k0 = it.k0 + KEYS * j;
-            const bool edge = k0 + KEYS - 1 > all_hi || k0 < all_lo;
-            float x[16];
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                x[i] = s[i] * a.scale2;
-                const int key = k0 + i / 4 * 8 + 4 * h + i % 4;
-                if (edge && (key > hi || key < lo)) x[i] = NEG_INF;
+            for (int i = 0; i < NS; i++) s = mfma32(*(const Vec8<T>*)(k + i * 512), q[i], s);
+            if constexpr (NS <= 8) {  // all operands on their way at once, where there are registers for them
+                __builtin_amdgcn_sched_group_barrier(0x100, NS, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, NS, 0);
             }
-            add_scores(ml, x);
+            const int k0 = it.k0 + KEYS * j;
+            if (k0 + KEYS - 1 > all_hi || k0 < all_lo) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int key = k0 + i / 4 * 8 + 4 * h + i % 4;
+                    if (key > hi || key < lo) s[i] = NEG_INF;
+                }
+            }
+            float top = fmaxf(s[0], s[1]);  // the compiler's: it waits for the products
+#pragma unroll
+            for (int i = 2; i < 16; i += 2) top = vmax3(top, s[i], s[i + 1]);
+            top = vmax(ml.x, top * a.scale2);
+            const float ref = top == NEG_INF ? 0.f : top;
+            float sum = ml.x == NEG_INF ? ml.y : ml.y * fast_exp2(ml.x - ref), more = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                sum += fast_exp2(__builtin_fmaf(s[i], a.scale2, -ref));
+                more += fast_exp2(__builtin_fmaf(s[i + 1], a.scale2, -ref));
+            }
+            ml = make_float2(top, sum + more);
         }
+        landed<0>();  // copies that no block needs write the ring no more behind this
         ml = merge(ml, shuffled(ml, 32));
-        if (h == 0 && row < it.rows) a.stats[it.stat + 32 * w + r] = ml;
+        if (h || row >= it.rows) continue;
+        if (it.whole) ml = final_of(a, ml, it.tok0, it.head, row);
+        a.stats[it.stat + row - it.row0] = ml;
     }
 }
 
-// ---- sums over few rows' kept scores: a thread a key ----
+// Several pieces of many rows' statistics: 16 lanes a row, 16 rows of an item a work-group.
+constexpr int MERGE_WAYS = SCORE_ROWS / 16;
+__global__ void __launch_bounds__(256) merge_kernel(Args a, const Merge* __restrict__ items, const int* __restrict__ nitems) {
+    const int count = *uniform(nitems) * MERGE_WAYS, lane = threadIdx.x % 16;
+    for (int n = blockIdx.x; n < count; n += gridDim.x) {
+        const Uniform<int> u = uniform((const int*)(items + n / MERGE_WAYS));
+        const Merge it{u[0], u[1], u[2], u[3], u[4], u[5], u[6], 0};
+        const int row = it.r0 + n % MERGE_WAYS * 16 + (int)threadIdx.x / 16;
+        float2 all = make_float2(NEG_INF, 0.f);
+        for (int p0 = 0; p0 < it.pieces; p0 += 128) {
+            float2 x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int p = p0 + 16 * i + lane;
+                x[i] = row < it.r1 && p < it.pieces ? a.stats[it.stat + (size_t)p * it.rows + row] : make_float2(NEG_INF, 0.f);
+            }
+#pragma unroll
+            for (int y = 4; y; y /= 2)
+#pragma unroll
+                for (int i = 0; i < y; i++) x[i] = merge(x[i], x[i + y]);
+            all = merge(all, x[0]);
+        }
+#pragma unroll
+        for (int i = 1; i < 16; i *= 2) all = merge(all, shuffled(all, i));
+        if (lane == 0 && row < it.r1) a.stats[it.stat + row] = final_of(a, all, it.tok0, it.head, row);
+    }
+}
+
+// ---- sums over few rows' kept scores ----
 __global__ void __launch_bounds__(256) sum_few(Args a, const Sum* __restrict__ items, const int* __restrict__ nitems) {
     __shared__ float2 f[32];
-    __shared__ int odd;  // a row whose weights are no numbers where it sees, and nothing all the same where it does not
+    __shared__ int odd;
     const int count = *uniform(nitems), tid = threadIdx.x;
     for (int n = blockIdx.x; n < count; n += gridDim.x) {
         const Sum it = load_sum(items + n);
-        const int rows = min(it.rows, (a.rows - it.tok0) * a.group);  // that the call has
         __syncthreads();  // the item before has been read
         if (tid == 0) odd = 0;
         __syncthreads();
-        {  // 8 lanes a row
-            const int row = tid / 8;
-            float2 s = make_float2(NEG_INF, 0.f);
-            if (row < rows)
-                for (int p = tid % 8; p < it.pieces; p += 8) s = merge(s, a.stats[it.stat + p * it.rows + row]);
+        // 8 lanes a row
+        const int row = tid / 8, rows = min(it.rows, (a.rows - it.tok0) * a.group);
+        float2 s = make_float2(NEG_INF, 0.f);
+        if (row < rows)
+            for (int p = tid % 8; p < it.pieces; p += 8) s = merge(s, a.stats[it.stat + p * it.rows + row]);
 #pragma unroll
-            for (int i = 1; i < 8; i *= 2) s = merge(s, shuffled(s, i));
-            if (tid % 8 == 0 && row < rows) {
-                f[row] = s = factor_of(a, s, it.head * a.group + row % a.group);
-                if (!(s.y < -NEG_INF)) odd = 1;
-            }
-        }
+        for (int i = 1; i < 8; i *= 2) s = merge(s, shuffled(s, i));
+        if (tid % 8 == 0 && row < rows) put_factor(a, s, it.head, row, f, odd);
         __syncthreads();
-        float* const weights = a.weights + it.seq * a.seq_stride + it.head * a.stride;
-        for (int key = it.k0 + tid; key < it.k1; key += 256) {
-            const int i = key - it.s0;
-            const float* const s = a.work + it.scores + (size_t)(i / KEYS) * KEYS * it.rows + i % KEYS;
-            float sum = 0.f;
-#pragma unroll 8
-            for (int r = 0; r < rows; r++) sum += fast_exp2(s[r * KEYS] - f[r].x) * f[r].y;
-            if (odd) {
-                sum = 0.f;
-                for (int r = 0; r < rows; r++) {
-                    const int pos = it.pos0 + r / a.group;
-                    if (key <= pos && (!a.window || key > pos - a.window)) sum += fast_exp2(s[r * KEYS] - f[r].x) * f[r].y;
-                }
-            }
-            weights[key] = (a.decay == 0.f ? 0.f : a.decay * weights[key]) + sum;
-        }
+        sum_kept(a, it.seq, it.head, it.pos0, it.k0, it.k1, it.rows, rows, it.scores, it.s0, f, odd);
     }
 }
 
-// ---- sums over many rows: 4 waves of 64 keys against the same rows, 32 at a time through LDS ----
-// S[32 rows][32 keys] = Q . K^T (32x32x16), K in registers: lane (x, h) has key x, rows 8c + 4h + i, so a key's sum over the
-// rows stays in its lane.
+// ---- sums over many rows: 8 waves of 32 keys in registers, the rows through the ring ----
+// A row tile lies in LDS as its operands are read, [8 dims][row][8], and its final statistics behind it. Sums over the rows stay by row
+// and key in the lanes' registers until the end.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) sum_rows(Args a, const Sum* __restrict__ items, const int* __restrict__ nitems) {
-    constexpr int NS = D / 16, PER = D / 64;  // 16-byte pieces of a row tile that a thread brings
-    __shared__ __attribute__((aligned(16))) T sq[2][32][D + 8];
-    __shared__ __attribute__((aligned(16))) float sm[2][32], sr[2][32];
-    __shared__ __attribute__((aligned(16))) int sp[2][32];
-    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), x = lane & 31, h = lane >> 5;
+__global__ void __launch_bounds__(512) sum_rows(Args a, const Sum* __restrict__ items, const int* __restrict__ nitems) {
+    constexpr int NS = D / 16, TILE = 32 * D * 2, SLOT = TILE + 256, PER = D == 64 ? 1 : D / 128;  // (heads of 64: two waves bring the same)
+    __shared__ __attribute__((aligned(1024))) unsigned char ring[RING_TILES * SLOT];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x = lane & 31, h = lane >> 5;
+    const int piece0 = w * PER % (D / 16);
+    const unsigned lds = (unsigned)(uintptr_t)(lds_void*)ring;
     const int count = *uniform(nitems);
+    // rows go on 32 at a time: tokens and heads of the group
+    const int tok_by = 32 / a.group, head_by = 32 % a.group;
+    const int64_t by = tok_by * a.q_tok + head_by * a.q_head, wrap = a.q_tok - a.group * a.q_head;
     for (int n = blockIdx.x; n < count; n += gridDim.x) {
         const Sum it = load_sum(items + n);
         const Keys<D> keys(a, it.seq, it.head);
         float* const weights = a.weights + it.seq * a.seq_stride + it.head * a.stride;
+        const int there = (int)min((long long)it.r1, (long long)(a.rows - it.tok0) * a.group);  // rows that the call has
         for (int k0 = it.k0; k0 < it.k1; k0 += SUM_KEYS) {
-            const int first = k0 + 64 * w;  // the wave's keys; behind the last the last block again, not counted
-            Vec8<T> k[2][NS];
-#pragma unroll
-            for (int b = 0; b < 2; b++) {
-                const char* const p = keys.block(min(first + 32 * b, (it.k1 - 1) / KEYS * KEYS)) + (x >> 4) * 16 * D * 2 + h * 256 + (x & 15) * 16;
-#pragma unroll
-                for (int s = 0; s < NS; s++) k[b][s] = load8((const T*)(p + s * 512));
-            }
-            float sum[2] = {0.f, 0.f};
-            Vec8<T> next[PER];
-            float2 stat;
-            int pos;
-            auto bring = [&](int r0) INLINE {  // rows r0 .. r0 + 31 and their statistics, 8 lanes a row
-#pragma unroll
-                for (int i = 0; i < PER; i++) {
-                    const int c = tid + 256 * i, row = r0 + c / (D / 8), tok = it.tok0 + row / a.group;
-                    const bool is = row < it.r1 && tok < a.rows;
-                    next[i] = is ? load8((const T*)a.q + (int64_t)tok * a.q_tok + (it.head * a.group + row % a.group) * a.q_head + c % (D / 8) * 8)
-                                 : Vec8<T>{};
-                }
-                const int row = r0 + tid / 8;
-                stat = make_float2(NEG_INF, 0.f);
-                if (row < it.r1)
-                    for (int p = tid % 8; p < it.pieces; p += 8) stat = merge(stat, a.stats[it.stat + p * it.rows + row]);
-                pos = it.pos0 + row / a.group;
-            };
-            auto put = [&](int r0, int to) INLINE {
-#pragma unroll
-                for (int i = 0; i < PER; i++) {
-                    const int c = tid + 256 * i;
-                    *(Vec8<T>*)&sq[to][c / (D / 8)][c % (D / 8) * 8] = next[i];
-                }
-#pragma unroll
-                for (int i = 1; i < 8; i *= 2) stat = merge(stat, shuffled(stat, i));
-                if (tid % 8 == 0) {
-                    const int row = r0 + tid / 8;
-                    const bool is = row < it.r1 && it.tok0 + row / a.group < a.rows;
-                    // a row that is none weighs nothing: exp2(0 - inf) * 0
-                    const float2 f = is ? factor_of(a, stat, it.head * a.group + row % a.group) : make_float2(-NEG_INF, 0.f);
-                    sm[to][tid / 8] = f.x;
-                    sr[to][tid / 8] = f.y;
-                    sp[to][tid / 8] = is ? pos : -1;
-                }
-            };
-            const long long there = min((long long)it.r1, (long long)(a.rows - it.tok0) * a.group);  // rows that the call has
+            const int first = k0 + 32 * w;  // the wave's keys; behind the last the last block again, not counted
             // the first rows that see any of these keys
-            int r0 = max(it.r0, (int)(min((long long)(k0 - it.pos0) * a.group, (long long)it.rows)) / KEYS * KEYS);
-            __syncthreads();  // the rows before have been read
-            if (r0 < it.r1) {
-                bring(r0);
-                put(r0, 0);
+            const int r0 = max(it.r0, (int)(min((long long)(k0 - it.pos0) * a.group, (long long)it.rows)) / KEYS * KEYS);
+            const int tiles = max(0, (there - r0 + 31) / 32);
+            int row = r0 + x, rem = row % a.group;  // of the next tile to come
+            const T* src = (const T*)a.q + (int64_t)(it.tok0 + row / a.group) * a.q_tok + (it.head * a.group + rem) * a.q_head + piece0 * 16 + h * 8;
+            const T* const q0 = (const T*)a.q + (int64_t)(it.tok0 + r0 / a.group) * a.q_tok + (it.head * a.group + r0 % a.group) * a.q_head + piece0 * 16 + h * 8;
+            auto issue = [&](int j) INLINE {  // (rows behind the last: the first again; tiles behind the last: its statistics)
+                const T* const p = row < there ? src : q0;
+                const unsigned to = lds + j % RING_TILES * SLOT;
+#pragma unroll
+                for (int i = 0; i < PER; i++) dma16v(p + i * 16, to + (piece0 + i) * 1024);
+                dma4v((const float*)(a.stats + it.stat + r0 + 32 * min(j, tiles - 1)) + lane, to + TILE);
+                row += 32;
+                rem += head_by;
+                src += by;
+                if (rem >= a.group) {
+                    rem -= a.group;
+                    src += wrap;
+                }
+            };
+            __syncthreads();  // the ring before has been read
+            if (tiles > 0)
+#pragma unroll
+                for (int j = 0; j < RING_TILES - 1; j++) issue(j);
+            Vec8<T> k[NS];
+            const char* const kp = keys.block(min(first, (it.k1 - 1) / KEYS * KEYS)) + (x >> 4) * 16 * D * 2 + h * 256 + (x & 15) * 16;
+#pragma unroll
+            for (int s = 0; s < NS; s++) k[s] = load8((const T*)(kp + s * 512));
+            arrived(k);
+            f32x16 sum = f32x16{};
+            for (int j = 0; j < tiles; j++) {
+                landed<(RING_TILES - 2) * (PER + 1)>();
+                lds_barrier();
+                issue(j + RING_TILES - 1);
+                const unsigned char* const slot = ring + j % RING_TILES * SLOT;
+                const float2 f = ((const float2*)(slot + TILE))[x];
+                f32x16 s = f32x16{};
+#pragma unroll
+                for (int i = 0; i < NS; i++) s = mfma32(k[i], *(const Vec8<T>*)(slot + (2 * i + h) * 512 + x * 16), s);
+                const int at = r0 + 32 * j;
+                const int low = it.pos0 + at / a.group, high = it.pos0 + (at + 31) / a.group;
+                if (at + 32 > there || first + 31 > low || (a.window && first < high - a.window + 1)) {
+                    // the lane's keys as seen from the last that its row sees, in [0, span): one comparison each
+                    const int pos = at + x < there ? it.pos0 + (at + x) / a.group : -1;
+                    const unsigned span = pos < 0 ? 0 : a.window ? a.window : pos + 1;
+                    int back = pos - first - 4 * h;
+                    asm volatile("" : "+v"(back));  // (here: the keys in registers through the loop otherwise)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float y = fast_exp2(__builtin_fmaf(s[i], a.scale2, -f.x)) * f.y;
+                        if ((unsigned)(back - i / 4 * 8 - i % 4) < span) sum[i] += y;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) sum[i] = __builtin_fmaf(fast_exp2(__builtin_fmaf(s[i], a.scale2, -f.x)), f.y, sum[i]);
+                }
+            }
+            landed<0>();  // copies that no tile needs write the ring no more behind this
+            __syncthreads();
+            float* const sums = (float*)ring;  // of the work-group's keys
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                float y = reduce16(sum[i], [](float p, float q) { return p + q; });
+                y += __shfl_xor(y, 16);
+                if (x == 0) sums[32 * w + i / 4 * 8 + 4 * h + i % 4] = y;
             }
             __syncthreads();
-            for (int at = 0; r0 < it.r1; r0 += 32, at ^= 1) {
-                const bool more = r0 + 32 < it.r1;
-                if (more) bring(r0 + 32);
-                f32x16 s[2] = {f32x16{}, f32x16{}};
-#pragma unroll
-                for (int i = 0; i < NS; i++) {
-                    const Vec8<T> q = *(const Vec8<T>*)&sq[at][x][16 * i + 8 * h];
-#pragma unroll
-                    for (int b = 0; b < 2; b++) s[b] = mfma32(q, k[b][i], s[b]);
-                }
-                // rows from r0 on at it.pos0 + r0 / group and behind
-                const int low = it.pos0 + r0 / a.group, high = it.pos0 + (r0 + 31) / a.group;
-#pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    const int key = first + 32 * b + x;
-                    const bool edge = r0 + 32 > there || first + 32 * b + 31 > low || (a.window && first + 32 * b < high - a.window + 1);
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const f32x4 m = *(const f32x4*)&sm[at][8 * c + 4 * h], f = *(const f32x4*)&sr[at][8 * c + 4 * h];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            float y = __builtin_fmaf(s[b][4 * c + i], a.scale2, -m[i]);
-                            y = fast_exp2(y) * f[i];
-                            if (edge) {
-                                const int p = sp[at][8 * c + 4 * h + i];
-                                if (key > p || (a.window && key < p - a.window + 1)) y = 0.f;
-                            }
-                            sum[b] += y;
-                        }
-                    }
-                }
-                if (more) put(r0 + 32, at ^ 1);
-                __syncthreads();
-            }
-#pragma unroll
-            for (int b = 0; b < 2; b++) {
-                const float y = sum[b] + __shfl_xor(sum[b], 32);
-                const int key = first + 32 * b + x;
-                if (h || key >= it.k1) continue;
+            const int key = k0 + (int)threadIdx.x;
+            if (threadIdx.x < SUM_KEYS && key < it.k1) {
+                const float y = sums[threadIdx.x];
                 if (it.part >= 0) a.work[it.part + key - it.k0] = y;
                 else weights[key] = (a.decay == 0.f ? 0.f : a.decay * weights[key]) + y;
             }
@@ -394,6 +486,7 @@ __global__ void __launch_bounds__(256) fade_kernel(Args a, const Fade* __restric
         for (int key = it.k0 + threadIdx.x; key < it.k1; key += 256) {
             const float* const p = a.work + it.part + key - it.k0;
             float sum = 0.f;
+#pragma unroll 8
             for (int s = 0; s < it.sums; s++) sum += p[(size_t)s * it.stride];
             weights[key] = (a.decay == 0.f ? 0.f : a.decay * weights[key]) + sum;
         }
@@ -627,16 +720,18 @@ __global__ void __launch_bounds__(1024) pack_kernel(WeightsAt w, const Eviction*
 template <typename T, int D>
 hipError_t weigh_as(const Args& a, const int* batch, const WeighLists& l, const int* grid, hipStream_t s) {
     hipError_t e = hipSuccess;
-    auto go = [&](auto kernel, int list, auto* items) {
+    auto go = [&](auto kernel, int list, auto* items, int threads = 256) {
         if (!grid[list] || e != hipSuccess) return;
-        kernel<<<dim3(grid[list]), dim3(256), 0, s>>>(a, items, batch + list);
+        const int groups = list == MERGES ? std::min(grid[list], MOST_GRID / MERGE_WAYS) * MERGE_WAYS : grid[list];
+        kernel<<<dim3(groups), dim3(threads), 0, s>>>(a, items, batch + list);
         e = hipGetLastError();
     };
     go(score_few<T, D, 1>, SCORE_FEW, (const Score*)(batch + l.at[SCORE_FEW]));
     go(score_few<T, D, 2>, SCORE_SOME, (const Score*)(batch + l.at[SCORE_SOME]));
     go(score_rows<T, D>, SCORE_MANY, (const Score*)(batch + l.at[SCORE_MANY]));
+    go(merge_kernel, MERGES, (const Merge*)(batch + l.at[MERGES]));
     go(sum_few, SUM_FEW, (const Sum*)(batch + l.at[SUM_FEW]));
-    go(sum_rows<T, D>, SUM_MANY, (const Sum*)(batch + l.at[SUM_MANY]));
+    go(sum_rows<T, D>, SUM_MANY, (const Sum*)(batch + l.at[SUM_MANY]), 512);
     go(fade_kernel, FADES, (const Fade*)(batch + l.at[FADES]));
     return e;
 }

@@ -62,12 +62,14 @@ struct Kept : Weights {
             const WeighPlan& p = next[w];
             if (!none) {
                 for (int k = 0; k <= SCORE_MANY; k++) c[k] = (int)p.scores[k].size();
+                c[MERGES] = (int)p.merges.size();
                 for (int k = 0; k < 2; k++) c[SUM_FEW + k] = (int)p.sums[k].size();
                 c[FADES] = (int)p.fades.size();
             }
             put(base, c, COUNTS);
             if (none) continue;
             for (int k = 0; k <= SCORE_MANY; k++) put(base + lists_at.at[k], p.scores[k].data(), p.scores[k].size() * (sizeof(Score) / 4));
+            put(base + lists_at.at[MERGES], p.merges.data(), p.merges.size() * (sizeof(Merge) / 4));
             for (int k = 0; k < 2; k++) put(base + lists_at.at[SUM_FEW + k], p.sums[k].data(), p.sums[k].size() * (sizeof(Sum) / 4));
             put(base + lists_at.at[FADES], p.fades.data(), p.fades.size() * (sizeof(Fade) / 4));
         }
@@ -86,7 +88,7 @@ WeightSizes weight_sizes(const mpg_config& c, int last) {
     s.stride = ((size_t)c.ctx + 31) / 32 * 32;
     s.weights = (size_t)c.layers * c.seqs * c.kv_heads * s.stride;
     const long long counted = last ? std::min((long long)c.tokens, (long long)std::min(c.seqs, c.tokens) * last) : c.tokens;
-    s.stats = counted * c.q_heads + STATS_MORE;
+    s.stats = counted * c.q_heads + STATS_MORE;  // (and a tile of rows behind: the last is read whole)
     // scores of up to 32 rows of every position of the pool, as far as that is not too much
     s.work = (size_t)std::min<double>(WORK_MOST, 32. * c.pages * c.page * c.kv_heads);
     s.picks = (size_t)c.layers * c.kv_heads * c.pages * c.page;
@@ -95,14 +97,14 @@ WeightSizes weight_sizes(const mpg_config& c, int last) {
     size_t at = COUNTS;
     for (int k = 0; k < WEIGH_LISTS; k++) {
         s.l.at[k] = at;
-        at += entries * (k <= SCORE_MANY ? sizeof(Score) : k < FADES ? sizeof(Sum) : sizeof(Fade)) / 4;
+        at += entries * (k <= SCORE_MANY ? sizeof(Score) : k == MERGES ? sizeof(Merge) : k < FADES ? sizeof(Sum) : sizeof(Fade)) / 4;
     }
     s.l.words = at;
     s.words = s.l.words * MPG_WINDOWS_MAX + c.seqs;
     return s;
 }
 double bytes_of(const WeightSizes& s, const mpg_config& c) {
-    return 4. * s.weights + 8. * s.stats + 4. * s.work + 4. * s.picks + 4. * s.words + sizeof(Eviction) * (double)c.seqs;
+    return 4. * s.weights + 8. * (s.stats + KEYS) + 4. * s.work + 4. * s.picks + 4. * s.words + sizeof(Eviction) * (double)c.seqs;
 }
 
 int check_last(const char* who, int last) {
@@ -143,7 +145,7 @@ static int keep_weights(mpg_t* h, int last) {
     hipError_t e = words < 1ull << 32 ? hipSuccess : hipErrorOutOfMemory;
     if (e == hipSuccess) e = hipMalloc((void**)&dev, words * 4);
     if (e == hipSuccess) e = hipMalloc((void**)&k->at.p, s.weights * 4);
-    if (e == hipSuccess) e = hipMalloc((void**)&k->stats, s.stats * 8);
+    if (e == hipSuccess) e = hipMalloc((void**)&k->stats, (s.stats + KEYS) * 8);
     if (e == hipSuccess) e = hipMalloc((void**)&k->work, s.work * 4);
     if (e == hipSuccess) e = hipMalloc((void**)&k->picks, s.picks * 4);
     if (e == hipSuccess) e = hipMalloc((void**)&k->entries, sizeof(Eviction) * c.seqs);
@@ -210,7 +212,9 @@ int mpg_weigh(mpg_t* h, int layer, int rows, const void* q, int64_t q_tok, int64
     a.stats = k->stats;
     a.work = k->work;
     int grid[WEIGH_LISTS];
-    auto size = [&](int list) { return list <= SCORE_MANY ? p.scores[list].size() : list < FADES ? p.sums[list - SUM_FEW].size() : p.fades.size(); };
+    auto size = [&](int list) {
+        return list <= SCORE_MANY ? p.scores[list].size() : list == MERGES ? p.merges.size() : list < FADES ? p.sums[list - SUM_FEW].size() : p.fades.size();
+    };
     for (int l = 0; l < WEIGH_LISTS; l++) grid[l] = cap ? GRAPH_WEIGH : (int)std::min<size_t>(size(l), MOST_GRID);
     if (!cap && decay == 1) {  // what is not given anything stays as it is
         bool sums = false;

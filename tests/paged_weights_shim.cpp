@@ -29,6 +29,7 @@ void shim_weigh(int q_heads, int kv_heads, int head_dim, int n, const int* membe
     for (int i = 0; i < n; i++) batch.push_back({members[3 * i], members[3 * i + 1], members[3 * i + 2]});
     plan_weigh(Shape{q_heads, kv_heads, head_dim}, batch, window, last, WeighRoom{stats, work}, plan);
     for (int k = 0; k <= SCORE_MANY; k++) sizes[k] = (int)plan.scores[k].size();
+    sizes[MERGES] = (int)plan.merges.size();
     for (int k = 0; k < 2; k++) sizes[SUM_FEW + k] = (int)plan.sums[k].size();
     sizes[FADES] = (int)plan.fades.size();
 }
@@ -37,6 +38,9 @@ void shim_scores(int list, int* out) {  // 12 ints each
 }
 void shim_sums(int list, int* out) {  // 16 ints each
     for (size_t i = 0; i < plan.sums[list].size(); i++) *(Sum*)(out + 16 * i) = plan.sums[list][i];
+}
+void shim_merges(int* out) {  // 8 ints each
+    for (size_t i = 0; i < plan.merges.size(); i++) *(Merge*)(out + 8 * i) = plan.merges[i];
 }
 void shim_fades(int* out) {  // 8 ints each
     for (size_t i = 0; i < plan.fades.size(); i++) *(Fade*)(out + 8 * i) = plan.fades[i];

@@ -31,20 +31,21 @@ def ints(xs):
 
 
 def weigh(L, kv, group, batch, window, last, stats, work):
-    sizes = ints([0] * 6)
+    sizes = ints([0] * 7)
     L.shim_weigh(kv * group, kv, 64, len(batch), ints([x for m in batch for x in m]), window, last, ctypes.c_longlong(stats),
                  ctypes.c_longlong(work), sizes)
-    scores, sums, fades = [], [], ints([0] * (8 * sizes[5]))
+    scores, sums, fades, merges = [], [], ints([0] * (8 * sizes[6])), ints([0] * (8 * sizes[3]))
     for k in range(3):
         buf = ints([0] * (12 * sizes[k]))
         L.shim_scores(k, buf)
-        scores.append([buf[12 * i:12 * i + 10] for i in range(sizes[k])])
+        scores.append([buf[12 * i:12 * i + 11] for i in range(sizes[k])])
     for k in range(2):
-        buf = ints([0] * (16 * sizes[3 + k]))
+        buf = ints([0] * (16 * sizes[4 + k]))
         L.shim_sums(k, buf)
-        sums.append([buf[16 * i:16 * i + 14] for i in range(sizes[3 + k])])
-    L.shim_fades(fades)
-    return scores, sums, [fades[8 * i:8 * i + 7] for i in range(sizes[5])]
+        sums.append([buf[16 * i:16 * i + 14] for i in range(sizes[4 + k])])
+    L.shim_fades(fades), L.shim_merges(merges)
+    return (scores, sums, [fades[8 * i:8 * i + 7] for i in range(sizes[6])],
+            [merges[8 * i:8 * i + 7] for i in range(sizes[3])])
 
 
 def covers(spans, lo, hi):
@@ -54,40 +55,55 @@ def covers(spans, lo, hi):
 
 
 def check(L, kv, group, batch, window, last, stats, work):
-    scores, sums, fades = weigh(L, kv, group, batch, window, last, stats, work)
+    scores, sums, fades, merges = weigh(L, kv, group, batch, window, last, stats, work)
     tokens = sum(c for _, c, _ in batch)
     most = L.shim_entries(kv * group, kv, max(tokens, 1), len(batch))
-    assert all(len(x) <= most for x in scores + sums + [fades])
+    assert all(len(x) <= most for x in scores + sums + [fades, merges])
     seqs, at = {}, 0
     for s, c, n in batch:
         m = min(last or c, c)
         at += c
         if m:
             seqs[s] = (at - m, m * group, n - m, n)  # first counted token, rows, its position, length
-    stat, pieces, spans, kept = {}, {}, {}, {}
+    stat, spans, kept, whole, weights, parts, pairs = {}, {}, {}, {}, {}, {}, {}
     for kind, items in enumerate(scores):
-        for seq, head, tok0, rows, row0, pos0, k0, k1, st, keep in items:
+        for seq, head, tok0, rows, row0, pos0, k0, k1, st, keep, final in items:
             assert (tok0, rows, pos0) == seqs[seq][:3] and k0 % 32 == 0 and 0 <= k0 <= k1 <= seqs[seq][3]
             assert (row0 == 0 and rows <= (16, 32)[kind] and keep >= 0 and k0 < k1) if kind < 2 else keep == -1
             for r in range(row0, min(row0 + 128, rows)):
                 i = st + r - row0
                 assert 0 <= i < stats and i not in stat
                 stat[i] = (seq, head, r)
+                if final:
+                    assert (seq, head, r) not in whole
+                    whole[seq, head, r] = i
+            if final and kind < 2:  # it takes its sums itself
+                weights.setdefault((seq, head), []).append((k0, k1))
+                pairs.setdefault((seq, head), []).append((k0, k1, 0, rows))
                 spans.setdefault((seq, head, r), []).append((k0, k1))
             if keep >= 0:
                 kept.setdefault((seq, head), []).append((keep, keep + (k1 - k0 + 31) // 32 * 32 * rows, k0))
+    by_tok0 = {v[0]: s for s, v in seqs.items()}
+    for head, tok0, rows, r0, r1, st, n in merges:
+        seq = by_tok0[tok0]
+        assert n > 1 and rows == seqs[seq][1] and 0 <= r0 < r1 <= rows
+        for r in range(r0, r1):
+            assert all(stat[st + p * rows + r] == (seq, head, r) for p in range(n)) and (seq, head, r) not in whole
+            whole[seq, head, r] = st + r
     for (seq, _, r), s in spans.items():
         pos = seqs[seq][2] + r // group
         assert covers(s, max(0, pos - window + 1) if window else 0, pos + 1)
     used = sorted((a, b) for v in kept.values() for a, b, _ in v)
     assert all(x[1] <= y[0] for x, y in zip(used, used[1:])) and (not used or (used[0][0] >= 0 and used[-1][1] <= work))
-    weights, parts, pairs = {}, {}, {}
     for kind, items in enumerate(sums):
         for seq, head, tok0, rows, pos0, k0, k1, r0, r1, st, n, sc, s0, part in items:
             assert (tok0, rows, pos0) == seqs[seq][:3] and 0 <= k0 < k1 <= seqs[seq][3] and k0 % 32 == 0
             assert (r0, r1) == (0, rows) if kind == 0 else r0 % 32 == 0 and 0 <= r0 <= rows and r1 <= rows
             for r in range(rows):
-                assert all(stat[st + p * rows + r] == (seq, head, r) for p in range(n))
+                if kind == 0:
+                    assert all(stat[st + p * rows + r] == (seq, head, r) for p in range(n))
+                else:  # the final ones
+                    assert whole[seq, head, r] == st + r
             if kind == 0:
                 for a, b, first in kept[seq, head]:  # the scores lie where they are read: block by block from s0
                     assert a == sc + (first - s0) * rows
