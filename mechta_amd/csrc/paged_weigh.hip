@@ -498,7 +498,7 @@ constexpr int CHANGES = 128;  // of a launch, in its arguments
 struct ChangeList {
     Change c[CHANGES];
 };
-constexpr int SPAN = 4096;  // positions of a work-group
+constexpr int SPAN = 4096;  // positions of a work-group, 16 a thread
 template <bool COPY>
 __global__ void __launch_bounds__(256) change_kernel(WeightsAt w, ChangeList list, int n, int spans, size_t all) {
     for (size_t i = blockIdx.x; i < all; i += gridDim.x) {  // (layer and head, change, span)
@@ -508,8 +508,17 @@ __global__ void __launch_bounds__(256) change_kernel(WeightsAt w, ChangeList lis
         const Change x = list.c[c];
         float* const p = w.p + w.at(layer, x.seq, head) + x.a;
         const float* const from = COPY ? w.p + w.at(layer, x.other, head) + x.a : nullptr;
-        const int end = min(x.count, (span + 1) * SPAN);
-        for (int j = span * SPAN + threadIdx.x; j < end; j += 256) p[j] = COPY ? from[j] : 0.f;
+        const int first = span * SPAN, end = min(x.count, first + SPAN);
+        if (x.a % 4 == 0 && end - first == SPAN) {  // whole, 16 bytes a time
+            f32x4 y[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) y[j] = COPY ? ((const f32x4*)(from + first))[threadIdx.x + 256 * j] : f32x4{};
+#pragma unroll
+            for (int j = 0; j < 4; j++) ((f32x4*)(p + first))[threadIdx.x + 256 * j] = y[j];
+        } else {
+#pragma unroll 4
+            for (int j = first + threadIdx.x; j < end; j += 256) p[j] = COPY ? from[j] : 0.f;
+        }
     }
 }
 
@@ -529,13 +538,15 @@ __device__ inline unsigned order_of(float x) {
     return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// The picks of one sequence, layer and head by a work-group: the least weight that stays, by four digits of eight bits from the
-// highest on, then the positions in order; of those with just that weight the first ones.
+// The picks of one sequence, layer and head by a work-group: the least weight that stays, by digits of 11, 11 and 10 bits from the
+// highest on, then the positions in order; of those with just that weight the first ones. 65,536 weights stay in registers from one
+// reading to the next, four neighbours a thread and 4,096; longer sequences are read again for each.
+constexpr int GROUP = 16, PICKED = 4096 * GROUP;
 __global__ void __launch_bounds__(1024) pick_kernel(WeightsAt w, EvictionList list, int n, int entry0, int first, int recent,
                                                     Eviction* __restrict__ entries, int* __restrict__ picks, size_t stride, int units) {
     // (at most EVICTIONS x 2^22 pairs of a sequence and a layer's head)
-    __shared__ int hist[256];
-    __shared__ int waves[16];
+    __shared__ int hist[2048];
+    __shared__ int waves[2][16];
     __shared__ int found[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     for (int b = blockIdx.x; b < n * units; b += gridDim.x) {
@@ -547,101 +558,142 @@ __global__ void __launch_bounds__(1024) pick_kernel(WeightsAt w, EvictionList li
         const int lo = first, hi = e.len - recent, want = e.keep - first - recent;
         for (int i = tid; i < first; i += 1024) to[i] = i;
         for (int i = tid; i < recent; i += 1024) to[e.keep - recent + i] = hi + i;
+        if (!want) continue;
+        unsigned v[GROUP][4];
+        auto bring = [&](int g0) INLINE {  // positions g0 .. g0 + PICKED - 1 (rows are whole runs of 32; what is not in [lo, hi) is not looked at)
+#pragma unroll
+            for (int t = 0; t < GROUP; t++) {
+                const int i = g0 + 4096 * t + 4 * tid;
+                if (g0 + 4096 * t >= hi) break;
+                f32x4 x = f32x4{};
+                if (i < hi) x = *(const f32x4*)(src + i);
+#pragma unroll
+                for (int y = 0; y < 4; y++) v[t][y] = order_of(x[y]);
+            }
+        };
         unsigned known = 0, mask = 0;  // the digits of the least weight that stays
         int left = want;               // of those that have them
-        for (int digit = 24; digit >= 0 && want; digit -= 8) {
+        bring(0);
+        for (int shift = 21; shift >= 0; shift = shift ? max(0, shift - 11) : -1) {  // 21, 10, 0: of 11, 11 and 10 bits
+            const unsigned digit = shift ? 2047 : 1023;
             __syncthreads();
-            if (tid < 256) hist[tid] = 0;
+            hist[tid] = hist[tid + 1024] = 0;
             __syncthreads();
-            for (int i = lo + tid; i < hi; i += 1024) {
-                const unsigned k = order_of(src[i]);
-                if ((k & mask) == known) atomicAdd(&hist[k >> digit & 255], 1);
-            }
-            __syncthreads();
-            if (tid < 64) {  // from the highest digit down: lane l has digits 255 - 4 l .. 252 - 4 l
-                int mine[4], sum = 0;
+            for (int g0 = 0; g0 < hi; g0 += PICKED) {
+                if (hi > PICKED) bring(g0);
 #pragma unroll
-                for (int x = 0; x < 4; x++) sum += mine[x] = hist[255 - 4 * lane - x];
-                int before = sum;
+                for (int t = 0; t < GROUP; t++) {
+                    if (g0 + 4096 * t >= hi) break;
 #pragma unroll
-                for (int x = 1; x < 64; x *= 2) {
-                    const int y = __shfl_up(before, x);
-                    if (lane >= x) before += y;
-                }
-                before -= sum;
-#pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    if (before < left && before + mine[x] >= left) {
-                        found[0] = 255 - 4 * lane - x;
-                        found[1] = left - before;
+                    for (int y = 0; y < 4; y++) {
+                        const int i = g0 + 4096 * t + 4 * tid + y;
+                        const bool is = i >= lo && i < hi && (v[t][y] & mask) == known;
+                        const unsigned at = v[t][y] >> shift & digit;
+                        const unsigned long long active = __ballot(is);
+                        if (!active) continue;
+                        // (weights that are all alike, those of new positions for one, would queue up for one address)
+                        const unsigned one = __builtin_amdgcn_readlane(at, __builtin_ctzll(active));
+                        if (__ballot(is && at == one) == active) {
+                            if (lane == 0) atomicAdd(&hist[one], __popcll(active));
+                        } else if (is) {
+                            atomicAdd(&hist[at], 1);
+                        }
                     }
-                    before += mine[x];
                 }
             }
             __syncthreads();
-            known |= (unsigned)found[0] << digit;
-            mask |= 255u << digit;
-            left = found[1];
-        }
-        // left: how many of those with just the least weight stay
-        int more = 0, same = 0;  // before the tile: heavier ones, ones of the least weight
-        for (int i0 = lo; i0 < hi && want; i0 += 4096) {
-            unsigned k[4];
-            int mine = 0;  // (heavier) + (same) << 16
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const int i = i0 + 4 * tid + x;
-                k[x] = i < hi ? order_of(src[i]) : 0;
-                if (i < hi) mine += k[x] > known ? 1 : k[x] == known ? 1 << 16 : 0;
-            }
-            int before = mine;
+            // from the highest digit down: thread t has digits 2047 - 2 t and 2046 - 2 t
+            const int h0 = hist[2047 - 2 * tid], h1 = hist[2046 - 2 * tid];
+            int before = h0 + h1;
 #pragma unroll
             for (int x = 1; x < 64; x *= 2) {
                 const int y = __shfl_up(before, x);
                 if (lane >= x) before += y;
             }
+            if (lane == 63) waves[0][wave] = before;
             __syncthreads();
-            if (lane == 63) waves[wave] = before;
+            before -= h0 + h1;
+#pragma unroll
+            for (int x = 0; x < 15; x++) {
+                const int y = waves[0][x];
+                if (x < wave) before += y;
+            }
+            if (before < left && before + h0 >= left) {
+                found[0] = 2047 - 2 * tid;
+                found[1] = left - before;
+            } else if (before + h0 < left && before + h0 + h1 >= left) {
+                found[0] = 2046 - 2 * tid;
+                found[1] = left - before - h0;
+            }
             __syncthreads();
-            int all = 0;
-            before -= mine;
-#pragma unroll
-            for (int x = 0; x < 16; x++) {
-                if (x < wave) before += waves[x];
-                all += waves[x];
-            }
-            int m = more + (before & 0xFFFF), s = same + (before >> 16);
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const int i = i0 + 4 * tid + x;
-                if (i >= hi) break;
-                if (k[x] > known) to[first + m++ + min(s, left)] = i;
-                else if (k[x] == known) {
-                    if (s < left) to[first + m + s] = i;
-                    s++;
-                }
-            }
-            more += all & 0xFFFF;
-            same += all >> 16;
+            known |= (unsigned)found[0] << shift;
+            mask |= digit << shift;
+            left = found[1];
         }
-        __syncthreads();
+        // left: how many of those with just the least weight stay
+        int more = 0, same = 0;  // before the tile: heavier ones, ones of the least weight
+        for (int g0 = 0; g0 < hi; g0 += PICKED) {
+            if (hi > PICKED) bring(g0);
+#pragma unroll
+            for (int t = 0; t < GROUP; t++) {
+                if (g0 + 4096 * t >= hi) break;
+                const int i0 = g0 + 4096 * t + 4 * tid;
+                int mine = 0;  // (heavier) + (same) << 16
+#pragma unroll
+                for (int y = 0; y < 4; y++)
+                    if (i0 + y >= lo && i0 + y < hi) mine += v[t][y] > known ? 1 : v[t][y] == known ? 1 << 16 : 0;
+                int before = mine;
+#pragma unroll
+                for (int x = 1; x < 64; x *= 2) {
+                    const int y = __shfl_up(before, x);
+                    if (lane >= x) before += y;
+                }
+                if (lane == 63) waves[t % 2][wave] = before;
+                __syncthreads();  // (one a tile: the other half of `waves` was read before the one before)
+                int all = 0;
+                before -= mine;
+#pragma unroll
+                for (int x = 0; x < 16; x++) {
+                    const int y = waves[t % 2][x];
+                    if (x < wave) before += y;
+                    all += y;
+                }
+                int m = more + (before & 0xFFFF), s = same + (before >> 16);
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    const int i = i0 + y;
+                    if (i < lo || i >= hi) continue;
+                    if (v[t][y] > known) to[first + m++ + min(s, left)] = i;
+                    else if (v[t][y] == known) {
+                        if (s < left) to[first + m + s] = i;
+                        s++;
+                    }
+                }
+                more += all & 0xFFFF;
+                same += all >> 16;
+            }
+            __syncthreads();
+        }
     }
 }
 
 // A new page's block of 32 positions of a head and layer, K or V: 16 bytes of K a thread (8 dims of a position), 16 bytes of V
-// (a dim of 8 positions, which come from 8 places). Positions behind the last that stays are left as they were.
+// (a dim of 8 positions, which come from 8 places), all on their way at once; `parts` work-groups share a block's dims where blocks are
+// few. Positions behind the last that stays are left as they were. Bound by memory, which gives whole lines: 128 bytes are 8
+// positions of 8 dims of K, or 8 dims of 8 positions of V, so that of a sequence cut to a quarter nearly all lines are read.
 template <int D>
 __global__ void __launch_bounds__(256) gather_kernel(unsigned short* __restrict__ pool, const int* __restrict__ table, int most_pages,
                                                      int page, int kv_heads, int units, size_t plane,
                                                      const Eviction* __restrict__ entries, const int* __restrict__ picks,
-                                                     size_t stride, PageList list) {
+                                                     size_t stride, int parts, PageList list) {
+    constexpr int ROUNDS = D / 64;  // of 256 units of 16 bytes
     __shared__ size_t from[KEYS];
     __shared__ int in[KEYS];
     typedef Vec8<unsigned short> Unit;
     const int tid = threadIdx.x, blocks = page / KEYS;
     const NewPage np = list.p[blockIdx.x / blocks];
-    const int block = blockIdx.x % blocks;
-    const bool is_v = blockIdx.z;
+    const int block = blockIdx.x % blocks, part = blockIdx.z / 2;
+    const bool is_v = blockIdx.z % 2;
     const Eviction e = entries[np.entry];
     const int p0 = np.nth * page + block * KEYS, count = min(KEYS, e.keep - p0);
     if (count <= 0) return;
@@ -657,41 +709,50 @@ __global__ void __launch_bounds__(256) gather_kernel(unsigned short* __restrict_
         __syncthreads();
         unsigned short* const to = base + ((size_t)np.page * kv_heads + head) * page * D + (size_t)block * KEYS * D;
         if (!is_v) {
-            for (int i = tid; i < KEYS * D / 8; i += 256) {
-                const int x = i % KEYS, c = i / KEYS;
-                if (x >= count) continue;
-                const int y = in[x];
-                *(Unit*)(to + x / 16 * 16 * D + c * 128 + x % 16 * 8) = *(const Unit*)(base + from[x] + y / 16 * 16 * D + c * 128 + y % 16 * 8);
-            }
+            const int x = tid % KEYS;
+            if (x >= count) continue;
+            const int y = in[x];
+            const unsigned short* const s = base + from[x] + y / 16 * 16 * D + y % 16 * 8;
+            unsigned short* const t = to + x / 16 * 16 * D + x % 16 * 8;
+            Unit u[ROUNDS];
+#pragma unroll
+            for (int i = 0; i < ROUNDS; i++)
+                if (i % parts == part) u[i] = *(const Unit*)(s + (tid / KEYS + 8 * i) * 128);
+#pragma unroll
+            for (int i = 0; i < ROUNDS; i++)
+                if (i % parts == part) *(Unit*)(t + (tid / KEYS + 8 * i) * 128) = u[i];
             continue;
         }
-        for (int i = tid; i < 4 * D; i += 256) {
-            const int g = i / D, d = i % D;
-            Unit u;
-            bool whole = true;
+        // (a round is 256 units: of heads of 256 one group of positions, of 128 two, of 64 all four)
+        Unit u[ROUNDS];
+#pragma unroll
+        for (int i = 0; i < ROUNDS; i++) {
+            if (i % parts != part) continue;
+            const int g = (tid + 256 * i) / D, d = (tid + 256 * i) % D;
 #pragma unroll
             for (int z = 0; z < 8; z++) {
-                const int x = 16 * (z / 4) + 4 * g + z % 4;
-                if (x < count) {
-                    const int y = in[x];
-                    u[z] = base[from[x] + (y % 16 / 4 * D + d) * 8 + y / 16 * 4 + y % 4];
-                } else {
-                    whole = false;
-                }
+                const int x = min(16 * (z / 4) + 4 * g + z % 4, count - 1), y = in[x];
+                u[i][z] = base[from[x] + (y % 16 / 4 * D + d) * 8 + y / 16 * 4 + y % 4];
             }
-            unsigned short* const o = to + i * 8;
-            if (whole) {
-                *(Unit*)o = u;
+        }
+#pragma unroll
+        for (int i = 0; i < ROUNDS; i++) {
+            if (i % parts != part) continue;
+            const int g = (tid + 256 * i) / D;
+            unsigned short* const o = to + (tid + 256 * i) * 8;
+            if (16 + 4 * g + 3 < count) {
+                *(Unit*)o = u[i];
             } else {
 #pragma unroll
                 for (int z = 0; z < 8; z++)
-                    if (16 * (z / 4) + 4 * g + z % 4 < count) o[z] = u[z];
+                    if (16 * (z / 4) + 4 * g + z % 4 < count) o[z] = u[i][z];
             }
         }
     }
 }
 
-// The weights that stay, in place: a position's goes to one that is not behind it, tile by tile.
+// The weights that stay, in place: a position's goes to one that is not behind it, 16,384 at a time.
+constexpr int PACKED = 16;
 __global__ void __launch_bounds__(1024) pack_kernel(WeightsAt w, const Eviction* __restrict__ entries, const int* __restrict__ picks,
                                                     size_t stride, int n, int units) {
     for (size_t b = blockIdx.x; b < (size_t)n * units; b += gridDim.x) {
@@ -699,20 +760,20 @@ __global__ void __launch_bounds__(1024) pack_kernel(WeightsAt w, const Eviction*
         const Eviction e = entries[b / units];
         float* const p = w.p + w.at(unit / w.kv_heads, e.seq, unit % w.kv_heads);
         const int* const from = picks + (size_t)unit * stride + e.off;
-        for (int i0 = 0; i0 < e.keep; i0 += 4096) {
-            float x[4];
+        // What a tile takes lies in it or behind it: it has been read when the tile is written, and tiles are on their way together.
+        for (int i0 = 0; i0 < e.keep; i0 += 1024 * PACKED) {
+            float x[PACKED];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int i = i0 + threadIdx.x + 1024 * j;
+            for (int j = 0; j < PACKED; j++) {
+                const int i = i0 + (int)threadIdx.x + 1024 * j;
                 x[j] = i < e.keep ? p[from[i]] : 0.f;
             }
             __syncthreads();
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int i = i0 + threadIdx.x + 1024 * j;
+            for (int j = 0; j < PACKED; j++) {
+                const int i = i0 + (int)threadIdx.x + 1024 * j;
                 if (i < e.keep) p[i] = x[j];
             }
-            __syncthreads();
         }
     }
 }
@@ -810,8 +871,10 @@ hipError_t launch_gather(const Geometry& g, char* pool, const int* table, const 
         const int m = std::min(NEW_PAGES, n - i);
         for (int j = 0; j < NEW_PAGES; j++) list.p[j] = j < m ? pages[i + j] : NewPage{0, 0, 0};
         const int units = g.layers * g.kv_heads;
-        kernel<<<dim3(m * (g.page / KEYS), std::min(units, 1024), 2), dim3(256), 0, s>>>(
-            (unsigned short*)pool, table, g.most_pages, g.page, g.kv_heads, units, g.plane_elems(), entries, picks, stride, list);
+        const long long groups = (long long)n * (g.page / KEYS) * units * 2;
+        const int parts = groups >= 2048 ? 1 : std::min(g.head_dim / 64, groups >= 1024 ? 2 : 4);
+        kernel<<<dim3(m * (g.page / KEYS), std::min(units, 1024), 2 * parts), dim3(256), 0, s>>>(
+            (unsigned short*)pool, table, g.most_pages, g.page, g.kv_heads, units, g.plane_elems(), entries, picks, stride, parts, list);
         if (const hipError_t err = hipGetLastError()) return err;
     }
     return hipSuccess;

@@ -235,7 +235,7 @@ static int evict(mpg_t* h, int n, const int* seq, const int* keep, int first, in
         if (keep[i] < 1 || (long long)first + recent > keep[i])
             return fail(MKV_E_ARG, "%s: %d positions kept, %d first and %d last ones among them", who, keep[i], first, recent);
     if (int rc = h->book.can_evict(who, n, seq, keep)) return rc;
-    // The device finds the rows that stay by the pages that the sequences have now, and learns of the new ones last.
+    // the device finds the rows that stay by the pages that the sequences have now
     if (const int rc = end_batch(h, who)) return rc;
     if (const int rc = upload_tables(h, who)) return rc;
     std::vector<Evicted> cut;
@@ -258,9 +258,8 @@ static int evict(mpg_t* h, int n, const int* seq, const int* keep, int first, in
         if (err == hipSuccess)
             err = launch_gather(h->g, h->pool, h->dev, k->entries, k->picks, stride, pages.data(), (int)pages.size(), h->stream);
         if (err != hipSuccess) return hip_fail(err, who);
-        // the old pages have been read: the new tables may go up. The weights move last, in one launch: whatever fails
-        // before it leaves them as they were.
-        if (const int rc = upload_tables(h, who)) return rc;
+        // The weights move last, in one launch: whatever fails before it leaves them as they were. (The new tables go up when the
+        // device next needs them.)
         err = launch_pack(k->at, k->entries, (int)e.size(), k->picks, stride, h->stream);
         return err == hipSuccess ? (int)MKV_OK : hip_fail(err, who);
     };
