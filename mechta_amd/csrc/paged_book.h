@@ -157,7 +157,7 @@ size_t most_joins(const Shape& g, int tokens, int seqs);
 struct Score {  // rows row0 .. of one kv head against keys [k0, k1): the reference and the sum of each to stats[stat ..]
     int seq, head, tok0, rows, row0, pos0;  // tok0, pos0: the first counted token and its position
     int k0, k1, stat;
-    int keep;        // few rows: where the scores go in the work space, by blocks of KEYS keys [row][key]
+    int keep;        // few rows: where the scores go in the work space, 16 keys behind 16 keys, [row][key]
     int whole;       // there is no other piece: many rows: what goes to stats is final; few: the sums are taken at once
     int pad;
 };

@@ -107,16 +107,16 @@ __device__ inline void sum_kept(const Args& a, int seq, int head, int pos0, int 
     float* const weights = a.weights + seq * a.seq_stride + head * a.stride;
     for (int key = k0 + (int)threadIdx.x; key < k1; key += 256) {
         const int i = key - s0;
-        const float* const s = a.work + scores + (size_t)(i / KEYS) * KEYS * rows + i % KEYS;
+        const float* const s = a.work + scores + (size_t)(i / 16) * 16 * rows + i % 16;
         const float was = a.decay == 0.f ? 0.f : a.decay * weights[key];
         float sum = 0.f;
 #pragma unroll 8
-        for (int r = 0; r < there; r++) sum += fast_exp2(s[r * KEYS] - f[r].x) * f[r].y;
+        for (int r = 0; r < there; r++) sum += fast_exp2(s[r * 16] - f[r].x) * f[r].y;
         if (odd) {
             sum = 0.f;
             for (int r = 0; r < there; r++) {
                 const int pos = pos0 + r / a.group;
-                if (key <= pos && (!a.window || key > pos - a.window)) sum += fast_exp2(s[r * KEYS] - f[r].x) * f[r].y;
+                if (key <= pos && (!a.window || key > pos - a.window)) sum += fast_exp2(s[r * 16] - f[r].x) * f[r].y;
             }
         }
         weights[key] = was + sum;
@@ -189,8 +189,8 @@ __global__ void __launch_bounds__(256) score_few(Args a, const Score* __restrict
                 add_scores(ml[t], x);
                 const int row = 16 * t + r;
                 if (row < it.rows) {
-                    *(f32x4*)(to + row * KEYS + 4 * g) = f32x4{x[0], x[1], x[2], x[3]};
-                    *(f32x4*)(to + row * KEYS + 16 + 4 * g) = f32x4{x[4], x[5], x[6], x[7]};
+                    *(f32x4*)(to + row * 16 + 4 * g) = f32x4{x[0], x[1], x[2], x[3]};
+                    *(f32x4*)(to + (it.rows + row) * 16 + 4 * g) = f32x4{x[4], x[5], x[6], x[7]};
                 }
             }
         }
