@@ -775,7 +775,8 @@ struct Segs {  // of a join; one that it does not have has no splits
         return (size_t)(part + s * stride + r);
     }
 };
-template <typename T, int D>
+// SHARED: there may be such (0.5 us more for the joins of a batch that has none).
+template <typename T, int D, bool SHARED>
 __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restrict__ joins, const int* __restrict__ njoins,
                                                    const Seg* __restrict__ segs) {
     __shared__ float factor[SPLITS_MOST];
@@ -792,7 +793,7 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
     for (int n = blockIdx.x / ways; n < count; n += gridDim.x / ways) {
         const Uniform<int> ji = uniform((const int*)(joins + n));
         const Join j{ji[0], ji[1], ji[2], ji[3], ji[4], ji[5], ji[6], ji[7]};
-        const Segs shared(segs + (size_t)n * LEVELS, j.segs);
+        const Segs shared(segs + (size_t)n * LEVELS, SHARED ? j.segs : 0);
         if (!j.wide) {
             constexpr int LANES = D / 4, GROUPS = 256 / LANES;
             const int d = tid % LANES * 4;
@@ -838,14 +839,14 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
                 four(j.part, j.count, j.splits, 0, false);
                 for (int s = 4; s < j.splits; s += 4) four(j.part, j.count, j.splits, s, true);
 #pragma unroll
-                for (int i = 0; i < LEVELS; i++)
+                for (int i = 0; i < (SHARED ? LEVELS : 0); i++)
                     for (int s = 0; s < shared.x[i].splits; s += 4) four(shared.x[i].part, shared.x[i].stride, shared.x[i].splits, s, true);
                 finish(tok, j.head * a.group + row % a.group, d, acc, top, total);
             }
             continue;
         }
         const int splits = j.splits + shared.splits;
-        if (j.wide == ROW_WIDE) {
+        if (SHARED && j.wide == ROW_WIDE) {
             constexpr int LANES = D / 4, GROUPS = 256 / LANES;
             const int group = tid / LANES, lane = tid % LANES;
             for (int r = way; r < j.count; r += ways) {
@@ -918,7 +919,7 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restric
             const int row = j.row0 + r, tok = j.tok0 + row / a.group;
             if (tok >= a.rows) continue;
             const size_t first = j.part + r;
-            auto partial = [&](int s) INLINE { return s < j.splits ? first + (size_t)s * j.count : shared.row(s - j.splits, r); };
+            auto partial = [&](int s) INLINE { return !SHARED || s < j.splits ? first + (size_t)s * j.count : shared.row(s - j.splits, r); };
             float top = NEG_INF;
             for (int s = tid; s < splits; s += 256) top = fmaxf(top, a.pm[partial(s)]);
             // the first splits' values are on their way meanwhile
@@ -1019,7 +1020,8 @@ hipError_t attend_as(const Geometry& g, const AttendArgs& x, const int* batch, c
                 ways = std::max(ways, j.wide == ROW_WIDE ? j.count : j.wide ? j.count * (D / JOIN_DIMS) : (j.count + groups - 1) / groups);
             }
         const int all = std::min(join_grid, MOST_GRID / ways) * ways;
-        join_kernel<T, D><<<dim3(all), dim3(256), 0, s>>>(a, (const Join*)(batch + l.joins), batch + KINDS, (const Seg*)(batch + l.segs));
+        const auto kernel = x.shared ? join_kernel<T, D, true> : join_kernel<T, D, false>;
+        kernel<<<dim3(all), dim3(256), 0, s>>>(a, (const Join*)(batch + l.joins), batch + KINDS, (const Seg*)(batch + l.segs));
         e = hipGetLastError();
     }
     return e;

@@ -57,6 +57,7 @@ struct AttendArgs {
     const Place* order;              // the tokens of shared tiles
     const std::vector<Join>* joins;  // the plan's, for the launch's shape
     bool captured;                   // a captured launch serves any plan
+    bool shared;                     // joins may have splits of shared keys
 };
 // grid[kind] work-groups for each kind of item (0: not launched), joins likewise; lists and counts on the device.
 hipError_t launch_attend(const Geometry& g, const AttendArgs& a, const int* batch, const Lists& l, const int* grid,

@@ -620,6 +620,7 @@ int mpg_attend(mpg_t* h, int layer, int rows, const void* q, int64_t q_tok, int6
     a.order = (const Place*)(h->dev + h->order_at);
     a.joins = &p.joins;
     a.captured = cap != 0;
+    a.shared = cap || !p.segs.empty();
     int grid[KINDS];
     for (int k = 0; k < KINDS; k++)
         grid[k] = cap ? (k < HALF ? GRAPH_GRID : GRAPH_CHUNKS) : (int)std::min<size_t>(p.items[k].size(), MOST_GRID);
