@@ -182,7 +182,7 @@ int mpg_attend(mpg_t* h, int layer, int rows, const void* q, int64_t q_tok, int6
 /* Device bytes that mpg_keep_weights allocates for a handle of this configuration (0 if it would refuse). */
 size_t mpg_weights_bytes(const mpg_config* c, int last);
 /* From here on the handle keeps weights: of each sequence of a batch, mpg_weigh counts the `last` last new tokens (0: all).
- * Before the handle's first positions and its first batch; it waits for the stream. */
+ * Before the handle's first mpg_reserve or mpg_begin; it waits for the stream. */
 int mpg_keep_weights(mpg_t* h, int last);
 /* Device address of a layer's weights: of (sequence, kv head, position) at sequence x *seq_stride + head x *head_stride +
  * position. A caller may write those of a sequence's positions, in order with the handle's stream. */

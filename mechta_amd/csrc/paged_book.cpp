@@ -741,7 +741,7 @@ void draft(const Shape& g, const std::vector<Member>& batch, const Share* share,
 }
 
 // What a draft takes, where sequences have keys in common.
-double cost_of(const Shape& g, const Share& share, int window, const std::vector<Member>& batch, const Draft& d) {
+double cost_of(const Shape& g, const Share& share, const Draft& d) {
     double distinct[KINDS] = {};  // keys of the lists for few rows, what several tiles have counted once
     for (int k : {FEW, SOME}) {
         std::vector<char> seen(share.ranges.size(), 0);
@@ -778,11 +778,11 @@ static void plan(const Shape& g, const std::vector<Member>& batch, const Share* 
     Draft best;
     draft(g, batch, share, window, APART, best);
     if (share) {
-        best.cost = cost_of(g, *share, window, batch, best);
+        best.cost = cost_of(g, *share, best);
         for (Way way : {STREAMED, TILED}) {
             Draft d;
             draft(g, batch, share, window, way, d);
-            d.cost = cost_of(g, *share, window, batch, d);
+            d.cost = cost_of(g, *share, d);
             if (d.cost < best.cost) best = std::move(d);
         }
     }

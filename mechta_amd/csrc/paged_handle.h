@@ -59,7 +59,7 @@ struct mpg_store {
     int nruns = 0, longest = 0;     // its runs, and the tokens of the longest
     bool listed = false;            // the lists on the device are a batch's: replays would do it
     std::vector<mkv::paged::Plan> plans, next;  // per window, of the batch and of the one that is being laid out
-    bool begun = false;             // a batch has stood: captured calls may hold the handle's addresses
+    bool used = false;              // sequences have had positions: captured calls may hold the handle's addresses
     size_t shift_at = 0;            // word offset in dev of the sequences' evicted positions; 0: nothing is ever evicted
     std::unique_ptr<mkv::paged::Weights> weights;  // none: the handle keeps no weights
 };

@@ -438,6 +438,7 @@ int mpg_reserve(mpg_t* h, int n, const int* seq, const int* count) {
     MPG_HOST_CALL(h, "mpg_reserve");
     return guarded("mpg_reserve", [&] {
         if (int rc = h->book.reserve("mpg_reserve", n, seq, count)) return rc;
+        h->used = true;
         return settle(
             h, {}, "mpg_reserve", [&] { h->book.undo_reserve(n, seq, count); }, [&] { return clear_new(h, n, seq, count, "mpg_reserve"); });
     });
@@ -472,7 +473,6 @@ static int lay_out(mpg_t* h, int n, const int* seq, const int* count, bool share
     }
     if (int rc = upload(h, &runs, &h->next, &common.order, who)) return rc;
     if (h->weights) h->weights->stands();
-    h->begun = true;
     h->listed = true;
     h->plans.swap(h->next);
     h->tokens = tok;
@@ -489,6 +489,7 @@ static int begin(mpg_t* h, int n, const int* seq, const int* count, int* tokens,
         if (sum > h->c.tokens)
             return fail(MKV_E_ARG, "%s: %lld tokens, the handle's batches have at most %d", who, sum, h->c.tokens);
         if (int rc = h->book.reserve(who, n, seq, count)) return rc;
+        h->used = true;
         try {
             const int rc = lay_out(h, n, seq, count, shared, who);
             if (rc) h->book.undo_reserve(n, seq, count);

@@ -124,9 +124,7 @@ size_t mpg_weights_bytes(const mpg_config* c, int last) {
 static int keep_weights(mpg_t* h, int last) {
     if (int rc = check_last("mpg_keep_weights", last)) return rc;
     if (h->weights) return fail(MKV_E_ARG, "mpg_keep_weights: the handle keeps them already");
-    if (h->begun) return fail(MKV_E_ARG, "mpg_keep_weights: before the handle's first batch");
-    for (int n : h->book.len)
-        if (n) return fail(MKV_E_ARG, "mpg_keep_weights: before the sequences have positions");
+    if (h->used) return fail(MKV_E_ARG, "mpg_keep_weights: sequences have had positions already");
     const mpg_config& c = h->c;
     const WeightSizes s = weight_sizes(c, last);
     const double all = bytes_of(s, c);
@@ -163,7 +161,6 @@ static int keep_weights(mpg_t* h, int last) {
     h->shift_at = h->words + s.l.words * MPG_WINDOWS_MAX;
     h->words = words;
     h->g.shift = dev + h->shift_at;
-    std::fill(h->book.fresh.begin(), h->book.fresh.end(), 0);
     h->weights = std::move(k);
     return MKV_OK;
 }

@@ -358,7 +358,7 @@ class PagedKv:
         """Cuts each of the sequences that is longer to `keep` positions (a number, or one for each): its `first` first and
         `recent` last ones and, for each layer and K/V head by itself, those of the largest weights between them."""
         a, ap = _ints(seqs)
-        b, bp = _ints([keep] * len(a) if isinstance(keep, int) else keep, len(a), "keep")
+        b, bp = _ints(keep if hasattr(keep, "__iter__") else [keep] * len(a), len(a), "keep")
         _check(self._lib.mpg_evict(self._h, len(a), ap, bp, _int(first, "first"), _int(recent, "recent")))
 
     def weights(self, layer):
