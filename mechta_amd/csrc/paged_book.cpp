@@ -319,7 +319,7 @@ constexpr int LEAST_KEYS = 128;  // of a piece: a tile for each wave of few rows
 // Pieces of a kind's tiles: about as many as CUs. Few rows stream fastest from 216 work-groups (1 token at 131,072
 // positions of 2 x 256: 128 / 192 / 216 / 240 / 256 / 512 of them 59.1 / 51.4 / 51.3 / 52.0 / 52.6 / 59.8 us; 64 sequences of 4 x 128 at
 // 3,000: 256 / 512 / 768 64.1 / 69.5 / 71.9) -- or from 256 where 216 would leave a quarter of them without work.
-constexpr int CUS = 256, STREAMS = 216;
+constexpr int STREAMS = 216;
 // Few rows that none of the tiles is worth a join for: 512 keys of 64 or 128 dims, 256 of 256. (Whole / split, us: a token of
 // 4 x 128 at 400 / 513 / 700 positions 5.8, 6.1, 8.9 / 6.9, 6.9, 7.6; of 12 sequences 9.1, 9.2, 11.6 / 9.1, 9.5, 11.0; of
 // 2 x 256 at 200 / 300 / 400 9.1, 10.9, 12.7 / 10.0, 9.7, 9.5; of 12 9.7, 11.8, 13.6 / 11.1, 11.5, 11.8.)
@@ -930,7 +930,7 @@ void plan_weigh(const Shape& g, const std::vector<Member>& batch, int window, in
         const long long blocks = (m.len - k0 + KEYS - 1) / KEYS, kept = blocks * KEYS * rows * heads;
         rows_left += (long long)rows * heads;
         Weighed w{m.seq, tok0, rows, pos0, k0, m.len, -1};
-        if (rows <= TILE_ROWS[SOME] && work + kept <= room.work) {
+        if (rows <= TILE_ROWS[SOME] && work + kept <= room.work - WEIGH_PARTS) {
             w.scores = (int)work;
             work += kept;
             few_keys += (long long)(m.len - k0) * heads;
@@ -988,7 +988,6 @@ void plan_weigh(const Shape& g, const std::vector<Member>& batch, int window, in
     // Many rows: bound by the matrix units and the exponentials. Tiles of rows against all their keys, split where they are few.
     more = 0;
     constexpr int PLACES = 2 * CUS;
-    constexpr int SUM_PLACES = 6 * CUS - 64;
     const long long many_length = std::max<long long>(LEAST_KEYS, (tile_keys + PLACES - 1) / PLACES) / KEYS;
     long long key_tiles = 0, row_tiles = 0;
     for (const Weighed& w : many) {

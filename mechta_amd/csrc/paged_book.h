@@ -188,6 +188,9 @@ struct WeighRoom {
 };
 constexpr int SCORE_ROWS = 128, SUM_KEYS = 256;  // of a tile: rows of SCORE_MANY, keys of SUM_MANY
 constexpr int WEIGH_MOST = 4096;                 // entries of a list at most, besides one for each tile of SCORE_ROWS or sequence, and head
+constexpr int CUS = 256;
+constexpr int SUM_PLACES = 6 * CUS - 64;         // work-groups that take many rows' sums, about
+constexpr int WEIGH_PARTS = (SUM_PLACES + WEIGH_MOST) * SUM_KEYS;  // floats of the room: those sums' parts, which always find room
 size_t weigh_entries(const Shape& g, int tokens, int seqs);
 void plan_weigh(const Shape& g, const std::vector<Member>& batch, int window, int last, const WeighRoom& room, WeighPlan& out);
 

@@ -15,7 +15,7 @@ namespace {
 
 // Work-groups of a captured weighing, of whatever batch it finds.
 constexpr int GRAPH_WEIGH = 1024;
-constexpr long long WORK_MOST = 1ll << 26;  // floats: kept scores and partial sums
+constexpr long long WORK_MOST = 1ll << 28;  // floats: kept scores
 constexpr long long STATS_MORE = 1ll << 18;  // statistics of rows in more than one piece
 
 struct Kept : Weights {
@@ -89,8 +89,10 @@ WeightSizes weight_sizes(const mpg_config& c, int last) {
     s.weights = (size_t)c.layers * c.seqs * c.kv_heads * s.stride;
     const long long counted = last ? std::min((long long)c.tokens, (long long)std::min(c.seqs, c.tokens) * last) : c.tokens;
     s.stats = counted * c.q_heads + STATS_MORE;  // (and a tile of rows behind: the last is read whole)
-    // scores of up to 32 rows of every position of the pool, as far as that is not too much
-    s.work = (size_t)std::min<double>(WORK_MOST, 32. * c.pages * c.page * c.kv_heads);
+    // Scores of a token of each sequence, however many of them share their pages, and of up to 32 rows of every position of the pool,
+    // as far as that is not too much; what finds no room is scored twice.
+    s.work = (size_t)(std::min<double>(WORK_MOST, std::max(32. * c.pages * c.page * c.kv_heads,
+                                                           (double)s.stride * std::min(c.seqs, c.tokens) * c.q_heads)) + WEIGH_PARTS);
     s.picks = (size_t)c.layers * c.kv_heads * c.pages * c.page;
     const Shape g{c.q_heads, c.kv_heads, c.head_dim};
     const size_t entries = weigh_entries(g, c.tokens, c.seqs);

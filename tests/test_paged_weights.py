@@ -153,6 +153,16 @@ def test_large_batches_stay_inside_their_lists(shim):
         check(shim, kv, group, batch, 0, last, tokens * kv * group + (1 << 18), 1 << 26)
 
 
+@pytest.mark.parametrize("more", [0, 5000, 200000, 3000000])
+def test_parts_of_sums_find_room_behind_the_scores(shim, more):
+    for kv, group, prompt in [(4, 8, 4096), (2, 4, 700), (1, 1, 3000)]:
+        batch = [(s, 1 + s % 3, 900 + 410 * s) for s in range(20)] + [(30, prompt, prompt + 100)]
+        tokens = sum(c for _, c, _ in batch)
+        scores, sums, fades, kept = check(shim, kv, group, batch, 0, 0, tokens * kv * group + 1000, shim.shim_parts() + more)
+        assert all(end <= more for _, end in kept)  # scores stay in the room that is theirs
+        assert any(f[5] > 1 for f in fades)  # and sums are split
+
+
 # ---- eviction in the book ----
 
 class Book:
