@@ -731,7 +731,7 @@ __global__ void __launch_bounds__(512) chunk_rows(Args a, const Item* __restrict
             if (kg == 0) finish_rows(low);
             else finish_rows(high);
         }
-        if (it.part >= 0 && kg == 0 && h == 0 && row <= last_row) {
+        if (it.part >= 0 && kg == 0 && h == 0 && is) {
             a.pm[it.part + 32 * wr + r] = m;
             a.pl[it.part + 32 * wr + r] = l;
         }
@@ -775,195 +775,202 @@ struct Segs {  // of a join; one that it does not have has no splits
         return (size_t)(part + s * stride + r);
     }
 };
-// SHARED: there may be such (0.5 us more for the joins of a batch that has none).
+// SHARED: the join may have such.
+template <typename T, int D, bool SHARED>
+__device__ __forceinline__ void join_rows(const Args& a, const Join& j, const Seg* segs, int way, int ways, float (&factor)[SPLITS_MOST],
+                                          f32x4 (&sa)[16][16], float (&red)[2][4]) {
+    const int tid = threadIdx.x;
+    auto finish = [&](int tok, int head, int d, f32x4 acc, float m, float l) INLINE {
+        acc *= row_factor(a, head, m, l);
+        const float x[4] = {acc[0], acc[1], acc[2], acc[3]};
+        store_out<T, D, 4>(a, tok, head, d, x);
+    };
+    const Segs shared(segs, SHARED ? j.segs : 0);
+    if (!j.wide) {
+        constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+        const int d = tid % LANES * 4;
+        for (int r = way * GROUPS + tid / LANES; r < j.count; r += ways * GROUPS) {
+            const int row = j.row0 + r, tok = j.tok0 + row / a.group;
+            if (tok >= a.rows) continue;
+            f32x4 acc = f32x4{};
+            float top = NEG_INF, total = 0.f;
+            // splits s0 .. s0 + 3 of those at `part`; behind the last: the last again, not counted
+            auto four = [&](int part, int stride, int splits, int s0, bool begun) INLINE {
+                float m[4], l[4];
+                f32x4 x[4];
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    const size_t at = part + r + (size_t)min(s0 + s, splits - 1) * stride;
+                    m[s] = a.pm[at];
+                    l[s] = a.pl[at];
+                    x[s] = *(const f32x4*)(a.pacc + at * D + d);
+                }
+                const float was = top;
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    if (s0 + s >= splits) {
+                        m[s] = NEG_INF;
+                        l[s] = 0.f;
+                        x[s] = f32x4{};
+                    }
+                    top = fmaxf(top, m[s]);
+                }
+                if (begun) {
+                    const float f = was == NEG_INF ? 0.f : fast_exp2(was - top);
+                    acc *= f;
+                    total *= f;
+                }
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    const float f = m[s] == NEG_INF ? 0.f : fast_exp2(m[s] - top);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[i] += f * x[s][i];
+                    total += f * l[s];
+                }
+            };
+            four(j.part, j.count, j.splits, 0, false);
+            for (int s = 4; s < j.splits; s += 4) four(j.part, j.count, j.splits, s, true);
+#pragma unroll
+            for (int i = 0; i < (SHARED ? LEVELS : 0); i++)
+                for (int s = 0; s < shared.x[i].splits; s += 4) four(shared.x[i].part, shared.x[i].stride, shared.x[i].splits, s, true);
+            finish(tok, j.head * a.group + row % a.group, d, acc, top, total);
+        }
+        return;
+    }
+    const int splits = j.splits + shared.splits;
+    if (SHARED && j.wide == ROW_WIDE) {
+        constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+        const int group = tid / LANES, lane = tid % LANES;
+        for (int r = way; r < j.count; r += ways) {
+            const int row = j.row0 + r, tok = j.tok0 + row / a.group;
+            if (tok >= a.rows) continue;
+            f32x4 acc = f32x4{};
+            float top = NEG_INF, total = 0.f;
+            for (int s0 = 4 * group; s0 < splits; s0 += 4 * GROUPS) {  // behind the last the last again, not counted
+                float m[4], l[4];
+                f32x4 x[4];
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    const int at = min(s0 + s, splits - 1);
+                    const size_t p = at < j.splits ? j.part + r + (size_t)at * j.count : shared.row(at - j.splits, r);
+                    m[s] = a.pm[p];
+                    l[s] = a.pl[p];
+                    x[s] = *(const f32x4*)(a.pacc + p * D + lane * 4);
+                }
+                const float was = top;
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    if (s0 + s >= splits) {
+                        m[s] = NEG_INF;
+                        l[s] = 0.f;
+                        x[s] = f32x4{};
+                    }
+                    top = fmaxf(top, m[s]);
+                }
+                const float f = was == NEG_INF ? 0.f : fast_exp2(was - top);
+                acc *= f;
+                total *= f;
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    const float f = m[s] == NEG_INF ? 0.f : fast_exp2(m[s] - top);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[i] += f * x[s][i];
+                    total += f * l[s];
+                }
+            }
+            __syncthreads();  // the row before has been read
+            (&sa[0][0])[tid] = acc;
+            if (lane == 0) {
+                factor[group] = top;
+                factor[16 + group] = total;
+            }
+            lds_barrier();
+            if (group) continue;
+            float all = top;
+#pragma unroll
+            for (int x = 1; x < GROUPS; x++) all = fmaxf(all, factor[x]);
+            const float f = top == NEG_INF ? 0.f : fast_exp2(top - all);
+            acc *= f;
+            total *= f;
+#pragma unroll
+            for (int x = 1; x < GROUPS; x++) {
+                const float f = factor[x] == NEG_INF ? 0.f : fast_exp2(factor[x] - all);
+                const f32x4 y = (&sa[0][0])[x * LANES + lane];
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[i] += f * y[i];
+                total += f * factor[16 + x];
+            }
+            finish(tok, j.head * a.group + row % a.group, lane * 4, acc, all, total);
+        }
+        return;
+    }
+    constexpr int PER_ROW = D / JOIN_DIMS;
+    const int part = tid / 16, lane = tid % 16;
+    for (int u = way; u < j.count * PER_ROW; u += ways) {
+        const int r = u / PER_ROW, d = u % PER_ROW * JOIN_DIMS + lane * 4;
+        const int row = j.row0 + r, tok = j.tok0 + row / a.group;
+        if (tok >= a.rows) continue;
+        const size_t first = j.part + r;
+        auto partial = [&](int s) INLINE { return !SHARED || s < j.splits ? first + (size_t)s * j.count : shared.row(s - j.splits, r); };
+        float top = NEG_INF;
+        for (int s = tid; s < splits; s += 256) top = fmaxf(top, a.pm[partial(s)]);
+        // the first splits' values are on their way meanwhile
+        constexpr int EARLY = 8;
+        f32x4 x[EARLY];
+#pragma unroll
+        for (int i = 0; i < EARLY; i++) x[i] = *(const f32x4*)(a.pacc + partial(min(part + 16 * i, splits - 1)) * D + d);
+#pragma unroll
+        for (int i = 1; i < 64; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
+        __syncthreads();  // the row before has been read
+        if (tid % 64 == 0) red[0][tid / 64] = top;
+        lds_barrier();
+        top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+        float total = 0.f;
+        for (int s = tid; s < splits; s += 256) {
+            const size_t at = partial(s);
+            const float m = a.pm[at], f = m == NEG_INF ? 0.f : fast_exp2(m - top);
+            factor[s] = f;
+            total += f * a.pl[at];
+        }
+#pragma unroll
+        for (int i = 1; i < 64; i *= 2) total += __shfl_xor(total, i);
+        if (tid % 64 == 0) red[1][tid / 64] = total;
+        lds_barrier();
+        total = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+        f32x4 acc = f32x4{};
+        auto add = [&](int s, f32x4 y) INLINE {
+            const float f = factor[s];
+#pragma unroll
+            for (int c = 0; c < 4; c++) acc[c] += f * y[c];
+        };
+#pragma unroll
+        for (int i = 0; i < EARLY; i++)
+            if (part + 16 * i < splits) add(part + 16 * i, x[i]);
+#pragma unroll 4
+        for (int s = part + 16 * EARLY; s < splits; s += 16) add(s, *(const f32x4*)(a.pacc + partial(s) * D + d));
+        sa[part][lane] = acc;
+        lds_barrier();
+        if (part) continue;
+        acc = sa[0][lane];
+#pragma unroll
+        for (int i = 1; i < 16; i++) acc += sa[i][lane];
+        finish(tok, j.head * a.group + row % a.group, d, acc, top, total);
+    }
+}
 template <typename T, int D, bool SHARED>
 __global__ void __launch_bounds__(256) join_kernel(Args a, const Join* __restrict__ joins, const int* __restrict__ njoins,
                                                    const Seg* __restrict__ segs) {
     __shared__ float factor[SPLITS_MOST];
     __shared__ __attribute__((aligned(16))) f32x4 sa[16][16];
     __shared__ float red[2][4];
-    const int count = *uniform(njoins), tid = threadIdx.x;
-    auto finish = [&](int tok, int head, int d, f32x4 acc, float m, float l) INLINE {
-        acc *= row_factor(a, head, m, l);
-        const float x[4] = {acc[0], acc[1], acc[2], acc[3]};
-        store_out<T, D, 4>(a, tok, head, d, x);
-    };
+    const int count = *uniform(njoins);
     // work-groups of a join: as many as there are for each
     const int ways = max(1, (int)gridDim.x / max(1, count)), way = blockIdx.x % ways;
     for (int n = blockIdx.x / ways; n < count; n += gridDim.x / ways) {
         const Uniform<int> ji = uniform((const int*)(joins + n));
         const Join j{ji[0], ji[1], ji[2], ji[3], ji[4], ji[5], ji[6], ji[7]};
-        const Segs shared(segs + (size_t)n * LEVELS, SHARED ? j.segs : 0);
-        if (!j.wide) {
-            constexpr int LANES = D / 4, GROUPS = 256 / LANES;
-            const int d = tid % LANES * 4;
-            for (int r = way * GROUPS + tid / LANES; r < j.count; r += ways * GROUPS) {
-                const int row = j.row0 + r, tok = j.tok0 + row / a.group;
-                if (tok >= a.rows) continue;
-                f32x4 acc = f32x4{};
-                float top = NEG_INF, total = 0.f;
-                // splits s0 .. s0 + 3 of those at `part`; behind the last: the last again, not counted
-                auto four = [&](int part, int stride, int splits, int s0, bool begun) INLINE {
-                    float m[4], l[4];
-                    f32x4 x[4];
-#pragma unroll
-                    for (int s = 0; s < 4; s++) {
-                        const size_t at = part + r + (size_t)min(s0 + s, splits - 1) * stride;
-                        m[s] = a.pm[at];
-                        l[s] = a.pl[at];
-                        x[s] = *(const f32x4*)(a.pacc + at * D + d);
-                    }
-                    const float was = top;
-#pragma unroll
-                    for (int s = 0; s < 4; s++) {
-                        if (s0 + s >= splits) {
-                            m[s] = NEG_INF;
-                            l[s] = 0.f;
-                            x[s] = f32x4{};
-                        }
-                        top = fmaxf(top, m[s]);
-                    }
-                    if (begun) {
-                        const float f = was == NEG_INF ? 0.f : fast_exp2(was - top);
-                        acc *= f;
-                        total *= f;
-                    }
-#pragma unroll
-                    for (int s = 0; s < 4; s++) {
-                        const float f = m[s] == NEG_INF ? 0.f : fast_exp2(m[s] - top);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) acc[i] += f * x[s][i];
-                        total += f * l[s];
-                    }
-                };
-                four(j.part, j.count, j.splits, 0, false);
-                for (int s = 4; s < j.splits; s += 4) four(j.part, j.count, j.splits, s, true);
-#pragma unroll
-                for (int i = 0; i < (SHARED ? LEVELS : 0); i++)
-                    for (int s = 0; s < shared.x[i].splits; s += 4) four(shared.x[i].part, shared.x[i].stride, shared.x[i].splits, s, true);
-                finish(tok, j.head * a.group + row % a.group, d, acc, top, total);
-            }
-            continue;
-        }
-        const int splits = j.splits + shared.splits;
-        if (SHARED && j.wide == ROW_WIDE) {
-            constexpr int LANES = D / 4, GROUPS = 256 / LANES;
-            const int group = tid / LANES, lane = tid % LANES;
-            for (int r = way; r < j.count; r += ways) {
-                const int row = j.row0 + r, tok = j.tok0 + row / a.group;
-                if (tok >= a.rows) continue;
-                f32x4 acc = f32x4{};
-                float top = NEG_INF, total = 0.f;
-                for (int s0 = 4 * group; s0 < splits; s0 += 4 * GROUPS) {  // behind the last the last again, not counted
-                    float m[4], l[4];
-                    f32x4 x[4];
-#pragma unroll
-                    for (int s = 0; s < 4; s++) {
-                        const int at = min(s0 + s, splits - 1);
-                        const size_t p = at < j.splits ? j.part + r + (size_t)at * j.count : shared.row(at - j.splits, r);
-                        m[s] = a.pm[p];
-                        l[s] = a.pl[p];
-                        x[s] = *(const f32x4*)(a.pacc + p * D + lane * 4);
-                    }
-                    const float was = top;
-#pragma unroll
-                    for (int s = 0; s < 4; s++) {
-                        if (s0 + s >= splits) {
-                            m[s] = NEG_INF;
-                            l[s] = 0.f;
-                            x[s] = f32x4{};
-                        }
-                        top = fmaxf(top, m[s]);
-                    }
-                    const float f = was == NEG_INF ? 0.f : fast_exp2(was - top);
-                    acc *= f;
-                    total *= f;
-#pragma unroll
-                    for (int s = 0; s < 4; s++) {
-                        const float f = m[s] == NEG_INF ? 0.f : fast_exp2(m[s] - top);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) acc[i] += f * x[s][i];
-                        total += f * l[s];
-                    }
-                }
-                __syncthreads();  // the row before has been read
-                (&sa[0][0])[tid] = acc;
-                if (lane == 0) {
-                    factor[group] = top;
-                    factor[16 + group] = total;
-                }
-                lds_barrier();
-                if (group) continue;
-                float all = top;
-#pragma unroll
-                for (int x = 1; x < GROUPS; x++) all = fmaxf(all, factor[x]);
-                const float f = top == NEG_INF ? 0.f : fast_exp2(top - all);
-                acc *= f;
-                total *= f;
-#pragma unroll
-                for (int x = 1; x < GROUPS; x++) {
-                    const float f = factor[x] == NEG_INF ? 0.f : fast_exp2(factor[x] - all);
-                    const f32x4 y = (&sa[0][0])[x * LANES + lane];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) acc[i] += f * y[i];
-                    total += f * factor[16 + x];
-                }
-                finish(tok, j.head * a.group + row % a.group, lane * 4, acc, all, total);
-            }
-            continue;
-        }
-        constexpr int PER_ROW = D / JOIN_DIMS;
-        const int part = tid / 16, lane = tid % 16;
-        for (int u = way; u < j.count * PER_ROW; u += ways) {
-            const int r = u / PER_ROW, d = u % PER_ROW * JOIN_DIMS + lane * 4;
-            const int row = j.row0 + r, tok = j.tok0 + row / a.group;
-            if (tok >= a.rows) continue;
-            const size_t first = j.part + r;
-            auto partial = [&](int s) INLINE { return !SHARED || s < j.splits ? first + (size_t)s * j.count : shared.row(s - j.splits, r); };
-            float top = NEG_INF;
-            for (int s = tid; s < splits; s += 256) top = fmaxf(top, a.pm[partial(s)]);
-            // the first splits' values are on their way meanwhile
-            constexpr int EARLY = 8;
-            f32x4 x[EARLY];
-#pragma unroll
-            for (int i = 0; i < EARLY; i++) x[i] = *(const f32x4*)(a.pacc + partial(min(part + 16 * i, splits - 1)) * D + d);
-#pragma unroll
-            for (int i = 1; i < 64; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
-            __syncthreads();  // the row before has been read
-            if (tid % 64 == 0) red[0][tid / 64] = top;
-            lds_barrier();
-            top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-            float total = 0.f;
-            for (int s = tid; s < splits; s += 256) {
-                const size_t at = partial(s);
-                const float m = a.pm[at], f = m == NEG_INF ? 0.f : fast_exp2(m - top);
-                factor[s] = f;
-                total += f * a.pl[at];
-            }
-#pragma unroll
-            for (int i = 1; i < 64; i *= 2) total += __shfl_xor(total, i);
-            if (tid % 64 == 0) red[1][tid / 64] = total;
-            lds_barrier();
-            total = red[1][0] + red[1][1] + red[1][2] + red[1][3];
-            f32x4 acc = f32x4{};
-            auto add = [&](int s, f32x4 y) INLINE {
-                const float f = factor[s];
-#pragma unroll
-                for (int c = 0; c < 4; c++) acc[c] += f * y[c];
-            };
-#pragma unroll
-            for (int i = 0; i < EARLY; i++)
-                if (part + 16 * i < splits) add(part + 16 * i, x[i]);
-#pragma unroll 4
-            for (int s = part + 16 * EARLY; s < splits; s += 16) add(s, *(const f32x4*)(a.pacc + partial(s) * D + d));
-            sa[part][lane] = acc;
-            lds_barrier();
-            if (part) continue;
-            acc = sa[0][lane];
-#pragma unroll
-            for (int i = 1; i < 16; i++) acc += sa[i][lane];
-            finish(tok, j.head * a.group + row % a.group, d, acc, top, total);
-        }
+        if (SHARED && j.segs) join_rows<T, D, true>(a, j, segs + (size_t)n * LEVELS, way, ways, factor, sa, red);
+        else join_rows<T, D, false>(a, j, nullptr, way, ways, factor, sa, red);
     }
 }
 
