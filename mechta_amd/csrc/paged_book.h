@@ -175,6 +175,7 @@ struct Sum {  // keys [k0, k1) from rows [r0, r1)
 struct Fade {  // weights of keys [k0, k1), faded, plus `sums` partial sums, of key k0 + i at part + s * stride + i
     int seq, head, k0, k1, part, sums, stride, pad;
 };
+constexpr int MERGE_WAYS = 8;  // work-groups of a merge: 16 rows each
 // few: up to 16 rows, some: up to 32, many: tiles of 128
 enum { SCORE_FEW, SCORE_SOME, SCORE_MANY, MERGES, SUM_FEW, SUM_MANY, FADES, WEIGH_LISTS };
 struct WeighPlan {

@@ -327,7 +327,6 @@ __global__ void __launch_bounds__(256) score_rows(Args a, const Score* __restric
 }
 
 // Several pieces of many rows' statistics: 16 lanes a row, 16 rows of an item a work-group.
-constexpr int MERGE_WAYS = SCORE_ROWS / 16;
 __global__ void __launch_bounds__(256) merge_kernel(Args a, const Merge* __restrict__ items, const int* __restrict__ nitems) {
     const int count = *uniform(nitems) * MERGE_WAYS, lane = threadIdx.x % 16;
     for (int n = blockIdx.x; n < count; n += gridDim.x) {
@@ -783,8 +782,7 @@ hipError_t weigh_as(const Args& a, const int* batch, const WeighLists& l, const 
     hipError_t e = hipSuccess;
     auto go = [&](auto kernel, int list, auto* items, int threads = 256) {
         if (!grid[list] || e != hipSuccess) return;
-        const int groups = list == MERGES ? std::min(grid[list], MOST_GRID / MERGE_WAYS) * MERGE_WAYS : grid[list];
-        kernel<<<dim3(groups), dim3(threads), 0, s>>>(a, items, batch + list);
+        kernel<<<dim3(grid[list]), dim3(threads), 0, s>>>(a, items, batch + list);
         e = hipGetLastError();
     };
     go(score_few<T, D, 1>, SCORE_FEW, (const Score*)(batch + l.at[SCORE_FEW]));

@@ -13,8 +13,9 @@ using namespace mkv::paged;
 
 namespace {
 
-// Work-groups of a captured weighing, of whatever batch it finds.
-constexpr int GRAPH_WEIGH = 1024;
+// Work-groups of each kernel of a captured weighing, of whatever batch it finds. (1 token at 300 positions of 2 x 256, 64 at 3,000 and 4 of one
+// sequence at 65,536 of 4 x 128, in a graph: 15.3 / 58.5 / 50.0 us; with 8,192 for the merges 16.6 / 60.1 / 51.6, with 512 of each kind 15.2 / 60.8 / 65.8.)
+constexpr int GRAPH_WEIGH = 1024, GRAPH_MERGES = 512;
 constexpr long long WORK_MOST = 1ll << 28;  // floats: kept scores
 constexpr long long STATS_MORE = 1ll << 18;  // statistics of rows in more than one piece
 
@@ -202,7 +203,7 @@ int mpg_weigh(mpg_t* h, int layer, int rows, const void* q, int64_t q_tok, int64
     a.pool = h->pool;
     a.layer = layer;
     a.window = h->kinds[w];
-    a.rows = rows;
+    a.rows = std::min(rows, h->c.tokens);  // (a batch has no more; rows x group stays a number of 32 bits)
     a.table = h->dev;
     a.q = Rows{q, q_tok, q_head};
     a.sinks = sinks;
@@ -212,9 +213,9 @@ int mpg_weigh(mpg_t* h, int layer, int rows, const void* q, int64_t q_tok, int64
     a.work = k->work;
     int grid[WEIGH_LISTS];
     auto size = [&](int list) {
-        return list <= SCORE_MANY ? p.scores[list].size() : list == MERGES ? p.merges.size() : list < FADES ? p.sums[list - SUM_FEW].size() : p.fades.size();
+        return list <= SCORE_MANY ? p.scores[list].size() : list == MERGES ? p.merges.size() * MERGE_WAYS : list < FADES ? p.sums[list - SUM_FEW].size() : p.fades.size();
     };
-    for (int l = 0; l < WEIGH_LISTS; l++) grid[l] = cap ? GRAPH_WEIGH : (int)std::min<size_t>(size(l), MOST_GRID);
+    for (int l = 0; l < WEIGH_LISTS; l++) grid[l] = cap ? l == MERGES ? GRAPH_MERGES : GRAPH_WEIGH : (int)std::min<size_t>(size(l), MOST_GRID);
     if (!cap && decay == 1) {  // what is not given anything stays as it is
         bool sums = false;
         for (const Fade& f : p.fades) sums |= f.sums > 0;

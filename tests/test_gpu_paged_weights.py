@@ -527,6 +527,19 @@ def test_fewer_rows_than_the_batch_in_a_replay(torch_gpu, pg):
             at += c
 
 
+@pytest.mark.parametrize("tokens", [1, 5])
+def test_as_many_rows_as_there_are_numbers(torch_gpu, pg, tokens):
+    """Rows behind the batch's last are not read, however many the call says there are."""
+    import ctypes
+    m = Model(torch_gpu, pg, 2, 8, 64, "f16", 64)
+    m.begin([0], [600])
+    m.begin([0, 1], [tokens, tokens])
+    q = m.weigh(run=False)
+    rc = m.kv._lib.mpg_weigh(m.kv._h, 0, 2 ** 31 - 1, ctypes.c_void_p(q.data_ptr()), q.stride(0), q.stride(1), 64 ** -0.5, None, 1.0)
+    assert rc == 0
+    m.check()
+
+
 def test_another_current_stream(torch_gpu, pg):
     torch = torch_gpu
     m = Model(torch, pg, 1, 8, 64, "f16", 32)
