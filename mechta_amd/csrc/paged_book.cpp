@@ -905,6 +905,19 @@ void plan_shared(const Shape& g, const std::vector<Member>& batch, const Share& 
 
 // ---- accumulated attention weights ----
 
+bool may_weigh(const Shape& g, int tokens, int seqs, int ctx, int window, int last, const WeighRoom& room, int list) {
+    const long long rows = (long long)(last ? std::min(last, tokens) : tokens) * (g.q_heads / g.kv_heads);
+    // (a sequence's scores are of whole blocks of keys)
+    const double scores = (double)std::min(seqs, tokens) * ((ctx + KEYS - 1) / KEYS * KEYS) * rows * g.kv_heads;
+    const bool many = rows > TILE_ROWS[SOME] || scores > room.work - WEIGH_PARTS;
+    switch (list) {
+        case SCORE_SOME: return rows > TILE_ROWS[FEW];
+        case SCORE_MANY: case MERGES: case SUM_MANY: return many;
+        case FADES: return many || window;
+        default: return true;
+    }
+}
+
 size_t weigh_entries(const Shape& g, int tokens, int seqs) {
     const size_t group = g.q_heads / g.kv_heads;
     return ((size_t)tokens * group / SCORE_ROWS + 2 * (size_t)std::min(seqs, tokens)) * g.kv_heads + WEIGH_MOST;

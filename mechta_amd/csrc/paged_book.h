@@ -192,6 +192,8 @@ constexpr int WEIGH_MOST = 4096;                 // entries of a list at most, b
 constexpr int CUS = 256;
 constexpr int SUM_PLACES = 6 * CUS - 64;         // work-groups that take many rows' sums, about
 constexpr int WEIGH_PARTS = (SUM_PLACES + WEIGH_MOST) * SUM_KEYS;  // floats of the room: those sums' parts, which always find room
+// Whether a batch of up to `tokens` tokens of up to `seqs` sequences of up to `ctx` positions can have entries in a list.
+bool may_weigh(const Shape& g, int tokens, int seqs, int ctx, int window, int last, const WeighRoom& room, int list);
 size_t weigh_entries(const Shape& g, int tokens, int seqs);
 void plan_weigh(const Shape& g, const std::vector<Member>& batch, int window, int last, const WeighRoom& room, WeighPlan& out);
 

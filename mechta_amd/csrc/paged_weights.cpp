@@ -215,7 +215,11 @@ int mpg_weigh(mpg_t* h, int layer, int rows, const void* q, int64_t q_tok, int64
     auto size = [&](int list) {
         return list <= SCORE_MANY ? p.scores[list].size() : list == MERGES ? p.merges.size() * MERGE_WAYS : list < FADES ? p.sums[list - SUM_FEW].size() : p.fades.size();
     };
-    for (int l = 0; l < WEIGH_LISTS; l++) grid[l] = cap ? l == MERGES ? GRAPH_MERGES : GRAPH_WEIGH : (int)std::min<size_t>(size(l), MOST_GRID);
+    // a captured call has the kernels that some batch of the handle needs
+    for (int l = 0; l < WEIGH_LISTS; l++)
+        grid[l] = cap ? !may_weigh(h->shape, h->c.tokens, h->c.seqs, h->c.ctx, a.window, k->last, k->room, l) ? 0
+                        : l == MERGES ? GRAPH_MERGES : GRAPH_WEIGH
+                      : (int)std::min<size_t>(size(l), MOST_GRID);
     if (!cap && decay == 1) {  // what is not given anything stays as it is
         bool sums = false;
         for (const Fade& f : p.fades) sums |= f.sums > 0;

@@ -45,6 +45,9 @@ void shim_merges(int* out) {  // 8 ints each
 void shim_fades(int* out) {  // 8 ints each
     for (size_t i = 0; i < plan.fades.size(); i++) *(Fade*)(out + 8 * i) = plan.fades[i];
 }
+int shim_may(int q_heads, int kv_heads, int tokens, int seqs, int ctx, int window, int last, long long work, int list) {
+    return may_weigh(Shape{q_heads, kv_heads, 64}, tokens, seqs, ctx, window, last, WeighRoom{0, work}, list);
+}
 int shim_parts() { return WEIGH_PARTS; }
 size_t shim_entries(int q_heads, int kv_heads, int tokens, int seqs) { return weigh_entries(Shape{q_heads, kv_heads, 64}, tokens, seqs); }
 

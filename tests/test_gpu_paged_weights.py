@@ -493,6 +493,31 @@ def test_captured_weighing_follows_the_batch(torch_gpu, pg):
     m.kv.set_stream(torch.cuda.current_stream())
 
 
+@pytest.mark.parametrize("last,window", [(1, 0), (1, 40), (4, 0)])
+def test_captured_weighing_of_few_rows(torch_gpu, pg, last, window):
+    """A cache that counts a token or a few of each sequence, whose graphs have fewer kernels."""
+    torch = torch_gpu
+    stream = torch.cuda.Stream()
+    m = Model(torch, pg, 2, 8, 64, "bf16", 64, last=last, window=window)
+    m.begin([0, 1, 2], [700, 40, 3])
+    m.weigh()
+    m.begin([0], [1])
+    rows = 300
+    q = m.rnd(rows, 16, 64)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    m.kv.set_stream(stream)
+    with torch.cuda.graph(graph, stream=stream):
+        m.kv.weigh(0, q, decay=0.5)
+    m.kv.set_stream(torch.cuda.current_stream())
+    for seqs, counts in [([0], [1]), ([2, 0, 1], [1, 200, 4]), ([1], [40]), ([0, 1], [1, 1])]:
+        m.begin(seqs, counts)
+        graph.replay()
+        torch.cuda.synchronize()
+        m.weigh(q=q[:sum(counts)], decay=0.5, run=False)
+        m.check(what=f"{seqs} {counts}")
+
+
 def test_fewer_rows_than_the_batch_in_a_replay(torch_gpu, pg):
     """Tokens behind the captured rows are left out, of what they give as of what they are given."""
     torch = torch_gpu

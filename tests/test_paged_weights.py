@@ -163,6 +163,28 @@ def test_parts_of_sums_find_room_behind_the_scores(shim, more):
         assert any(f[5] > 1 for f in fades)  # and sums are split
 
 
+@pytest.mark.parametrize("seed", range(40))
+def test_lists_that_no_batch_fills_are_known_before(shim, seed):
+    r = random.Random(70 + seed)
+    kv, group, last, window = r.choice([1, 2]), r.choice([1, 4, 8, 16, 17]), r.choice([0, 1, 2, 4]), r.choice([0, 33])
+    seqs, ctx, tokens = r.choice([1, 3, 8]), r.choice([31, 700, 5000]), r.choice([1, 4, 40])
+    work = shim.shim_parts() + r.choice([0, 20000, 1 << 26])
+    may = [shim.shim_may(kv * group, kv, tokens, seqs, ctx, window, last, ctypes.c_longlong(work), k) for k in range(7)]
+    seen = [0] * 7
+    for _ in range(30):
+        left, batch = tokens, []
+        for s in range(seqs):
+            c = min(r.choice([0, 1, 1, 2, 4, 40]), left, ctx)
+            left -= c
+            batch.append((s, c, min(ctx, c + r.choice([0, 40, 600, 5000]))))
+        scores, sums, fades, merges = weigh(shim, kv, group, batch, window, last, 1 << 20, work)
+        seen = [a or bool(x) for a, x in zip(seen, scores + [merges] + sums + [fades])]
+    assert all(b or not a for a, b in zip(seen, may))
+    if work > 1 << 26:  # and no more than that: few rows find room
+        rows = min(last or tokens, tokens) * group
+        assert may == [1, rows > 16, rows > 32, rows > 32, 1, rows > 32, rows > 32 or window > 0]
+
+
 # ---- eviction in the book ----
 
 class Book:
