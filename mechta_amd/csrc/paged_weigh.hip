@@ -530,23 +530,31 @@ struct PageList {
     NewPage p[NEW_PAGES];
 };
 
-// Weights in an order of whole numbers; NaN weighs most, both zeros the same.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// Weights in an order of whole numbers, from 0x7FFFFF on; NaN weighs most, both zeros the same.
 __device__ inline unsigned order_of(float x) {
     if (x != x) return ~0u;
     const unsigned u = __float_as_uint(x == 0.f ? 0.f : x);
     return u >> 31 ? ~u : u | 0x80000000u;
 }
 
+__device__ inline int before_lane(unsigned long long lanes) {  // how many of them lie below this one
+    return __builtin_amdgcn_mbcnt_hi((unsigned)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)lanes, 0));
+}
+
 // The picks of one sequence, layer and head by a work-group: the least weight that stays, by digits of 11, 11 and 10 bits from the
 // highest on, then the positions in order; of those with just that weight the first ones. 65,536 weights stay in registers from one
-// reading to the next, four neighbours a thread and 4,096; longer sequences are read again for each.
-constexpr int GROUP = 16, PICKED = 4096 * GROUP;
+// reading to the next, four neighbours a thread and 4,096; longer sequences are read again for each. Each digit is counted in four places by
+// lane: weights are of few magnitudes, and lanes that count the same wait for each other.
+constexpr int GROUP = 16, PICKED = 4096 * GROUP, COUNTED = 4;
 __global__ void __launch_bounds__(1024) pick_kernel(WeightsAt w, EvictionList list, int n, int entry0, int first, int recent,
                                                     Eviction* __restrict__ entries, int* __restrict__ picks, size_t stride, int units) {
     // (at most EVICTIONS x 2^22 pairs of a sequence and a layer's head)
-    __shared__ int hist[2048];
-    __shared__ int waves[2][16];
-    __shared__ int found[2];
+    __shared__ __attribute__((aligned(16))) int hist[2048 * COUNTED];
+    __shared__ int waves[16];
+    __shared__ int2 before_of[GROUP * 16];  // tile by tile, of each wave: heavier ones before it, ones of the least weight
+    __shared__ int found[3];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     for (int b = blockIdx.x; b < n * units; b += gridDim.x) {
         const int c = b / units, unit = b % units;
@@ -559,7 +567,7 @@ __global__ void __launch_bounds__(1024) pick_kernel(WeightsAt w, EvictionList li
         for (int i = tid; i < recent; i += 1024) to[e.keep - recent + i] = hi + i;
         if (!want) continue;
         unsigned v[GROUP][4];
-        auto bring = [&](int g0) INLINE {  // positions g0 .. g0 + PICKED - 1 (rows are whole runs of 32; what is not in [lo, hi) is not looked at)
+        auto bring = [&](int g0) INLINE {  // positions g0 .. g0 + PICKED - 1 (rows are whole runs of 32); 0 for what is not in [lo, hi)
 #pragma unroll
             for (int t = 0; t < GROUP; t++) {
                 const int i = g0 + 4096 * t + 4 * tid;
@@ -567,7 +575,7 @@ __global__ void __launch_bounds__(1024) pick_kernel(WeightsAt w, EvictionList li
                 f32x4 x = f32x4{};
                 if (i < hi) x = *(const f32x4*)(src + i);
 #pragma unroll
-                for (int y = 0; y < 4; y++) v[t][y] = order_of(x[y]);
+                for (int y = 0; y < 4; y++) v[t][y] = i + y >= lo && i + y < hi ? order_of(x[y]) : 0;
             }
         };
         unsigned known = 0, mask = 0;  // the digits of the least weight that stays
@@ -576,7 +584,8 @@ __global__ void __launch_bounds__(1024) pick_kernel(WeightsAt w, EvictionList li
         for (int shift = 21; shift >= 0; shift = shift ? max(0, shift - 11) : -1) {  // 21, 10, 0: of 11, 11 and 10 bits
             const unsigned digit = shift ? 2047 : 1023;
             __syncthreads();
-            hist[tid] = hist[tid + 1024] = 0;
+#pragma unroll
+            for (int x = 0; x < 2; x++) ((i32x4*)hist)[tid + 1024 * x] = i32x4{};
             __syncthreads();
             for (int g0 = 0; g0 < hi; g0 += PICKED) {
                 if (hi > PICKED) bring(g0);
@@ -585,92 +594,109 @@ __global__ void __launch_bounds__(1024) pick_kernel(WeightsAt w, EvictionList li
                     if (g0 + 4096 * t >= hi) break;
 #pragma unroll
                     for (int y = 0; y < 4; y++) {
-                        const int i = g0 + 4096 * t + 4 * tid + y;
-                        const bool is = i >= lo && i < hi && (v[t][y] & mask) == known;
-                        const unsigned at = v[t][y] >> shift & digit;
-                        const unsigned long long active = __ballot(is);
-                        if (!active) continue;
-                        // (weights that are all alike, those of new positions for one, would queue up for one address)
-                        const unsigned one = __builtin_amdgcn_readlane(at, __builtin_ctzll(active));
-                        if (__ballot(is && at == one) == active) {
-                            if (lane == 0) atomicAdd(&hist[one], __popcll(active));
-                        } else if (is) {
-                            atomicAdd(&hist[at], 1);
-                        }
+                        if (v[t][y] && (v[t][y] & mask) == known) atomicAdd(&hist[(v[t][y] >> shift & digit) * COUNTED + lane % COUNTED], 1);
                     }
                 }
             }
             __syncthreads();
             // from the highest digit down: thread t has digits 2047 - 2 t and 2046 - 2 t
-            const int h0 = hist[2047 - 2 * tid], h1 = hist[2046 - 2 * tid];
+            auto counted = [&](int d) INLINE {
+                const i32x4 x = ((const i32x4*)hist)[d];
+                return x[0] + x[1] + x[2] + x[3];
+            };
+            const int h0 = counted(2047 - 2 * tid), h1 = counted(2046 - 2 * tid);
             int before = h0 + h1;
 #pragma unroll
             for (int x = 1; x < 64; x *= 2) {
                 const int y = __shfl_up(before, x);
                 if (lane >= x) before += y;
             }
-            if (lane == 63) waves[0][wave] = before;
+            if (lane == 63) waves[wave] = before;
             __syncthreads();
             before -= h0 + h1;
 #pragma unroll
             for (int x = 0; x < 15; x++) {
-                const int y = waves[0][x];
+                const int y = waves[x];
                 if (x < wave) before += y;
             }
             if (before < left && before + h0 >= left) {
                 found[0] = 2047 - 2 * tid;
                 found[1] = left - before;
+                found[2] = h0;
             } else if (before + h0 < left && before + h0 + h1 >= left) {
                 found[0] = 2046 - 2 * tid;
                 found[1] = left - before - h0;
+                found[2] = h1;
             }
             __syncthreads();
-            known |= (unsigned)found[0] << shift;
+            known |= (unsigned)__builtin_amdgcn_readfirstlane(found[0]) << shift;
             mask |= digit << shift;
-            left = found[1];
+            left = __builtin_amdgcn_readfirstlane(found[1]);
+            if (left == __builtin_amdgcn_readfirstlane(found[2])) {  // all with these digits stay, whatever the others: those above the number below
+                known--;
+                left = 0;
+                break;
+            }
         }
-        // left: how many of those with just the least weight stay
-        int more = 0, same = 0;  // before the tile: heavier ones, ones of the least weight
+        // left: how many of those with just the least weight stay (no weight's number is 0: `known` never went below)
+        int2 all = make_int2(0, 0);  // before the tiles: heavier ones, ones of the least weight
         for (int g0 = 0; g0 < hi; g0 += PICKED) {
             if (hi > PICKED) bring(g0);
+            if (wave == 0)
+#pragma unroll
+                for (int x = 0; x < GROUP / 4; x++) before_of[lane + 64 * x] = make_int2(0, 0);
+            __syncthreads();
 #pragma unroll
             for (int t = 0; t < GROUP; t++) {
                 if (g0 + 4096 * t >= hi) break;
-                const int i0 = g0 + 4096 * t + 4 * tid;
-                int mine = 0;  // (heavier) + (same) << 16
-#pragma unroll
-                for (int y = 0; y < 4; y++)
-                    if (i0 + y >= lo && i0 + y < hi) mine += v[t][y] > known ? 1 : v[t][y] == known ? 1 << 16 : 0;
-                int before = mine;
-#pragma unroll
-                for (int x = 1; x < 64; x *= 2) {
-                    const int y = __shfl_up(before, x);
-                    if (lane >= x) before += y;
-                }
-                if (lane == 63) waves[t % 2][wave] = before;
-                __syncthreads();  // (one a tile: the other half of `waves` was read before the one before)
-                int all = 0;
-                before -= mine;
-#pragma unroll
-                for (int x = 0; x < 16; x++) {
-                    const int y = waves[t % 2][x];
-                    if (x < wave) before += y;
-                    all += y;
-                }
-                int m = more + (before & 0xFFFF), s = same + (before >> 16);
+                int2 mine = make_int2(0, 0);
 #pragma unroll
                 for (int y = 0; y < 4; y++) {
-                    const int i = i0 + y;
-                    if (i < lo || i >= hi) continue;
-                    if (v[t][y] > known) to[first + m++ + min(s, left)] = i;
+                    mine.x += __popcll(__ballot(v[t][y] > known));
+                    mine.y += __popcll(__ballot(v[t][y] == known));
+                }
+                if (lane == 0) before_of[16 * t + wave] = mine;
+            }
+            __syncthreads();
+            // every wave adds up all 256 itself, four a lane, and takes its own
+            int2 four[4], sum = make_int2(0, 0);
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int2 y = before_of[4 * lane + x];
+                four[x] = sum;
+                sum = make_int2(sum.x + y.x, sum.y + y.y);
+            }
+            int2 upto = sum;
+#pragma unroll
+            for (int x = 1; x < 64; x *= 2) {
+                const int y = __shfl_up(upto.x, x), z = __shfl_up(upto.y, x);
+                if (lane >= x) upto = make_int2(upto.x + y, upto.y + z);
+            }
+            const int2 start = make_int2(all.x + upto.x - sum.x, all.y + upto.y - sum.y);
+            const int x_of = wave % 4;
+            const int2 own = make_int2(start.x + (x_of == 0 ? four[0].x : x_of == 1 ? four[1].x : x_of == 2 ? four[2].x : four[3].x),
+                                       start.y + (x_of == 0 ? four[0].y : x_of == 1 ? four[1].y : x_of == 2 ? four[2].y : four[3].y));
+            asm volatile("" : "+s"(known));  // (compared anew: the lanes' answers of all tiles do not fit in registers)
+#pragma unroll
+            for (int t = 0; t < GROUP; t++) {
+                if (g0 + 4096 * t >= hi) break;
+                const int i0 = g0 + 4096 * t + 4 * tid, from = 4 * t + wave / 4;  // the lane that has the wave's
+                int m = __builtin_amdgcn_readlane(own.x, from), s = __builtin_amdgcn_readlane(own.y, from);
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    m += before_lane(__ballot(v[t][y] > known));
+                    s += before_lane(__ballot(v[t][y] == known));
+                }
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    if (v[t][y] > known) to[first + m++ + min(s, left)] = i0 + y;
                     else if (v[t][y] == known) {
-                        if (s < left) to[first + m + s] = i;
+                        if (s < left) to[first + m + s] = i0 + y;
                         s++;
                     }
                 }
-                more += all & 0xFFFF;
-                same += all >> 16;
             }
+            all = make_int2(all.x + __builtin_amdgcn_readlane(upto.x, 63), all.y + __builtin_amdgcn_readlane(upto.y, 63));
             __syncthreads();
         }
     }
