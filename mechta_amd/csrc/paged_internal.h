@@ -101,12 +101,14 @@ struct Eviction {  // `keep` of a sequence's `len` positions; their indexes at `
 struct NewPage {  // page `nth` of a sequence (entry of the evictions) is `page` now
     int entry, nth, page;
 };
-// Which positions stay: to picks[(layer * kv_heads + head) * stride + off ..], in order; `entries` keeps the list for the others.
+// Which positions stay: to picks[(layer * kv_heads + head) * stride + off ..], in order, and their weights likewise to `kept`; `entries`
+// has the list for the others.
 hipError_t launch_pick(const Geometry& g, const WeightsAt& w, const Eviction* e, int n, int first, int recent, Eviction* entries,
-                       int* picks, size_t stride, hipStream_t s);
+                       int* picks, float* kept, size_t stride, hipStream_t s);
 hipError_t launch_gather(const Geometry& g, char* pool, const int* table, const Eviction* entries, const int* picks, size_t stride,
                          const NewPage* pages, int n, hipStream_t s);
-hipError_t launch_pack(const WeightsAt& w, const Eviction* entries, int n, const int* picks, size_t stride, hipStream_t s);
+// The weights that stay to their places; longest: the most positions that stay of a sequence.
+hipError_t launch_pack(const WeightsAt& w, const Eviction* entries, int n, int longest, const float* kept, size_t stride, hipStream_t s);
 
 }  // namespace paged
 }  // namespace mkv

@@ -539,6 +539,7 @@ __device__ inline unsigned order_of(float x) {
     return u >> 31 ? ~u : u | 0x80000000u;
 }
 
+__device__ inline float weight_of(unsigned x) { return __uint_as_float(x >> 31 ? x & 0x7FFFFFFF : ~x); }
 __device__ inline int before_lane(unsigned long long lanes) {  // how many of them lie below this one
     return __builtin_amdgcn_mbcnt_hi((unsigned)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)lanes, 0));
 }
@@ -549,7 +550,8 @@ __device__ inline int before_lane(unsigned long long lanes) {  // how many of th
 // lane: weights are of few magnitudes, and lanes that count the same wait for each other.
 constexpr int GROUP = 16, PICKED = 4096 * GROUP, COUNTED = 4;
 __global__ void __launch_bounds__(1024) pick_kernel(WeightsAt w, EvictionList list, int n, int entry0, int first, int recent,
-                                                    Eviction* __restrict__ entries, int* __restrict__ picks, size_t stride, int units) {
+                                                    Eviction* __restrict__ entries, int* __restrict__ picks, float* __restrict__ kept,
+                                                    size_t stride, int units) {
     // (at most EVICTIONS x 2^22 pairs of a sequence and a layer's head)
     __shared__ __attribute__((aligned(16))) int hist[2048 * COUNTED];
     __shared__ int waves[16];
@@ -561,10 +563,16 @@ __global__ void __launch_bounds__(1024) pick_kernel(WeightsAt w, EvictionList li
         const Eviction e = list.e[c];
         if (unit == 0 && tid == 0) entries[entry0 + c] = e;
         int* const to = picks + (size_t)unit * stride + e.off;
+        float* const heavy = kept + (size_t)unit * stride + e.off;
         const float* const src = w.p + w.at(unit / w.kv_heads, e.seq, unit % w.kv_heads);
         const int lo = first, hi = e.len - recent, want = e.keep - first - recent;
-        for (int i = tid; i < first; i += 1024) to[i] = i;
-        for (int i = tid; i < recent; i += 1024) to[e.keep - recent + i] = hi + i;
+        auto pick = [&](int k, int i, float x) INLINE {
+            to[k] = i;
+            heavy[k] = x;
+        };
+        for (int i = tid; i < first; i += 1024) pick(i, i, src[i]);
+#pragma unroll 4
+        for (int i = tid; i < recent; i += 1024) pick(e.keep - recent + i, hi + i, src[hi + i]);
         if (!want) continue;
         unsigned v[GROUP][4];
         auto bring = [&](int g0) INLINE {  // positions g0 .. g0 + PICKED - 1 (rows are whole runs of 32); 0 for what is not in [lo, hi)
@@ -689,9 +697,9 @@ __global__ void __launch_bounds__(1024) pick_kernel(WeightsAt w, EvictionList li
                 }
 #pragma unroll
                 for (int y = 0; y < 4; y++) {
-                    if (v[t][y] > known) to[first + m++ + min(s, left)] = i0 + y;
+                    if (v[t][y] > known) pick(first + m++ + min(s, left), i0 + y, weight_of(v[t][y]));
                     else if (v[t][y] == known) {
-                        if (s < left) to[first + m + s] = i0 + y;
+                        if (s < left) pick(first + m + s, i0 + y, weight_of(v[t][y]));
                         s++;
                     }
                 }
@@ -742,7 +750,7 @@ __global__ void __launch_bounds__(256) gather_kernel(unsigned short* __restrict_
             Unit u[ROUNDS];
 #pragma unroll
             for (int i = 0; i < ROUNDS; i++)
-                if (i % parts == part) u[i] = *(const Unit*)(s + (tid / KEYS + 8 * i) * 128);
+                if (i % parts == part) u[i] = __builtin_nontemporal_load((const Unit*)(s + (tid / KEYS + 8 * i) * 128));
 #pragma unroll
             for (int i = 0; i < ROUNDS; i++)
                 if (i % parts == part) *(Unit*)(t + (tid / KEYS + 8 * i) * 128) = u[i];
@@ -776,30 +784,16 @@ __global__ void __launch_bounds__(256) gather_kernel(unsigned short* __restrict_
     }
 }
 
-// The weights that stay, in place: a position's goes to one that is not behind it, 16,384 at a time.
-constexpr int PACKED = 16;
-__global__ void __launch_bounds__(1024) pack_kernel(WeightsAt w, const Eviction* __restrict__ entries, const int* __restrict__ picks,
-                                                    size_t stride, int n, int units) {
-    for (size_t b = blockIdx.x; b < (size_t)n * units; b += gridDim.x) {
+// The weights that stay, from where the picks have put them.
+__global__ void __launch_bounds__(256) pack_kernel(WeightsAt w, const Eviction* __restrict__ entries, const float* __restrict__ kept,
+                                                   size_t stride, size_t all, int units) {
+    for (size_t b = blockIdx.x; b < all; b += gridDim.x) {
         const int unit = (int)(b % units);
         const Eviction e = entries[b / units];
         float* const p = w.p + w.at(unit / w.kv_heads, e.seq, unit % w.kv_heads);
-        const int* const from = picks + (size_t)unit * stride + e.off;
-        // What a tile takes lies in it or behind it: it has been read when the tile is written, and tiles are on their way together.
-        for (int i0 = 0; i0 < e.keep; i0 += 1024 * PACKED) {
-            float x[PACKED];
-#pragma unroll
-            for (int j = 0; j < PACKED; j++) {
-                const int i = i0 + (int)threadIdx.x + 1024 * j;
-                x[j] = i < e.keep ? p[from[i]] : 0.f;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < PACKED; j++) {
-                const int i = i0 + (int)threadIdx.x + 1024 * j;
-                if (i < e.keep) p[i] = x[j];
-            }
-        }
+        const float* const from = kept + (size_t)unit * stride + e.off;
+#pragma unroll 4
+        for (int i = blockIdx.y * 256 + threadIdx.x; i < e.keep; i += gridDim.y * 256) p[i] = from[i];
     }
 }
 
@@ -874,14 +868,14 @@ hipError_t launch_weigh(const Geometry& g, const WeightsAt& w, const WeighArgs& 
 }
 
 hipError_t launch_pick(const Geometry& g, const WeightsAt& w, const Eviction* e, int n, int first, int recent, Eviction* entries,
-                       int* picks, size_t stride, hipStream_t s) {
+                       int* picks, float* kept, size_t stride, hipStream_t s) {
     const int units = g.layers * g.kv_heads;
     for (int i = 0; i < n; i += EVICTIONS) {
         EvictionList list;
         const int m = std::min(EVICTIONS, n - i);
         for (int j = 0; j < EVICTIONS; j++) list.e[j] = j < m ? e[i + j] : Eviction{0, 0, 0, 0};
         pick_kernel<<<dim3((unsigned)std::min<long long>((long long)m * units, MOST_GRID)), dim3(1024), 0, s>>>(w, list, m, i, first, recent, entries,
-                                                                                                    picks, stride, units);
+                                                                                                    picks, kept, stride, units);
         if (const hipError_t err = hipGetLastError()) return err;
     }
     return hipSuccess;
@@ -904,9 +898,11 @@ hipError_t launch_gather(const Geometry& g, char* pool, const int* table, const 
     return hipSuccess;
 }
 
-hipError_t launch_pack(const WeightsAt& w, const Eviction* entries, int n, const int* picks, size_t stride, hipStream_t s) {
+hipError_t launch_pack(const WeightsAt& w, const Eviction* entries, int n, int longest, const float* kept, size_t stride, hipStream_t s) {
     const int units = w.layers * w.kv_heads;
-    pack_kernel<<<dim3((unsigned)std::min<long long>((long long)n * units, MOST_GRID / 4)), dim3(1024), 0, s>>>(w, entries, picks, stride, n, units);
+    const size_t all = (size_t)n * units;
+    pack_kernel<<<dim3((unsigned)std::min<size_t>(all, MOST_GRID / 64), std::min((longest + 1023) / 1024, 64)), dim3(256), 0, s>>>(
+        w, entries, kept, stride, all, units);
     return hipGetLastError();
 }
 

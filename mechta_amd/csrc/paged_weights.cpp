@@ -28,13 +28,14 @@ struct Kept : Weights {
     size_t batch_at = 0;         // word offset in dev
     float* stats = nullptr;      // pairs
     float* work = nullptr;
-    int* picks = nullptr;        // [layer][kv head][positions of the pool]
+    int* picks = nullptr;        // [layer][kv head][positions of the pool]: of an eviction, the positions that stay
+    float* heavy = nullptr;      // and their weights
     Eviction* entries = nullptr;  // [seqs]
     std::vector<WeighPlan> plans, next;  // per window
     std::vector<int> counts;     // COUNTS a window, of `next`
 
     ~Kept() override {
-        for (void* p : {(void*)at.p, (void*)stats, (void*)work, (void*)picks, (void*)entries})
+        for (void* p : {(void*)at.p, (void*)stats, (void*)work, (void*)picks, (void*)heavy, (void*)entries})
             if (p) (void)hipFree(p);
     }
     int changes(bool copy, int n, const int* seq, const int* from, const int* count, const int* other, const char* who) {
@@ -107,7 +108,7 @@ WeightSizes weight_sizes(const mpg_config& c, int last) {
     return s;
 }
 double bytes_of(const WeightSizes& s, const mpg_config& c) {
-    return 4. * s.weights + 8. * (s.stats + KEYS) + 4. * s.work + 4. * s.picks + 4. * s.words + sizeof(Eviction) * (double)c.seqs;
+    return 4. * s.weights + 8. * (s.stats + KEYS) + 4. * s.work + 8. * s.picks + 4. * s.words + sizeof(Eviction) * (double)c.seqs;
 }
 
 int check_last(const char* who, int last) {
@@ -149,6 +150,7 @@ static int keep_weights(mpg_t* h, int last) {
     if (e == hipSuccess) e = hipMalloc((void**)&k->stats, (s.stats + KEYS) * 8);
     if (e == hipSuccess) e = hipMalloc((void**)&k->work, s.work * 4);
     if (e == hipSuccess) e = hipMalloc((void**)&k->picks, s.picks * 4);
+    if (e == hipSuccess) e = hipMalloc((void**)&k->heavy, s.picks * 4);
     if (e == hipSuccess) e = hipMalloc((void**)&k->entries, sizeof(Eviction) * c.seqs);
     if (e == hipSuccess) e = hipMemsetAsync(dev, 0, words * 4, h->stream);
     if (e == hipSuccess) e = hipMemsetAsync(k->at.p, 0, s.weights * 4, h->stream);
@@ -249,22 +251,23 @@ static int evict(mpg_t* h, int n, const int* seq, const int* keep, int first, in
         if (cut.empty()) return (int)MKV_OK;
         std::vector<Eviction> e;
         std::vector<NewPage> pages;
-        int off = 0;
+        int off = 0, longest = 0;
         for (const Evicted& c : cut) {
             const int m = h->book.len[c.seq];
+            longest = std::max(longest, m);
             const std::vector<int>& t = h->book.table[c.seq];
             for (int p = 0; p < (int)t.size(); p++) pages.push_back({(int)e.size(), p, t[p]});
             e.push_back({c.seq, c.len, m, off});
             off += m;
         }
         const size_t stride = (size_t)h->c.pages * h->c.page;
-        hipError_t err = launch_pick(h->g, k->at, e.data(), (int)e.size(), first, recent, k->entries, k->picks, stride, h->stream);
+        hipError_t err = launch_pick(h->g, k->at, e.data(), (int)e.size(), first, recent, k->entries, k->picks, k->heavy, stride, h->stream);
         if (err == hipSuccess)
             err = launch_gather(h->g, h->pool, h->dev, k->entries, k->picks, stride, pages.data(), (int)pages.size(), h->stream);
         if (err != hipSuccess) return hip_fail(err, who);
         // The weights move last, in one launch: whatever fails before it leaves them as they were. (The new tables go up when the
         // device next needs them.)
-        err = launch_pack(k->at, k->entries, (int)e.size(), k->picks, stride, h->stream);
+        err = launch_pack(k->at, k->entries, (int)e.size(), longest, k->heavy, stride, h->stream);
         return err == hipSuccess ? (int)MKV_OK : hip_fail(err, who);
     };
     int rc;

@@ -27,15 +27,16 @@ hipError_t launch_weigh(const Geometry&, const WeightsAt&, const WeighArgs&, con
     return hipSuccess;
 }
 // every second of the positions between, whatever they weigh
-hipError_t launch_pick(const Geometry& g, const WeightsAt&, const Eviction* e, int n, int first, int recent, Eviction* entries, int* picks,
-                       size_t stride, hipStream_t) {
+hipError_t launch_pick(const Geometry& g, const WeightsAt& w, const Eviction* e, int n, int first, int recent, Eviction* entries, int* picks,
+                       float* heavy, size_t stride, hipStream_t) {
     for (int i = 0; i < n; i++) {
         if (const hipError_t err = step(hipErrorLaunchFailure)) return err;
         entries[i] = e[i];
         for (int u = 0; u < g.layers * g.kv_heads; u++)
             for (int k = 0, m = 0; k < e[i].keep; k++) {
                 const int mid = e[i].keep - first - recent, free = e[i].len - first - recent - mid;
-                picks[u * stride + e[i].off + k] = k < first ? k : k < first + mid ? first + std::min(free, ++m) + k - first : e[i].len - e[i].keep + k;
+                const int p = picks[u * stride + e[i].off + k] = k < first ? k : k < first + mid ? first + std::min(free, ++m) + k - first : e[i].len - e[i].keep + k;
+                heavy[u * stride + e[i].off + k] = w.p[w.at(u / w.kv_heads, e[i].seq, u % w.kv_heads) + p];
             }
     }
     return hipSuccess;
@@ -56,12 +57,12 @@ hipError_t launch_gather(const Geometry& g, char* pool, const int* table, const 
     }
     return hipSuccess;
 }
-hipError_t launch_pack(const WeightsAt& w, const Eviction* entries, int n, const int* picks, size_t stride, hipStream_t) {
+hipError_t launch_pack(const WeightsAt& w, const Eviction* entries, int n, int longest, const float* heavy, size_t stride, hipStream_t) {
     if (const hipError_t err = step(hipErrorLaunchFailure)) return err;
     for (int i = 0; i < n; i++)
         for (int u = 0; u < w.layers * w.kv_heads; u++) {
             float* const p = w.p + w.at(u / w.kv_heads, entries[i].seq, u % w.kv_heads);
-            for (int k = 0; k < entries[i].keep; k++) p[k] = p[picks[u * stride + entries[i].off + k]];
+            for (int k = 0; k < std::min(longest, entries[i].keep); k++) p[k] = heavy[u * stride + entries[i].off + k];
         }
     return hipSuccess;
 }
