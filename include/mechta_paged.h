@@ -16,7 +16,8 @@
  * or until pages change hands (mpg_fork, mpg_copy, mpg_free, mpg_compact, mpg_set_len, mpg_reserve, mpg_evict): then appends and
  * attention are refused until a new mpg_begin.
  *
- * Ordering: every call is enqueued on the handle's HIP stream; none waits, except mpg_create, mpg_sync and mpg_destroy.
+ * Ordering: every call is enqueued on the handle's HIP stream; none waits, except mpg_create, mpg_keep_weights, mpg_sync and
+ * mpg_destroy.
  * What goes up to the device (mpg_begin; the page calls that end a batch; mpg_read_rows, uncaptured, where pages are new)
  * goes through four pinned buffers: such a call waits where the stream is four of them behind, and for a larger buffer
  * when it needs one. Calls of one handle come from one thread at a time and run
@@ -190,8 +191,8 @@ int mpg_weights(const mpg_t* h, int layer, float** base, int64_t* seq_stride, in
 /* For each sequence of the batch with new tokens, each kv head and each of its positions j: weight = decay x weight + the sum,
  * over the counted tokens and the query heads of the kv head, of the attention weights of j (mpg_attend's softmax, with its
  * scale, window and sinks; after the layer's mpg_append). Other sequences' weights are left as they are. decay >= 0: 1
- * accumulates, 0 starts afresh whatever was there. q, rows: mpg_attend's, rotated. All in f32. A score that is NaN or plus infinity makes
- * all that its row sees NaN. */
+ * accumulates, 0 starts afresh whatever was there. q, rows: mpg_attend's, rotated. All in f32. A score that is NaN or plus
+ * infinity, or minus infinity in all that a row sees without a sink, makes all that its row sees NaN. */
 int mpg_weigh(mpg_t* h, int layer, int rows, const void* q, int64_t q_tok, int64_t q_head, float scale, const float* sinks,
               float decay);
 /* Cuts each of n different sequences of more than keep[i] positions to keep[i] >= 1: its first `first` and last `recent` ones

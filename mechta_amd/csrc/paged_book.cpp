@@ -329,9 +329,9 @@ constexpr int WIDE_SPLITS = 8, WIDE_ROWS = 512;
 // sequences of a token on a prompt of 4,096 of 4 x 128: 4 12.2 / 14.7, 8 13.4 / 14.6, 16 18.0 / 14.7; 8 and 16 of 2 x 256 15.8 / 17.9,
 // 20.1 / 18.9.)
 constexpr int WIDE_SHARED = 512 * 64;
-// Rows and splits of a shared batch that are joined a row a work-group. (Whole calls, us, so / D / 4 lanes a row: 8 verifies of 4 tokens at
-// 65,536, 2 x 256, 512 rows of 54 splits 61.2 / 66; 16 tokens on 16,384 of 4 x 128 23.9 / 26.9; 64 tokens, 2,048 rows of up to 40 42.5 / 39.6,
-// of 8 x 64 35.7 / 31.)
+// Rows and splits of a shared batch that are joined a row a work-group. (Whole calls, us, so / D / 4 lanes a row: 8 verifies of 4
+// tokens at 65,536, 2 x 256, 512 rows of 54 splits 61.2 / 66; 16 tokens on 16,384 of 4 x 128 23.9 / 26.9; 64 tokens, 2,048 rows of
+// up to 40 42.5 / 39.6, of 8 x 64 35.7 / 31.)
 constexpr int ROW_SPLITS = 16, ROW_ROWS = 1024;
 }  // namespace
 
@@ -549,6 +549,7 @@ int splits_room(int rows, int kv_heads, int part, int more) {
 namespace {
 // Which of a batch's common positions are attended once for all that have them. Apart they are read once for each (though the
 // later readings may find them in a cache); together they cost a launch more, or tiles among those there, and their partials.
+// What is found here is worth a draft; whether it is attended so, the model of the whole call says (cost_of).
 struct Sharer {
     static constexpr int LEAST = 128;         // positions of a range
     static constexpr int LEAST_SPARED = 512;  // positions that a range spares its sequences, in all
@@ -629,8 +630,10 @@ namespace {
 struct Common {
     int rows = 0, tok0 = 0, k0 = 0, splits = 0, part = 0;
 };
-// How a batch's work may be cut. APART: every sequence by itself. STREAMED: what they share in tiles of 32 rows beside their own, all by
-// few_rows. TILED: what they share in a chunk's tiles where it has more than 32 rows.
+// How a batch's work may be cut. APART: every sequence by itself. STREAMED: what they share in tiles of 32 rows beside their own, all
+// by few_rows. TILED: what they share in a chunk's tiles where it has more than 32 rows. (Whole calls, us, 2 / 4 / 8 / 16 / 64 tokens on
+// a prompt of 16,384 of 4 x 128, 32 heads: apart 16.7 / 23.4 / 38.9 / 55 / 123, where the later readings come out of the L2s at 17 TB/s;
+// streamed 14.8 / 15.8 / 19.1 / 30.9 / 48; tiled 13.8 / 21 / 20.6 / 26.8 / 39.)
 enum Way { APART, STREAMED, TILED };
 struct Draft {
     std::vector<Tile> tiles[KINDS];
@@ -701,7 +704,8 @@ void draft(const Shape& g, const std::vector<Member>& batch, const Share* share,
         }
         any = true;
         auto tiles = [&](int kind) {
-            for (int row = 0; row < c.rows; row += TILE_ROWS[kind]) by_kind[kind].push_back({share->members[r.first], c.tok0, row, c.k0, r.k1, kind, (int)x});
+            for (int row = 0; row < c.rows; row += TILE_ROWS[kind])
+                by_kind[kind].push_back({share->members[r.first], c.tok0, row, c.k0, r.k1, kind, (int)x});
         };
         if (c.rows <= TILE_ROWS[SOME] || way == STREAMED) {
             tiles(c.rows <= TILE_ROWS[FEW] && way != STREAMED ? FEW : SOME);
@@ -961,9 +965,10 @@ void plan_weigh(const Shape& g, const std::vector<Member>& batch, int window, in
         return (int)std::max(1ll, std::min(p, most));
     };
     int more = 0;
-    // Few rows: bound by the keys' stream. Whole where they are short, which spares the launch for their sums (a token at 300 positions of
-    // 2 x 256 6.2 us, in three pieces 8.4; 12 windows of 545 keys of 4 x 128 9.3 and 9.2); else in about four pieces a CU. (The statistics of 64 sequences at 500 .. 8,001 positions of 4 x 128 in 428 / 640 / 1,160 / 2,300 work-groups: 45.5 / 44.1 / 42.3 /
-    // 41.5 us.)
+    // Few rows: bound by the keys' stream. Whole where they are short, which spares the launch for their sums (a token at 300
+    // positions of 2 x 256 6.2 us, in three pieces 8.4; 12 windows of 545 keys of 4 x 128 9.3 and 9.2); else in about four pieces a
+    // CU. (The statistics of 64 sequences at 500 .. 8,001 positions of 4 x 128 in 428 / 640 / 1,160 / 2,300 work-groups: 45.5 / 44.1
+    // / 42.3 / 41.5 us.)
     constexpr int WHOLE_FEW = 512;
     const long long few_length = std::max<long long>(LEAST_KEYS, (few_keys + 4 * CUS - 1) / (4 * CUS)) / KEYS;
     for (const Weighed& w : few) {
@@ -981,7 +986,8 @@ void plan_weigh(const Shape& g, const std::vector<Member>& batch, int window, in
                     {w.seq, h, w.tok0, w.rows, 0, w.pos0, w.k0 + a * KEYS, std::min(w.len, w.k0 + b * KEYS), stat + p * w.rows,
                      scores + a * KEYS * w.rows, pieces == 1, 0});
             }
-            if (pieces > 1) out.sums[0].push_back({w.seq, h, w.tok0, w.rows, w.pos0, w.k0, w.len, 0, w.rows, stat, pieces, scores, w.k0, -1, {0, 0}});
+            if (pieces > 1)
+                out.sums[0].push_back({w.seq, h, w.tok0, w.rows, w.pos0, w.k0, w.len, 0, w.rows, stat, pieces, scores, w.k0, -1, {0, 0}});
         }
     }
     // their sums by ranges of keys
@@ -1011,7 +1017,9 @@ void plan_weigh(const Shape& g, const std::vector<Member>& batch, int window, in
         }
     }
     const int per = (int)std::max(1ll, (key_tiles + WEIGH_MOST / 2 - 1) / (WEIGH_MOST / 2));  // key tiles of a work-group
-    const long long chunk = per > 1 ? 1ll << 40 : std::max<long long>(4, (row_tiles + SUM_PLACES - 1) / SUM_PLACES) * KEYS;  // rows of one
+    // rows of one (at least 4 tiles of them: 15 sequences in a window of 513, prompts of 33 .. 700 among them, 35.3 us; 8 and 16 tiles
+    // 38.7 and 45.9, where a batch has fewer parts to add up)
+    const long long chunk = per > 1 ? 1ll << 40 : std::max<long long>(4, (row_tiles + SUM_PLACES - 1) / SUM_PLACES) * KEYS;
     for (const Weighed& w : many) {
         const int units = (w.len - w.k0 + KEYS - 1) / KEYS;
         int pieces = 0;
@@ -1035,20 +1043,23 @@ void plan_weigh(const Shape& g, const std::vector<Member>& batch, int window, in
                 for (int p = 0; p < pieces; p++) {  // (a piece without keys leaves its rows' statistics empty)
                     const int a = std::max(lo, w.k0 + (int)((long long)units * p / pieces) * KEYS);
                     const int b = std::min(end, w.k0 + (int)((long long)units * (p + 1) / pieces) * KEYS);
-                    out.scores[SCORE_MANY].push_back({w.seq, h, w.tok0, w.rows, r, w.pos0, a, std::max(a, b), stat + p * w.rows + r, -1, pieces == 1, 0});
+                    out.scores[SCORE_MANY].push_back(
+                        {w.seq, h, w.tok0, w.rows, r, w.pos0, a, std::max(a, b), stat + p * w.rows + r, -1, pieces == 1, 0});
                 }
             }
             for (int k = w.k0; k < w.len; k += SUM_KEYS * per) {
                 const int end = std::min(w.len, k + SUM_KEYS * per);
                 const int r0 = (int)std::min<long long>(w.rows, std::max(0ll, (long long)(k - w.pos0) * group)) / KEYS * KEYS;
-                const int r1 = window ? (int)std::min<long long>(w.rows, std::max(0ll, ((long long)end - 1 + window - w.pos0) * group)) : w.rows;
+                const long long seen = std::max(0ll, ((long long)end - 1 + window - w.pos0) * group);
+                const int r1 = window ? (int)std::min<long long>(w.rows, seen) : w.rows;
                 int sums = (int)std::max(1ll, (std::max(0, r1 - r0) + chunk - 1) / chunk);
                 if (sums > 1 && work + (long long)sums * SUM_KEYS > room.work) sums = 1;
                 for (int x = 0; x < sums; x++) {
                     const int units_of = (std::max(0, r1 - r0) + KEYS - 1) / KEYS;
                     const int a = r0 + (int)((long long)units_of * x / sums) * KEYS;
                     const int b = std::min(std::max(r0, r1), r0 + (int)((long long)units_of * (x + 1) / sums) * KEYS);
-                    out.sums[1].push_back({w.seq, h, w.tok0, w.rows, w.pos0, k, end, a, b, stat, pieces, -1, 0, sums > 1 ? (int)work + x * SUM_KEYS : -1, {0, 0}});
+                    out.sums[1].push_back({w.seq, h, w.tok0, w.rows, w.pos0, k, end, a, b, stat, pieces, -1, 0,
+                                           sums > 1 ? (int)work + x * SUM_KEYS : -1, {0, 0}});
                 }
                 if (sums > 1) {
                     out.fades.push_back({w.seq, h, k, end, (int)work, sums, SUM_KEYS, 0});

@@ -89,7 +89,8 @@ struct Item {
     int part;        // first row of the split partials it writes, -1: it writes the output
     int split;
     int top;         // 0, or the tile is of keys that several sequences have (seq is one of them): its tokens are entries tok0 ..
-                     // of the batch's order, all behind the keys, the furthest at position top - 1; pos0: the end of the keys, k1 or behind it
+                     // of the batch's order, all behind the keys, the furthest at position top - 1; pos0: the end of the keys, k1 or
+                     // behind it
     int pad;
 };
 // Join of a tile's splits: split s of row r at part + s * count + r, and those of the shared tiles that its rows are in, Seg
@@ -149,7 +150,6 @@ void plan_shared(const Shape& g, const std::vector<Member>& batch, const Share& 
 // Entries a plan of `tokens` tokens of `seqs` sequences can have at most.
 size_t most_items(const Shape& g, int tokens, int seqs);
 size_t most_joins(const Shape& g, int tokens, int seqs);
-
 
 // ---- accumulated attention weights ----
 // Per window, the work of weighing a batch: what each position is given by the sequences' counted tokens (rows = counted

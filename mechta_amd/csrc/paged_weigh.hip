@@ -96,7 +96,7 @@ __device__ inline Sum load_sum(const Sum* p) {
     return Sum{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], x[8], x[9], x[10], x[11], x[12], x[13], {0, 0}};
 }
 
-// ---- few rows' kept scores summed up: a thread a key ----
+// ---- few rows' kept scores summed up: a thread a key, a row's scores of 16 neighbours in one 64-byte run ----
 __device__ inline void put_factor(const Args& a, float2 s, int head, int row, float2* f, int& odd) {
     f[row] = s = factor_of(a, s, head * a.group + row % a.group);
     if (!(s.y < -NEG_INF)) odd = 1;  // its weights are no numbers where it sees, and nothing all the same where it does not
@@ -126,7 +126,10 @@ __device__ inline void sum_kept(const Args& a, int seq, int head, int pos0, int 
 // ---- statistics of few rows, NRT x 16 of them, with their scores ----
 // 4 waves, each with every fourth block of 32 keys, its K straight from memory into the operands of the 16x16x32 products, the
 // next block's on its way meanwhile. Lane (r, g): row r, keys 4g + i and 16 + 4g + i of the block; each lane has an m and l of
-// its own until the end. Where there is no other piece, the sums are taken at once. Bound by memory.
+// its own until the end. Where there is no other piece, the sums are taken at once. Bound by memory: 64 sequences of a token at
+// 500 .. 8,001 positions of 4 x 128, 185 MB of K, 41 us; 8 of them are the 23 MB of scores that it writes (33 without, 5.5 TB/s),
+// 16 keys of a row behind the other, whole lines a store, which spare the second reading of K. One token at 300 positions of
+// 2 x 256, a launch: 6.0 us.
 template <typename T, int D, int NRT>
 __global__ void __launch_bounds__(256) score_few(Args a, const Score* __restrict__ items, const int* __restrict__ nitems) {
     constexpr int NS = D / 32;
@@ -219,8 +222,10 @@ __global__ void __launch_bounds__(256) score_few(Args a, const Score* __restrict
 // Both readings compute S^T[32 keys][32 rows] = K . Q^T (32x32x16): lane (r, h) has row r, keys 8c + 4h + i, so a row's statistics,
 // and what turns its scores into weights, are its lane's. One side stays in registers, 32 rows or 32 keys a wave; the other comes
 // by direct loads into a ring in LDS that the work-group's waves share, tiles of 32, one barrier a tile: what lands is
-// waited for by each wave before the barrier, and what is overwritten behind it has been read before it. Bound by the vector units (an
-// exponential and two to three others a score, in either reading) and the products beside them.
+// waited for by each wave before the barrier, and what is overwritten behind it has been read before it. Bound by the vector
+// units (an exponential, 8 cycles of a wave, and two to three others a score, in either reading) and the products, which run beside
+// them only in part: a prompt of 4,096 of 32 heads on 4 x 128, 68.7 GFLOP a reading, 84 us for the statistics (0.82 PFLOP/s; without
+// the exponentials 80, without the products 69) and 112 for the sums (0.61; 107 and 77).
 constexpr int RING_TILES = 4;
 // 64 lanes x 16 or 4 bytes from addresses of their own, to `lds` and behind
 __device__ inline void dma16v(const void* src, unsigned lds) {
@@ -326,7 +331,8 @@ __global__ void __launch_bounds__(256) score_rows(Args a, const Score* __restric
     }
 }
 
-// Several pieces of many rows' statistics: 16 lanes a row, 16 rows of an item a work-group.
+// Several pieces of many rows' statistics: 16 lanes a row, 16 rows of an item a work-group, up to 8 pieces a lane on their way at
+// once. Bound by latency: 512 rows of 125 pieces 3.9 us.
 __global__ void __launch_bounds__(256) merge_kernel(Args a, const Merge* __restrict__ items, const int* __restrict__ nitems) {
     const int count = *uniform(nitems) * MERGE_WAYS, lane = threadIdx.x % 16;
     for (int n = blockIdx.x; n < count; n += gridDim.x) {
@@ -354,6 +360,7 @@ __global__ void __launch_bounds__(256) merge_kernel(Args a, const Merge* __restr
 }
 
 // ---- sums over few rows' kept scores ----
+// Bound by the reading of the scores, from caches as far as they are there: 23 MB of 64 sequences 7.3 us.
 __global__ void __launch_bounds__(256) sum_few(Args a, const Sum* __restrict__ items, const int* __restrict__ nitems) {
     __shared__ float2 f[32];
     __shared__ int odd;
@@ -377,8 +384,9 @@ __global__ void __launch_bounds__(256) sum_few(Args a, const Sum* __restrict__ i
 }
 
 // ---- sums over many rows: 8 waves of 32 keys in registers, the rows through the ring ----
-// A row tile lies in LDS as its operands are read, [8 dims][row][8], and its final statistics behind it. Sums over the rows stay by row
-// and key in the lanes' registers until the end.
+// A row tile lies in LDS as its operands are read, [8 dims][row][8], and its final statistics behind it. Sums over the rows stay by
+// row and key in the lanes' registers until the end. (4 waves of 64 keys: 235 us for both readings of the prompt above, against 188,
+// registers in memory; the next tile's products among this one's exponentials by hand 230.)
 template <typename T, int D>
 __global__ void __launch_bounds__(512) sum_rows(Args a, const Sum* __restrict__ items, const int* __restrict__ nitems) {
     constexpr int NS = D / 16, TILE = 32 * D * 2, SLOT = TILE + 256, PER = D == 64 ? 1 : D / 128;  // (heads of 64: two waves bring the same)
@@ -401,8 +409,9 @@ __global__ void __launch_bounds__(512) sum_rows(Args a, const Sum* __restrict__ 
             const int r0 = max(it.r0, (int)(min((long long)(k0 - it.pos0) * a.group, (long long)it.rows)) / KEYS * KEYS);
             const int tiles = max(0, (there - r0 + 31) / 32);
             int row = r0 + x, rem = row % a.group;  // of the next tile to come
-            const T* src = (const T*)a.q + (int64_t)(it.tok0 + row / a.group) * a.q_tok + (it.head * a.group + rem) * a.q_head + piece0 * 16 + h * 8;
-            const T* const q0 = (const T*)a.q + (int64_t)(it.tok0 + r0 / a.group) * a.q_tok + (it.head * a.group + r0 % a.group) * a.q_head + piece0 * 16 + h * 8;
+            const T* const own = (const T*)a.q + it.head * a.group * a.q_head + piece0 * 16 + h * 8;
+            const T* src = own + (int64_t)(it.tok0 + row / a.group) * a.q_tok + rem * a.q_head;
+            const T* const q0 = own + (int64_t)(it.tok0 + r0 / a.group) * a.q_tok + r0 % a.group * a.q_head;
             auto issue = [&](int j) INLINE {  // (rows behind the last: the first again; tiles behind the last: its statistics)
                 const T* const p = row < there ? src : q0;
                 const unsigned to = lds + j % RING_TILES * SLOT;
@@ -474,7 +483,7 @@ __global__ void __launch_bounds__(512) sum_rows(Args a, const Sum* __restrict__ 
     }
 }
 
-// ---- weights that fade, and partial sums that join them ----
+// ---- weights that fade, and partial sums that join them: bound by latency, 4.7 us of the prompt's 4 x 4,096 positions ----
 __global__ void __launch_bounds__(256) fade_kernel(Args a, const Fade* __restrict__ items, const int* __restrict__ nitems) {
     const int count = *uniform(nitems);
     for (int n = blockIdx.x; n < count; n += gridDim.x) {
@@ -492,7 +501,7 @@ __global__ void __launch_bounds__(256) fade_kernel(Args a, const Fade* __restric
     }
 }
 
-// ---- weights of positions that are new, or another sequence's ----
+// ---- weights of positions that are new, or another sequence's: 20 x 65,536 copied in 4.7 us ----
 constexpr int CHANGES = 128;  // of a launch, in its arguments
 struct ChangeList {
     Change c[CHANGES];
@@ -546,8 +555,9 @@ __device__ inline int before_lane(unsigned long long lanes) {  // how many of th
 
 // The picks of one sequence, layer and head by a work-group: the least weight that stays, by digits of 11, 11 and 10 bits from the
 // highest on, then the positions in order; of those with just that weight the first ones. 65,536 weights stay in registers from one
-// reading to the next, four neighbours a thread and 4,096; longer sequences are read again for each. Each digit is counted in four places by
-// lane: weights are of few magnitudes, and lanes that count the same wait for each other.
+// reading to the next, four neighbours a thread and 4,096; longer sequences are read again for each. Each digit is counted in four
+// places by lane: weights are of few magnitudes, and lanes that count the same wait for each other. Bound by latency, barriers and
+// these counts: 20 x 65,536 43 us (counted in one place, with sums over the lanes for the kept ones' places, 62), 2,000 9.4.
 constexpr int GROUP = 16, PICKED = 4096 * GROUP, COUNTED = 4;
 __global__ void __launch_bounds__(1024) pick_kernel(WeightsAt w, EvictionList list, int n, int entry0, int first, int recent,
                                                     Eviction* __restrict__ entries, int* __restrict__ picks, float* __restrict__ kept,
@@ -601,9 +611,9 @@ __global__ void __launch_bounds__(1024) pick_kernel(WeightsAt w, EvictionList li
                 for (int t = 0; t < GROUP; t++) {
                     if (g0 + 4096 * t >= hi) break;
 #pragma unroll
-                    for (int y = 0; y < 4; y++) {
-                        if (v[t][y] && (v[t][y] & mask) == known) atomicAdd(&hist[(v[t][y] >> shift & digit) * COUNTED + lane % COUNTED], 1);
-                    }
+                    for (int y = 0; y < 4; y++)
+                        if (v[t][y] && (v[t][y] & mask) == known)
+                            atomicAdd(&hist[(v[t][y] >> shift & digit) * COUNTED + lane % COUNTED], 1);
                 }
             }
             __syncthreads();
@@ -713,7 +723,10 @@ __global__ void __launch_bounds__(1024) pick_kernel(WeightsAt w, EvictionList li
 // A new page's block of 32 positions of a head and layer, K or V: 16 bytes of K a thread (8 dims of a position), 16 bytes of V
 // (a dim of 8 positions, which come from 8 places), all on their way at once; `parts` work-groups share a block's dims where blocks are
 // few. Positions behind the last that stays are left as they were. Bound by memory, which gives whole lines: 128 bytes are 8
-// positions of 8 dims of K, or 8 dims of 8 positions of V, so that of a sequence cut to a quarter nearly all lines are read.
+// positions of 8 dims of K, or 8 dims of 8 positions of V, so that of a sequence cut to a quarter nearly all lines are read: 65,536
+// to 16,384 of 10 layers of 2 x 256 280 us, 335 MB written and 1.16 GB read, 5.35 TB/s. K comes past the caches (nothing else is
+// in its lines that another work-group takes; through them 0.7% slower); V through them, a line serves 4 loads of a wave (past
+// them 12% slower).
 template <int D>
 __global__ void __launch_bounds__(256) gather_kernel(unsigned short* __restrict__ pool, const int* __restrict__ table, int most_pages,
                                                      int page, int kv_heads, int units, size_t plane,
@@ -784,7 +797,7 @@ __global__ void __launch_bounds__(256) gather_kernel(unsigned short* __restrict_
     }
 }
 
-// The weights that stay, from where the picks have put them.
+// The weights that stay, from where the picks have put them: 20 x 16,384 5 us. (Gathered by position, in place, 14.5.)
 __global__ void __launch_bounds__(256) pack_kernel(WeightsAt w, const Eviction* __restrict__ entries, const float* __restrict__ kept,
                                                    size_t stride, size_t all, int units) {
     for (size_t b = blockIdx.x; b < all; b += gridDim.x) {
@@ -817,7 +830,9 @@ hipError_t weigh_as(const Args& a, const int* batch, const WeighLists& l, const 
 
 template <typename T>
 hipError_t weigh_dim(int dim, const Args& a, const int* batch, const WeighLists& l, const int* grid, hipStream_t s) {
-    return dim == 64 ? weigh_as<T, 64>(a, batch, l, grid, s) : dim == 128 ? weigh_as<T, 128>(a, batch, l, grid, s) : weigh_as<T, 256>(a, batch, l, grid, s);
+    return dim == 64    ? weigh_as<T, 64>(a, batch, l, grid, s)
+           : dim == 128 ? weigh_as<T, 128>(a, batch, l, grid, s)
+                        : weigh_as<T, 256>(a, batch, l, grid, s);
 }
 
 template <bool COPY>

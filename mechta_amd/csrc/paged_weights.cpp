@@ -13,8 +13,9 @@ using namespace mkv::paged;
 
 namespace {
 
-// Work-groups of each kernel of a captured weighing, of whatever batch it finds. (1 token at 300 positions of 2 x 256, 64 at 3,000 and 4 of one
-// sequence at 65,536 of 4 x 128, in a graph: 15.3 / 58.5 / 50.0 us; with 8,192 for the merges 16.6 / 60.1 / 51.6, with 512 of each kind 15.2 / 60.8 / 65.8.)
+// Work-groups of each kernel of a captured weighing, of whatever batch it finds. (1 token at 300 positions of 2 x 256, 64 at 3,000 and 4
+// of one sequence at 65,536 of 4 x 128, in a graph: 15.3 / 58.5 / 50.0 us; with 8,192 for the merges 16.6 / 60.1 / 51.6, with 512 of
+// each kind 15.2 / 60.8 / 65.8. Of a handle that counts a token of each sequence, whose graphs have two kernels: 7.4 / 50.6.)
 constexpr int GRAPH_WEIGH = 1024, GRAPH_MERGES = 512;
 constexpr long long WORK_MOST = 1ll << 28;  // floats: kept scores
 constexpr long long STATS_MORE = 1ll << 18;  // statistics of rows in more than one piece
@@ -215,7 +216,10 @@ int mpg_weigh(mpg_t* h, int layer, int rows, const void* q, int64_t q_tok, int64
     a.work = k->work;
     int grid[WEIGH_LISTS];
     auto size = [&](int list) {
-        return list <= SCORE_MANY ? p.scores[list].size() : list == MERGES ? p.merges.size() * MERGE_WAYS : list < FADES ? p.sums[list - SUM_FEW].size() : p.fades.size();
+        return list <= SCORE_MANY ? p.scores[list].size()
+               : list == MERGES   ? p.merges.size() * MERGE_WAYS
+               : list < FADES     ? p.sums[list - SUM_FEW].size()
+                                  : p.fades.size();
     };
     // a captured call has the kernels that some batch of the handle needs
     for (int l = 0; l < WEIGH_LISTS; l++)
