@@ -531,12 +531,13 @@ __global__ void __launch_bounds__(256) change_kernel(WeightsAt w, ChangeList lis
 }
 
 // ---- eviction ----
-constexpr int EVICTIONS = 128, NEW_PAGES = 256;
+constexpr int EVICTIONS = 128, NEW_PAGES = 480;  // of a launch, in its arguments (4 KB)
 struct EvictionList {
     Eviction e[EVICTIONS];
 };
+// a new page: 27 bits of page and 5 of the entry's, 11 more and 17 of which page of the sequence it is (the limits of mpg_create)
 struct PageList {
-    NewPage p[NEW_PAGES];
+    unsigned p[NEW_PAGES][2];
 };
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -737,7 +738,8 @@ __global__ void __launch_bounds__(256) gather_kernel(unsigned short* __restrict_
     __shared__ int in[KEYS];
     typedef Vec8<unsigned short> Unit;
     const int tid = threadIdx.x, blocks = page / KEYS;
-    const NewPage np = list.p[blockIdx.x / blocks];
+    const unsigned n0 = list.p[blockIdx.x / blocks][0], n1 = list.p[blockIdx.x / blocks][1];
+    const NewPage np{(int)(n0 >> 27 | (n1 & 0x7FF) << 5), (int)(n1 >> 11), (int)(n0 & 0x7FFFFFF)};
     const int block = blockIdx.x % blocks, part = blockIdx.z / 2;
     const bool is_v = blockIdx.z % 2;
     const Eviction e = entries[np.entry];
@@ -902,7 +904,11 @@ hipError_t launch_gather(const Geometry& g, char* pool, const int* table, const 
     for (int i = 0; i < n; i += NEW_PAGES) {
         PageList list;
         const int m = std::min(NEW_PAGES, n - i);
-        for (int j = 0; j < NEW_PAGES; j++) list.p[j] = j < m ? pages[i + j] : NewPage{0, 0, 0};
+        for (int j = 0; j < NEW_PAGES; j++) {
+            const NewPage np = j < m ? pages[i + j] : NewPage{0, 0, 0};
+            list.p[j][0] = (unsigned)np.page | (unsigned)np.entry << 27;
+            list.p[j][1] = (unsigned)np.entry >> 5 | (unsigned)np.nth << 11;
+        }
         const int units = g.layers * g.kv_heads;
         const long long groups = (long long)n * (g.page / KEYS) * units * 2;
         const int parts = groups >= 2048 ? 1 : std::min(g.head_dim / 64, groups >= 1024 ? 2 : 4);

@@ -578,6 +578,26 @@ def test_another_current_stream(torch_gpu, pg):
         m.check([0])
 
 
+def test_two_caches_on_two_streams(torch_gpu, pg):
+    """Each has its own room to work in: calls of one run beside the other's."""
+    torch = torch_gpu
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    with torch.cuda.stream(streams[0]):
+        a = Model(torch, pg, 2, 4, 64, "bf16", 64)
+    with torch.cuda.stream(streams[1]):
+        b = Model(torch, pg, 1, 8, 128, "f16", 32, last=4)
+    for step in range(6):
+        for m, s in ((a, streams[0]), (b, streams[1])):
+            with torch.cuda.stream(s):
+                m.begin([0, 1, 2], [300, 1, 40] if step % 2 else [1, 60, 2], shared=step > 3)
+                m.weigh(decay=0.9)
+                if step == 3:
+                    m.evict([0], [100], first=2, recent=30)
+    for m, s in ((a, streams[0]), (b, streams[1])):
+        with torch.cuda.stream(s):
+            m.check()
+
+
 def test_refusals(torch_gpu, pg):
     torch = torch_gpu
 
