@@ -385,8 +385,8 @@ __global__ void __launch_bounds__(256) sum_few(Args a, const Sum* __restrict__ i
 
 // ---- sums over many rows: 8 waves of 32 keys in registers, the rows through the ring ----
 // A row tile lies in LDS as its operands are read, [8 dims][row][8], and its final statistics behind it. Sums over the rows stay by
-// row and key in the lanes' registers until the end. (4 waves of 64 keys: 235 us for both readings of the prompt above, against 188,
-// registers in memory; the next tile's products among this one's exponentials by hand 230.)
+// row and key in the lanes' registers until the end. (4 waves of 64 keys, some of whose registers go to memory: 235 us for both
+// readings of the prompt above, against 188; the next tile's products among this one's exponentials by hand: 230.)
 template <typename T, int D>
 __global__ void __launch_bounds__(512) sum_rows(Args a, const Sum* __restrict__ items, const int* __restrict__ nitems) {
     constexpr int NS = D / 16, TILE = 32 * D * 2, SLOT = TILE + 256, PER = D == 64 ? 1 : D / 128;  // (heads of 64: two waves bring the same)
