@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <iterator>
 
 #include "../../include/mechta_kv.h"
 
@@ -726,8 +727,9 @@ void draft(const Shape& g, const std::vector<Member>& batch, const Share* share,
     // Few rows among a chunk's tiles fill CUs that its last ones leave idle, and spare a launch, often two. (us apart / among:
     // 512 tokens and 12 decodes at 500 .. 4,000 positions 31.8 / 23.9 of 4 x 128, 40.8 / 30.6 of 2 x 256; 100 and 20 at 100
     // .. 400 21.9 / 13.9, 31.8 / 19.8. 64 tokens and 60 decodes at 500 .. 8,000 of 4 x 128 92.7 / 114: those stay apart.)
-    std::vector<Tile> both = by_kind[HALF];
-    for (int k : {FEW, SOME}) both.insert(both.end(), by_kind[k].begin(), by_kind[k].end());
+    std::vector<Tile> both = by_kind[HALF];  // (of a streamed range's tiles of 32 rows those that a chunk's tiles begin with)
+    for (int k : {FEW, SOME})
+        std::copy_if(by_kind[k].begin(), by_kind[k].end(), std::back_inserter(both), [](const Tile& t) { return t.row0 % TILE_ROWS[HALF] == 0; });
     double together = 1e30;
     const bool mixed = !by_kind[HALF].empty() && both.size() > by_kind[HALF].size();
     const long long joint = mixed ? chunk_length(both, g, HALF, together) : 0;
