@@ -124,7 +124,11 @@ int guarded(const char* who, F f) {  // no exception crosses the C boundary
     if (const int cap = capturing(h, who))                                                                   \
         return cap < 0 ? cap : fail(MKV_E_ARG, "%s: the stream is capturing; page calls run outside a graph", who)
 
-// paged_store.cpp: the batch that stands ends; what the device does not know of the page tables and shifts goes up.
+// paged_store.cpp: words of a handle's tables and lists on the device, which with those of its weights are fewer than WORDS_MOST
+// (an upload's offsets are numbers of 32 bits).
+constexpr size_t WORDS_MOST = 1ull << 32;
+size_t handle_words(const mpg_config& c);
+// The batch that stands ends; what the device does not know of the page tables and shifts goes up.
 int end_batch(mpg_store* h, const char* who);
 int upload_tables(mpg_store* h, const char* who);
 

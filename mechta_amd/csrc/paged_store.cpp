@@ -220,6 +220,7 @@ int upload(mpg_store* h, const std::vector<Run>* runs, const std::vector<Plan>* 
 
 }  // namespace
 
+size_t mkv::paged::handle_words(const mpg_config& c) { return sizes(c, MPG_WINDOWS_MAX).words; }
 int mkv::paged::upload_tables(mpg_store* h, const char* who) { return upload(h, nullptr, nullptr, nullptr, who); }
 
 // What replays of captured calls do once pages have changed hands and no batch stands: nothing. The batch stands until the

@@ -115,6 +115,13 @@ double bytes_of(const WeightSizes& s, const mpg_config& c) {
 int check_last(const char* who, int last) {
     return last < 0 ? fail(MKV_E_ARG, "%s: the last %d tokens", who, last) : MKV_OK;
 }
+// What is refused before anything is allocated.
+int check_sizes(const char* who, const WeightSizes& s, const mpg_config& c) {
+    const double all = bytes_of(s, c);
+    if (all > 1ll << 48) return fail(MKV_E_NOMEM, "%s: %g bytes", who, all);
+    const size_t words = handle_words(c) + s.words;
+    return words < WORDS_MOST ? (int)MKV_OK : fail(MKV_E_NOMEM, "%s: lists of %zu words", who, words);
+}
 
 }  // namespace
 
@@ -122,8 +129,8 @@ extern "C" {
 
 size_t mpg_weights_bytes(const mpg_config* c, int last) {
     if (!mpg_bytes(c) || check_last("mpg_weights_bytes", last)) return 0;
-    const double b = bytes_of(weight_sizes(*c, last), *c);
-    return b > 1ll << 48 ? 0 : (size_t)b;
+    const WeightSizes s = weight_sizes(*c, last);
+    return check_sizes("mpg_weights_bytes", s, *c) ? 0 : (size_t)bytes_of(s, *c);
 }
 
 static int keep_weights(mpg_t* h, int last) {
@@ -132,8 +139,7 @@ static int keep_weights(mpg_t* h, int last) {
     if (h->used) return fail(MKV_E_ARG, "mpg_keep_weights: sequences have had positions already");
     const mpg_config& c = h->c;
     const WeightSizes s = weight_sizes(c, last);
-    const double all = bytes_of(s, c);
-    if (all > 1ll << 48) return fail(MKV_E_NOMEM, "mpg_keep_weights: %g bytes", all);
+    if (int rc = check_sizes("mpg_keep_weights", s, c)) return rc;
     std::unique_ptr<Kept> k(new Kept);
     k->h = h;
     k->last = last;
@@ -145,8 +151,7 @@ static int keep_weights(mpg_t* h, int last) {
     // the lists and shifts go where the handle's uploads go: behind what is there
     const size_t words = h->words + s.words;
     int* dev = nullptr;
-    hipError_t e = words < 1ull << 32 ? hipSuccess : hipErrorOutOfMemory;
-    if (e == hipSuccess) e = hipMalloc((void**)&dev, words * 4);
+    hipError_t e = hipMalloc((void**)&dev, words * 4);
     if (e == hipSuccess) e = hipMalloc((void**)&k->at.p, s.weights * 4);
     if (e == hipSuccess) e = hipMalloc((void**)&k->stats, (s.stats + KEYS) * 8);
     if (e == hipSuccess) e = hipMalloc((void**)&k->work, s.work * 4);
@@ -159,7 +164,7 @@ static int keep_weights(mpg_t* h, int last) {
     if (e != hipSuccess) {
         (void)hipGetLastError();
         if (dev) (void)hipFree(dev);
-        return fail(MKV_E_NOMEM, "mpg_keep_weights: %.0f bytes: %s", all, hipGetErrorString(e));
+        return fail(MKV_E_NOMEM, "mpg_keep_weights: %.0f bytes: %s", bytes_of(s, c), hipGetErrorString(e));
     }
     (void)hipFree(h->dev);
     h->dev = dev;
