@@ -294,8 +294,14 @@ int mpg_rotate(const mpg_turns* r, int fmt, int rows, int heads, int dim, const 
     return e == hipSuccess ? MKV_OK : hip_fail(e, "mpg_rotate");
 }
 
+// What is refused before anything is allocated.
+static int check_words(const char* who, const mpg_config& c) {
+    const size_t words = handle_words(c);
+    return words < WORDS_MOST ? (int)MKV_OK : fail(MKV_E_NOMEM, "%s: lists of %zu words", who, words);
+}
+
 size_t mpg_bytes(const mpg_config* c) {
-    if (check_config("mpg_bytes", c)) return 0;
+    if (check_config("mpg_bytes", c) || check_words("mpg_bytes", *c)) return 0;
     const Sizes s = sizes(*c, MPG_WINDOWS_MAX);
     return s.pool + (s.words + s.part) * 4;
 }
@@ -304,6 +310,7 @@ static int create(mpg_t** out, const mpg_config* c, const int* windows, const mp
     if (!out) return fail(MKV_E_ARG, "mpg_create: NULL argument");
     *out = nullptr;
     if (int rc = check_config("mpg_create", c)) return rc;
+    if (int rc = check_words("mpg_create", *c)) return rc;
     if (rope) {
         if (int rc = check_rope("mpg_create", rope)) return rc;
         if (rope->dim > c->head_dim)
@@ -340,7 +347,7 @@ static int create(mpg_t** out, const mpg_config* c, const int* windows, const mp
     h->book.init(c->pages, c->page, c->seqs, c->ctx);
     if (const int cap = capturing(h, "mpg_create"))
         return cap < 0 ? cap : fail(MKV_E_ARG, "mpg_create: the stream is capturing");
-    hipError_t e = s.words < 1ull << 32 ? hipGetDevice(&h->device) : hipErrorOutOfMemory;
+    hipError_t e = hipGetDevice(&h->device);
     if (e == hipSuccess) e = hipMalloc((void**)&h->pool, s.pool);
     if (e == hipSuccess) e = hipMalloc((void**)&h->dev, s.words * 4);
     if (e == hipSuccess) e = hipMalloc((void**)&h->part, s.part * 4);

@@ -19,3 +19,15 @@ def test_weights_bytes_of_what_is_refused(more):
     assert b"mpg_weights_bytes: lists of" in L.mkv_last_error()
     more["seqs"] = more["tokens"] = 1000
     assert L.mpg_weights_bytes(config(**more), 1) > 0
+
+
+# lists past 2^32 words
+@pytest.mark.parametrize("more", [dict(q_heads=1024, kv_heads=1024, tokens=262144), dict(q_heads=512, kv_heads=256, seqs=65536, tokens=65536, ctx=8192)])
+def test_bytes_of_what_is_refused(more):
+    L = paged.lib()
+    assert L.mpg_bytes(config(**more)) == 0 and b"mpg_bytes: lists of" in L.mkv_last_error()
+    h = ctypes.c_void_p(1)
+    assert L.mpg_create(ctypes.byref(h), config(**more), None, None, None) == -7 and h.value is None
+    assert b"mpg_create: lists of" in L.mkv_last_error()
+    more["tokens"] = more["seqs"] = 100
+    assert L.mpg_bytes(config(**more)) > 0
