@@ -2,7 +2,7 @@
  * (libmechta_kv.so). Error codes are the MKV_E_* of mechta_kv.h and the message of a failed call is in
  * mkv_last_error(); a refused call changes nothing and enqueues nothing, and one that fails on its way to the device (MKV_E_HIP,
  * or MKV_E_NOMEM of the host) leaves every sequence as it was, so that it can be made again, and the batch too, unless it
- * was the copying of pages that failed: then no batch stands.
+ * was the copying of pages that failed, or mpg_evict: then no batch stands.
  *
  * A handle owns a pool of `pages` pages. A page holds `page` consecutive positions of one sequence, K and V of every
  * layer. Sequences are numbered 0 .. seqs - 1; a sequence is the list of its pages and a length, both kept on the host
@@ -198,8 +198,9 @@ int mpg_weigh(mpg_t* h, int layer, int rows, const void* q, int64_t q_tok, int64
 /* Cuts each of n different sequences of more than keep[i] positions to keep[i] >= 1: its first `first` and last `recent` ones
  * and, for each layer and kv head by itself, those of the largest weights between them (of equal ones the lowest positions; NaN
  * weighs most). K, V and weights stay in order, on new pages: the pool needs as many free pages as keep[i] positions of each
- * take, before the old ones are given back (MKV_E_NOMEM). Layers with a window need `recent` to be no less than it. A batch ends,
- * as with every call that changes pages. */
+ * take, before the old ones are given back (MKV_E_NOMEM; of sequences cut in calls of their own each finds the pages that the ones
+ * before gave back). Layers with a window need `recent` to be no less than it. A batch ends, as with every call that changes
+ * pages. */
 int mpg_evict(mpg_t* h, int n, const int* seq, const int* keep, int first, int recent);
 /* The position of a sequence's next token: its length, and what has been evicted of it. */
 int mpg_position(const mpg_t* h, int seq, int* position);

@@ -632,7 +632,8 @@ struct Common {
     int rows = 0, tok0 = 0, k0 = 0, splits = 0, part = 0;
 };
 // How a batch's work may be cut. APART: every sequence by itself. STREAMED: what they share in tiles of 32 rows beside their own, all
-// by few_rows. TILED: what they share in a chunk's tiles where it has more than 32 rows. (Whole calls, us, 2 / 4 / 8 / 16 / 64 tokens on
+// by few_rows (or, where few rows go among a chunk's tiles, with them). TILED: what they share in a chunk's tiles where it has more than
+// 32 rows. (Whole calls, us, 2 / 4 / 8 / 16 / 64 tokens on
 // a prompt of 16,384 of 4 x 128, 32 heads: apart 16.7 / 23.4 / 38.9 / 55 / 123, where the later readings come out of the L2s at 17 TB/s;
 // streamed 14.8 / 15.8 / 19.1 / 30.9 / 48; tiled 13.8 / 21 / 20.6 / 26.8 / 39.)
 enum Way { APART, STREAMED, TILED };
